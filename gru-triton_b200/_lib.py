@@ -44,7 +44,31 @@ class CGemmArgs(ctypes.Structure):
                 ("C", ctypes.c_void_p), ("ldc", ctypes.c_longlong), ("split_stride", ctypes.c_longlong)]
 
 
+class CGatedArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int) for n in ("T", "B", "H", "dtype", "candidate_tanh", "length_bytes")] +
+                [("gi", ctypes.c_void_p), ("gi_t", ctypes.c_longlong), ("gi_b", ctypes.c_longlong),
+                 ("h0", ctypes.c_void_p), ("h0_b", ctypes.c_longlong), ("lengths", ctypes.c_void_p),
+                 ("out", ctypes.c_void_p), ("out_t", ctypes.c_longlong), ("out_b", ctypes.c_longlong),
+                 ("h_T", ctypes.c_void_p), ("states", ctypes.c_void_p),
+                 ("dout", ctypes.c_void_p), ("dout_t", ctypes.c_longlong), ("dout_b", ctypes.c_longlong),
+                 ("dh_T", ctypes.c_void_p), ("dh_b", ctypes.c_longlong),
+                 ("dgi", ctypes.c_void_p), ("dgi_t", ctypes.c_longlong), ("dgi_b", ctypes.c_longlong),
+                 ("dh0", ctypes.c_void_p)])
+
+
+class CLinearArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int) for n in ("M", "K", "N", "dtype", "activation")] +
+                [("x", ctypes.c_void_p), ("ldx", ctypes.c_longlong), ("W", ctypes.c_void_p), ("ldw", ctypes.c_longlong),
+                 ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("ldr", ctypes.c_longlong),
+                 ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong), ("slope", ctypes.c_void_p), ("lds", ctypes.c_longlong),
+                 ("dy", ctypes.c_void_p), ("lddy", ctypes.c_longlong), ("dx", ctypes.c_void_p), ("dW", ctypes.c_void_p),
+                 ("db", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)])
+
+
 _P = ctypes.c_void_p
+_L = ctypes.c_longlong
+_NP = ctypes.POINTER(CGatedArgs)
+_AP = ctypes.POINTER(CLinearArgs)
 _GP = ctypes.POINTER(CGemmArgs)
 _QP = ctypes.POINTER(CQuant)
 _SP = ctypes.POINTER(CShape)
@@ -79,6 +103,13 @@ SIGNATURES = {
     "b200gru_column_sums": (_I, [_P, _Z, _I, _P, _P, _Z, _P]),
     "b200gru_calibration_workspace_bytes": (_Z, [_SP]),
     "b200gru_calibration_scan": (_I, [_SP, _P, _P, _P, _P, _I, ctypes.c_double, _P, _P, _I, _P, _P, _I, _P, _P, _Z, _P]),
+    "b200gru_gated_states_bytes": (_Z, [_I, _I, _I]),
+    "b200gru_gated_scan_forward": (_I, [_NP, _P]),
+    "b200gru_gated_scan_backward": (_I, [_NP, _P]),
+    "b200gru_gated_step": (_I, [_I, _I, _I, _I, _P, _L, _P, _L, _P, _P, _L, _P]),
+    "b200gru_linear_act_workspace_bytes": (_Z, [_AP, _I]),
+    "b200gru_linear_act_forward": (_I, [_AP, _P]),
+    "b200gru_linear_act_backward": (_I, [_AP, _P]),
     "b200gru_device_status": (_I, [_I]),
     "b200gru_layer_sizes": (_I, [_P, _P]),
     "b200gru_layer_forward": (_I, [_P, _P, _P, _P]),

@@ -1,0 +1,148 @@
+"""Matrix product with bias, activation and residual in its epilogue.
+
+    y = act(x @ W^T + bias) + residual
+
+The product that makes the gates of a recurrence, that widens a feed-forward layer, or that takes a layer's
+output back into the stream of a model, without a second pass over its result.  ``tc.linear`` is its neighbour for
+quantised weights: float32 alone, no activation or residual.
+
+Element types float32, bfloat16 and float16, one for all tensors of a call; sums are float32.  float32 operands run as
+two row-scaled fp16 planes in three tensor-core products (22 significant bits, as ``tc.linear``'s).  What the backward
+needs of the activation is its slope, kept by the forward in float32 or, for the 16-bit types, in float16.  The
+same call repeats its bits.  CUDA tensors only; there is no fallback.  The reference's counterpart is ``F.linear``
+(src/gru_qat/gru_cell.py:410-435), without activation and residual.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Any, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._scan_common import require_cuda
+from .scan_gated import DTYPES, on_device, rows_contiguous, stream_of
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4, "tanh": 5}
+
+
+def _check(x, W, bias, residual, activation):
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}; got {activation!r}")
+    given = {k: v for k, v in (("x", x), ("W", W), ("bias", bias), ("residual", residual)) if v is not None}
+    if x.dtype not in DTYPES:
+        raise ValueError(f"x dtype must be float32, bfloat16 or float16; got {x.dtype}")
+    for name, t in given.items():
+        if t.dtype != x.dtype:
+            raise ValueError(f"{name} dtype must be x's, {x.dtype}; got {t.dtype}")
+    if W.dim() != 2 or x.dim() < 1 or x.shape[-1] != W.shape[1]:
+        raise ValueError(f"linear_act needs x[..., K] and W[N, K]; got {tuple(x.shape)} and {tuple(W.shape)}")
+    N, K = W.shape
+    if N == 0 or K == 0:
+        raise ValueError(f"N and K must be > 0; got N={N}, K={K}")
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"bias shape must be (N,)=({N},); got {tuple(bias.shape)}")
+    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
+        raise ValueError(f"residual shape must be {(*x.shape[:-1], N)}; got {tuple(residual.shape)}")
+    require_cuda(**given)
+    for name, t in given.items():
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as a matrix of rows, in place where its strides allow it."""
+    return rows_contiguous(t.reshape(-1, t.shape[-1]))
+
+
+def _fill(x, W, activation) -> _lib.CLinearArgs:
+    a = _lib.CLinearArgs()
+    a.M, a.K = x.shape
+    a.N = W.shape[0]
+    a.dtype, a.activation = DTYPES[x.dtype], ACTIVATIONS[activation]
+    a.x, a.ldx, a.W, a.ldw = x.data_ptr(), x.stride(0), W.data_ptr(), W.stride(0)
+    return a
+
+
+def _run(a, backward: bool, device) -> None:
+    lib = _lib.load()
+    n = lib.b200gru_linear_act_workspace_bytes(ctypes.byref(a), int(backward))
+    if n == ctypes.c_size_t(-1).value:
+        raise RuntimeError("linear_act: shape not supported")
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    call = lib.b200gru_linear_act_backward if backward else lib.b200gru_linear_act_forward
+    with on_device(device):
+        rc = call(ctypes.byref(a), stream_of(device))
+    if rc:
+        _lib._raise(rc, "linear_act backward" if backward else "linear_act")
+    _lib._after_call()
+
+
+def _forward(x, W, bias, residual, activation, want_slope: bool):
+    """(y[M, N], slope or None)."""
+    lead, N = x.shape[:-1], W.shape[0]
+    x, W = _rows(x), rows_contiguous(W)
+    M = x.shape[0]
+    y = torch.empty((M, N), device=x.device, dtype=x.dtype)
+    slope = None
+    if want_slope and activation != "none":
+        # rows padded to eight elements: 16-byte accesses at any width
+        slope = torch.empty((M, -(-N // 8) * 8), device=x.device, dtype=torch.float32 if x.dtype == torch.float32 else torch.float16)
+    if M:
+        a = _fill(x, W, activation)
+        if bias is not None:
+            bias = rows_contiguous(bias)
+            a.bias = bias.data_ptr()
+        if residual is not None:
+            residual = _rows(residual)
+            a.residual, a.ldr = residual.data_ptr(), residual.stride(0)
+        a.y, a.ldy = y.data_ptr(), N
+        if slope is not None:
+            a.slope, a.lds = slope.data_ptr(), slope.stride(0)
+        _run(a, False, x.device)
+    return y.reshape(*lead, N), slope
+
+
+class LinearActFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x, W, bias, residual, activation):
+        y, slope = _forward(x, W, bias, residual, activation, True)
+        ctx.save_for_backward(x, W, *([slope] if slope is not None else []))
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, dy):
+        x, W, *slope = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+        M, (N, K) = x.numel() // x.shape[-1], W.shape
+        fresh = torch.empty if M else torch.zeros
+        dW = fresh((N, K), device=x.device, dtype=x.dtype) if need_w else None
+        db = fresh((N,), device=x.device, dtype=x.dtype) if need_b else None
+        if M and (need_x or need_w or need_b):
+            x2, W2, dy2 = _rows(x), rows_contiguous(W), _rows(dy)
+            a = _fill(x2, W2, ctx.activation)
+            a.dy, a.lddy = dy2.data_ptr(), dy2.stride(0)
+            if slope:
+                a.slope, a.lds = slope[0].data_ptr(), slope[0].stride(0)
+            a.dx, a.dW, a.db = (None if t is None else t.data_ptr() for t in (dx, dW, db))
+            _run(a, True, x.device)
+        return dx, dW, db, (dy if need_r else None), None
+
+
+def linear_act(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: str = "none",
+               residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(x[..., K] @ W[N, K]^T + bias[N]) + residual[..., N]`` in x's type; differentiable in all four tensors.
+
+    ``activation``: none, relu, silu, gelu (the error-function form), sigmoid or tanh.  Rows may have any stride; a
+    residual has the result's shape (``expand`` a broadcast one)."""
+    _check(x, W, bias, residual, activation)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, W, bias, residual)):
+        return LinearActFunction.apply(x, W, bias, residual, activation)
+    return _forward(x, W, bias, residual, activation, False)[0]

@@ -272,6 +272,67 @@ int b200gru_layer_sizes(const int* dims, size_t* sizes);
 int b200gru_layer_forward(const int* dims, const float* quants, const void* const* ptrs, void* stream);
 int b200gru_layer_backward(const int* dims, const float* quants, const void* const* ptrs, void* stream);
 
+/* ---- gated linear recurrence -------------------------------------------------------------------
+ * The GRU update with gates from the input alone (no hidden weights), so its steps are affine maps of the state:
+ *   z = sigmoid(x)   n = tanh(c) or c   h_t = z h_{t-1} + (1 - z) n      gi[t][b] = (x[H], c[H])
+ * Element type of gi, out, dout, dgi: `dtype`; states are fp32.  Strides in elements, units of a row contiguous; inputs
+ * may have stride 0.  No reference counterpart.
+ *   lengths   steps of each row (int32 or int64, length_bytes 4 or 8), held inside [0, T]; NULL: T.  Behind a row's last
+ *             step nothing is read into its results, out and dgi are zero, and h_T[b] is the state after its last step
+ *             (h0[b] for a row without steps)
+ *   states    b200gru_gated_states_bytes(T, B, H), written by a forward that a backward follows, else NULL; the backward
+ *             recomputes the states between from gi
+ *   h0, dout, dh_T   NULL: zeros.   dh0   NULL: not wanted
+ * Results repeat their bits; those of a row depend on T and B to rounding. */
+enum { B200GRU_F32 = 0, B200GRU_BF16 = 1, B200GRU_F16 = 2 };
+typedef struct {
+  int T, B, H, dtype, candidate_tanh, length_bytes;
+  const void* gi; long long gi_t, gi_b;
+  const float* h0; long long h0_b;
+  const void* lengths;
+  void* out; long long out_t, out_b;
+  float* h_T;                        /* [B][H] */
+  float* states;
+  const void* dout; long long dout_t, dout_b;
+  const float* dh_T; long long dh_b;
+  void* dgi; long long dgi_t, dgi_b;
+  float* dh0;                        /* [B][H] */
+} b200gru_gated_args;
+size_t b200gru_gated_states_bytes(int T, int B, int H);
+int b200gru_gated_scan_forward(const b200gru_gated_args* args, void* stream);
+int b200gru_gated_scan_backward(const b200gru_gated_args* args, void* stream);
+/* One step: gi[B][2H] (row stride gi_b), h -> out[B][H] (contiguous, `dtype`) and h_new, which may be h itself. */
+int b200gru_gated_step(int dtype, int candidate_tanh, int B, int H, const void* gi, long long gi_b, const float* h,
+                       long long h_b, void* out, float* h_new, long long hn_b, void* stream);
+
+/* ---- product with bias, activation and residual -------------------------------------------------
+ *   y = act(x W^T + bias) + residual         x[M][K], W[N][K], bias[N], residual[M][N], y[M][N]
+ *   d = dy act'(pre)   dx = d W   dW = d^T x   db = sum over rows of d      (the residual's gradient is dy itself)
+ * All of `dtype`; row strides ld* in elements (inputs may have stride 0), rows contiguous; dx, dW and db are packed.
+ * bias, residual, dx, dW, db may be NULL.  slope: [M][lds], written by a forward that a backward follows (fp32 for
+ * fp32, else fp16) and read by it; NULL in inference and where there is no activation.  workspace: 256-byte aligned,
+ * b200gru_linear_act_workspace_bytes of the same arguments ((size_t)-1: invalid).  No reference counterpart (its
+ * projections are F.linear, src/gru_qat/gru_cell.py:410-435). */
+enum { B200GRU_ACT_NONE = 0, B200GRU_ACT_RELU = 1, B200GRU_ACT_SILU = 2, B200GRU_ACT_GELU = 3, B200GRU_ACT_SIGMOID = 4,
+       B200GRU_ACT_TANH = 5 };
+typedef struct {
+  int M, K, N, dtype, activation;
+  const void* x; long long ldx;
+  const void* W; long long ldw;
+  const void* bias;
+  const void* residual; long long ldr;
+  void* y; long long ldy;
+  void* slope; long long lds;
+  const void* dy; long long lddy;
+  void* dx;
+  void* dW;
+  void* db;
+  void* workspace; size_t workspace_bytes;
+} b200gru_linear_args;
+size_t b200gru_linear_act_workspace_bytes(const b200gru_linear_args* args, int backward);
+int b200gru_linear_act_forward(const b200gru_linear_args* args, void* stream);
+int b200gru_linear_act_backward(const b200gru_linear_args* args, void* stream);
+
 /* Diagonal backward for callers that cannot allocate device memory.  It has no counterpart in
  * the reference (whose wrappers always allocate their scratch with torch).  Same inputs, outputs
  * and results as b200gru_diagonal_backward, but no workspace argument: the partial sums go into a

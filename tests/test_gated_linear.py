@@ -1,0 +1,716 @@
+"""The gated linear recurrence (``scan_gated``) and the product with bias, activation and residual
+(``linear_act``) against plain implementations in 64 bits; refusals; the two together as a block.
+
+Tolerances (u = 2^-24, half a step of float32; ``half(t)`` = eps / 2 of an output type):
+
+* scan: a state is an average of candidates and h0, so at most M = max(|n|, |h0|).  A step's gates are off by at most
+  16 u of themselves, and what is not in proportion to 1 - z (the rounding of z, of the step, of a tile's product) by
+  3 u M a step: |error| <= u M (16 + 3 T).  The backward recurrence is the same sum over |dout|, ``gabs``, with a factor
+  |h - n| <= 2 M, and its slopes: u gabs max(1, 2 M) (32 + 6 T).
+* product: S = sum |x| |W| of a result.  Operands of two fp16 planes are off by 2^-23 each, their dropped product by 2^-24;
+  the tensor core truncates each of at most 32 steps of a chunk by 2 u, chunks of 64 or more terms add with u each:
+  u S (80 + K / 64).  An activation adds its own 8 u of its value, and multiplies by a slope below 1.2.
+* 16-bit gradients: d = dy * slope is rounded to the type, its slope to fp16: S_d (half(t) + 2^-11 + u (80 + K / 64)).
+* every result: half(t) of itself, and half the step of the smallest numbers of its type.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from gru_triton_b200 import _lib
+from gru_triton_b200.linear_act import ACTIVATIONS, linear_act
+from gru_triton_b200.scan_gated import gated_scan, gated_step
+
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ["fp32", "bf16", "fp16"]
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rounding(ref, dtype):
+    f = torch.finfo(dtype)
+    return half(dtype) * ref.abs() + f.tiny * f.eps / 2
+
+
+def close(got, ref, tol):
+    assert tuple(got.shape) == tuple(ref.shape)
+    off = (got.double() - ref).abs() - tol
+    assert bool(torch.isfinite(got.double()).all()) and bool((off <= 0).all()), \
+        f"off by {float((got.double() - ref).abs().max()):.3e}, allowed {float((tol + torch.zeros_like(ref)).min()):.3e}"
+
+
+# ---- the recurrence in 64 bits -------------------------------------------------------------------
+
+def scan64(gi, h0, lengths, candidate):
+    """(out, h_T, states before each step) one step after the other."""
+    gi = gi.double()
+    T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
+    h = torch.zeros(B, H, dtype=torch.float64, device=gi.device) if h0 is None else h0.double()
+    lengths = torch.full((B,), T, device=gi.device) if lengths is None else lengths.clamp(0, T)
+    outs, before = [], []
+    for t in range(T):
+        on = (t < lengths)[:, None]
+        x, c = gi[t, :, :H], gi[t, :, H:]
+        n = c.tanh() if candidate == "tanh" else c
+        before.append(h)
+        new = torch.sigmoid(x) * h + torch.sigmoid(-x) * n
+        h = torch.where(on, new, h)
+        outs.append(torch.where(on, new, torch.zeros_like(new)))
+    return torch.stack(outs), h, torch.stack(before)
+
+
+def scan64_backward(gi, lengths, candidate, before, dout, dh):
+    gi, dout, G = gi.double(), dout.double(), dh.double()
+    T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
+    lengths = torch.full((B,), T, device=gi.device) if lengths is None else lengths.clamp(0, T)
+    dgi = torch.zeros_like(gi)
+    for t in reversed(range(T)):
+        on = (t < lengths)[:, None]
+        x, c = gi[t, :, :H], gi[t, :, H:]
+        z, k = torch.sigmoid(x), torch.sigmoid(-x)
+        n, slope = (c.tanh(), c.cosh() ** -2) if candidate == "tanh" else (c, torch.ones_like(c))
+        g = G + dout[t]
+        dgi[t] = torch.where(on, torch.cat([g * (before[t] - n) * z * k, g * k * slope], 1), torch.zeros_like(gi[t]))
+        G = torch.where(on, z * g, G)
+    return dgi, G
+
+
+def scan_tolerance(gi, h0, T, candidate):
+    c = gi.double()[..., gi.shape[2] // 2:]
+    c = c[torch.isfinite(c)]
+    M = float(c.abs().max()) if candidate == "identity" and c.numel() else 1.0
+    M = max(M, 0.0 if h0 is None else float(h0.abs().max()))
+    return M, U * M * (16 + 3 * T)
+
+
+def problem(dtype, T, B, H, seed=0, lean=1.0, device="cuda"):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    gi = torch.randn(T, B, 2 * H, device=device, generator=gen) * 2
+    gi[..., :H] += lean
+    return (gi.to(dtype), torch.randn(B, H, device=device, generator=gen),
+            (torch.randn(T, B, H, device=device, generator=gen)).to(dtype), torch.randn(B, H, device=device, generator=gen))
+
+
+def check_scan(gi, h0, lengths, candidate, dout, dh):
+    T, dtype = gi.shape[0], gi.dtype
+    leaf = gi.detach().requires_grad_(True)
+    leaves = [leaf] if h0 is None else [leaf, h0.detach().requires_grad_(True)]
+    out, h_T = gated_scan(leaf, leaves[1] if h0 is not None else None, lengths=lengths, candidate=candidate)
+    grads = torch.autograd.grad((out, h_T), leaves, (dout, dh))
+    ref, ref_T, before = scan64(gi, h0, lengths, candidate)
+    M, tol = scan_tolerance(gi, h0, T, candidate)
+    close(out.detach(), ref, tol + rounding(ref, dtype))
+    close(h_T.detach(), ref_T, tol + rounding(ref_T, torch.float32))
+    inner, inner_T = gated_scan(gi, h0, lengths=lengths, candidate=candidate)          # the form without gradients
+    assert torch.equal(inner, out) and torch.equal(inner_T, h_T)
+    rdgi, rdh0 = scan64_backward(gi, lengths, candidate, before, dout, dh)
+    _, gabs = scan64_backward(gi, lengths, candidate, before, dout.abs(), dh.abs())
+    reach = float(max(gabs.max(), dh.abs().max(), dout[torch.isfinite(dout)].abs().sum(0).max() if dout.numel() else 0.0))
+    tol = U * reach * max(1.0, 2 * M) * (32 + 6 * T)
+    close(grads[0], rdgi, tol + rounding(rdgi, dtype))
+    if h0 is not None:
+        close(grads[1], rdh0, tol + rounding(rdh0, torch.float32))
+    return out, h_T, grads
+
+
+SCAN_SIZES = [(1, 1, 1), (1, 3, 33), (2, 1, 8), (7, 2, 64), (16, 40, 72), (17, 2, 64), (63, 2, 64), (64, 5, 40), (65, 3, 96),
+              (130, 1, 512), (300, 2, 72), (257, 19, 607), (1000, 1, 1024), (200, 64, 256), (2100, 1, 24)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T,B,H", SCAN_SIZES)
+def test_scan_matches_64_bits(dtype, T, B, H):
+    gi, h0, dout, dh = problem(dtype, T, B, H, seed=T + H)
+    check_scan(gi, h0, None, "tanh", dout, dh)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T,B,H", [(1, 2, 8), (40, 3, 65), (129, 4, 128), (700, 3, 200)])
+def test_scan_identity_candidate_without_h0(dtype, T, B, H):
+    gi, _, dout, dh = problem(dtype, T, B, H, seed=T + H)
+    check_scan(gi, None, None, "identity", dout, dh)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T,H", [(5, 16), (64, 32), (150, 72), (150, 33), (513, 64)])
+def test_scan_ragged_rows_ignore_their_padding(dtype, T, H, index):
+    """Rows of no, one, some and all steps, lengths out of range; what lies behind a row is NaN or infinite."""
+    lengths = torch.tensor([0, 1, T // 2, T - 1, T, -3, T + 9, min(T, 64), min(T, 65)], device="cuda", dtype=index)
+    B = lengths.numel()
+    gi, h0, dout, dh = problem(dtype, T, B, H, seed=T)
+    behind = torch.arange(T, device="cuda")[:, None] >= lengths[None]
+    clean_gi, clean_dout = gi.clone(), dout.clone()
+    gi[behind] = float("nan")
+    dout[behind] = float("inf")
+    gi[-1, 0] = float("-inf")
+    leaf, h = gi.requires_grad_(True), h0.requires_grad_(True)
+    out, h_T = gated_scan(leaf, h, lengths=lengths)
+    got = torch.autograd.grad((out, h_T), (leaf, h), (dout, dh))
+    ref = check_scan(clean_gi, h0.detach(), lengths, "tanh", clean_dout, dh)
+    assert torch.equal(out, ref[0]) and torch.equal(h_T, ref[1])
+    assert all(torch.equal(a, b) for a, b in zip(got, ref[2]))
+    assert bool((out[behind] == 0).all()) and bool((got[0][behind] == 0).all())
+    for b in (0, 5):                                             # rows without steps
+        assert torch.equal(h_T[b], h0[b]) and torch.equal(got[1][b], dh[b])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,B,H", [(1, 2, 24), (90, 2, 64), (90, 2, 33), (600, 2, 64)])
+def test_scan_saturated_gates_and_nan_stay_where_they_are(T, B, H):
+    gi, h0, dout, dh = problem(torch.float32, T, B, H, seed=3)
+    inf = float("inf")
+    gi[0, 0, :H], gi[T // 2, 0, 0], gi[T // 3, 1, H:] = inf, -inf, inf
+    gi[:, 1, 1] = 60.0                                            # holds for good
+    gi[:, 1, 2] = -60.0                                           # forgets at once
+    gi[:, :, H + 3] *= 1e-6                                       # candidates far below one keep their precision
+    check_scan(gi, h0, None, "tanh", dout, dh)
+    _, h_T = gated_scan(gi, h0)
+    rel = (h_T[0, 3].double() - scan64(gi, None, None, "tanh")[1][0, 3]).abs()
+    assert torch.equal(h_T[1, 1], h0[1, 1]) and float(rel) < 10
+    bad = gi.clone()
+    bad[T // 2, 0, 5] = float("nan")
+    out, _ = gated_scan(bad, h0)
+    ok, _ = gated_scan(gi, h0)
+    same = torch.ones(T, B, H, dtype=torch.bool, device="cuda")
+    same[T // 2:, 0, 5] = False
+    assert torch.equal(out[same], ok[same]) and bool(out[T // 2:, 0, 5].isnan().all())
+    if T > 4:                                                    # a NaN candidate reaches no earlier step's gradient
+        bad = gi.clone()
+        bad[T // 2, 0, H + 5] = float("nan")
+        leaf = bad.requires_grad_(True)
+        dgi, = torch.autograd.grad(gated_scan(leaf, h0)[0], leaf, dout)
+        assert bool(torch.isfinite(dgi[:T // 2]).all()) and bool(torch.isfinite(dgi[:, 1]).all())
+
+
+@pytest.mark.gpu
+def test_scan_small_candidates_keep_relative_precision():
+    gi, _, _, _ = problem(torch.float32, 100, 2, 64, seed=5)
+    gi[..., 64:] *= 1e-4
+    out, h_T = gated_scan(gi)
+    ref, ref_T, _ = scan64(gi, None, None, "tanh")
+    M = float(gi[..., 64:].abs().max())
+    close(out, ref, U * M * (16 + 300) + rounding(ref, torch.float32))
+    close(h_T, ref_T, U * M * (16 + 300) + rounding(ref_T, torch.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T", [3, 140])
+def test_scan_reads_any_layout(dtype, T):
+    B, H = 3, 64
+    gi, h0, dout, dh = problem(dtype, T, B, H, seed=7)
+    ref = check_scan(gi, h0, None, "tanh", dout, dh)
+
+    def wide(t, front, back):
+        big = torch.full((*t.shape[:-1], t.shape[-1] + front + back), float("nan"), dtype=t.dtype, device="cuda")
+        big[..., front:front + t.shape[-1]] = t
+        return big[..., front:front + t.shape[-1]]
+
+    forms = {"batch first": (gi.transpose(0, 1).contiguous().transpose(0, 1), dout.transpose(0, 1).contiguous().transpose(0, 1)),
+             "odd offset": (wide(gi, 1, 2), wide(dout, 3, 1)), "wide rows": (wide(gi, 8, 8), wide(dout, 0, 16)),
+             "units strided": (gi.repeat_interleave(2, -1)[..., ::2], dout.transpose(1, 2).contiguous().transpose(1, 2))}
+    for name, (g, d) in forms.items():
+        assert torch.equal(g, gi) and torch.equal(d, dout)
+        leaf, h = g.detach().requires_grad_(True), wide(h0, 1, 0).detach().requires_grad_(True)
+        out, h_T = gated_scan(leaf, h)
+        got = torch.autograd.grad((out, h_T), (leaf, h), (d, wide(dh, 2, 1)))
+        for a, b in zip((out, h_T, *got), (ref[0], ref[1], *ref[2])):
+            close(a.detach(), b.detach().double(), 2 * rounding(b.double(), dtype) + 64 * T * U * float(b.abs().max()))
+    # every step and row the same one: inputs of stride 0
+    one = gi[:1, :1].expand(T, B, 2 * H)
+    assert torch.equal(gated_scan(one)[0], gated_scan(one.contiguous())[0])
+    leaf = gi.detach().requires_grad_(True)
+    a, = torch.autograd.grad(gated_scan(leaf, h0)[0].sum(), leaf)                       # a gradient of stride 0
+    b, = torch.autograd.grad(gated_scan(leaf, h0)[0], leaf, torch.ones_like(dout))
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_scan_gradient_of_one_output_and_broadcast_state():
+    gi, h0, dout, dh = problem(torch.float32, 70, 4, 48, seed=9)
+    leaf = gi.requires_grad_(True)
+    out, h_T = gated_scan(leaf, h0)
+    zeros = torch.zeros_like(dout), torch.zeros_like(dh)
+    a = torch.autograd.grad(out, leaf, dout, retain_graph=True)[0]
+    assert torch.equal(a, torch.autograd.grad((out, h_T), leaf, (dout, zeros[1]), retain_graph=True)[0])
+    b = torch.autograd.grad(h_T, leaf, dh, retain_graph=True)[0]
+    assert torch.equal(b, torch.autograd.grad((out, h_T), leaf, (zeros[0], dh))[0])
+    row = h0[0].clone().requires_grad_(True)                     # one learnt state for every row
+    _, h_T = gated_scan(gi.detach(), row.expand(4, -1))
+    got, = torch.autograd.grad(h_T, row, dh)
+    full = h0[:1].expand(4, -1).contiguous().requires_grad_(True)
+    _, h_T = gated_scan(gi.detach(), full)
+    assert torch.equal(got, torch.autograd.grad(h_T, full, dh)[0].sum(0))
+
+
+@pytest.mark.gpu
+def test_scan_gradient_against_differences():
+    gi, h0, dout, dh = problem(torch.float32, 75, 2, 40, seed=11)
+    lengths = torch.tensor([75, 31], device="cuda")
+    leaf, h = gi.requires_grad_(True), h0.requires_grad_(True)
+    out, h_T = gated_scan(leaf, h, lengths=lengths)
+    got = torch.autograd.grad((out, h_T), (leaf, h), (dout, dh))
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    step = 1e-6
+    for which in (0, 1):
+        base = [gi.detach().double(), h0.detach().double()]
+        way = torch.randn(base[which].shape, device="cuda", generator=gen, dtype=torch.float64)
+        ends = []
+        for sign in (1, -1):
+            at = list(base)
+            at[which] = at[which] + sign * step * way
+            o, hT, _ = scan64(at[0], at[1], lengths, "tanh")
+            ends.append(float((o * dout.double()).sum() + (hT * dh.double()).sum()))
+        slope = (ends[0] - ends[1]) / (2 * step)
+        mine = float((got[which].double() * way).sum())
+        # the difference: step^2 times a third derivative, and 2^-53 of the sums over step; the gradient: as above
+        scale = float((got[which].double() * way).abs().sum())
+        assert abs(slope - mine) <= 1e-5 * scale
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("candidate", ["tanh", "identity"])
+@pytest.mark.parametrize("B,H", [(1, 1), (1, 256), (5, 33), (130, 1024)])
+def test_steps_walk_the_scan(dtype, candidate, B, H):
+    T = 6
+    gi, h0, _, _ = problem(dtype, T, B, H, seed=13)
+    ref, ref_T, _ = scan64(gi, h0, None, candidate)
+    _, tol = scan_tolerance(gi, h0, T, candidate)
+    h, state = h0, h0.clone()
+    for t in range(T):
+        out, h = gated_step(gi[t], h, candidate=candidate)
+        again, same = gated_step(gi[t], state, candidate=candidate, out_state=state)
+        assert same is state and torch.equal(state, h) and torch.equal(out, again)
+        close(out, ref[t], tol + rounding(ref[t], dtype))
+    close(h, ref_T, tol + rounding(ref_T, torch.float32))
+    pool = torch.full((2 * B, H + 5), 7.0, device="cuda")         # rows of a larger state table, every other one
+    pool[::2, :H] = h0
+    out, new = gated_step(gi[0], pool[::2, :H], candidate=candidate, out_state=pool[::2, :H])
+    assert torch.equal(new, gated_step(gi[0], h0, candidate=candidate)[1])
+    assert bool((pool[1::2] == 7).all()) and bool((pool[:, H:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_step_refuses_states_that_overlap_and_gradients():
+    gi, h0, _, _ = problem(torch.float32, 1, 4, 16)
+    big = torch.zeros(5, 16, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        gated_step(gi[0], big[:4], out_state=big[1:])
+    with pytest.raises(ValueError, match="rows"):
+        gated_step(gi[0], h0, out_state=h0[:1].expand(4, 16))
+    with pytest.raises(ValueError, match="gradients"):
+        gated_step(gi[0].requires_grad_(True), h0)
+    flat = torch.zeros(4, 32, device="cuda")
+    with pytest.raises(ValueError, match="gi"):
+        gated_step(flat, h0, out_state=flat[:, :16])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,B,H", [(9, 3, 40), (64, 32, 512), (500, 2, 96), (3000, 1, 128)])
+def test_scan_repeats_its_bits(T, B, H):
+    gi, h0, dout, dh = problem(torch.float32, T, B, H, seed=15)
+    lengths = torch.randint(0, T + 1, (B,), device="cuda")
+    runs = []
+    for _ in range(3):
+        leaf, h = gi.detach().requires_grad_(True), h0.detach().requires_grad_(True)
+        out, h_T = gated_scan(leaf, h, lengths=lengths)
+        runs.append((out.detach(), h_T.detach(), *torch.autograd.grad((out, h_T), (leaf, h), (dout, dh))))
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+@pytest.mark.gpu
+@pytest.mark.slow
+def test_scan_offsets_past_32_bits():
+    """gi and out of more than 2^31 elements: the last row agrees with the same row alone."""
+    T, B, H = 70016, 16, 1024
+    gi = torch.empty(T, B, 2 * H, device="cuda", dtype=torch.bfloat16)
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    row = torch.randn(T, 1, 2 * H, device="cuda", generator=gen).to(torch.bfloat16)
+    gi[:, :15] = 0
+    gi[:, 15:] = row
+    leaf = gi.requires_grad_(True)
+    out, h_T = gated_scan(leaf)
+    alone, alone_T = gated_scan(row)
+    assert float((out[:, 15:] - alone).abs().max()) <= 2 ** -6 and float((h_T[15] - alone_T[0]).abs().max()) <= 1e-5
+    assert bool((out[:, :15] == 0).all())
+    del alone
+    dgi, = torch.autograd.grad(out, leaf, row[..., :H].expand(T, B, H))
+    del out
+    leaf1 = row.requires_grad_(True)
+    ref, = torch.autograd.grad(gated_scan(leaf1)[0], leaf1, row.detach()[..., :H])
+    assert float((dgi[:, 15:].float() - ref.float()).abs().max()) <= 2 ** -7 * float(ref.float().abs().max())
+
+
+# ---- the product ------------------------------------------------------------------------------------
+
+def act64(pre, name):
+    return {"none": lambda v: v, "relu": torch.relu, "silu": lambda v: v * torch.sigmoid(v),
+            "gelu": lambda v: 0.5 * v * torch.erfc(-v / math.sqrt(2.0)), "sigmoid": torch.sigmoid, "tanh": torch.tanh}[name](pre)
+
+
+def linear_problem(dtype, M, K, N, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(M, K, device="cuda", generator=gen).to(dtype)
+    W = (torch.randn(N, K, device="cuda", generator=gen) / math.sqrt(K)).to(dtype)
+    bias = torch.randn(N, device="cuda", generator=gen).to(dtype)
+    residual = torch.randn(M, N, device="cuda", generator=gen).to(dtype)
+    return x, W, bias, residual, torch.randn(M, N, device="cuda", generator=gen).to(dtype)
+
+
+def check_linear(x, W, bias, residual, activation, dy):
+    dtype, K, N, M = x.dtype, W.shape[1], W.shape[0], x.shape[0]
+    leaves = [t.detach().requires_grad_(True) for t in (x, W) + (() if bias is None else (bias,)) + (() if residual is None else (residual,))]
+    it = iter(leaves[2:])
+    y = linear_act(leaves[0], leaves[1], None if bias is None else next(it), activation=activation,
+                   residual=None if residual is None else next(it))
+    got = torch.autograd.grad(y, leaves, dy)
+    inner = linear_act(x, W, bias, activation=activation, residual=residual)
+    assert torch.equal(inner, y)
+
+    x64, W64, dy64 = x.double(), W.double(), dy.double()
+    pre = x64 @ W64.t() + (0 if bias is None else bias.double())
+    pre.requires_grad_(True)
+    a = act64(pre, activation)
+    d, = torch.autograd.grad(a, pre, dy64)
+    pre, a = pre.detach(), a.detach()
+    ref = a if residual is None else a + residual.double()
+    S = x64.abs() @ W64.abs().t() + (0 if bias is None else bias.double().abs())
+    off_pre = U * S * (80 + K / 64)
+    close(y.detach(), ref, 1.2 * off_pre + 8 * U * (a.abs() + pre.abs() + ref.abs()) + rounding(ref, dtype))
+    # the slope's own error: |act''| <= 1 of the error of pre, a few units of itself; fp16 behind 16-bit types
+    off_d = dy64.abs() * (off_pre + 16 * U)
+    if activation == "relu":
+        off_d = dy64.abs() * (pre.abs() <= off_pre) + 0 * d      # the sign of pre decides
+    if dtype != torch.float32:
+        off_d = off_d + d.abs() * (2.0 ** -11 if activation != "none" else 0.0) + dy64.abs() * 2.0 ** -24
+    in_product = off_d + (half(dtype) * d.abs() if dtype != torch.float32 and activation != "none" else 0.0)
+    refs = [d @ W64, d.t() @ x64]
+    sums = [d.abs() @ W64.abs(), d.abs().t() @ x64.abs()]
+    carried = [in_product @ W64.abs(), in_product.t() @ x64.abs()]
+    for k, terms in ((0, N), (1, M)):
+        close(got[k], refs[k], carried[k] + U * sums[k] * (80 + terms / 64) + rounding(refs[k], dtype))
+    if bias is not None:
+        db = d.sum(0)
+        close(got[2], db, off_d.sum(0) + U * d.abs().sum(0) * (80 + M / 64) + rounding(db, dtype))
+    if residual is not None:
+        assert torch.equal(got[-1], dy)
+    return y, got
+
+
+LINEAR_SIZES = [(1, 1, 1), (1, 64, 64), (2, 100, 7), (3, 129, 250), (8, 512, 1024), (9, 256, 96), (16, 65, 33), (33, 1024, 512),
+                (64, 96, 260), (127, 63, 127), (128, 128, 128), (129, 72, 257), (300, 1000, 136), (1000, 120, 608), (2048, 512, 1024),
+                (700, 2050, 70), (5000, 40, 24), (4100, 136, 1032)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M,K,N", LINEAR_SIZES)
+def test_linear_matches_64_bits(dtype, M, K, N):
+    x, W, bias, residual, dy = linear_problem(dtype, M, K, N, seed=M + K + N)
+    check_linear(x, W, bias, residual, "silu", dy)
+    check_linear(x, W, None, None, "none", dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("activation", list(ACTIVATIONS))
+@pytest.mark.parametrize("M,K,N", [(3, 72, 40), (40, 256, 200), (400, 264, 520)])
+def test_linear_activations(dtype, activation, M, K, N):
+    x, W, bias, residual, dy = linear_problem(dtype, M, K, N, seed=M)
+    check_linear(x, W, bias, None, activation, dy)
+    check_linear(x, W * 3, bias, residual, activation, dy)       # saturated in part
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M", [2, 40, 300])
+def test_linear_reads_any_layout(dtype, M):
+    K, N = 136, 264
+    x, W, bias, residual, dy = linear_problem(dtype, M, K, N, seed=1)
+    y, grads = check_linear(x, W, bias, residual, "gelu", dy)
+
+    def wide(t, front, back):
+        big = torch.full((*t.shape[:-1], t.shape[-1] + front + back), float("nan"), dtype=t.dtype, device="cuda")
+        big[..., front:front + t.shape[-1]] = t
+        return big[..., front:front + t.shape[-1]]
+
+    def turned(t):
+        return t.t().contiguous().t()
+
+    forms = [(wide(x, 8, 16), wide(W, 16, 8), wide(residual, 8, 0), wide(dy, 0, 8)),
+             (wide(x, 1, 1), wide(W, 3, 1), wide(residual, 1, 1), wide(dy, 1, 2)),
+             (turned(x), turned(W), turned(residual), turned(dy))]
+    for fx, fW, fr, fd in forms:
+        leaves = [t.detach().requires_grad_(True) for t in (fx, fW, bias, fr)]
+        out = linear_act(*leaves[:3], activation="gelu", residual=leaves[3])
+        got = torch.autograd.grad(out, leaves, fd)
+        assert torch.equal(out, y)
+        assert all(torch.equal(a, b) for a, b in zip(got, grads))
+    three = x.reshape(2, M // 2, K)                              # leading axes
+    assert torch.equal(linear_act(three, W, bias, activation="gelu", residual=residual.reshape(2, M // 2, N)), y.reshape(2, M // 2, N))
+    back = three.transpose(0, 1)                                 # rows in another order
+    assert torch.equal(linear_act(back, W, bias), linear_act(back.contiguous(), W, bias))
+    assert torch.equal(linear_act(x[0], W, bias), linear_act(x[:1], W, bias)[0])
+    one = x[:1].expand(M, K)
+    assert torch.equal(linear_act(one, W, bias), linear_act(one.contiguous(), W, bias))
+    leaf = x.detach().requires_grad_(True)
+    a, = torch.autograd.grad(linear_act(leaf, W, bias, activation="gelu").sum(), leaf)
+    b, = torch.autograd.grad(linear_act(leaf, W, bias, activation="gelu"), leaf, torch.ones_like(dy))
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [5, 200])
+def test_linear_no_rows_some_gradients_and_special_values(M):
+    x, W, bias, residual, dy = linear_problem(torch.float32, M, 64, 48)
+    leaves = [t.detach().requires_grad_(True) for t in (x[:0], W, bias)]
+    y = linear_act(*leaves, activation="silu")
+    assert tuple(y.shape) == (0, 48)
+    got = torch.autograd.grad(y, leaves, dy[:0])
+    assert tuple(got[0].shape) == (0, 64) and not got[1].any() and not got[2].any()
+    full = [t.detach().requires_grad_(True) for t in (x, W, bias, residual)]
+    all_of = torch.autograd.grad(linear_act(*full[:3], activation="silu", residual=full[3]), full, dy)
+    for k in range(4):
+        some = [t.detach().requires_grad_(k == i) for i, t in enumerate((x, W, bias, residual))]
+        got, = torch.autograd.grad(linear_act(*some[:3], activation="silu", residual=some[3]), some[k], dy)
+        assert torch.equal(got, all_of[k])
+    # a row of NaN and one of infinities stay in their rows; a zero row gives act(bias)
+    bad = x.clone()
+    bad[1], bad[2], bad[3] = float("nan"), float("inf"), 0.0
+    for activation in ACTIVATIONS:
+        out = linear_act(bad, W, bias, activation=activation)
+        ok = linear_act(x, W, bias, activation=activation)
+        rest = [0, 4] + list(range(5, M))
+        assert torch.equal(out[rest], ok[rest]) and bool(out[1].isnan().all())
+        close(out[3], act64(bias.double(), activation), 32 * U * (1 + bias.double().abs()))
+    # saturated both ways
+    huge = torch.full((M, 64), 1e30, device="cuda")
+    one = torch.ones(2, 64, device="cuda")
+    one[1] = -1
+    for activation, (lo, hi) in {"relu": (0.0, None), "silu": (0.0, None), "gelu": (0.0, None), "sigmoid": (0.0, 1.0), "tanh": (-1.0, 1.0)}.items():
+        leaf = huge.detach().requires_grad_(True)
+        y = linear_act(leaf, one, activation=activation)
+        g, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+        assert bool((y[:, 1] == lo).all()) and (hi is None or bool((y[:, 0] == hi).all())) and bool((y[:, 0] > 0).all())
+        assert bool((g == (1.0 if hi is None else 0.0)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M,K,N", [(4, 300, 50), (48, 512, 640), (520, 512, 640), (9000, 128, 264)])
+def test_linear_repeats_its_bits(dtype, M, K, N):
+    x, W, bias, residual, dy = linear_problem(dtype, M, K, N)
+    runs = []
+    for _ in range(3):
+        leaves = [t.detach().requires_grad_(True) for t in (x, W, bias)]
+        y = linear_act(*leaves, activation="tanh", residual=residual)
+        runs.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+@pytest.mark.gpu
+def test_linear_small_rows_beside_large_ones():
+    """float32 rows and columns that differ by many powers of two keep their own precision."""
+    x, W, bias, _, dy = linear_problem(torch.float32, 300, 200, 160, seed=4)
+    x = x * (2.0 ** torch.randint(-30, 30, (300, 1), device="cuda"))
+    W = W * (2.0 ** torch.randint(-20, 20, (160, 1), device="cuda"))
+    y = linear_act(x, W)
+    ref = x.double() @ W.double().t()
+    S = x.double().abs() @ W.double().abs().t()
+    close(y, ref, U * S * (80 + 200 / 64) + rounding(ref, torch.float32))
+    leaf = x.requires_grad_(True)
+    wleaf = W.requires_grad_(True)
+    rows = dy * (2.0 ** torch.randint(-30, 30, (300, 1), device="cuda"))
+    dx, = torch.autograd.grad(linear_act(leaf, wleaf.detach()), leaf, rows)
+    ref = rows.double() @ W.double()
+    # a row of d is scaled as a whole after the weight rows' own powers of two are folded in
+    S = rows.double().abs() @ W.double().abs()
+    top = (rows.double().abs()[:, :, None] * W.double().abs().amax(1)[None, :, None]).amax(1)
+    close(dx, ref.detach(), U * S.detach() * (80 + 160 / 64) + 160 * 2.0 ** -38 * top.detach() + rounding(ref.detach(), torch.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.slow
+def test_linear_offsets_past_32_bits():
+    M, K, N = 2 ** 20 + 37, 64, 2056
+    x, W, bias, _, _ = linear_problem(torch.bfloat16, 2048, K, N)
+    xl = x.repeat(M // 2048 + 1, 1)[:M]
+    y = linear_act(xl, W, bias, activation="relu")
+    assert y.numel() > 2 ** 31
+    ref = linear_act(x, W, bias, activation="relu")
+    start = (M - 2048) // 2048 * 2048
+    assert torch.equal(y[start:start + 2048], ref) and torch.equal(y[-37:], ref[:37])
+
+
+# ---- streams, graphs, the two together ---------------------------------------------------------------
+
+def block(x, Wi, bi, Wo, bo, h0, lengths=None):
+    out, h_T = gated_scan(linear_act(x, Wi, bi), h0, lengths=lengths)
+    return linear_act(out, Wo, bo, activation="silu", residual=x), h_T
+
+
+def block_problem(dtype, T, B, K, H, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    make = lambda *s, scale=1.0: (torch.randn(*s, device="cuda", generator=gen) * scale).to(dtype)  # noqa: E731
+    return [make(T, B, K), make(2 * H, K, scale=K ** -0.5), make(2 * H), make(K, H, scale=H ** -0.5), make(K),
+            torch.randn(B, H, device="cuda", generator=gen)], make(T, B, K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T,B,K,H", [(20, 3, 40, 24), (70, 4, 72, 136), (130, 8, 256, 256)])
+def test_block_trains_and_serves(dtype, T, B, K, H):
+    tensors, dy = block_problem(dtype, T, B, K, H)
+    lengths = torch.randint(0, T + 1, (B,), device="cuda")
+    lengths[0] = T
+    leaves = [t.detach().requires_grad_(True) for t in tensors]
+    y, h_T = block(*leaves, lengths=lengths)
+    got = torch.autograd.grad(y, leaves, dy)
+
+    def block64(x, Wi, bi, Wo, bo, h0):
+        gi = x @ Wi.t() + bi
+        h, outs = h0, []
+        for t in range(T):
+            on = (t < lengths)[:, None]
+            new = torch.sigmoid(gi[t, :, :H]) * h + torch.sigmoid(-gi[t, :, :H]) * gi[t, :, H:].tanh()
+            h = torch.where(on, new, h)
+            outs.append(torch.where(on, new, torch.zeros_like(new)))
+        pre = torch.stack(outs) @ Wo.t() + bo
+        return pre * torch.sigmoid(pre) + x, h
+
+    wide = [t.detach().double().requires_grad_(True) for t in tensors]
+    ry, rh = block64(*wide)
+    ref = torch.autograd.grad(ry, wide, dy.double())
+    # relative to the norm: a handful of roundings of the type (gi, out, y; dout, dgi, dx), each half a step; memories of
+    # about ten steps repeat that of gi
+    bound = 16 * half(dtype) if dtype != torch.float32 else 512 * U
+    for a, b in zip((y.detach(), h_T.detach(), *got), (ry.detach(), rh.detach(), *ref)):
+        assert float((a.double() - b).norm() / b.norm()) <= bound
+    # the same rows token by token
+    x, Wi, bi, Wo, bo, h0 = tensors
+    state = h0.clone()
+    for t in range(int(lengths.min())):
+        out, _ = gated_step(linear_act(x[t], Wi, bi), state, out_state=state)
+        step = linear_act(out, Wo, bo, activation="silu", residual=x[t])
+        assert float((step.double() - ry[t]).norm() / ry[t].norm()) <= bound
+
+
+@pytest.mark.gpu
+def test_operators_on_another_stream():
+    tensors, dy = block_problem(torch.bfloat16, 90, 4, 64, 128)
+    ref = [t.detach().requires_grad_(True) for t in tensors]
+    want = torch.autograd.grad(block(*ref)[0], ref, dy)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        leaves = [t.detach().requires_grad_(True) for t in tensors]
+        got = torch.autograd.grad(block(*leaves)[0], leaves, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("T,B,K,H", [(1, 2, 64, 64), (90, 4, 64, 128), (600, 16, 128, 256)])
+def test_operators_replay_in_graphs(dtype, T, B, K, H):
+    """Two captured training steps of different inputs, replayed in turn and beside each other on two streams."""
+    from gru_triton_b200.graphed import GraphedStep
+
+    def step(x, Wi, bi, Wo, bo, h0, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, Wi, bi, Wo, bo, h0)]
+        y, h_T = block(*leaves)
+        return (y.detach(), h_T.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    sets = [block_problem(dtype, T, B, K, H, seed=s) for s in (1, 2, 3)]
+    want = [step(*t, dy) for t, dy in sets]
+    graphs = [GraphedStep(step, [*t, dy]) for t, dy in sets[:2]]
+    for k in (0, 1, 0):
+        got = graphs[k](*sets[k][0], sets[k][1])
+        assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
+    got = graphs[0](*sets[2][0], sets[2][1])                     # new inputs in the captured step
+    assert all(torch.equal(a, b) for a, b in zip(got, want[2]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[k](*sets[k][0], sets[k][1])
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(torch.equal(a, b) for a, b in zip(graphs[k].static_outputs, want[k]))
+    _lib.check_device_status()
+
+
+# ---- refusals (no GPU) --------------------------------------------------------------------------------
+
+def test_scan_refusals():
+    gi, h0 = torch.zeros(4, 2, 16), torch.zeros(2, 8)
+    for bad, match in [((gi, h0), "CUDA"), ((gi.double(), h0), "dtype"), ((gi[..., :15], h0), "2H"), ((gi[0], h0), "2H"),
+                       ((gi[:0], h0), "T"), ((gi[:, :0], h0[:0]), "B"), ((gi[..., :0], h0[:, :0]), "H"),
+                       ((gi, h0.half()), "float32"), ((gi, h0[:1]), "shape")]:
+        with pytest.raises(ValueError, match=match):
+            gated_scan(*bad)
+    with pytest.raises(ValueError, match="candidate"):
+        gated_scan(gi, h0, candidate="relu")
+    for lengths, match in [(torch.zeros(2), "int32 or int64"), (torch.zeros(3, dtype=torch.int64), "shape"),
+                           (torch.zeros(2, dtype=torch.int64), "CUDA")]:
+        with pytest.raises(ValueError, match=match):
+            gated_scan(gi, h0, lengths=lengths)
+    for bad, match in [((gi[0], h0), "CUDA"), ((gi, h0), "2H"), ((gi[0], h0.double()), "float32"), ((gi[0, :0], h0[:0]), "B"),
+                       ((gi[0], h0[:, :4]), "shape")]:
+        with pytest.raises(ValueError, match=match):
+            gated_step(*bad)
+    with pytest.raises(ValueError, match="out_state"):
+        gated_step(gi[0], h0, out_state=h0.half())
+
+
+def test_linear_refusals():
+    x, W, b, r = torch.zeros(4, 16), torch.zeros(8, 16), torch.zeros(8), torch.zeros(4, 8)
+    for args, kw, match in [((x, W, b), {}, "CUDA"), ((x.double(), W.double()), {}, "dtype"), ((x, W.half()), {}, "W dtype"),
+                            ((x, W[:, :8]), {}, "N, K"), ((x, W[0]), {}, "N, K"), ((x, W[:0]), {}, "N=0"), ((x, W, b[:4]), {}, "bias"),
+                            ((x, W, b), {"residual": r[:1]}, "residual"), ((x, W, b), {"activation": "swish"}, "activation"),
+                            ((x, W, b.half()), {}, "bias dtype"), ((x[:, :0], W[:, :0]), {}, "K=0")]:
+        with pytest.raises(ValueError, match=match):
+            linear_act(*args, **kw)
+
+
+def test_library_refuses_bad_arguments():
+    """The C entries answer with a status before any device work."""
+    import ctypes
+    lib = _lib.load()
+    a = _lib.CGatedArgs()
+    assert lib.b200gru_gated_scan_forward(None, None) == 1 and lib.b200gru_gated_scan_backward(ctypes.byref(a), None) == 1
+    a.T = a.B = a.H = 4
+    a.gi = 256
+    assert lib.b200gru_gated_scan_forward(ctypes.byref(a), None) == 1                   # no outputs
+    a.dtype = 3
+    assert lib.b200gru_gated_scan_forward(ctypes.byref(a), None) == 1
+    a.dtype, a.lengths, a.length_bytes = 0, 256, 2
+    assert lib.b200gru_gated_scan_forward(ctypes.byref(a), None) == 1
+    assert lib.b200gru_gated_states_bytes(65, 2, 3) == 2 * 2 * 3 * 4 and lib.b200gru_gated_states_bytes(0, 2, 3) == 0
+    assert lib.b200gru_gated_step(0, 1, 0, 4, 256, 8, 256, 4, 256, 256, 4, None) == 1
+    assert lib.b200gru_gated_step(0, 1, 2, 4, 256, 8, 256, 4, 256, 256, 3, None) == 1   # rows of the new state overlap
+    p = _lib.CLinearArgs()
+    bad = ctypes.c_size_t(-1).value
+    assert lib.b200gru_linear_act_workspace_bytes(ctypes.byref(p), 0) == bad and lib.b200gru_linear_act_forward(None, None) == 1
+    p.M = p.K = p.N = p.ldx = p.ldw = 8
+    p.x = p.W = 256
+    assert lib.b200gru_linear_act_workspace_bytes(ctypes.byref(p), 0) != bad
+    assert lib.b200gru_linear_act_forward(ctypes.byref(p), None) == 1                   # no y
+    assert lib.b200gru_linear_act_backward(ctypes.byref(p), None) == 1                  # no dy
+    p.dy, p.lddy, p.activation = 256, 8, 2
+    assert lib.b200gru_linear_act_backward(ctypes.byref(p), None) == 1                  # no slope
