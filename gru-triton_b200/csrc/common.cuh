@@ -180,6 +180,9 @@ int tc_read_status(int reset);       // tensor-core GEMM core (tc_gemm.cu)
 int tc_step_read_status(int reset);  // fused tensor-core step (tc_step.cu)
 int tc2_read_status(int reset);      // CTA-pair products (tc_gemm2.cu)
 }  // namespace tc
+namespace gated {
+int read_status(int reset);          // gated linear recurrence (gated_scan.cu)
+}  // namespace gated
 
 // Test hook (b200gru_test_select_kernels): slot 0 != 0 -> butterfly launches use the register /
 // global-twiddle kernels on every shape; slot 1 != 0 -> the diagonal forward uses the register-ring

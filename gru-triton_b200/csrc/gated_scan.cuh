@@ -61,11 +61,12 @@ struct Gate {
 //   tanh|c| = (1 - f) / (1 + f), dn/dc = 4 f / (1 + f)^2; below |c| = 1/8, where 1 - f cancels, the series
 //   c - c^3/3 + 2 c^5/15 (next term 17/315 c^7: 2e-7 of c at most).
 // Both quotients come from one reciprocal, of (1 + e)(1 + f) in [1, 4].  A NaN in one argument stays out of the other's gate.
-__device__ __forceinline__ Gate gate(float x, float c, bool with_tanh) {
+template <bool TANH>
+__device__ __forceinline__ Gate gate(float x, float c) {
   Gate g;
   const float e = expf(-fabsf(x));
   const float d = 1.f + e;
-  if (with_tanh) {
+  if (TANH) {
     const float f = expf(-2.f * fabsf(c));
     const float de = fminf(d, 2.f), df = fminf(1.f + f, 2.f);
     const float r = __frcp_rn(de * df);

@@ -510,19 +510,31 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 }  // namespace
 
-int make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, unsigned long long d0,
-                       unsigned long long d1, unsigned long long d2, unsigned long long stride1_bytes,
-                       unsigned long long stride2_bytes, unsigned box0, unsigned box1) {
+static int encode_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, unsigned long long d0,
+                     unsigned long long d1, unsigned long long d2, unsigned long long stride1_bytes,
+                     unsigned long long stride2_bytes, unsigned box0, unsigned box1, unsigned box2,
+                     CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encoder();
   if (fn == nullptr) return B200GRU_UNSUPPORTED;
   const cuuint64_t dims[3] = {d0, d1, d2};
   const cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
-  const cuuint32_t box[3] = {box0, box1, 1};
+  const cuuint32_t box[3] = {box0, box1, box2};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? B200GRU_OK : B200GRU_INVALID_ARGUMENT;
+}
+
+int make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, unsigned long long d0,
+                       unsigned long long d1, unsigned long long d2, unsigned long long stride1_bytes,
+                       unsigned long long stride2_bytes, unsigned box0, unsigned box1) {
+  return encode_3d(map, dtype, base, d0, d1, d2, stride1_bytes, stride2_bytes, box0, box1, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int make_tensor_map_rows(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, unsigned long long d0,
+                         unsigned long long d1, unsigned long long d2, unsigned long long stride1_bytes,
+                         unsigned long long stride2_bytes, unsigned box0, unsigned box2) {
+  return encode_3d(map, dtype, base, d0, d1, d2, stride1_bytes, stride2_bytes, box0, 1, box2, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 int launch_wait_timeout_probe(cudaStream_t st) {
