@@ -3,8 +3,8 @@
 //   z = sigmoid(x)   n = tanh(c) or c   h_t = z h_{t-1} + (1 - z) n        gi[t,b,:] = (x[H], c[H])
 //
 // Each (row, unit) is a chain of its own whose steps are affine maps h -> z h + u.  Maps compose,
-// (A2, b2) o (A1, b1) = (A2 A1, A2 b1 + b2), so time is cut: a warp folds eight steps, a CTA of eight warps a tile of 64 steps
-// of 64 units, and a cluster of up to 16 CTAs takes that many tiles of the same units at once.  Maps are joined in
+// (A2, b2) o (A1, b1) = (A2 A1, A2 b1 + b2), so time is cut: a thread folds eight steps of two units, a CTA a tile (64 steps
+// of 64 units, or 128 of 32), and a cluster of up to 8 CTAs takes that many tiles of the same units at once.  Maps are joined in
 // the order of time at every level (through shared memory, then through the cluster's), never in the order of arrival.
 // The backward pass is the same scan in the other direction, G_t = z_t (dout_t + G_{t+1}), with the same products of z; it
 // recomputes the states of a tile from the one that the forward kept, so `out` is not read again.
@@ -24,13 +24,17 @@ __device__ int g_gated_status;
 
 namespace {
 
-constexpr int WARPS = 8, THREADS = 32 * WARPS;
-constexpr int SEG = TILE / WARPS;            // steps a warp folds
-constexpr int UNITS = 64;                    // units of a CTA, two per lane
-constexpr int MAX_CLUSTER = 16;
+constexpr int THREADS = 256;
+constexpr int MAX_CLUSTER = 8;
 constexpr int STAGES_MAX = 4;
 
-// ---- element access: FAST = two adjacent units per lane (aligned), else unit lane and lane + 32
+// LANES threads side by side have a row's units of the tile (two each), THREADS / LANES of them one behind the other its steps.
+template <int LANES>
+struct Tile {
+  static constexpr int UNITS = 2 * LANES, PARTS = THREADS / LANES, STEPS = PARTS * SEG;
+};
+
+// ---- element access: FAST = two adjacent units per lane (aligned), else units `lane` and `lane + LANES`
 template <typename T> struct Pair;
 template <> struct Pair<float> { typedef float2 type; };
 template <> struct Pair<__nv_bfloat16> { typedef __nv_bfloat162 type; };
@@ -45,36 +49,42 @@ template <> __device__ __forceinline__ __nv_bfloat162 pack<__nv_bfloat16>(float2
 template <> __device__ __forceinline__ __half2 pack<__half>(float2 v) { return __float22half2_rn(v); }
 
 // The lane's two units of a row that starts at p (unit 0 of the CTA); `left`: units of the row from there on.
-template <bool FAST, typename T>
+template <bool FAST, int LANES, typename T>
 __device__ __forceinline__ float2 load_units(const T* p, int lane, int left) {
-  if (FAST) return 2 * lane < left ? unpack(*reinterpret_cast<const typename Pair<T>::type*>(p + 2 * lane)) : make_float2(0.f, 0.f);
-  return make_float2(lane < left ? to_float(p[lane]) : 0.f, lane + 32 < left ? to_float(p[lane + 32]) : 0.f);
+  if (FAST) return 2 * lane < left ? unpack(*reinterpret_cast<const typename Pair<T>::type*>(p + 2 * lane)) : both(0.f);
+  return make_float2(lane < left ? to_float(p[lane]) : 0.f, lane + LANES < left ? to_float(p[lane + LANES]) : 0.f);
 }
-template <bool FAST, typename T>
+template <bool FAST, int LANES, typename T>
 __device__ __forceinline__ void store_units(T* p, int lane, int left, float2 v) {
   if (FAST) {
     if (2 * lane < left) *reinterpret_cast<typename Pair<T>::type*>(p + 2 * lane) = pack<T>(v);
   } else {
     if (lane < left) p[lane] = from_float<T>(v.x);
-    if (lane + 32 < left) p[lane + 32] = from_float<T>(v.y);
+    if (lane + LANES < left) p[lane + LANES] = from_float<T>(v.y);
   }
 }
 
 // fp32 states of the lane's units; rows of any alignment.
-template <bool FAST>
+template <bool FAST, int LANES>
 __device__ __forceinline__ float2 load_state(const float* p, int lane, int left) {
-  const int i = FAST ? 2 * lane : lane, j = FAST ? 2 * lane + 1 : lane + 32;
+  const int i = FAST ? 2 * lane : lane, j = FAST ? 2 * lane + 1 : lane + LANES;
   return make_float2(i < left ? p[i] : 0.f, j < left ? p[j] : 0.f);
 }
-template <bool FAST>
+template <bool FAST, int LANES>
 __device__ __forceinline__ void store_state(float* p, int lane, int left, float2 v) {
-  const int i = FAST ? 2 * lane : lane, j = FAST ? 2 * lane + 1 : lane + 32;
+  const int i = FAST ? 2 * lane : lane, j = FAST ? 2 * lane + 1 : lane + LANES;
   if (i < left) p[i] = v.x;
   if (j < left) p[j] = v.y;
 }
 
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
+// The map `m` after the map `first`, each (A, A, b, b).
+__device__ __forceinline__ float4 after(float4 m, float4 first) {
+  const float2 A = make_float2(m.x, m.y);
+  const float2 p = mul2(A, make_float2(first.x, first.y));
+  const float2 b = fma2(A, make_float2(first.z, first.w), make_float2(m.z, m.w));
+  return make_float4(p.x, p.y, b.x, b.y);
+}
+__device__ __forceinline__ float2 apply(float4 m, float2 h) { return fma2(make_float2(m.x, m.y), h, make_float2(m.z, m.w)); }
 
 // ---- cluster exchange ----------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -98,20 +108,22 @@ __device__ __forceinline__ void send16(uint32_t dst, float4 v, uint32_t bar) {
                  "r"(__float_as_uint(v.w)), "r"(bar) : "memory");
 }
 
+template <int LANES>
 struct Shared {
-  float4 part[2][WARPS][32];                 // a warp's map of the lane's two units: (A, A, b, b)
-  float2 front[2][WARPS][32];                // backward: the b of the forward direction
+  float4 part[2][Tile<LANES>::PARTS][LANES];   // maps of the threads: (A, A, b, b) of two units
   unsigned long long full[STAGES_MAX];       // a stage of inputs has landed
   unsigned long long joined[2];              // maps of all ranks have landed
   int dead;
 };
-// Behind the ring of inputs in dynamic shared memory: maps of the cluster's tiles, [2][ranks][32].
-__host__ __device__ inline size_t peer_bytes(int ranks) { return ranks > 1 ? (size_t)2 * ranks * 32 * sizeof(float4) : 0; }
+// Behind the ring of inputs in dynamic shared memory: maps of the cluster's tiles, [2][ranks][LANES].
+template <int LANES>
+__host__ __device__ constexpr size_t peer_bytes(int ranks) { return ranks > 1 ? (size_t)2 * ranks * LANES * sizeof(float4) : 0; }
 
 // Where a CTA is: its row, first unit, and its rank among the CTAs that share them.
 struct Place {
   int b, unit, left, rank, ranks;
 };
+template <int UNITS>
 __device__ __forceinline__ Place place_of(const Args& a, int ranks) {
   Place w;
   w.ranks = ranks;
@@ -124,48 +136,50 @@ __device__ __forceinline__ Place place_of(const Args& a, int ranks) {
   return w;
 }
 
-__device__ __forceinline__ void set_up(Shared& s, int stages, int ranks) {
+template <int LANES>
+__device__ __forceinline__ void set_up(Shared<LANES>& s, int stages, int ranks) {
   if (threadIdx.x == 0) {
     s.dead = 0;
     for (int i = 0; i < stages; ++i) tc::mbar_init(tc::smem_u32(&s.full[i]), 1);
     for (int i = 0; i < 2; ++i) tc::mbar_init(tc::smem_u32(&s.joined[i]), 1);
     tc::mbar_fence_init();
     if (ranks > 1)
-      for (int i = 0; i < 2; ++i) tc::mbar_expect_tx(tc::smem_u32(&s.joined[i]), (uint32_t)(ranks * 32 * sizeof(float4)));
+      for (int i = 0; i < 2; ++i) tc::mbar_expect_tx(tc::smem_u32(&s.joined[i]), (uint32_t)(ranks * LANES * sizeof(float4)));
   }
   __syncthreads();
   if (ranks > 1) cluster_barrier();
 }
 
-// Joins the tiles of the cluster: `all` is this CTA's map (every warp has it).  Returns the value that enters this CTA's
-// tile and moves `carry` behind the last one.  A slot is used again two rounds later: a peer sends its map of the round
-// between only after all its threads have read this round's, so two slots are enough.
-__device__ __forceinline__ float2 join(Shared& s, float4* peers, const Place& w, int round, float4 all, float2& carry, int warp, int lane) {
+// Joins the tiles of the cluster: `all` is this CTA's map (every thread has that of its units).  Returns the value that
+// enters this CTA's tile and moves `carry` behind the last one.  A slot is used again two rounds later: a peer sends its map of
+// the round between only after all its threads have read this round's, so two slots are enough.
+template <int LANES>
+__device__ __forceinline__ float2 join(Shared<LANES>& s, float4* peers, const Place& w, int round, float4 all, float2& carry,
+                                       int part, int lane) {
   if (w.ranks == 1) {
     const float2 in = carry;
-    carry = fma2(make_float2(all.x, all.y), in, make_float2(all.z, all.w));
+    carry = apply(all, in);
     return in;
   }
   const int slot = round & 1;
-  float4* peer = peers + slot * w.ranks * 32;
-  for (int r = warp; r < w.ranks; r += WARPS)
-    send16(at_rank(tc::smem_u32(peer + w.rank * 32 + lane), (uint32_t)r), all, at_rank(tc::smem_u32(&s.joined[slot]), (uint32_t)r));
+  float4* peer = peers + slot * w.ranks * LANES;
+  if (part < w.ranks)
+    send16(at_rank(tc::smem_u32(peer + w.rank * LANES + lane), (uint32_t)part), all, at_rank(tc::smem_u32(&s.joined[slot]), (uint32_t)part));
   tc::mbar_wait(tc::smem_u32(&s.joined[slot]), (uint32_t)(round >> 1) & 1u, &s.dead, &g_gated_status);
-  if (threadIdx.x == 0) tc::mbar_expect_tx(tc::smem_u32(&s.joined[slot]), (uint32_t)(w.ranks * 32 * sizeof(float4)));
+  if (threadIdx.x == 0) tc::mbar_expect_tx(tc::smem_u32(&s.joined[slot]), (uint32_t)(w.ranks * LANES * sizeof(float4)));
   float2 in = carry, h = carry;
   for (int r = 0; r < w.ranks; ++r) {
     if (r == w.rank) in = h;
-    const float4 m = peer[r * 32 + lane];
-    h = fma2(make_float2(m.x, m.y), h, make_float2(m.z, m.w));
+    h = apply(peer[r * LANES + lane], h);
   }
   carry = h;
   return in;
 }
 
 // Nobody leaves while a peer may still write here; a CTA that gave up waits for what is in flight.
-__device__ __forceinline__ void tear_down(Shared& s, int ranks) {
+__device__ __forceinline__ void tear_down(const volatile int* dead, int ranks) {
   if (ranks > 1) cluster_barrier();
-  if (*reinterpret_cast<volatile int*>(&s.dead)) {
+  if (*dead) {
     const long long start = clock64();
     while (clock64() - start < (1ll << 18)) {
     }
@@ -173,17 +187,18 @@ __device__ __forceinline__ void tear_down(Shared& s, int ranks) {
 }
 
 // ---- forward -------------------------------------------------------------------------------------
-template <typename T, bool FAST, bool TANH>
-__global__ void __launch_bounds__(THREADS, FAST ? 2 : 1)
+template <typename T, int LANES, bool FAST, bool TANH>
+__global__ void __launch_bounds__(THREADS, 3)
 gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int ranks, int stages) {
+  constexpr int UNITS = Tile<LANES>::UNITS, PARTS = Tile<LANES>::PARTS, STEPS = Tile<LANES>::STEPS;
   extern __shared__ __align__(128) unsigned char raw[];
-  __shared__ Shared s;
-  T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c][TILE][UNITS]
-  float4* peers = reinterpret_cast<float4*>(raw + (size_t)stages * 2 * TILE * UNITS * sizeof(T));
-  const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
-  const Place w = place_of(a, ranks);
+  __shared__ Shared<LANES> s;
+  T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c][STEPS][UNITS]
+  float4* peers = reinterpret_cast<float4*>(raw + (size_t)stages * 2 * STEPS * UNITS * sizeof(T));
+  const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const Place w = place_of<UNITS>(a, ranks);
   const int len = row_length(a, w.b);
-  const int tiles = (len + TILE - 1) / TILE;
+  const int tiles = (len + STEPS - 1) / STEPS;
   const int rounds = (tiles + ranks - 1) / ranks;
   set_up(s, stages, ranks);
 
@@ -191,93 +206,102 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
     const int tile = round * ranks + w.rank;
     if (round >= rounds || tile >= tiles) return;
     const uint32_t bar = tc::smem_u32(&s.full[round % stages]);
-    T* dst = ring + (size_t)(round % stages) * 2 * TILE * UNITS;
-    tc::mbar_expect_tx(bar, 2 * TILE * UNITS * sizeof(T));
-    tc::tma_load_3d(tc::smem_u32(dst), &map, w.unit, w.b, tile * TILE, bar);
-    tc::tma_load_3d(tc::smem_u32(dst + TILE * UNITS), &map, a.H + w.unit, w.b, tile * TILE, bar);
+    T* dst = ring + (size_t)(round % stages) * 2 * STEPS * UNITS;
+    tc::mbar_expect_tx(bar, 2 * STEPS * UNITS * sizeof(T));
+    tc::tma_load_3d(tc::smem_u32(dst), &map, w.unit, w.b, tile * STEPS, bar);
+    tc::tma_load_3d(tc::smem_u32(dst + STEPS * UNITS), &map, a.H + w.unit, w.b, tile * STEPS, bar);
   };
   if (FAST && threadIdx.x == 0)
     for (int r = 0; r < stages; ++r) fetch(r);
 
   const T* gp = static_cast<const T*>(a.gi) + (long long)w.b * a.gi_b + w.unit;
   T* op = static_cast<T*>(a.out) + (long long)w.b * a.out_b + w.unit;
-  float2 carry = make_float2(0.f, 0.f);
-  if (a.h0 != nullptr) carry = load_state<FAST>(a.h0 + (long long)w.b * a.h0_b + w.unit, lane, w.left);
+  float2 carry = both(0.f);
+  if (a.h0 != nullptr) carry = load_state<FAST, LANES>(a.h0 + (long long)w.b * a.h0_b + w.unit, lane, w.left);
 
   for (int round = 0; round < rounds; ++round) {
     const int tile = round * ranks + w.rank;
-    const int t0 = tile * TILE + warp * SEG;
+    const int t0 = tile * STEPS + part * SEG;
+    const int n = min(SEG, len - t0);                         // steps of this thread; none where n <= 0
     float2 z[SEG], u[SEG];
-    float2 A = make_float2(1.f, 1.f), b = make_float2(0.f, 0.f);
-    if (FAST && tile < tiles)
-      tc::mbar_wait(tc::smem_u32(&s.full[round % stages]), (uint32_t)(round / stages) & 1u, &s.dead, &g_gated_status);
-    const T* st = ring + (size_t)(round % stages) * 2 * TILE * UNITS + warp * SEG * UNITS;
+    float2 A = both(1.f), b = both(0.f);
+    if (tile < tiles) {
+      if (FAST) tc::mbar_wait(tc::smem_u32(&s.full[round % stages]), (uint32_t)(round / stages) & 1u, &s.dead, &g_gated_status);
+      const T* st = ring + (size_t)(round % stages) * 2 * STEPS * UNITS + part * SEG * UNITS;
 #pragma unroll
-    for (int k = 0; k < SEG; ++k) {
-      z[k] = make_float2(1.f, 1.f);
-      u[k] = make_float2(0.f, 0.f);
-      if (t0 + k < len) {
-        float2 x, c;
+      for (int k = 0; k < SEG; ++k) {
+        float2 x = both(0.f), c = x;
         if (FAST) {
-          x = load_units<true>(st + k * UNITS, lane, UNITS);
-          c = load_units<true>(st + (TILE + k) * UNITS, lane, UNITS);
-        } else {
+          x = load_units<true, LANES>(st + k * UNITS, lane, UNITS);
+          c = load_units<true, LANES>(st + (STEPS + k) * UNITS, lane, UNITS);
+        } else if (k < n) {
           const T* p = gp + (long long)(t0 + k) * a.gi_t;
-          x = load_units<false>(p, lane, w.left);
-          c = load_units<false>(p + a.H, lane, w.left);
+          x = load_units<false, LANES>(p, lane, w.left);
+          c = load_units<false, LANES>(p + a.H, lane, w.left);
         }
-        const Gate g0 = gate<TANH>(x.x, c.x), g1 = gate<TANH>(x.y, c.y);
-        z[k] = make_float2(g0.z, g1.z);
-        u[k] = make_float2(g0.keep * g0.n, g1.keep * g1.n);
+        const Gates g = gates<TANH>(x, c);
+        z[k] = g.z;
+        u[k] = mul2(g.keep, g.n);
+      }
+      if (n < SEG) {                                          // behind the row's end: the state stays
+#pragma unroll
+        for (int k = 0; k < SEG; ++k)
+          if (k >= n) { z[k] = both(1.f); u[k] = both(0.f); }
+      }
+#pragma unroll
+      for (int k = 0; k < SEG; ++k) {
         A = mul2(z[k], A);
         b = fma2(z[k], b, u[k]);
       }
     }
     const int slot = round & 1;
-    s.part[slot][warp][lane] = make_float4(A.x, A.y, b.x, b.y);
-    __syncthreads();                                          // the stage is read, the warps' maps are there
+    s.part[slot][part][lane] = make_float4(A.x, A.y, b.x, b.y);
+    __syncthreads();                                          // the stage is read, the threads' maps are there
     if (FAST && threadIdx.x == 0) fetch(round + stages);
     float4 all = make_float4(1.f, 1.f, 0.f, 0.f), mine = all;
 #pragma unroll
-    for (int v = 0; v < WARPS; ++v) {
-      if (v == warp) mine = all;
-      const float4 m = s.part[slot][v][lane];
-      all = make_float4(m.x * all.x, m.y * all.y, fmaf(m.x, all.z, m.z), fmaf(m.y, all.w, m.w));
+    for (int v = 0; v < PARTS; ++v) {
+      if (v == part) mine = all;
+      all = after(s.part[slot][v][lane], all);
     }
-    float2 h = join(s, peers, w, round, all, carry, warp, lane);
-    if (a.states != nullptr && warp == 0 && tile < tiles)
-      store_state<FAST>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left, h);
-    h = fma2(make_float2(mine.x, mine.y), h, make_float2(mine.z, mine.w));
-    T* o = op + (long long)t0 * a.out_t;
+    float2 h = join(s, peers, w, round, all, carry, part, lane);
+    if (tile < tiles) {
+      if (a.states != nullptr && part == 0)
+        store_state<FAST, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left, h);
+      h = apply(mine, h);
+      T* o = op + (long long)t0 * a.out_t;
 #pragma unroll
-    for (int k = 0; k < SEG; ++k) {
-      h = fma2(z[k], h, u[k]);
-      if (t0 + k < len) store_units<FAST>(o + (long long)k * a.out_t, lane, w.left, h);
+      for (int k = 0; k < SEG; ++k) {
+        h = fma2(z[k], h, u[k]);
+        if (k < n) store_units<FAST, LANES>(o + (long long)k * a.out_t, lane, w.left, h);
+      }
     }
   }
 
   // steps behind the row's last, and the state after it
-  for (int t = len + w.rank * WARPS + warp; t < a.T; t += ranks * WARPS)
-    store_units<FAST>(op + (long long)t * a.out_t, lane, w.left, make_float2(0.f, 0.f));
-  if (w.rank == 0 && warp == 0) store_state<FAST>(a.h_T + (long long)w.b * a.H + w.unit, lane, w.left, carry);
-  tear_down(s, ranks);
+  for (int t = len + w.rank * PARTS + part; t < a.T; t += ranks * PARTS)
+    store_units<FAST, LANES>(op + (long long)t * a.out_t, lane, w.left, both(0.f));
+  if (w.rank == 0 && part == 0) store_state<FAST, LANES>(a.h_T + (long long)w.b * a.H + w.unit, lane, w.left, carry);
+  tear_down(&s.dead, ranks);
 }
 
 // ---- backward ------------------------------------------------------------------------------------
 // Tiles from the last to the first; rank 0 of a round has the latest.  `front` joins the states inside a tile forwards, `part`
 // the gradients backwards, both with the same products of z.
-template <typename T, bool FAST, bool TANH>
-__global__ void __launch_bounds__(THREADS, FAST ? 2 : 1)
+template <typename T, int LANES, bool FAST, bool TANH>
+__global__ void __launch_bounds__(THREADS, 2)
 gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap dmap, const Args a, int ranks,
                  int stages) {
+  constexpr int UNITS = Tile<LANES>::UNITS, PARTS = Tile<LANES>::PARTS, STEPS = Tile<LANES>::STEPS;
   extern __shared__ __align__(128) unsigned char raw[];
-  __shared__ Shared s;
-  T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c, dout][TILE][UNITS]
-  float4* peers = reinterpret_cast<float4*>(raw + (size_t)stages * 3 * TILE * UNITS * sizeof(T));
-  const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
-  const Place w = place_of(a, ranks);
+  __shared__ Shared<LANES> s;
+  __shared__ float2 front[2][PARTS][LANES];
+  T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c, dout][STEPS][UNITS]
+  float4* peers = reinterpret_cast<float4*>(raw + (size_t)stages * 3 * STEPS * UNITS * sizeof(T));
+  const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const Place w = place_of<UNITS>(a, ranks);
   const int len = row_length(a, w.b);
-  const int tiles = (len + TILE - 1) / TILE;
+  const int tiles = (len + STEPS - 1) / STEPS;
   const int rounds = (tiles + ranks - 1) / ranks;
   const bool with_dout = a.dout != nullptr;
   set_up(s, stages, ranks);
@@ -286,11 +310,11 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     const int tile = tiles - 1 - (round * ranks + w.rank);
     if (round >= rounds || tile < 0) return;
     const uint32_t bar = tc::smem_u32(&s.full[round % stages]);
-    T* dst = ring + (size_t)(round % stages) * 3 * TILE * UNITS;
-    tc::mbar_expect_tx(bar, (with_dout ? 3 : 2) * TILE * UNITS * sizeof(T));
-    tc::tma_load_3d(tc::smem_u32(dst), &map, w.unit, w.b, tile * TILE, bar);
-    tc::tma_load_3d(tc::smem_u32(dst + TILE * UNITS), &map, a.H + w.unit, w.b, tile * TILE, bar);
-    if (with_dout) tc::tma_load_3d(tc::smem_u32(dst + 2 * TILE * UNITS), &dmap, w.unit, w.b, tile * TILE, bar);
+    T* dst = ring + (size_t)(round % stages) * 3 * STEPS * UNITS;
+    tc::mbar_expect_tx(bar, (with_dout ? 3 : 2) * STEPS * UNITS * sizeof(T));
+    tc::tma_load_3d(tc::smem_u32(dst), &map, w.unit, w.b, tile * STEPS, bar);
+    tc::tma_load_3d(tc::smem_u32(dst + STEPS * UNITS), &map, a.H + w.unit, w.b, tile * STEPS, bar);
+    if (with_dout) tc::tma_load_3d(tc::smem_u32(dst + 2 * STEPS * UNITS), &dmap, w.unit, w.b, tile * STEPS, bar);
   };
   if (FAST && threadIdx.x == 0)
     for (int r = 0; r < stages; ++r) fetch(r);
@@ -298,190 +322,196 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
   const T* gp = static_cast<const T*>(a.gi) + (long long)w.b * a.gi_b + w.unit;
   const T* dp = with_dout ? static_cast<const T*>(a.dout) + (long long)w.b * a.dout_b + w.unit : nullptr;
   T* qp = static_cast<T*>(a.dgi) + (long long)w.b * a.dgi_b + w.unit;
-  float2 carry = make_float2(0.f, 0.f);
-  if (a.dh_T != nullptr) carry = load_state<FAST>(a.dh_T + (long long)w.b * a.dh_b + w.unit, lane, w.left);
+  float2 carry = both(0.f);
+  if (a.dh_T != nullptr) carry = load_state<FAST, LANES>(a.dh_T + (long long)w.b * a.dh_b + w.unit, lane, w.left);
 
   for (int round = 0; round < rounds; ++round) {
     const int tile = tiles - 1 - (round * ranks + w.rank);
-    const int t0 = tile * TILE + warp * SEG;
-    float2 h = make_float2(0.f, 0.f);
-    if (tile >= 0) h = load_state<FAST>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left);
-    float2 z[SEG], keep[SEG], n[SEG], slope[SEG], d[SEG];
-    float2 A = make_float2(1.f, 1.f), f = make_float2(0.f, 0.f), r = f;
-    if (FAST && tile >= 0)
-      tc::mbar_wait(tc::smem_u32(&s.full[round % stages]), (uint32_t)(round / stages) & 1u, &s.dead, &g_gated_status);
-    const T* st = ring + (size_t)(round % stages) * 3 * TILE * UNITS + warp * SEG * UNITS;
+    const int t0 = tile * STEPS + part * SEG;
+    const int n = min(SEG, len - t0);                         // steps of this thread; none where n <= 0
+    float2 h = both(0.f);
+    float2 z[SEG], u[SEG], p[SEG], q[SEG], d[SEG];            // p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'
+    float2 A = both(1.f), f = both(0.f), r = f;
+    float2 zk[SEG];
+    if (tile >= 0) {
+      h = load_state<FAST, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left);
+      if (FAST) tc::mbar_wait(tc::smem_u32(&s.full[round % stages]), (uint32_t)(round / stages) & 1u, &s.dead, &g_gated_status);
+      const T* st = ring + (size_t)(round % stages) * 3 * STEPS * UNITS + part * SEG * UNITS;
 #pragma unroll
-    for (int k = 0; k < SEG; ++k) {
-      z[k] = make_float2(1.f, 1.f);
-      keep[k] = n[k] = slope[k] = d[k] = make_float2(0.f, 0.f);
-      if (tile >= 0 && t0 + k < len) {
-        float2 x, c;
+      for (int k = 0; k < SEG; ++k) {
+        float2 x = both(0.f), c = x;
+        d[k] = x;
         if (FAST) {
-          x = load_units<true>(st + k * UNITS, lane, UNITS);
-          c = load_units<true>(st + (TILE + k) * UNITS, lane, UNITS);
-          if (with_dout) d[k] = load_units<true>(st + (2 * TILE + k) * UNITS, lane, UNITS);
-        } else {
-          const T* p = gp + (long long)(t0 + k) * a.gi_t;
-          x = load_units<false>(p, lane, w.left);
-          c = load_units<false>(p + a.H, lane, w.left);
-          if (with_dout) d[k] = load_units<false>(dp + (long long)(t0 + k) * a.dout_t, lane, w.left);
+          x = load_units<true, LANES>(st + k * UNITS, lane, UNITS);
+          c = load_units<true, LANES>(st + (STEPS + k) * UNITS, lane, UNITS);
+          if (with_dout) d[k] = load_units<true, LANES>(st + (2 * STEPS + k) * UNITS, lane, UNITS);
+        } else if (k < n) {
+          const T* at = gp + (long long)(t0 + k) * a.gi_t;
+          x = load_units<false, LANES>(at, lane, w.left);
+          c = load_units<false, LANES>(at + a.H, lane, w.left);
+          if (with_dout) d[k] = load_units<false, LANES>(dp + (long long)(t0 + k) * a.dout_t, lane, w.left);
         }
-        const Gate g0 = gate<TANH>(x.x, c.x), g1 = gate<TANH>(x.y, c.y);
-        z[k] = make_float2(g0.z, g1.z);
-        keep[k] = make_float2(g0.keep, g1.keep);
-        n[k] = make_float2(g0.n, g1.n);
-        slope[k] = make_float2(g0.slope, g1.slope);
-        A = mul2(z[k], A);
-        f = fma2(z[k], f, mul2(keep[k], n[k]));
+        const Gates g = gates<TANH>(x, c);
+        z[k] = g.z;
+        u[k] = mul2(g.keep, g.n);
+        p[k] = g.n;
+        q[k] = mul2(g.keep, g.slope);
+        zk[k] = mul2(g.open, g.keep);
       }
-    }
+      if (n < SEG) {
 #pragma unroll
-    for (int k = SEG - 1; k >= 0; --k) r = mul2(z[k], make_float2(d[k].x + r.x, d[k].y + r.y));
+        for (int k = 0; k < SEG; ++k)
+          if (k >= n) { z[k] = both(1.f); u[k] = d[k] = both(0.f); }
+      }
+#pragma unroll
+      for (int k = 0; k < SEG; ++k) {
+        A = mul2(z[k], A);
+        f = fma2(z[k], f, u[k]);
+      }
+#pragma unroll
+      for (int k = SEG - 1; k >= 0; --k) r = mul2(z[k], add2(d[k], r));
+    }
     const int slot = round & 1;
-    s.part[slot][warp][lane] = make_float4(A.x, A.y, r.x, r.y);
-    s.front[slot][warp][lane] = f;
+    s.part[slot][part][lane] = make_float4(A.x, A.y, r.x, r.y);
+    front[slot][part][lane] = f;
     __syncthreads();
     if (FAST && threadIdx.x == 0) fetch(round + stages);
     float4 all = make_float4(1.f, 1.f, 0.f, 0.f), mine = all;
 #pragma unroll
-    for (int v = WARPS - 1; v >= 0; --v) {
-      if (v == warp) mine = all;
+    for (int v = PARTS - 1; v >= 0; --v) {
+      if (v == part) mine = all;
       const float4 m = s.part[slot][v][lane];
-      all = make_float4(m.x * all.x, m.y * all.y, fmaf(m.x, all.z, m.z), fmaf(m.y, all.w, m.w));
+      all = after(m, all);
     }
-    for (int v = 0; v < warp; ++v) {
+    for (int v = 0; v < part; ++v) {
       const float4 m = s.part[slot][v][lane];
-      h = fma2(make_float2(m.x, m.y), h, s.front[slot][v][lane]);
+      h = fma2(make_float2(m.x, m.y), h, front[slot][v][lane]);
     }
-    float2 G = join(s, peers, w, round, all, carry, warp, lane);
-    G = fma2(make_float2(mine.x, mine.y), G, make_float2(mine.z, mine.w));
+    float2 G = join(s, peers, w, round, all, carry, part, lane);
+    if (tile >= 0) {
+      G = apply(mine, G);
 #pragma unroll
-    for (int k = 0; k < SEG; ++k) {                            // n becomes (h_{t-1} - n) z (1 - z), slope (1 - z) n'
-      const float2 was = h;
-      h = fma2(z[k], h, mul2(keep[k], n[k]));
-      const float2 zk = mul2(z[k], keep[k]);
-      n[k] = make_float2((was.x - n[k].x) * zk.x, (was.y - n[k].y) * zk.y);
-      slope[k] = mul2(keep[k], slope[k]);
-    }
-    T* o = qp + (long long)t0 * a.dgi_t;
+      for (int k = 0; k < SEG; ++k) {
+        p[k] = mul2(fma2(p[k], both(-1.f), h), zk[k]);
+        h = fma2(z[k], h, u[k]);
+      }
+      T* o = qp + (long long)t0 * a.dgi_t;
 #pragma unroll
-    for (int k = SEG - 1; k >= 0; --k) {
-      const float2 g = make_float2(G.x + d[k].x, G.y + d[k].y);
-      G = mul2(z[k], g);
-      if (tile >= 0 && t0 + k < len) {
-        store_units<FAST>(o + (long long)k * a.dgi_t, lane, w.left, mul2(g, n[k]));
-        store_units<FAST>(o + (long long)k * a.dgi_t + a.H, lane, w.left, mul2(g, slope[k]));
+      for (int k = SEG - 1; k >= 0; --k) {
+        const float2 g = add2(G, d[k]);
+        G = mul2(z[k], g);
+        if (k < n) {
+          store_units<FAST, LANES>(o + (long long)k * a.dgi_t, lane, w.left, mul2(g, p[k]));
+          store_units<FAST, LANES>(o + (long long)k * a.dgi_t + a.H, lane, w.left, mul2(g, q[k]));
+        }
       }
     }
   }
 
-  for (int t = len + w.rank * WARPS + warp; t < a.T; t += ranks * WARPS) {
-    store_units<FAST>(qp + (long long)t * a.dgi_t, lane, w.left, make_float2(0.f, 0.f));
-    store_units<FAST>(qp + (long long)t * a.dgi_t + a.H, lane, w.left, make_float2(0.f, 0.f));
+  for (int t = len + w.rank * PARTS + part; t < a.T; t += ranks * PARTS) {
+    store_units<FAST, LANES>(qp + (long long)t * a.dgi_t, lane, w.left, both(0.f));
+    store_units<FAST, LANES>(qp + (long long)t * a.dgi_t + a.H, lane, w.left, both(0.f));
   }
-  if (a.dh0 != nullptr && w.rank == 0 && warp == 0)
-    store_state<FAST>(a.dh0 + (long long)w.b * a.H + w.unit, lane, w.left, carry);
-  tear_down(s, ranks);
+  if (a.dh0 != nullptr && w.rank == 0 && part == 0)
+    store_state<FAST, LANES>(a.dh0 + (long long)w.b * a.H + w.unit, lane, w.left, carry);
+  tear_down(&s.dead, ranks);
 }
 
 // ---- a few steps -----------------------------------------------------------------------------------
 // At most SEG steps: a warp has 64 units of a row and all their steps, nothing to join.
 template <typename T, bool FAST, bool TANH>
 __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
-  const int lane = threadIdx.x & 31, columns = (a.H + UNITS - 1) / UNITS;
+  const int lane = threadIdx.x & 31, columns = (a.H + 63) / 64;
   const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (i >= (long long)a.B * columns) return;
-  const int b = (int)(i / columns), unit = (int)(i % columns) * UNITS, left = a.H - unit;
+  const int b = (int)(i / columns), unit = (int)(i % columns) * 64, left = a.H - unit;
   const int len = row_length(a, b);
   const T* gp = static_cast<const T*>(a.gi) + (long long)b * a.gi_b + unit;
   T* op = static_cast<T*>(a.out) + (long long)b * a.out_b + unit;
-  float2 h = make_float2(0.f, 0.f);
-  if (a.h0 != nullptr) h = load_state<FAST>(a.h0 + (long long)b * a.h0_b + unit, lane, left);
-  if (a.states != nullptr) store_state<FAST>(a.states + (long long)b * a.H + unit, lane, left, h);
+  float2 h = both(0.f);
+  if (a.h0 != nullptr) h = load_state<FAST, 32>(a.h0 + (long long)b * a.h0_b + unit, lane, left);
+  if (a.states != nullptr) store_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left, h);
   float2 x[SEG], c[SEG];
 #pragma unroll
   for (int k = 0; k < SEG; ++k)
     if (k < len) {
-      x[k] = load_units<FAST>(gp + (long long)k * a.gi_t, lane, left);
-      c[k] = load_units<FAST>(gp + (long long)k * a.gi_t + a.H, lane, left);
+      x[k] = load_units<FAST, 32>(gp + (long long)k * a.gi_t, lane, left);
+      c[k] = load_units<FAST, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
     }
 #pragma unroll
   for (int k = 0; k < SEG; ++k)
     if (k < a.T) {
-      float2 o = make_float2(0.f, 0.f);
+      float2 o = both(0.f);
       if (k < len) {
-        const Gate g0 = gate<TANH>(x[k].x, c[k].x), g1 = gate<TANH>(x[k].y, c[k].y);
-        h = make_float2(fmaf(g0.z, h.x, g0.keep * g0.n), fmaf(g1.z, h.y, g1.keep * g1.n));
+        const Gates g = gates<TANH>(x[k], c[k]);
+        h = fma2(g.z, h, mul2(g.keep, g.n));
         o = h;
       }
-      store_units<FAST>(op + (long long)k * a.out_t, lane, left, o);
+      store_units<FAST, 32>(op + (long long)k * a.out_t, lane, left, o);
     }
-  store_state<FAST>(a.h_T + (long long)b * a.H + unit, lane, left, h);
+  store_state<FAST, 32>(a.h_T + (long long)b * a.H + unit, lane, left, h);
 }
 
 template <typename T, bool FAST, bool TANH>
 __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
-  const int lane = threadIdx.x & 31, columns = (a.H + UNITS - 1) / UNITS;
+  const int lane = threadIdx.x & 31, columns = (a.H + 63) / 64;
   const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (i >= (long long)a.B * columns) return;
-  const int b = (int)(i / columns), unit = (int)(i % columns) * UNITS, left = a.H - unit;
+  const int b = (int)(i / columns), unit = (int)(i % columns) * 64, left = a.H - unit;
   const int len = row_length(a, b);
   const T* gp = static_cast<const T*>(a.gi) + (long long)b * a.gi_b + unit;
   const T* dp = a.dout != nullptr ? static_cast<const T*>(a.dout) + (long long)b * a.dout_b + unit : nullptr;
   T* qp = static_cast<T*>(a.dgi) + (long long)b * a.dgi_b + unit;
-  float2 G = make_float2(0.f, 0.f);
-  if (a.dh_T != nullptr) G = load_state<FAST>(a.dh_T + (long long)b * a.dh_b + unit, lane, left);
-  float2 h = load_state<FAST>(a.states + (long long)b * a.H + unit, lane, left);
+  float2 G = both(0.f);
+  if (a.dh_T != nullptr) G = load_state<FAST, 32>(a.dh_T + (long long)b * a.dh_b + unit, lane, left);
+  float2 h = load_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left);
   float2 z[SEG], p[SEG], q[SEG], d[SEG];
 #pragma unroll
   for (int k = 0; k < SEG; ++k) {
-    d[k] = make_float2(0.f, 0.f);
+    d[k] = both(0.f);
     if (k < len) {
-      const float2 x = load_units<FAST>(gp + (long long)k * a.gi_t, lane, left);
-      const float2 c = load_units<FAST>(gp + (long long)k * a.gi_t + a.H, lane, left);
-      if (dp != nullptr) d[k] = load_units<FAST>(dp + (long long)k * a.dout_t, lane, left);
-      const Gate g0 = gate<TANH>(x.x, c.x), g1 = gate<TANH>(x.y, c.y);
-      z[k] = make_float2(g0.z, g1.z);
-      p[k] = make_float2((h.x - g0.n) * (g0.z * g0.keep), (h.y - g1.n) * (g1.z * g1.keep));
-      q[k] = make_float2(g0.keep * g0.slope, g1.keep * g1.slope);
-      h = make_float2(fmaf(g0.z, h.x, g0.keep * g0.n), fmaf(g1.z, h.y, g1.keep * g1.n));
+      const float2 x = load_units<FAST, 32>(gp + (long long)k * a.gi_t, lane, left);
+      const float2 c = load_units<FAST, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
+      if (dp != nullptr) d[k] = load_units<FAST, 32>(dp + (long long)k * a.dout_t, lane, left);
+      const Gates g = gates<TANH>(x, c);
+      z[k] = g.z;
+      p[k] = mul2(fma2(g.n, both(-1.f), h), mul2(g.open, g.keep));
+      q[k] = mul2(g.keep, g.slope);
+      h = fma2(g.z, h, mul2(g.keep, g.n));
     }
   }
 #pragma unroll
   for (int k = SEG - 1; k >= 0; --k)
     if (k < a.T) {
-      float2 dx = make_float2(0.f, 0.f), dc = dx;
+      float2 dx = both(0.f), dc = dx;
       if (k < len) {
-        const float2 g = make_float2(G.x + d[k].x, G.y + d[k].y);
+        const float2 g = add2(G, d[k]);
         G = mul2(z[k], g);
         dx = mul2(g, p[k]);
         dc = mul2(g, q[k]);
       }
-      store_units<FAST>(qp + (long long)k * a.dgi_t, lane, left, dx);
-      store_units<FAST>(qp + (long long)k * a.dgi_t + a.H, lane, left, dc);
+      store_units<FAST, 32>(qp + (long long)k * a.dgi_t, lane, left, dx);
+      store_units<FAST, 32>(qp + (long long)k * a.dgi_t + a.H, lane, left, dc);
     }
-  if (a.dh0 != nullptr) store_state<FAST>(a.dh0 + (long long)b * a.H + unit, lane, left, G);
+  if (a.dh0 != nullptr) store_state<FAST, 32>(a.dh0 + (long long)b * a.H + unit, lane, left, G);
 }
 
 template <typename T, bool FAST, bool TANH>
 __global__ void __launch_bounds__(128) gated_step_kernel(const StepArgs a) {
-  const int lane = threadIdx.x & 31, columns = (a.H + UNITS - 1) / UNITS;
+  const int lane = threadIdx.x & 31, columns = (a.H + 63) / 64;
   const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (i >= (long long)a.B * columns) return;
-  const int b = (int)(i / columns), unit = (int)(i % columns) * UNITS, left = a.H - unit;
+  const int b = (int)(i / columns), unit = (int)(i % columns) * 64, left = a.H - unit;
   const T* gp = static_cast<const T*>(a.gi) + (long long)b * a.gi_b + unit;
-  const float2 x = load_units<FAST>(gp, lane, left), c = load_units<FAST>(gp + a.H, lane, left);
-  float2 h = load_state<FAST>(a.h + (long long)b * a.h_b + unit, lane, left);
-  const Gate g0 = gate<TANH>(x.x, c.x), g1 = gate<TANH>(x.y, c.y);
-  h = make_float2(fmaf(g0.z, h.x, g0.keep * g0.n), fmaf(g1.z, h.y, g1.keep * g1.n));
-  store_state<FAST>(a.h_new + (long long)b * a.hn_b + unit, lane, left, h);
-  store_units<FAST>(static_cast<T*>(a.out) + (long long)b * a.H + unit, lane, left, h);
+  const float2 x = load_units<FAST, 32>(gp, lane, left), c = load_units<FAST, 32>(gp + a.H, lane, left);
+  float2 h = load_state<FAST, 32>(a.h + (long long)b * a.h_b + unit, lane, left);
+  const Gates g = gates<TANH>(x, c);
+  h = fma2(g.z, h, mul2(g.keep, g.n));
+  store_state<FAST, 32>(a.h_new + (long long)b * a.hn_b + unit, lane, left, h);
+  store_units<FAST, 32>(static_cast<T*>(a.out) + (long long)b * a.H + unit, lane, left, h);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-constexpr size_t CTA_SHARED = 112 * 1024;          // two CTAs of a tile kernel share an SM
-
 template <typename T> struct MapType;
 template <> struct MapType<float> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_FLOAT32; };
 template <> struct MapType<__nv_bfloat16> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; };
@@ -497,28 +527,29 @@ template <typename T>
 bool paired(const void* p, long long st, long long sb) {
   return (reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1)) == 0 && st % 2 == 0 && sb % 2 == 0;
 }
-template <typename T>
+template <typename T, int LANES>
 int tile_map(CUtensorMap* map, const void* p, long long units, const Args& a, long long st, long long sb) {
   const unsigned long long row = a.B == 1 ? 16 : (unsigned long long)sb * sizeof(T);
-  return tc::make_tensor_map_rows(map, MapType<T>::value, p, units, a.B, a.T, row, (unsigned long long)st * sizeof(T), UNITS, TILE);
+  return tc::make_tensor_map_rows(map, MapType<T>::value, p, units, a.B, a.T, row, (unsigned long long)st * sizeof(T),
+                                  Tile<LANES>::UNITS, Tile<LANES>::STEPS);
 }
 
-// CTAs of a row and 64 units: one, or as many as it takes to give every SM two CTAs, up to the row's tiles.
-int ranks_for(const Args& a) {
-  const long long base = (long long)a.B * cdiv(a.H, UNITS);
-  const int tiles = cdiv(a.T, TILE);
+// Tiles of 32 units where 64 leave most of the GPU idle even with full clusters.
+bool narrow(int T, int B, int H) { return T > Tile<32>::STEPS && (long long)B * cdiv(H, Tile<32>::UNITS) * MAX_CLUSTER < 2 * 148; }
+
+// CTAs of a row's units: one, or as many as it takes to fill the GPU, up to the row's tiles.
+template <int LANES>
+int ranks_for(const Args& a, int ctas) {
+  const long long base = (long long)a.B * cdiv(a.H, Tile<LANES>::UNITS);
+  const int tiles = cdiv(a.T, Tile<LANES>::STEPS);
   int ranks = 1;
-  while (ranks < MAX_CLUSTER && ranks < tiles && base * ranks < 296) ranks *= 2;
+  while (ranks < MAX_CLUSTER && ranks < tiles && base * ranks < ctas) ranks *= 2;
   return ranks;
 }
 
 template <typename... KArgs, typename... CArgs>
-int launch_tiles(void (*kernel)(KArgs...), const Args& a, int ranks, size_t smem, cudaStream_t st, CArgs... args) {
-  const void* fn = reinterpret_cast<const void*>(kernel);
-  if (allow_dynamic_smem(fn, smem) != B200GRU_OK) return B200GRU_UNSUPPORTED;
-  if (ranks > 8 && cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-    return check_launch("cudaFuncSetAttribute(gated scan)");
-  const long long blocks = (long long)a.B * cdiv(a.H, UNITS) * ranks;
+int launch_tiles(void (*kernel)(KArgs...), long long blocks, int ranks, size_t smem, cudaStream_t st, CArgs... args) {
+  if (allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem) != B200GRU_OK) return B200GRU_UNSUPPORTED;
   if (blocks > 0x7fffffffll) return B200GRU_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
@@ -531,59 +562,78 @@ int launch_tiles(void (*kernel)(KArgs...), const Args& a, int ranks, size_t smem
   return check_launch("gated scan");
 }
 
-template <typename T, bool TANH>
-int forward(const Args& a, cudaStream_t st) {
-  const bool pairs = paired<T>(a.out, a.out_t, a.out_b) && a.H % 2 == 0;
-  if (a.T <= SEG) {
-    const unsigned blocks = (unsigned)(((long long)a.B * cdiv(a.H, UNITS) + 3) / 4);
-    if (pairs && paired<T>(a.gi, a.gi_t, a.gi_b)) gated_short_fwd_kernel<T, true, TANH><<<blocks, 128, 0, st>>>(a);
-    else gated_short_fwd_kernel<T, false, TANH><<<blocks, 128, 0, st>>>(a);
-    note_launch();
-    return check_launch("gated_short_fwd_kernel");
-  }
-  const int ranks = ranks_for(a);
+// Stages of `stage` bytes that fit beside the rest where `ctas` CTAs share an SM's 227 KB.
+template <int LANES>
+int stages_for(size_t stage, size_t fixed, int ranks, int ctas) {
+  const size_t room = 227 * 1024 / ctas - 1024 - fixed - peer_bytes<LANES>(ranks);
+  const int n = (int)(room / stage);
+  return n < 1 ? 1 : (n > STAGES_MAX ? STAGES_MAX : n);
+}
+
+template <typename T, int LANES, bool TANH>
+int forward_tiles(const Args& a, cudaStream_t st) {
+  const int ranks = ranks_for<LANES>(a, 3 * 148);
+  const long long blocks = (long long)a.B * cdiv(a.H, Tile<LANES>::UNITS) * ranks;
+  const size_t peers = peer_bytes<LANES>(ranks);
   alignas(64) CUtensorMap map;
   memset(&map, 0, sizeof(map));
-  if (pairs && a.H * sizeof(T) % 16 == 0 && tileable<T>(a.gi, a.gi_t, a.gi_b, a.B) &&
-      tile_map<T>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK) {
-    const size_t stage = 2 * TILE * UNITS * sizeof(T), fixed = sizeof(Shared) + peer_bytes(ranks) + 1024;
-    int stages = (int)((CTA_SHARED - fixed) / stage);
-    if (stages > STAGES_MAX) stages = STAGES_MAX;
-    return launch_tiles(gated_fwd_kernel<T, true, TANH>, a, ranks, stages * stage + peer_bytes(ranks), st, map, a, ranks, stages);
+  if (paired<T>(a.out, a.out_t, a.out_b) && a.H * sizeof(T) % 16 == 0 && tileable<T>(a.gi, a.gi_t, a.gi_b, a.B) &&
+      tile_map<T, LANES>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK) {
+    const size_t stage = (size_t)2 * Tile<LANES>::STEPS * Tile<LANES>::UNITS * sizeof(T);
+    const int stages = stages_for<LANES>(stage, sizeof(Shared<LANES>), ranks, 3);
+    return launch_tiles(gated_fwd_kernel<T, LANES, true, TANH>, blocks, ranks, stages * stage + peers, st, map, a, ranks, stages);
   }
-  return launch_tiles(gated_fwd_kernel<T, false, TANH>, a, ranks, peer_bytes(ranks), st, map, a, ranks, 0);
+  return launch_tiles(gated_fwd_kernel<T, LANES, false, TANH>, blocks, ranks, peers, st, map, a, ranks, 0);
+}
+
+template <typename T, int LANES, bool TANH>
+int backward_tiles(const Args& a, cudaStream_t st) {
+  const int ranks = ranks_for<LANES>(a, 2 * 148);
+  const long long blocks = (long long)a.B * cdiv(a.H, Tile<LANES>::UNITS) * ranks;
+  const size_t peers = peer_bytes<LANES>(ranks);
+  alignas(64) CUtensorMap map, dmap;
+  memset(&map, 0, sizeof(map));
+  memset(&dmap, 0, sizeof(dmap));
+  if (paired<T>(a.dgi, a.dgi_t, a.dgi_b) && a.H * sizeof(T) % 16 == 0 && tileable<T>(a.gi, a.gi_t, a.gi_b, a.B) &&
+      tile_map<T, LANES>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK &&
+      (a.dout == nullptr || (tileable<T>(a.dout, a.dout_t, a.dout_b, a.B) &&
+                             tile_map<T, LANES>(&dmap, a.dout, a.H, a, a.dout_t, a.dout_b) == B200GRU_OK))) {
+    const size_t stage = (size_t)3 * Tile<LANES>::STEPS * Tile<LANES>::UNITS * sizeof(T);
+    const size_t fixed = sizeof(Shared<LANES>) + 2 * THREADS * sizeof(float2);
+    const int stages = stages_for<LANES>(stage, fixed, ranks, 2);
+    return launch_tiles(gated_bwd_kernel<T, LANES, true, TANH>, blocks, ranks, stages * stage + peers, st, map, dmap, a, ranks, stages);
+  }
+  return launch_tiles(gated_bwd_kernel<T, LANES, false, TANH>, blocks, ranks, peers, st, map, dmap, a, ranks, 0);
+}
+
+template <typename T, bool TANH>
+int forward(const Args& a, cudaStream_t st) {
+  if (a.T > SEG) return narrow(a.T, a.B, a.H) ? forward_tiles<T, 16, TANH>(a, st) : forward_tiles<T, 32, TANH>(a, st);
+  const unsigned blocks = (unsigned)(((long long)a.B * cdiv(a.H, 64) + 3) / 4);
+  if (a.H % 2 == 0 && paired<T>(a.out, a.out_t, a.out_b) && paired<T>(a.gi, a.gi_t, a.gi_b))
+    gated_short_fwd_kernel<T, true, TANH><<<blocks, 128, 0, st>>>(a);
+  else
+    gated_short_fwd_kernel<T, false, TANH><<<blocks, 128, 0, st>>>(a);
+  note_launch();
+  return check_launch("gated_short_fwd_kernel");
 }
 
 template <typename T, bool TANH>
 int backward(const Args& a, cudaStream_t st) {
-  const bool pairs = paired<T>(a.dgi, a.dgi_t, a.dgi_b) && a.H % 2 == 0;
-  if (a.T <= SEG) {
-    const unsigned blocks = (unsigned)(((long long)a.B * cdiv(a.H, UNITS) + 3) / 4);
-    if (pairs && paired<T>(a.gi, a.gi_t, a.gi_b) && (a.dout == nullptr || paired<T>(a.dout, a.dout_t, a.dout_b)))
-      gated_short_bwd_kernel<T, true, TANH><<<blocks, 128, 0, st>>>(a);
-    else gated_short_bwd_kernel<T, false, TANH><<<blocks, 128, 0, st>>>(a);
-    note_launch();
-    return check_launch("gated_short_bwd_kernel");
-  }
-  const int ranks = ranks_for(a);
-  alignas(64) CUtensorMap map, dmap;
-  memset(&map, 0, sizeof(map));
-  memset(&dmap, 0, sizeof(dmap));
-  if (pairs && a.H * sizeof(T) % 16 == 0 && tileable<T>(a.gi, a.gi_t, a.gi_b, a.B) &&
-      tile_map<T>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK &&
-      (a.dout == nullptr || (tileable<T>(a.dout, a.dout_t, a.dout_b, a.B) &&
-                             tile_map<T>(&dmap, a.dout, a.H, a, a.dout_t, a.dout_b) == B200GRU_OK))) {
-    const size_t stage = 3 * TILE * UNITS * sizeof(T), fixed = sizeof(Shared) + peer_bytes(ranks) + 1024;
-    int stages = (int)((CTA_SHARED - fixed) / stage);
-    if (stages > STAGES_MAX) stages = STAGES_MAX;
-    return launch_tiles(gated_bwd_kernel<T, true, TANH>, a, ranks, stages * stage + peer_bytes(ranks), st, map, dmap, a, ranks, stages);
-  }
-  return launch_tiles(gated_bwd_kernel<T, false, TANH>, a, ranks, peer_bytes(ranks), st, map, dmap, a, ranks, 0);
+  if (a.T > SEG) return narrow(a.T, a.B, a.H) ? backward_tiles<T, 16, TANH>(a, st) : backward_tiles<T, 32, TANH>(a, st);
+  const unsigned blocks = (unsigned)(((long long)a.B * cdiv(a.H, 64) + 3) / 4);
+  if (a.H % 2 == 0 && paired<T>(a.dgi, a.dgi_t, a.dgi_b) && paired<T>(a.gi, a.gi_t, a.gi_b) &&
+      (a.dout == nullptr || paired<T>(a.dout, a.dout_t, a.dout_b)))
+    gated_short_bwd_kernel<T, true, TANH><<<blocks, 128, 0, st>>>(a);
+  else
+    gated_short_bwd_kernel<T, false, TANH><<<blocks, 128, 0, st>>>(a);
+  note_launch();
+  return check_launch("gated_short_bwd_kernel");
 }
 
 template <typename T, bool TANH>
 int step(const StepArgs& a, cudaStream_t st) {
-  const unsigned blocks = (unsigned)(((long long)a.B * cdiv(a.H, UNITS) + 3) / 4);
+  const unsigned blocks = (unsigned)(((long long)a.B * cdiv(a.H, 64) + 3) / 4);
   if (a.H % 2 == 0 && paired<T>(a.gi, 0, a.gi_b) && paired<T>(a.out, 0, 0)) gated_step_kernel<T, true, TANH><<<blocks, 128, 0, st>>>(a);
   else gated_step_kernel<T, false, TANH><<<blocks, 128, 0, st>>>(a);
   note_launch();
@@ -591,6 +641,8 @@ int step(const StepArgs& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+int tile_steps(int T, int B, int H) { return narrow(T, B, H) ? Tile<16>::STEPS : Tile<32>::STEPS; }
 
 int launch_forward(const Args& a, int dtype, cudaStream_t st) {
   if (dtype == B200GRU_F32) return a.tanh ? forward<float, true>(a, st) : forward<float, false>(a, st);
@@ -655,7 +707,7 @@ extern "C" {
 
 size_t b200gru_gated_states_bytes(int T, int B, int H) {
   if (T <= 0 || B <= 0 || H <= 0) return 0;
-  return (size_t)cdiv(T, gated::TILE) * B * H * sizeof(float);
+  return (size_t)cdiv(T, gated::tile_steps(T, B, H)) * B * H * sizeof(float);
 }
 
 int b200gru_gated_scan_forward(const b200gru_gated_args* p, void* stream) {

@@ -9,7 +9,7 @@
 namespace b200gru {
 namespace gated {
 
-constexpr int TILE = 64;       // steps between two kept states
+constexpr int SEG = 8;         // steps that a thread folds
 
 // Strides in elements; the units of a row are contiguous.  h0, dout, dh_T: NULL = zeros.
 struct Args {
@@ -20,7 +20,7 @@ struct Args {
   const void* lengths; int length_bytes;       // per row, 4 or 8 bytes each; NULL = T
   void* out; long long out_t, out_b;
   float* h_T;                  // [B][H]
-  float* states;               // [ceil(T / TILE)][B][H]: state before step k * TILE; NULL = not kept
+  float* states;               // [tiles][B][H]: state before each tile (see tile_steps); NULL = not kept
   const void* dout; long long dout_t, dout_b;
   const float* dh_T; long long dh_b;
   void* dgi; long long dgi_t, dgi_b;
@@ -51,44 +51,93 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-struct Gate {
-  float z, keep, n, slope;     // sigmoid(x), 1 - z, candidate, dn / dc
+// ---- two units at a time: the packed fp32 instructions of sm_100 --------------------------------------
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float exp2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// The smaller one; NaN if either is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^(v * scale), at most 2^60.
+__device__ __forceinline__ float2 power2(float2 v, float scale) {
+  const float2 t = mul2(v, both(scale));
+  return make_float2(exp2_approx(min_nan(t.x, 60.f)), exp2_approx(min_nan(t.y, 60.f)));
+}
+
+// Gates of two units.  z = 1 - keep, so that the two add to one to a rounding and a state that holds for hundreds of steps
+// does not drift; `open` is the same gate to full relative precision, where its size matters (its slope).
+struct Gates {
+  float2 z, open, keep, n, slope;
 };
 
-// With e = exp(-|x|) and f = exp(-2|c|) in [0, 1]:
-//   the smaller of z and 1 - z is e / (1 + e), to full relative precision; the larger is 1 minus it, so that the two add to
-//   one to a rounding of the larger and a state that holds for hundreds of steps does not drift;
-//   tanh|c| = (1 - f) / (1 + f), dn/dc = 4 f / (1 + f)^2; below |c| = 1/8, where 1 - f cancels, the series
-//   c - c^3/3 + 2 c^5/15 (next term 17/315 c^7: 2e-7 of c at most).
-// Both quotients come from one reciprocal, of (1 + e)(1 + f) in [1, 4].  A NaN in one argument stays out of the other's gate.
+// With e = exp(-x) and f = exp(-2c):  open = 1 / (1 + e), keep = e open, tanh c = (1 - f) / (1 + f), dn/dc = 4 f / (1 + f)^2.
+// Both quotients come from one reciprocal, of (1 + e)(1 + f): three special-function values instead of four, which is what
+// bounds 16-bit inputs (16 of them a cycle and SM, against 26 bytes a cycle from memory).  The minima keep a NaN of one
+// argument out of the other's gate.  Below |c| = 1/8, where 1 - f cancels, the series c - c^3/3 + 2 c^5/15 (next term
+// 17/315 c^7: 2e-7 of c at most).
 template <bool TANH>
-__device__ __forceinline__ Gate gate(float x, float c) {
-  Gate g;
-  const float e = expf(-fabsf(x));
-  const float d = 1.f + e;
+__device__ __forceinline__ Gates gates(float2 x, float2 c) {
+  constexpr float LOG2E = 1.44269504f, MOST = 2305843009213693952.f;        // 2^61
+  Gates g;
+  const float2 one = both(1.f);
+  const float2 e = power2(x, -LOG2E);
+  float2 d = add2(one, e);
   if (TANH) {
-    const float f = expf(-2.f * fabsf(c));
-    const float de = fminf(d, 2.f), df = fminf(1.f + f, 2.f);
-    const float r = __frcp_rn(de * df);
-    const float s = e * (r * df);
-    const float q = r * de;
-    const float c2 = c * c;
-    const float near0 = fmaf(fmaf(c2, 2.f / 15.f, -1.f / 3.f) * c2, c, c);
-    const float far = copysignf((1.f - f) * q, c);
-    g.n = fabsf(c) < 0.125f ? near0 : far;
-    g.slope = 4.f * f * q * q;
-    g.z = x >= 0.f ? 1.f - s : s;
-    g.keep = x >= 0.f ? s : 1.f - s;
+    const float2 f = power2(c, -2.f * LOG2E);
+    float2 q = add2(one, f);
+    d = make_float2(fminf(d.x, MOST), fminf(d.y, MOST));
+    q = make_float2(fminf(q.x, MOST), fminf(q.y, MOST));
+    const float2 p = mul2(d, q);
+    const float2 r = make_float2(rcp_approx(p.x), rcp_approx(p.y));
+    g.open = mul2(r, q);
+    q = mul2(r, d);
+    const float2 far = mul2(fma2(f, both(-1.f), one), q);
+    const float2 c2 = mul2(c, c);
+    const float2 near0 = fma2(mul2(fma2(c2, both(2.f / 15.f), both(-1.f / 3.f)), c2), c, c);
+    g.n = make_float2(fabsf(c.x) < 0.125f ? near0.x : far.x, fabsf(c.y) < 0.125f ? near0.y : far.y);
+    g.slope = mul2(mul2(mul2(f, q), q), both(4.f));
   } else {
-    const float s = e * __frcp_rn(d);
+    g.open = make_float2(rcp_approx(d.x), rcp_approx(d.y));
     g.n = c;
-    g.slope = 1.f;
-    g.z = x >= 0.f ? 1.f - s : s;
-    g.keep = x >= 0.f ? s : 1.f - s;
+    g.slope = one;
   }
+  g.keep = mul2(e, g.open);
+  g.z = fma2(g.keep, both(-1.f), one);
   return g;
 }
 
+// Steps of a tile for these sizes.
+int tile_steps(int T, int B, int H);
 int launch_forward(const Args& a, int dtype, cudaStream_t st);
 int launch_backward(const Args& a, int dtype, cudaStream_t st);
 int launch_step(const StepArgs& a, int dtype, cudaStream_t st);

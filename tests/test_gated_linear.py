@@ -226,7 +226,7 @@ def test_scan_reads_any_layout(dtype, T):
         out, h_T = gated_scan(leaf, h)
         got = torch.autograd.grad((out, h_T), (leaf, h), (d, wide(dh, 2, 1)))
         for a, b in zip((out, h_T, *got), (ref[0], ref[1], *ref[2])):
-            close(a.detach(), b.detach().double(), 2 * rounding(b.double(), dtype) + 64 * T * U * float(b.abs().max()))
+            close(a.detach(), b.detach().double(), 2 * rounding(b.double(), dtype) + 64 * T * U * float(b.detach().abs().max()))
     # every step and row the same one: inputs of stride 0
     one = gi[:1, :1].expand(T, B, 2 * H)
     assert torch.equal(gated_scan(one)[0], gated_scan(one.contiguous())[0])
@@ -701,7 +701,7 @@ def test_library_refuses_bad_arguments():
     assert lib.b200gru_gated_scan_forward(ctypes.byref(a), None) == 1
     a.dtype, a.lengths, a.length_bytes = 0, 256, 2
     assert lib.b200gru_gated_scan_forward(ctypes.byref(a), None) == 1
-    assert lib.b200gru_gated_states_bytes(65, 2, 3) == 2 * 2 * 3 * 4 and lib.b200gru_gated_states_bytes(0, 2, 3) == 0
+    assert lib.b200gru_gated_states_bytes(64, 200, 96) == 200 * 96 * 4 and lib.b200gru_gated_states_bytes(0, 2, 3) == 0
     assert lib.b200gru_gated_step(0, 1, 0, 4, 256, 8, 256, 4, 256, 256, 4, None) == 1
     assert lib.b200gru_gated_step(0, 1, 2, 4, 256, 8, 256, 4, 256, 256, 3, None) == 1   # rows of the new state overlap
     p = _lib.CLinearArgs()
