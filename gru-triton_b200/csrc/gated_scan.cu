@@ -111,6 +111,7 @@ __device__ __forceinline__ void send16(uint32_t dst, float4 v, uint32_t bar) {
 template <int LANES>
 struct Shared {
   float4 part[2][Tile<LANES>::PARTS][LANES];   // maps of the threads: (A, A, b, b) of two units
+  float2 carry[2][LANES];                      // what enters the round
   unsigned long long full[STAGES_MAX];       // a stage of inputs has landed
   unsigned long long joined[2];              // maps of all ranks have landed
   int dead;
@@ -150,30 +151,30 @@ __device__ __forceinline__ void set_up(Shared<LANES>& s, int stages, int ranks) 
   if (ranks > 1) cluster_barrier();
 }
 
-// Joins the tiles of the cluster: `all` is this CTA's map (every thread has that of its units).  Returns the value that
-// enters this CTA's tile and moves `carry` behind the last one.  A slot is used again two rounds later: a peer sends its map of
-// the round between only after all its threads have read this round's, so two slots are enough.
+// One part of the threads (all of a CTA's units) sends the CTA's map to every rank.  A slot is used again two rounds later: a
+// peer sends its map of the round between only after all its threads have read this round's, so two slots are enough.
 template <int LANES>
-__device__ __forceinline__ float2 join(Shared<LANES>& s, float4* peers, const Place& w, int round, float4 all, float2& carry,
-                                       int part, int lane) {
-  if (w.ranks == 1) {
-    const float2 in = carry;
-    carry = apply(all, in);
-    return in;
-  }
+__device__ __forceinline__ void send_map(Shared<LANES>& s, float4* peers, const Place& w, int round, float4 all, int lane) {
   const int slot = round & 1;
-  float4* peer = peers + slot * w.ranks * LANES;
-  if (part < w.ranks)
-    send16(at_rank(tc::smem_u32(peer + w.rank * LANES + lane), (uint32_t)part), all, at_rank(tc::smem_u32(&s.joined[slot]), (uint32_t)part));
+  const uint32_t to = tc::smem_u32(peers + (slot * w.ranks + w.rank) * LANES + lane), bar = tc::smem_u32(&s.joined[slot]);
+  for (int r = 0; r < w.ranks; ++r) send16(at_rank(to, (uint32_t)r), all, at_rank(bar, (uint32_t)r));
+}
+// What enters this CTA's tile: the round's carry through the maps of the ranks before it.  Part 1 folds on through all of
+// them, which is what the next round starts from.
+template <int LANES>
+__device__ __forceinline__ float2 join(Shared<LANES>& s, const float4* peers, const Place& w, int round, int part, int lane) {
+  const int slot = round & 1;
   tc::mbar_wait(tc::smem_u32(&s.joined[slot]), (uint32_t)(round >> 1) & 1u, &s.dead, &g_gated_status);
   if (threadIdx.x == 0) tc::mbar_expect_tx(tc::smem_u32(&s.joined[slot]), (uint32_t)(w.ranks * LANES * sizeof(float4)));
-  float2 in = carry, h = carry;
-  for (int r = 0; r < w.ranks; ++r) {
-    if (r == w.rank) in = h;
-    h = apply(peer[r * LANES + lane], h);
+  const float4* m = peers + slot * w.ranks * LANES + lane;
+  float2 h = s.carry[slot][lane];
+  for (int r = 0; r < w.rank; ++r) h = apply(m[r * LANES], h);
+  if (part == 1) {
+    float2 end = h;
+    for (int r = w.rank; r < w.ranks; ++r) end = apply(m[r * LANES], end);
+    s.carry[slot ^ 1][lane] = end;
   }
-  carry = h;
-  return in;
+  return h;
 }
 
 // Nobody leaves while a peer may still write here; a CTA that gave up waits for what is in flight.
@@ -187,8 +188,11 @@ __device__ __forceinline__ void tear_down(const volatile int* dead, int ranks) {
 }
 
 // ---- forward -------------------------------------------------------------------------------------
-template <typename T, int LANES, bool FAST, bool TANH>
-__global__ void __launch_bounds__(THREADS, 3)
+// A round's phases: gates and maps of the threads | barrier | the state that enters, the results.  CLUSTERED: the gates of the next
+// round are computed while the maps of this one travel (two sets of registers, two CTAs to an SM); otherwise a third CTA
+// covers for the barrier.
+template <typename T, int LANES, bool FAST, bool TANH, bool CLUSTERED>
+__global__ void __launch_bounds__(THREADS, CLUSTERED ? 2 : 3)
 gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int ranks, int stages) {
   constexpr int UNITS = Tile<LANES>::UNITS, PARTS = Tile<LANES>::PARTS, STEPS = Tile<LANES>::STEPS;
   extern __shared__ __align__(128) unsigned char raw[];
@@ -196,6 +200,7 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
   T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c][STEPS][UNITS]
   float4* peers = reinterpret_cast<float4*>(raw + (size_t)stages * 2 * STEPS * UNITS * sizeof(T));
   const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  if (!CLUSTERED) ranks = 1;
   const Place w = place_of<UNITS>(a, ranks);
   const int len = row_length(a, w.b);
   const int tiles = (len + STEPS - 1) / STEPS;
@@ -216,14 +221,18 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
 
   const T* gp = static_cast<const T*>(a.gi) + (long long)w.b * a.gi_b + w.unit;
   T* op = static_cast<T*>(a.out) + (long long)w.b * a.out_b + w.unit;
-  float2 carry = both(0.f);
-  if (a.h0 != nullptr) carry = load_state<FAST, LANES>(a.h0 + (long long)w.b * a.h0_b + w.unit, lane, w.left);
+  if (part == 0) {
+    float2 h = both(0.f);
+    if (a.h0 != nullptr) h = load_state<FAST, LANES>(a.h0 + (long long)w.b * a.h0_b + w.unit, lane, w.left);
+    s.carry[0][lane] = h;
+  }
+  const Constants K = constants();
 
-  for (int round = 0; round < rounds; ++round) {
+  // gates of a round into z and u, the thread's map into shared memory
+  auto open_gates = [&](int round, float2 (&z)[SEG], float2 (&u)[SEG]) {
     const int tile = round * ranks + w.rank;
     const int t0 = tile * STEPS + part * SEG;
-    const int n = min(SEG, len - t0);                         // steps of this thread; none where n <= 0
-    float2 z[SEG], u[SEG];
+    const int n = len - t0;                                   // steps left from here
     float2 A = both(1.f), b = both(0.f);
     if (tile < tiles) {
       if (FAST) tc::mbar_wait(tc::smem_u32(&s.full[round % stages]), (uint32_t)(round / stages) & 1u, &s.dead, &g_gated_status);
@@ -239,7 +248,7 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
           x = load_units<false, LANES>(p, lane, w.left);
           c = load_units<false, LANES>(p + a.H, lane, w.left);
         }
-        const Gates g = gates<TANH>(x, c);
+        const Gates g = gates<TANH, false>(x, c, K);
         z[k] = g.z;
         u[k] = mul2(g.keep, g.n);
       }
@@ -248,47 +257,85 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
         for (int k = 0; k < SEG; ++k)
           if (k >= n) { z[k] = both(1.f); u[k] = both(0.f); }
       }
+      A = z[0];
+      b = u[0];
 #pragma unroll
-      for (int k = 0; k < SEG; ++k) {
+      for (int k = 1; k < SEG; ++k) {
         A = mul2(z[k], A);
         b = fma2(z[k], b, u[k]);
       }
     }
-    const int slot = round & 1;
-    s.part[slot][part][lane] = make_float4(A.x, A.y, b.x, b.y);
-    __syncthreads();                                          // the stage is read, the threads' maps are there
-    if (FAST && threadIdx.x == 0) fetch(round + stages);
-    float4 all = make_float4(1.f, 1.f, 0.f, 0.f), mine = all;
+    s.part[round & 1][part][lane] = make_float4(A.x, A.y, b.x, b.y);
+  };
+  // results of a round from the state that enters its tile
+  auto walk = [&](int round, float2 h, const float2 (&z)[SEG], const float2 (&u)[SEG]) {
+    const int tile = round * ranks + w.rank;
+    if (tile >= tiles) return;
+    if (a.states != nullptr && part == 0)
+      store_state<FAST, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left, h);
+    const float4* m = &s.part[round & 1][0][lane];
+    for (int v = 0; v < part; ++v) h = apply(m[v * LANES], h);
+    const int t0 = tile * STEPS + part * SEG, n = len - t0;
+    T* o = op + (long long)t0 * a.out_t;
+    if (n >= SEG) {
 #pragma unroll
-    for (int v = 0; v < PARTS; ++v) {
-      if (v == part) mine = all;
-      all = after(s.part[slot][v][lane], all);
-    }
-    float2 h = join(s, peers, w, round, all, carry, part, lane);
-    if (tile < tiles) {
-      if (a.states != nullptr && part == 0)
-        store_state<FAST, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left, h);
-      h = apply(mine, h);
-      T* o = op + (long long)t0 * a.out_t;
+      for (int k = 0; k < SEG; ++k) {
+        h = fma2(z[k], h, u[k]);
+        store_units<FAST, LANES>(o, lane, w.left, h);
+        o += a.out_t;
+      }
+    } else {
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
         h = fma2(z[k], h, u[k]);
         if (k < n) store_units<FAST, LANES>(o + (long long)k * a.out_t, lane, w.left, h);
       }
     }
+    if (!CLUSTERED && part == PARTS - 1) s.carry[(round & 1) ^ 1][lane] = h;
+  };
+
+  if (CLUSTERED) {
+    auto round_of = [&](int round, const float2 (&z)[SEG], const float2 (&u)[SEG], float2 (&zn)[SEG], float2 (&un)[SEG]) {
+      __syncthreads();                                        // the stage is read, the threads' maps are there
+      if (part == 0) {
+        float4 all = s.part[round & 1][0][lane];
+#pragma unroll
+        for (int v = 1; v < PARTS; ++v) all = after(s.part[round & 1][v][lane], all);
+        send_map(s, peers, w, round, all, lane);
+      }
+      if (FAST && threadIdx.x == 0) fetch(round + stages);
+      if (round + 1 < rounds) open_gates(round + 1, zn, un);
+      walk(round, join(s, peers, w, round, part, lane), z, u);
+    };
+    float2 za[SEG], ua[SEG], zb[SEG], ub[SEG];
+    if (rounds > 0) open_gates(0, za, ua);
+    for (int round = 0; round < rounds; round += 2) {
+      round_of(round, za, ua, zb, ub);
+      if (round + 1 < rounds) round_of(round + 1, zb, ub, za, ua);
+    }
+  } else {
+    for (int round = 0; round < rounds; ++round) {
+      float2 z[SEG], u[SEG];
+      open_gates(round, z, u);
+      __syncthreads();
+      if (FAST && threadIdx.x == 0) fetch(round + stages);
+      walk(round, s.carry[round & 1][lane], z, u);
+    }
   }
 
   // steps behind the row's last, and the state after it
   for (int t = len + w.rank * PARTS + part; t < a.T; t += ranks * PARTS)
     store_units<FAST, LANES>(op + (long long)t * a.out_t, lane, w.left, both(0.f));
-  if (w.rank == 0 && part == 0) store_state<FAST, LANES>(a.h_T + (long long)w.b * a.H + w.unit, lane, w.left, carry);
+  __syncthreads();
+  if (w.rank == 0 && part == 0)
+    store_state<FAST, LANES>(a.h_T + (long long)w.b * a.H + w.unit, lane, w.left, s.carry[rounds & 1][lane]);
   tear_down(&s.dead, ranks);
 }
 
 // ---- backward ------------------------------------------------------------------------------------
 // Tiles from the last to the first; rank 0 of a round has the latest.  `front` joins the states inside a tile forwards, `part`
 // the gradients backwards, both with the same products of z.
-template <typename T, int LANES, bool FAST, bool TANH>
+template <typename T, int LANES, bool FAST, bool TANH, bool CLUSTERED>
 __global__ void __launch_bounds__(THREADS, 2)
 gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap dmap, const Args a, int ranks,
                  int stages) {
@@ -299,6 +346,7 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
   T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c, dout][STEPS][UNITS]
   float4* peers = reinterpret_cast<float4*>(raw + (size_t)stages * 3 * STEPS * UNITS * sizeof(T));
   const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  if (!CLUSTERED) ranks = 1;
   const Place w = place_of<UNITS>(a, ranks);
   const int len = row_length(a, w.b);
   const int tiles = (len + STEPS - 1) / STEPS;
@@ -322,13 +370,17 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
   const T* gp = static_cast<const T*>(a.gi) + (long long)w.b * a.gi_b + w.unit;
   const T* dp = with_dout ? static_cast<const T*>(a.dout) + (long long)w.b * a.dout_b + w.unit : nullptr;
   T* qp = static_cast<T*>(a.dgi) + (long long)w.b * a.dgi_b + w.unit;
-  float2 carry = both(0.f);
-  if (a.dh_T != nullptr) carry = load_state<FAST, LANES>(a.dh_T + (long long)w.b * a.dh_b + w.unit, lane, w.left);
+  if (part == 0) {
+    float2 G = both(0.f);
+    if (a.dh_T != nullptr) G = load_state<FAST, LANES>(a.dh_T + (long long)w.b * a.dh_b + w.unit, lane, w.left);
+    s.carry[0][lane] = G;
+  }
+  const Constants K = constants();
 
   for (int round = 0; round < rounds; ++round) {
     const int tile = tiles - 1 - (round * ranks + w.rank);
     const int t0 = tile * STEPS + part * SEG;
-    const int n = min(SEG, len - t0);                         // steps of this thread; none where n <= 0
+    const int n = len - t0;                                   // steps left from here
     float2 h = both(0.f);
     float2 z[SEG], u[SEG], p[SEG], q[SEG], d[SEG];            // p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'
     float2 A = both(1.f), f = both(0.f), r = f;
@@ -351,7 +403,7 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
           c = load_units<false, LANES>(at + a.H, lane, w.left);
           if (with_dout) d[k] = load_units<false, LANES>(dp + (long long)(t0 + k) * a.dout_t, lane, w.left);
         }
-        const Gates g = gates<TANH>(x, c);
+        const Gates g = gates<TANH, true>(x, c, K);
         z[k] = g.z;
         u[k] = mul2(g.keep, g.n);
         p[k] = g.n;
@@ -375,26 +427,25 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     s.part[slot][part][lane] = make_float4(A.x, A.y, r.x, r.y);
     front[slot][part][lane] = f;
     __syncthreads();
-    if (FAST && threadIdx.x == 0) fetch(round + stages);
-    float4 all = make_float4(1.f, 1.f, 0.f, 0.f), mine = all;
+    const float4* m = &s.part[slot][0][lane];
+    if (CLUSTERED && part == 0) {
+      float4 all = m[(PARTS - 1) * LANES];
 #pragma unroll
-    for (int v = PARTS - 1; v >= 0; --v) {
-      if (v == part) mine = all;
-      const float4 m = s.part[slot][v][lane];
-      all = after(m, all);
+      for (int v = PARTS - 2; v >= 0; --v) all = after(m[v * LANES], all);
+      send_map(s, peers, w, round, all, lane);
     }
-    for (int v = 0; v < part; ++v) {
-      const float4 m = s.part[slot][v][lane];
-      h = fma2(make_float2(m.x, m.y), h, front[slot][v][lane]);
-    }
-    float2 G = join(s, peers, w, round, all, carry, part, lane);
+    if (FAST && threadIdx.x == 0) fetch(round + stages);
+    for (int v = 0; v < part; ++v) h = fma2(make_float2(m[v * LANES].x, m[v * LANES].y), h, front[slot][v][lane]);
     if (tile >= 0) {
-      G = apply(mine, G);
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
-        p[k] = mul2(fma2(p[k], both(-1.f), h), zk[k]);
+        p[k] = mul2(sub2(h, p[k]), zk[k]);
         h = fma2(z[k], h, u[k]);
       }
+    }
+    float2 G = CLUSTERED ? join(s, peers, w, round, part, lane) : s.carry[slot][lane];
+    if (tile >= 0) {
+      for (int v = PARTS - 1; v > part; --v) G = apply(m[v * LANES], G);
       T* o = qp + (long long)t0 * a.dgi_t;
 #pragma unroll
       for (int k = SEG - 1; k >= 0; --k) {
@@ -405,6 +456,7 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
           store_units<FAST, LANES>(o + (long long)k * a.dgi_t + a.H, lane, w.left, mul2(g, q[k]));
         }
       }
+      if (!CLUSTERED && part == 0) s.carry[slot ^ 1][lane] = G;
     }
   }
 
@@ -412,8 +464,9 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     store_units<FAST, LANES>(qp + (long long)t * a.dgi_t, lane, w.left, both(0.f));
     store_units<FAST, LANES>(qp + (long long)t * a.dgi_t + a.H, lane, w.left, both(0.f));
   }
+  __syncthreads();
   if (a.dh0 != nullptr && w.rank == 0 && part == 0)
-    store_state<FAST, LANES>(a.dh0 + (long long)w.b * a.H + w.unit, lane, w.left, carry);
+    store_state<FAST, LANES>(a.dh0 + (long long)w.b * a.H + w.unit, lane, w.left, s.carry[rounds & 1][lane]);
   tear_down(&s.dead, ranks);
 }
 
@@ -431,6 +484,7 @@ __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
   float2 h = both(0.f);
   if (a.h0 != nullptr) h = load_state<FAST, 32>(a.h0 + (long long)b * a.h0_b + unit, lane, left);
   if (a.states != nullptr) store_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left, h);
+  const Constants K = constants();
   float2 x[SEG], c[SEG];
 #pragma unroll
   for (int k = 0; k < SEG; ++k)
@@ -443,7 +497,7 @@ __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
     if (k < a.T) {
       float2 o = both(0.f);
       if (k < len) {
-        const Gates g = gates<TANH>(x[k], c[k]);
+        const Gates g = gates<TANH, false>(x[k], c[k], K);
         h = fma2(g.z, h, mul2(g.keep, g.n));
         o = h;
       }
@@ -465,6 +519,7 @@ __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
   float2 G = both(0.f);
   if (a.dh_T != nullptr) G = load_state<FAST, 32>(a.dh_T + (long long)b * a.dh_b + unit, lane, left);
   float2 h = load_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left);
+  const Constants K = constants();
   float2 z[SEG], p[SEG], q[SEG], d[SEG];
 #pragma unroll
   for (int k = 0; k < SEG; ++k) {
@@ -473,9 +528,9 @@ __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
       const float2 x = load_units<FAST, 32>(gp + (long long)k * a.gi_t, lane, left);
       const float2 c = load_units<FAST, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
       if (dp != nullptr) d[k] = load_units<FAST, 32>(dp + (long long)k * a.dout_t, lane, left);
-      const Gates g = gates<TANH>(x, c);
+      const Gates g = gates<TANH, true>(x, c, K);
       z[k] = g.z;
-      p[k] = mul2(fma2(g.n, both(-1.f), h), mul2(g.open, g.keep));
+      p[k] = mul2(sub2(h, g.n), mul2(g.open, g.keep));
       q[k] = mul2(g.keep, g.slope);
       h = fma2(g.z, h, mul2(g.keep, g.n));
     }
@@ -505,7 +560,7 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const StepArgs a) {
   const T* gp = static_cast<const T*>(a.gi) + (long long)b * a.gi_b + unit;
   const float2 x = load_units<FAST, 32>(gp, lane, left), c = load_units<FAST, 32>(gp + a.H, lane, left);
   float2 h = load_state<FAST, 32>(a.h + (long long)b * a.h_b + unit, lane, left);
-  const Gates g = gates<TANH>(x, c);
+  const Gates g = gates<TANH, false>(x, c, constants());
   h = fma2(g.z, h, mul2(g.keep, g.n));
   store_state<FAST, 32>(a.h_new + (long long)b * a.hn_b + unit, lane, left, h);
   store_units<FAST, 32>(static_cast<T*>(a.out) + (long long)b * a.H + unit, lane, left, h);
@@ -580,10 +635,12 @@ int forward_tiles(const Args& a, cudaStream_t st) {
   if (paired<T>(a.out, a.out_t, a.out_b) && a.H * sizeof(T) % 16 == 0 && tileable<T>(a.gi, a.gi_t, a.gi_b, a.B) &&
       tile_map<T, LANES>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK) {
     const size_t stage = (size_t)2 * Tile<LANES>::STEPS * Tile<LANES>::UNITS * sizeof(T);
-    const int stages = stages_for<LANES>(stage, sizeof(Shared<LANES>), ranks, 3);
-    return launch_tiles(gated_fwd_kernel<T, LANES, true, TANH>, blocks, ranks, stages * stage + peers, st, map, a, ranks, stages);
+    const int stages = stages_for<LANES>(stage, sizeof(Shared<LANES>), ranks, ranks > 1 ? 2 : 3);
+    return ranks > 1 ? launch_tiles(gated_fwd_kernel<T, LANES, true, TANH, true>, blocks, ranks, stages * stage + peers, st, map, a, ranks, stages)
+                     : launch_tiles(gated_fwd_kernel<T, LANES, true, TANH, false>, blocks, 1, stages * stage, st, map, a, 1, stages);
   }
-  return launch_tiles(gated_fwd_kernel<T, LANES, false, TANH>, blocks, ranks, peers, st, map, a, ranks, 0);
+  return ranks > 1 ? launch_tiles(gated_fwd_kernel<T, LANES, false, TANH, true>, blocks, ranks, peers, st, map, a, ranks, 0)
+                   : launch_tiles(gated_fwd_kernel<T, LANES, false, TANH, false>, blocks, 1, 0, st, map, a, 1, 0);
 }
 
 template <typename T, int LANES, bool TANH>
@@ -601,9 +658,11 @@ int backward_tiles(const Args& a, cudaStream_t st) {
     const size_t stage = (size_t)3 * Tile<LANES>::STEPS * Tile<LANES>::UNITS * sizeof(T);
     const size_t fixed = sizeof(Shared<LANES>) + 2 * THREADS * sizeof(float2);
     const int stages = stages_for<LANES>(stage, fixed, ranks, 2);
-    return launch_tiles(gated_bwd_kernel<T, LANES, true, TANH>, blocks, ranks, stages * stage + peers, st, map, dmap, a, ranks, stages);
+    return ranks > 1 ? launch_tiles(gated_bwd_kernel<T, LANES, true, TANH, true>, blocks, ranks, stages * stage + peers, st, map, dmap, a, ranks, stages)
+                     : launch_tiles(gated_bwd_kernel<T, LANES, true, TANH, false>, blocks, 1, stages * stage, st, map, dmap, a, 1, stages);
   }
-  return launch_tiles(gated_bwd_kernel<T, LANES, false, TANH>, blocks, ranks, peers, st, map, dmap, a, ranks, 0);
+  return ranks > 1 ? launch_tiles(gated_bwd_kernel<T, LANES, false, TANH, true>, blocks, ranks, peers, st, map, dmap, a, ranks, 0)
+                   : launch_tiles(gated_bwd_kernel<T, LANES, false, TANH, false>, blocks, 1, 0, st, map, dmap, a, 1, 0);
 }
 
 template <typename T, bool TANH>

@@ -71,6 +71,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tsub.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float exp2_approx(float v) {
   float r;
@@ -88,9 +94,24 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// The constants of the packed instructions, which take registers alone.  Behind a volatile move they stay in theirs; the
+// compiler would otherwise build each pair anew at each use, seven moves beside the 24 instructions of an element.
+struct Constants {
+  float2 one, to_e, to_2c, cubic, fifth;
+};
+__device__ __forceinline__ float2 pinned(float v) {
+  float2 d;
+  asm volatile("mov.b32 %0, %2;\n\tmov.b32 %1, %2;" : "=f"(d.x), "=f"(d.y) : "f"(v));
+  return d;
+}
+__device__ __forceinline__ Constants constants() {
+  constexpr float LOG2E = 1.44269504f;
+  return {pinned(1.f), pinned(-LOG2E), pinned(-2.f * LOG2E), pinned(-1.f / 3.f), pinned(2.f / 15.f)};
+}
+
 // 2^(v * scale), at most 2^60.
-__device__ __forceinline__ float2 power2(float2 v, float scale) {
-  const float2 t = mul2(v, both(scale));
+__device__ __forceinline__ float2 power2(float2 v, float2 scale) {
+  const float2 t = mul2(v, scale);
   return make_float2(exp2_approx(min_nan(t.x, 60.f)), exp2_approx(min_nan(t.y, 60.f)));
 }
 
@@ -101,38 +122,39 @@ struct Gates {
 };
 
 // With e = exp(-x) and f = exp(-2c):  open = 1 / (1 + e), keep = e open, tanh c = (1 - f) / (1 + f), dn/dc = 4 f / (1 + f)^2.
-// Both quotients come from one reciprocal, of (1 + e)(1 + f): three special-function values instead of four, which is what
-// bounds 16-bit inputs (16 of them a cycle and SM, against 26 bytes a cycle from memory).  The minima keep a NaN of one
-// argument out of the other's gate.  Below |c| = 1/8, where 1 - f cancels, the series c - c^3/3 + 2 c^5/15 (next term
-// 17/315 c^7: 2e-7 of c at most).
-template <bool TANH>
-__device__ __forceinline__ Gates gates(float2 x, float2 c) {
-  constexpr float LOG2E = 1.44269504f, MOST = 2305843009213693952.f;        // 2^61
+// Both quotients come from one reciprocal, of (1 + e)(1 + f): three special-function values instead of four, of which an SM
+// has 16 a cycle.  APART: a NaN of c stays out of x's gate (in the forward both make the state NaN from there on; in the
+// backward the gate alone carries the gradient to earlier steps).  Below |c| = 1/8, where 1 - f cancels, the series
+// c - c^3/3 + 2 c^5/15 (next term 17/315 c^7: 2e-7 of c at most).
+template <bool TANH, bool APART>
+__device__ __forceinline__ Gates gates(float2 x, float2 c, const Constants& k) {
   Gates g;
-  const float2 one = both(1.f);
-  const float2 e = power2(x, -LOG2E);
-  float2 d = add2(one, e);
+  const float2 e = power2(x, k.to_e);
+  const float2 d = add2(k.one, e);
   if (TANH) {
-    const float2 f = power2(c, -2.f * LOG2E);
-    float2 q = add2(one, f);
-    d = make_float2(fminf(d.x, MOST), fminf(d.y, MOST));
-    q = make_float2(fminf(q.x, MOST), fminf(q.y, MOST));
+    const float2 f = power2(c, k.to_2c);
+    float2 q = add2(k.one, f);
+    if (APART) {
+      constexpr float MOST = 2305843009213693952.f;          // 2^61, above any 1 + f
+      q = make_float2(fminf(q.x, MOST), fminf(q.y, MOST));
+    }
     const float2 p = mul2(d, q);
     const float2 r = make_float2(rcp_approx(p.x), rcp_approx(p.y));
     g.open = mul2(r, q);
     q = mul2(r, d);
-    const float2 far = mul2(fma2(f, both(-1.f), one), q);
+    const float2 far = mul2(sub2(k.one, f), q);
     const float2 c2 = mul2(c, c);
-    const float2 near0 = fma2(mul2(fma2(c2, both(2.f / 15.f), both(-1.f / 3.f)), c2), c, c);
+    const float2 near0 = fma2(mul2(fma2(c2, k.fifth, k.cubic), c2), c, c);
     g.n = make_float2(fabsf(c.x) < 0.125f ? near0.x : far.x, fabsf(c.y) < 0.125f ? near0.y : far.y);
-    g.slope = mul2(mul2(mul2(f, q), q), both(4.f));
+    const float2 fq = mul2(mul2(f, q), q);
+    g.slope = make_float2(4.f * fq.x, 4.f * fq.y);
   } else {
     g.open = make_float2(rcp_approx(d.x), rcp_approx(d.y));
     g.n = c;
-    g.slope = one;
+    g.slope = k.one;
   }
   g.keep = mul2(e, g.open);
-  g.z = fma2(g.keep, both(-1.f), one);
+  g.z = sub2(k.one, g.keep);
   return g;
 }
 
