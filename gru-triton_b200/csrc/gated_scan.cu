@@ -40,9 +40,12 @@ template <> struct Pair<float> { typedef float2 type; };
 template <> struct Pair<__nv_bfloat16> { typedef __nv_bfloat162 type; };
 template <> struct Pair<__half> { typedef __half2 type; };
 
-__device__ __forceinline__ float2 unpack(float2 v) { return v; }
-__device__ __forceinline__ float2 unpack(__nv_bfloat162 v) { return __bfloat1622float2(v); }
-__device__ __forceinline__ float2 unpack(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ P2 unpack(float2 v) { return pair(v.x, v.y); }
+__device__ __forceinline__ P2 unpack(__nv_bfloat162 v) {        // a bf16 is the upper half of an fp32
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(&v);
+  return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ P2 unpack(__half2 v) { return unpack(__half22float2(v)); }
 template <typename T> __device__ __forceinline__ typename Pair<T>::type pack(float2 v);
 template <> __device__ __forceinline__ float2 pack<float>(float2 v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat162 pack<__nv_bfloat16>(float2 v) { return __float22bfloat162_rn(v); }
@@ -50,12 +53,13 @@ template <> __device__ __forceinline__ __half2 pack<__half>(float2 v) { return _
 
 // The lane's two units of a row that starts at p (unit 0 of the CTA); `left`: units of the row from there on.
 template <bool FAST, int LANES, typename T>
-__device__ __forceinline__ float2 load_units(const T* p, int lane, int left) {
+__device__ __forceinline__ P2 load_units(const T* p, int lane, int left) {
   if (FAST) return 2 * lane < left ? unpack(*reinterpret_cast<const typename Pair<T>::type*>(p + 2 * lane)) : both(0.f);
-  return make_float2(lane < left ? to_float(p[lane]) : 0.f, lane + LANES < left ? to_float(p[lane + LANES]) : 0.f);
+  return pair(lane < left ? to_float(p[lane]) : 0.f, lane + LANES < left ? to_float(p[lane + LANES]) : 0.f);
 }
 template <bool FAST, int LANES, typename T>
-__device__ __forceinline__ void store_units(T* p, int lane, int left, float2 v) {
+__device__ __forceinline__ void store_units(T* p, int lane, int left, P2 pv) {
+  const float2 v = split(pv);
   if (FAST) {
     if (2 * lane < left) *reinterpret_cast<typename Pair<T>::type*>(p + 2 * lane) = pack<T>(v);
   } else {
@@ -66,25 +70,25 @@ __device__ __forceinline__ void store_units(T* p, int lane, int left, float2 v) 
 
 // fp32 states of the lane's units; rows of any alignment.
 template <bool FAST, int LANES>
-__device__ __forceinline__ float2 load_state(const float* p, int lane, int left) {
+__device__ __forceinline__ P2 load_state(const float* p, int lane, int left) {
   const int i = FAST ? 2 * lane : lane, j = FAST ? 2 * lane + 1 : lane + LANES;
-  return make_float2(i < left ? p[i] : 0.f, j < left ? p[j] : 0.f);
+  return pair(i < left ? p[i] : 0.f, j < left ? p[j] : 0.f);
 }
 template <bool FAST, int LANES>
-__device__ __forceinline__ void store_state(float* p, int lane, int left, float2 v) {
+__device__ __forceinline__ void store_state(float* p, int lane, int left, P2 pv) {
+  const float2 v = split(pv);
   const int i = FAST ? 2 * lane : lane, j = FAST ? 2 * lane + 1 : lane + LANES;
   if (i < left) p[i] = v.x;
   if (j < left) p[j] = v.y;
 }
 
-// The map `m` after the map `first`, each (A, A, b, b).
-__device__ __forceinline__ float4 after(float4 m, float4 first) {
-  const float2 A = make_float2(m.x, m.y);
-  const float2 p = mul2(A, make_float2(first.x, first.y));
-  const float2 b = fma2(A, make_float2(first.z, first.w), make_float2(m.z, m.w));
-  return make_float4(p.x, p.y, b.x, b.y);
-}
-__device__ __forceinline__ float2 apply(float4 m, float2 h) { return fma2(make_float2(m.x, m.y), h, make_float2(m.z, m.w)); }
+// A map of two units as it lies in shared memory: 16 bytes.
+struct __align__(16) Map {
+  P2 A, b;
+};
+// The map `m` after the map `first`.
+__device__ __forceinline__ Map after(const Map& m, const Map& first) { return {mul2(m.A, first.A), fma2(m.A, first.b, m.b)}; }
+__device__ __forceinline__ P2 apply(const Map& m, P2 h) { return fma2(m.A, h, m.b); }
 
 // ---- cluster exchange ----------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -102,23 +106,22 @@ __device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
   return r;
 }
 // 16 bytes into a peer's shared memory, counted on a barrier of the peer.
-__device__ __forceinline__ void send16(uint32_t dst, float4 v, uint32_t bar) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
-               ::"r"(dst), "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)),
-                 "r"(__float_as_uint(v.w)), "r"(bar) : "memory");
+__device__ __forceinline__ void send16(uint32_t dst, const Map& m, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];"
+               ::"r"(dst), "l"(m.A.v), "l"(m.b.v), "r"(bar) : "memory");
 }
 
 template <int LANES>
 struct Shared {
-  float4 part[2][Tile<LANES>::PARTS][LANES];   // maps of the threads: (A, A, b, b) of two units
-  float2 carry[2][LANES];                      // what enters the round
+  Map part[2][Tile<LANES>::PARTS][LANES];      // maps of the threads
+  P2 carry[2][LANES];                          // what enters the round
   unsigned long long full[STAGES_MAX];       // a stage of inputs has landed
   unsigned long long joined[2];              // maps of all ranks have landed
   int dead;
 };
 // Behind the ring of inputs in dynamic shared memory: maps of the cluster's tiles, [2][ranks][LANES].
 template <int LANES>
-__host__ __device__ constexpr size_t peer_bytes(int ranks) { return ranks > 1 ? (size_t)2 * ranks * LANES * sizeof(float4) : 0; }
+__host__ __device__ constexpr size_t peer_bytes(int ranks) { return ranks > 1 ? (size_t)2 * ranks * LANES * sizeof(Map) : 0; }
 
 // Where a CTA is: its row, first unit, and its rank among the CTAs that share them.
 struct Place {
@@ -145,7 +148,7 @@ __device__ __forceinline__ void set_up(Shared<LANES>& s, int stages, int ranks) 
     for (int i = 0; i < 2; ++i) tc::mbar_init(tc::smem_u32(&s.joined[i]), 1);
     tc::mbar_fence_init();
     if (ranks > 1)
-      for (int i = 0; i < 2; ++i) tc::mbar_expect_tx(tc::smem_u32(&s.joined[i]), (uint32_t)(ranks * LANES * sizeof(float4)));
+      for (int i = 0; i < 2; ++i) tc::mbar_expect_tx(tc::smem_u32(&s.joined[i]), (uint32_t)(ranks * LANES * sizeof(Map)));
   }
   __syncthreads();
   if (ranks > 1) cluster_barrier();
@@ -154,7 +157,7 @@ __device__ __forceinline__ void set_up(Shared<LANES>& s, int stages, int ranks) 
 // One part of the threads (all of a CTA's units) sends the CTA's map to every rank.  A slot is used again two rounds later: a
 // peer sends its map of the round between only after all its threads have read this round's, so two slots are enough.
 template <int LANES>
-__device__ __forceinline__ void send_map(Shared<LANES>& s, float4* peers, const Place& w, int round, float4 all, int lane) {
+__device__ __forceinline__ void send_map(Shared<LANES>& s, Map* peers, const Place& w, int round, Map all, int lane) {
   const int slot = round & 1;
   const uint32_t to = tc::smem_u32(peers + (slot * w.ranks + w.rank) * LANES + lane), bar = tc::smem_u32(&s.joined[slot]);
   for (int r = 0; r < w.ranks; ++r) send16(at_rank(to, (uint32_t)r), all, at_rank(bar, (uint32_t)r));
@@ -162,20 +165,29 @@ __device__ __forceinline__ void send_map(Shared<LANES>& s, float4* peers, const 
 // What enters this CTA's tile: the round's carry through the maps of the ranks before it.  Part 1 folds on through all of
 // them, which is what the next round starts from.
 template <int LANES>
-__device__ __forceinline__ float2 join(Shared<LANES>& s, const float4* peers, const Place& w, int round, int part, int lane) {
+__device__ __forceinline__ P2 join(Shared<LANES>& s, const Map* peers, const Place& w, int round, int part, int lane) {
   const int slot = round & 1;
   tc::mbar_wait(tc::smem_u32(&s.joined[slot]), (uint32_t)(round >> 1) & 1u, &s.dead, &g_gated_status);
-  if (threadIdx.x == 0) tc::mbar_expect_tx(tc::smem_u32(&s.joined[slot]), (uint32_t)(w.ranks * LANES * sizeof(float4)));
-  const float4* m = peers + slot * w.ranks * LANES + lane;
-  float2 h = s.carry[slot][lane];
+  if (threadIdx.x == 0) tc::mbar_expect_tx(tc::smem_u32(&s.joined[slot]), (uint32_t)(w.ranks * LANES * sizeof(Map)));
+  const Map* m = peers + slot * w.ranks * LANES + lane;
+  P2 h = s.carry[slot][lane];
   for (int r = 0; r < w.rank; ++r) h = apply(m[r * LANES], h);
   if (part == 1) {
-    float2 end = h;
+    P2 end = h;
     for (int r = w.rank; r < w.ranks; ++r) end = apply(m[r * LANES], end);
     s.carry[slot ^ 1][lane] = end;
   }
   return h;
 }
+
+// Stage of the ring and the phase of its barrier, moved on once a round (a division of the round would cost as much as eight
+// elements).
+struct Ring {
+  int stage, phase;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) { stage = 0; phase ^= 1; }
+  }
+};
 
 // Nobody leaves while a peer may still write here; a CTA that gave up waits for what is in flight.
 __device__ __forceinline__ void tear_down(const volatile int* dead, int ranks) {
@@ -198,7 +210,7 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
   extern __shared__ __align__(128) unsigned char raw[];
   __shared__ Shared<LANES> s;
   T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c][STEPS][UNITS]
-  float4* peers = reinterpret_cast<float4*>(raw + (size_t)stages * 2 * STEPS * UNITS * sizeof(T));
+  Map* peers = reinterpret_cast<Map*>(raw + (size_t)stages * 2 * STEPS * UNITS * sizeof(T));
   const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES;
   if (!CLUSTERED) ranks = 1;
   const Place w = place_of<UNITS>(a, ranks);
@@ -207,39 +219,41 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
   const int rounds = (tiles + ranks - 1) / ranks;
   set_up(s, stages, ranks);
 
-  auto fetch = [&](int round) {                               // one thread
+  auto fetch = [&](int round, int stage) {                    // one thread
     const int tile = round * ranks + w.rank;
     if (round >= rounds || tile >= tiles) return;
-    const uint32_t bar = tc::smem_u32(&s.full[round % stages]);
-    T* dst = ring + (size_t)(round % stages) * 2 * STEPS * UNITS;
+    const uint32_t bar = tc::smem_u32(&s.full[stage]);
+    T* dst = ring + (size_t)stage * 2 * STEPS * UNITS;
     tc::mbar_expect_tx(bar, 2 * STEPS * UNITS * sizeof(T));
     tc::tma_load_3d(tc::smem_u32(dst), &map, w.unit, w.b, tile * STEPS, bar);
     tc::tma_load_3d(tc::smem_u32(dst + STEPS * UNITS), &map, a.H + w.unit, w.b, tile * STEPS, bar);
   };
   if (FAST && threadIdx.x == 0)
-    for (int r = 0; r < stages; ++r) fetch(r);
+    for (int r = 0; r < stages; ++r) fetch(r, r);
 
   const T* gp = static_cast<const T*>(a.gi) + (long long)w.b * a.gi_b + w.unit;
   T* op = static_cast<T*>(a.out) + (long long)w.b * a.out_b + w.unit;
   if (part == 0) {
-    float2 h = both(0.f);
+    P2 h = both(0.f);
     if (a.h0 != nullptr) h = load_state<FAST, LANES>(a.h0 + (long long)w.b * a.h0_b + w.unit, lane, w.left);
     s.carry[0][lane] = h;
   }
   const Constants K = constants();
 
+  Ring at = {0, 0};
+
   // gates of a round into z and u, the thread's map into shared memory
-  auto open_gates = [&](int round, float2 (&z)[SEG], float2 (&u)[SEG]) {
+  auto open_gates = [&](int round, P2 (&z)[SEG], P2 (&u)[SEG]) {
     const int tile = round * ranks + w.rank;
     const int t0 = tile * STEPS + part * SEG;
     const int n = len - t0;                                   // steps left from here
-    float2 A = both(1.f), b = both(0.f);
+    P2 A = both(1.f), b = both(0.f);
     if (tile < tiles) {
-      if (FAST) tc::mbar_wait(tc::smem_u32(&s.full[round % stages]), (uint32_t)(round / stages) & 1u, &s.dead, &g_gated_status);
-      const T* st = ring + (size_t)(round % stages) * 2 * STEPS * UNITS + part * SEG * UNITS;
+      if (FAST) tc::mbar_wait(tc::smem_u32(&s.full[at.stage]), (uint32_t)at.phase, &s.dead, &g_gated_status);
+      const T* st = ring + (size_t)at.stage * 2 * STEPS * UNITS + part * SEG * UNITS;
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
-        float2 x = both(0.f), c = x;
+        P2 x = both(0.f), c = x;
         if (FAST) {
           x = load_units<true, LANES>(st + k * UNITS, lane, UNITS);
           c = load_units<true, LANES>(st + (STEPS + k) * UNITS, lane, UNITS);
@@ -265,15 +279,15 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
         b = fma2(z[k], b, u[k]);
       }
     }
-    s.part[round & 1][part][lane] = make_float4(A.x, A.y, b.x, b.y);
+    s.part[round & 1][part][lane] = Map{A, b};
   };
   // results of a round from the state that enters its tile
-  auto walk = [&](int round, float2 h, const float2 (&z)[SEG], const float2 (&u)[SEG]) {
+  auto walk = [&](int round, P2 h, const P2 (&z)[SEG], const P2 (&u)[SEG]) {
     const int tile = round * ranks + w.rank;
     if (tile >= tiles) return;
     if (a.states != nullptr && part == 0)
       store_state<FAST, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left, h);
-    const float4* m = &s.part[round & 1][0][lane];
+    const Map* m = &s.part[round & 1][0][lane];
     for (int v = 0; v < part; ++v) h = apply(m[v * LANES], h);
     const int t0 = tile * STEPS + part * SEG, n = len - t0;
     T* o = op + (long long)t0 * a.out_t;
@@ -295,19 +309,20 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
   };
 
   if (CLUSTERED) {
-    auto round_of = [&](int round, const float2 (&z)[SEG], const float2 (&u)[SEG], float2 (&zn)[SEG], float2 (&un)[SEG]) {
+    auto round_of = [&](int round, const P2 (&z)[SEG], const P2 (&u)[SEG], P2 (&zn)[SEG], P2 (&un)[SEG]) {
       __syncthreads();                                        // the stage is read, the threads' maps are there
       if (part == 0) {
-        float4 all = s.part[round & 1][0][lane];
+        Map all = s.part[round & 1][0][lane];
 #pragma unroll
         for (int v = 1; v < PARTS; ++v) all = after(s.part[round & 1][v][lane], all);
         send_map(s, peers, w, round, all, lane);
       }
-      if (FAST && threadIdx.x == 0) fetch(round + stages);
+      if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
+      at.next(stages);
       if (round + 1 < rounds) open_gates(round + 1, zn, un);
       walk(round, join(s, peers, w, round, part, lane), z, u);
     };
-    float2 za[SEG], ua[SEG], zb[SEG], ub[SEG];
+    P2 za[SEG], ua[SEG], zb[SEG], ub[SEG];
     if (rounds > 0) open_gates(0, za, ua);
     for (int round = 0; round < rounds; round += 2) {
       round_of(round, za, ua, zb, ub);
@@ -315,10 +330,11 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
     }
   } else {
     for (int round = 0; round < rounds; ++round) {
-      float2 z[SEG], u[SEG];
+      P2 z[SEG], u[SEG];
       open_gates(round, z, u);
       __syncthreads();
-      if (FAST && threadIdx.x == 0) fetch(round + stages);
+      if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
+      at.next(stages);
       walk(round, s.carry[round & 1][lane], z, u);
     }
   }
@@ -342,9 +358,9 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
   constexpr int UNITS = Tile<LANES>::UNITS, PARTS = Tile<LANES>::PARTS, STEPS = Tile<LANES>::STEPS;
   extern __shared__ __align__(128) unsigned char raw[];
   __shared__ Shared<LANES> s;
-  __shared__ float2 front[2][PARTS][LANES];
+  __shared__ P2 front[2][PARTS][LANES];
   T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c, dout][STEPS][UNITS]
-  float4* peers = reinterpret_cast<float4*>(raw + (size_t)stages * 3 * STEPS * UNITS * sizeof(T));
+  Map* peers = reinterpret_cast<Map*>(raw + (size_t)stages * 3 * STEPS * UNITS * sizeof(T));
   const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES;
   if (!CLUSTERED) ranks = 1;
   const Place w = place_of<UNITS>(a, ranks);
@@ -354,53 +370,54 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
   const bool with_dout = a.dout != nullptr;
   set_up(s, stages, ranks);
 
-  auto fetch = [&](int round) {                               // one thread
+  auto fetch = [&](int round, int stage) {                    // one thread
     const int tile = tiles - 1 - (round * ranks + w.rank);
     if (round >= rounds || tile < 0) return;
-    const uint32_t bar = tc::smem_u32(&s.full[round % stages]);
-    T* dst = ring + (size_t)(round % stages) * 3 * STEPS * UNITS;
+    const uint32_t bar = tc::smem_u32(&s.full[stage]);
+    T* dst = ring + (size_t)stage * 3 * STEPS * UNITS;
     tc::mbar_expect_tx(bar, (with_dout ? 3 : 2) * STEPS * UNITS * sizeof(T));
     tc::tma_load_3d(tc::smem_u32(dst), &map, w.unit, w.b, tile * STEPS, bar);
     tc::tma_load_3d(tc::smem_u32(dst + STEPS * UNITS), &map, a.H + w.unit, w.b, tile * STEPS, bar);
     if (with_dout) tc::tma_load_3d(tc::smem_u32(dst + 2 * STEPS * UNITS), &dmap, w.unit, w.b, tile * STEPS, bar);
   };
   if (FAST && threadIdx.x == 0)
-    for (int r = 0; r < stages; ++r) fetch(r);
+    for (int r = 0; r < stages; ++r) fetch(r, r);
 
   const T* gp = static_cast<const T*>(a.gi) + (long long)w.b * a.gi_b + w.unit;
   const T* dp = with_dout ? static_cast<const T*>(a.dout) + (long long)w.b * a.dout_b + w.unit : nullptr;
   T* qp = static_cast<T*>(a.dgi) + (long long)w.b * a.dgi_b + w.unit;
   if (part == 0) {
-    float2 G = both(0.f);
+    P2 G = both(0.f);
     if (a.dh_T != nullptr) G = load_state<FAST, LANES>(a.dh_T + (long long)w.b * a.dh_b + w.unit, lane, w.left);
     s.carry[0][lane] = G;
   }
   const Constants K = constants();
 
+  Ring at = {0, 0};
   for (int round = 0; round < rounds; ++round) {
     const int tile = tiles - 1 - (round * ranks + w.rank);
     const int t0 = tile * STEPS + part * SEG;
     const int n = len - t0;                                   // steps left from here
-    float2 h = both(0.f);
-    float2 z[SEG], u[SEG], p[SEG], q[SEG], d[SEG];            // p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'
-    float2 A = both(1.f), f = both(0.f), r = f;
-    float2 zk[SEG];
+    P2 h = both(0.f);
+    P2 z[SEG], u[SEG], p[SEG], q[SEG], d[SEG];            // p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'
+    P2 A = both(1.f), f = both(0.f), r = f;
+    P2 zk[SEG];
     if (tile >= 0) {
       h = load_state<FAST, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left);
-      if (FAST) tc::mbar_wait(tc::smem_u32(&s.full[round % stages]), (uint32_t)(round / stages) & 1u, &s.dead, &g_gated_status);
-      const T* st = ring + (size_t)(round % stages) * 3 * STEPS * UNITS + part * SEG * UNITS;
+      if (FAST) tc::mbar_wait(tc::smem_u32(&s.full[at.stage]), (uint32_t)at.phase, &s.dead, &g_gated_status);
+      const T* st = ring + (size_t)at.stage * 3 * STEPS * UNITS + part * SEG * UNITS;
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
-        float2 x = both(0.f), c = x;
+        P2 x = both(0.f), c = x;
         d[k] = x;
         if (FAST) {
           x = load_units<true, LANES>(st + k * UNITS, lane, UNITS);
           c = load_units<true, LANES>(st + (STEPS + k) * UNITS, lane, UNITS);
           if (with_dout) d[k] = load_units<true, LANES>(st + (2 * STEPS + k) * UNITS, lane, UNITS);
         } else if (k < n) {
-          const T* at = gp + (long long)(t0 + k) * a.gi_t;
-          x = load_units<false, LANES>(at, lane, w.left);
-          c = load_units<false, LANES>(at + a.H, lane, w.left);
+          const T* row = gp + (long long)(t0 + k) * a.gi_t;
+          x = load_units<false, LANES>(row, lane, w.left);
+          c = load_units<false, LANES>(row + a.H, lane, w.left);
           if (with_dout) d[k] = load_units<false, LANES>(dp + (long long)(t0 + k) * a.dout_t, lane, w.left);
         }
         const Gates g = gates<TANH, true>(x, c, K);
@@ -424,18 +441,19 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
       for (int k = SEG - 1; k >= 0; --k) r = mul2(z[k], add2(d[k], r));
     }
     const int slot = round & 1;
-    s.part[slot][part][lane] = make_float4(A.x, A.y, r.x, r.y);
+    s.part[slot][part][lane] = Map{A, r};
     front[slot][part][lane] = f;
     __syncthreads();
-    const float4* m = &s.part[slot][0][lane];
+    const Map* m = &s.part[slot][0][lane];
     if (CLUSTERED && part == 0) {
-      float4 all = m[(PARTS - 1) * LANES];
+      Map all = m[(PARTS - 1) * LANES];
 #pragma unroll
       for (int v = PARTS - 2; v >= 0; --v) all = after(m[v * LANES], all);
       send_map(s, peers, w, round, all, lane);
     }
-    if (FAST && threadIdx.x == 0) fetch(round + stages);
-    for (int v = 0; v < part; ++v) h = fma2(make_float2(m[v * LANES].x, m[v * LANES].y), h, front[slot][v][lane]);
+    if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
+    at.next(stages);
+    for (int v = 0; v < part; ++v) h = fma2(m[v * LANES].A, h, front[slot][v][lane]);
     if (tile >= 0) {
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
@@ -443,13 +461,13 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         h = fma2(z[k], h, u[k]);
       }
     }
-    float2 G = CLUSTERED ? join(s, peers, w, round, part, lane) : s.carry[slot][lane];
+    P2 G = CLUSTERED ? join(s, peers, w, round, part, lane) : s.carry[slot][lane];
     if (tile >= 0) {
       for (int v = PARTS - 1; v > part; --v) G = apply(m[v * LANES], G);
       T* o = qp + (long long)t0 * a.dgi_t;
 #pragma unroll
       for (int k = SEG - 1; k >= 0; --k) {
-        const float2 g = add2(G, d[k]);
+        const P2 g = add2(G, d[k]);
         G = mul2(z[k], g);
         if (k < n) {
           store_units<FAST, LANES>(o + (long long)k * a.dgi_t, lane, w.left, mul2(g, p[k]));
@@ -481,11 +499,11 @@ __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
   const int len = row_length(a, b);
   const T* gp = static_cast<const T*>(a.gi) + (long long)b * a.gi_b + unit;
   T* op = static_cast<T*>(a.out) + (long long)b * a.out_b + unit;
-  float2 h = both(0.f);
+  P2 h = both(0.f);
   if (a.h0 != nullptr) h = load_state<FAST, 32>(a.h0 + (long long)b * a.h0_b + unit, lane, left);
   if (a.states != nullptr) store_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left, h);
   const Constants K = constants();
-  float2 x[SEG], c[SEG];
+  P2 x[SEG], c[SEG];
 #pragma unroll
   for (int k = 0; k < SEG; ++k)
     if (k < len) {
@@ -495,7 +513,7 @@ __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
 #pragma unroll
   for (int k = 0; k < SEG; ++k)
     if (k < a.T) {
-      float2 o = both(0.f);
+      P2 o = both(0.f);
       if (k < len) {
         const Gates g = gates<TANH, false>(x[k], c[k], K);
         h = fma2(g.z, h, mul2(g.keep, g.n));
@@ -516,17 +534,17 @@ __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
   const T* gp = static_cast<const T*>(a.gi) + (long long)b * a.gi_b + unit;
   const T* dp = a.dout != nullptr ? static_cast<const T*>(a.dout) + (long long)b * a.dout_b + unit : nullptr;
   T* qp = static_cast<T*>(a.dgi) + (long long)b * a.dgi_b + unit;
-  float2 G = both(0.f);
+  P2 G = both(0.f);
   if (a.dh_T != nullptr) G = load_state<FAST, 32>(a.dh_T + (long long)b * a.dh_b + unit, lane, left);
-  float2 h = load_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left);
+  P2 h = load_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left);
   const Constants K = constants();
-  float2 z[SEG], p[SEG], q[SEG], d[SEG];
+  P2 z[SEG], p[SEG], q[SEG], d[SEG];
 #pragma unroll
   for (int k = 0; k < SEG; ++k) {
     d[k] = both(0.f);
     if (k < len) {
-      const float2 x = load_units<FAST, 32>(gp + (long long)k * a.gi_t, lane, left);
-      const float2 c = load_units<FAST, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
+      const P2 x = load_units<FAST, 32>(gp + (long long)k * a.gi_t, lane, left);
+      const P2 c = load_units<FAST, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
       if (dp != nullptr) d[k] = load_units<FAST, 32>(dp + (long long)k * a.dout_t, lane, left);
       const Gates g = gates<TANH, true>(x, c, K);
       z[k] = g.z;
@@ -538,9 +556,9 @@ __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
 #pragma unroll
   for (int k = SEG - 1; k >= 0; --k)
     if (k < a.T) {
-      float2 dx = both(0.f), dc = dx;
+      P2 dx = both(0.f), dc = dx;
       if (k < len) {
-        const float2 g = add2(G, d[k]);
+        const P2 g = add2(G, d[k]);
         G = mul2(z[k], g);
         dx = mul2(g, p[k]);
         dc = mul2(g, q[k]);
@@ -558,8 +576,8 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const StepArgs a) {
   if (i >= (long long)a.B * columns) return;
   const int b = (int)(i / columns), unit = (int)(i % columns) * 64, left = a.H - unit;
   const T* gp = static_cast<const T*>(a.gi) + (long long)b * a.gi_b + unit;
-  const float2 x = load_units<FAST, 32>(gp, lane, left), c = load_units<FAST, 32>(gp + a.H, lane, left);
-  float2 h = load_state<FAST, 32>(a.h + (long long)b * a.h_b + unit, lane, left);
+  const P2 x = load_units<FAST, 32>(gp, lane, left), c = load_units<FAST, 32>(gp + a.H, lane, left);
+  P2 h = load_state<FAST, 32>(a.h + (long long)b * a.h_b + unit, lane, left);
   const Gates g = gates<TANH, false>(x, c, constants());
   h = fma2(g.z, h, mul2(g.keep, g.n));
   store_state<FAST, 32>(a.h_new + (long long)b * a.hn_b + unit, lane, left, h);
@@ -656,7 +674,7 @@ int backward_tiles(const Args& a, cudaStream_t st) {
       (a.dout == nullptr || (tileable<T>(a.dout, a.dout_t, a.dout_b, a.B) &&
                              tile_map<T, LANES>(&dmap, a.dout, a.H, a, a.dout_t, a.dout_b) == B200GRU_OK))) {
     const size_t stage = (size_t)3 * Tile<LANES>::STEPS * Tile<LANES>::UNITS * sizeof(T);
-    const size_t fixed = sizeof(Shared<LANES>) + 2 * THREADS * sizeof(float2);
+    const size_t fixed = sizeof(Shared<LANES>) + 2 * THREADS * sizeof(P2);
     const int stages = stages_for<LANES>(stage, fixed, ranks, 2);
     return ranks > 1 ? launch_tiles(gated_bwd_kernel<T, LANES, true, TANH, true>, blocks, ranks, stages * stage + peers, st, map, dmap, a, ranks, stages)
                      : launch_tiles(gated_bwd_kernel<T, LANES, true, TANH, false>, blocks, 1, stages * stage, st, map, dmap, a, 1, stages);

@@ -52,32 +52,42 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
 // ---- two units at a time: the packed fp32 instructions of sm_100 --------------------------------------
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+// Both values in one 64-bit register, as the instructions take them.  (As a pair of floats, put together for each
+// instruction, the compiler spent ten moves beside 60 instructions of a pair.)
+struct P2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ P2 pair(float x, float y) {
+  P2 p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float2 split(P2 p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+  return f;
+}
+__device__ __forceinline__ P2 fma2(P2 a, P2 b, P2 c) {
+  P2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return d;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ P2 mul2(P2 a, P2 b) {
+  P2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
   return d;
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ P2 add2(P2 a, P2 b) {
+  P2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
   return d;
 }
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tsub.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ P2 sub2(P2 a, P2 b) {
+  P2 d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
   return d;
 }
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ P2 both(float v) { return pair(v, v); }
 __device__ __forceinline__ float exp2_approx(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -97,12 +107,12 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 // The constants of the packed instructions, which take registers alone.  Behind a volatile move they stay in theirs; the
 // compiler would otherwise build each pair anew at each use, seven moves beside the 24 instructions of an element.
 struct Constants {
-  float2 one, to_e, to_2c, cubic, fifth;
+  P2 one, to_e, to_2c, cubic, fifth;
 };
-__device__ __forceinline__ float2 pinned(float v) {
-  float2 d;
-  asm volatile("mov.b32 %0, %2;\n\tmov.b32 %1, %2;" : "=f"(d.x), "=f"(d.y) : "f"(v));
-  return d;
+__device__ __forceinline__ P2 pinned(float v) {
+  P2 p;
+  asm volatile("mov.b64 %0, {%1, %1};" : "=l"(p.v) : "f"(v));
+  return p;
 }
 __device__ __forceinline__ Constants constants() {
   constexpr float LOG2E = 1.44269504f;
@@ -110,15 +120,19 @@ __device__ __forceinline__ Constants constants() {
 }
 
 // 2^(v * scale), at most 2^60.
-__device__ __forceinline__ float2 power2(float2 v, float2 scale) {
-  const float2 t = mul2(v, scale);
-  return make_float2(exp2_approx(min_nan(t.x, 60.f)), exp2_approx(min_nan(t.y, 60.f)));
+__device__ __forceinline__ P2 power2(P2 v, P2 scale) {
+  const float2 t = split(mul2(v, scale));
+  return pair(exp2_approx(min_nan(t.x, 60.f)), exp2_approx(min_nan(t.y, 60.f)));
+}
+__device__ __forceinline__ P2 reciprocal2(P2 v) {
+  const float2 f = split(v);
+  return pair(rcp_approx(f.x), rcp_approx(f.y));
 }
 
 // Gates of two units.  z = 1 - keep, so that the two add to one to a rounding and a state that holds for hundreds of steps
 // does not drift; `open` is the same gate to full relative precision, where its size matters (its slope).
 struct Gates {
-  float2 z, open, keep, n, slope;
+  P2 z, open, keep, n, slope;
 };
 
 // With e = exp(-x) and f = exp(-2c):  open = 1 / (1 + e), keep = e open, tanh c = (1 - f) / (1 + f), dn/dc = 4 f / (1 + f)^2.
@@ -127,29 +141,28 @@ struct Gates {
 // backward the gate alone carries the gradient to earlier steps).  Below |c| = 1/8, where 1 - f cancels, the series
 // c - c^3/3 + 2 c^5/15 (next term 17/315 c^7: 2e-7 of c at most).
 template <bool TANH, bool APART>
-__device__ __forceinline__ Gates gates(float2 x, float2 c, const Constants& k) {
+__device__ __forceinline__ Gates gates(P2 x, P2 c, const Constants& k) {
   Gates g;
-  const float2 e = power2(x, k.to_e);
-  const float2 d = add2(k.one, e);
+  const P2 e = power2(x, k.to_e);
+  const P2 d = add2(k.one, e);
   if (TANH) {
-    const float2 f = power2(c, k.to_2c);
-    float2 q = add2(k.one, f);
+    const P2 f = power2(c, k.to_2c);
+    P2 q = add2(k.one, f);
     if (APART) {
       constexpr float MOST = 2305843009213693952.f;          // 2^61, above any 1 + f
-      q = make_float2(fminf(q.x, MOST), fminf(q.y, MOST));
+      const float2 s = split(q);
+      q = pair(fminf(s.x, MOST), fminf(s.y, MOST));
     }
-    const float2 p = mul2(d, q);
-    const float2 r = make_float2(rcp_approx(p.x), rcp_approx(p.y));
+    const P2 r = reciprocal2(mul2(d, q));
     g.open = mul2(r, q);
     q = mul2(r, d);
-    const float2 far = mul2(sub2(k.one, f), q);
-    const float2 c2 = mul2(c, c);
-    const float2 near0 = fma2(mul2(fma2(c2, k.fifth, k.cubic), c2), c, c);
-    g.n = make_float2(fabsf(c.x) < 0.125f ? near0.x : far.x, fabsf(c.y) < 0.125f ? near0.y : far.y);
-    const float2 fq = mul2(mul2(f, q), q);
-    g.slope = make_float2(4.f * fq.x, 4.f * fq.y);
+    const P2 c2 = mul2(c, c);
+    const float2 far = split(mul2(sub2(k.one, f), q)), near0 = split(fma2(mul2(fma2(c2, k.fifth, k.cubic), c2), c, c)), at = split(c);
+    g.n = pair(fabsf(at.x) < 0.125f ? near0.x : far.x, fabsf(at.y) < 0.125f ? near0.y : far.y);
+    const P2 fq = mul2(mul2(f, q), q), twice = add2(fq, fq);
+    g.slope = add2(twice, twice);
   } else {
-    g.open = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    g.open = reciprocal2(d);
     g.n = c;
     g.slope = k.one;
   }
