@@ -21,7 +21,8 @@ LIB_PATH = os.path.join(LIB_DIR, os.environ.get("B200GRU_LIB_NAME", "libb200gru.
 
 SOURCES = ["api.cu", "diag_scan.cu", "block_scan.cu", "block_gemm.cu", "butterfly_scan.cu", "butterfly_scan2.cu",
            "tc_gemm.cu", "tc_gemm2.cu", "tc_cluster.cu", "tc_step.cu", "tc_scan.cu", "weight_prep.cu", "tc_api.cu", "calib_scan.cu", "layer.cu",
-           "gated_scan.cu", "linear_act.cu"]
+           "gated_scan.cu", "linear_act.cu", "linear_gemm_f32.cu", "linear_gemm_bf16.cu", "linear_gemm_f16.cu",
+           "linear_gemm_partial.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

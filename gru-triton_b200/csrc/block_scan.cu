@@ -1061,8 +1061,9 @@ extern "C" int b200gru_device_status(int reset) {
   const int c = tcc::read_status(reset);
   const int g2 = tc::tc2_read_status(reset);
   const int g3 = gated::read_status(reset);
-  if (d < 0 || f < 0 || g < 0 || s < 0 || c < 0 || g2 < 0 || g3 < 0) return -1;
-  return (v != 0 || d != 0 || f != 0 || g != 0 || s != 0 || c != 0 || g2 != 0 || g3 != 0) ? 1 : 0;
+  const int l = lin::read_status(reset);
+  if (d < 0 || f < 0 || g < 0 || s < 0 || c < 0 || g2 < 0 || g3 < 0 || l < 0) return -1;
+  return (v != 0 || d != 0 || f != 0 || g != 0 || s != 0 || c != 0 || g2 != 0 || g3 != 0 || l != 0) ? 1 : 0;
 }
 
 }  // namespace b200gru

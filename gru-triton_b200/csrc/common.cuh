@@ -183,6 +183,9 @@ int tc2_read_status(int reset);      // CTA-pair products (tc_gemm2.cu)
 namespace gated {
 int read_status(int reset);          // gated linear recurrence (gated_scan.cu)
 }  // namespace gated
+namespace lin {
+int read_status(int reset);          // products with bias, activation and residual (linear_gemm.cuh)
+}  // namespace lin
 
 // Test hook (b200gru_test_select_kernels): slot 0 != 0 -> butterfly launches use the register /
 // global-twiddle kernels on every shape; slot 1 != 0 -> the diagonal forward uses the register-ring

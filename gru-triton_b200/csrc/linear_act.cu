@@ -1,124 +1,661 @@
 // y = act(x W^T + bias) + residual and its gradients.
 //
 //   d = dy * act'(pre)   dx = d W   dW = d^T x   db = sum over rows of d   (the residual's gradient is dy)
+//
+// Three products of one tensor-core kernel (linear_gemm.cuh); here: the operands' preparation, the joining of K slices, the
+// kernel for a few rows, and who runs when.
+//
+// fp32 operands become two fp16 planes scaled by powers of two.  A scale has to factor out of the sum, so it follows the index
+// that is not summed: forward, rows of x and rows of W; dx, rows of d (the scales of W's rows, which are summed here,
+// folded into d first); dW, columns of d (the scales of x's rows folded in first).  So x and W need one form each.
 
-#include "linear_act.cuh"
+#include "linear_gemm.cuh"
 
 namespace b200gru {
 namespace lin {
 
 namespace {
 
-constexpr int TILE = 64, DEPTH = 16, PAD = 4;
+inline long long pad8(long long n) { return (n + 7) / 8 * 8; }
 
-// C(m, n) = sum_k a(m, k) b(n, k) for operands given as functions; a 64 x 64 tile by 256 threads, 4 x 4 results each.
-template <typename LoadA, typename LoadB, typename Store>
-__device__ __forceinline__ void tile_product(int M, int N, int K, LoadA a, LoadB b, Store store) {
-  __shared__ float sa[DEPTH][TILE + PAD], sb[DEPTH][TILE + PAD];
-  const int m0 = blockIdx.y * TILE, n0 = blockIdx.x * TILE;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += DEPTH) {
-    for (int e = threadIdx.x; e < TILE * DEPTH; e += 256) {
-      const int r = e / DEPTH, k = e % DEPTH;
-      sa[k][r] = (m0 + r < M && k0 + k < K) ? a(m0 + r, k0 + k) : 0.f;
-      sb[k][r] = (n0 + r < N && k0 + k < K) ? b(n0 + r, k0 + k) : 0.f;
+// ---- operands ------------------------------------------------------------------------------------------
+// 16-bit rows that TMA cannot read where they lie (odd widths, bases or strides): copied to padded rows.
+__global__ void __launch_bounds__(256) pack_rows_kernel(const unsigned short* __restrict__ src, long long ld, unsigned short* __restrict__ dst,
+                                                        long long dld, int rows, int cols) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const unsigned short* s = src + (long long)row * ld;
+  unsigned short* d = dst + (long long)row * dld;
+  for (int c = lane; c < dld; c += 32) d[c] = c < cols ? s[c] : (unsigned short)0;
+}
+
+struct HiLo { __half hi, lo; };
+__device__ __forceinline__ HiLo hi_lo(float x) {
+  HiLo r;
+  r.hi = __float2half_rn(x);
+  r.lo = __float2half_rn(x - __half2float(r.hi));
+  return r;
+}
+
+// Four values of a row from column c on; zeros behind its end.
+template <bool VEC>
+__device__ __forceinline__ float4 four(const float* row, int c, int cols) {
+  if (VEC) return c < cols ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  return make_float4(c < cols ? row[c] : 0.f, c + 1 < cols ? row[c + 1] : 0.f, c + 2 < cols ? row[c + 2] : 0.f, c + 3 < cols ? row[c + 3] : 0.f);
+}
+__device__ __forceinline__ void store_planes(__half* d, long long plane, float4 v) {
+  const HiLo a = hi_lo(v.x), b = hi_lo(v.y), c = hi_lo(v.z), e = hi_lo(v.w);
+  __half h[4] = {a.hi, b.hi, c.hi, e.hi}, l[4] = {a.lo, b.lo, c.lo, e.lo};
+  *reinterpret_cast<uint2*>(d) = *reinterpret_cast<uint2*>(h);
+  *reinterpret_cast<uint2*>(d + plane) = *reinterpret_cast<uint2*>(l);
+}
+__device__ __forceinline__ float largest(float4 v, float m) {
+  return fmaxf(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), m);
+}
+__device__ __forceinline__ float4 times(float4 v, float s) { return make_float4(v.x * s, v.y * s, v.z * s, v.w * s); }
+__device__ __forceinline__ float4 times(float4 v, float4 s) { return make_float4(v.x * s.x, v.y * s.y, v.z * s.z, v.w * s.w); }
+
+// A row into two fp16 planes, scaled so that its largest element lies in [2^14, 2^15): 22 significant bits of all elements down
+// to 2^-17 of it.  One warp per row; the second read of the row comes from L1.
+template <bool VEC>
+__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, long long ld, __half* __restrict__ dst, long long dld,
+                                                         long long plane, int rows, int cols, float* __restrict__ inv) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const float* s = src + (long long)row * ld;
+  float mx = 0.f;
+#pragma unroll 4
+  for (int c = lane * 4; c < cols; c += 128) mx = largest(four<VEC>(s, c, cols), mx);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+  float scale, back;
+  pow2_row_scale(mx, &scale, &back);
+  if (lane == 0) inv[row] = back;
+  __half* d = dst + (long long)row * dld;
+#pragma unroll 4
+  for (int c = lane * 4; c < dld; c += 128) store_planes(d + c, plane, times(four<VEC>(s, c, cols), scale));
+}
+
+// ---- the gradient behind the activation ------------------------------------------------------------------
+// d = dy * slope; its column sums (one partial per row slice), and for fp32 the largest |d inv_x| of each column beside them.
+// A CTA has 64 x V columns and a slice of rows, four rows at a time.
+struct GradArgs {
+  int M, N;
+  const void* dy; long long lddy;
+  const void* slope; long long lds;
+  void* d; long long ldd;               // 16-bit types: d, rows padded with zeros; NULL: not wanted
+  const float* x_inv;                   // fp32: scales of x's rows
+  float* sums; float* tops;             // [slices][ldp]
+  long long ldp;
+  int rows_per_slice;
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void grad_values(const GradArgs& a, long long m, int n, float (&v)[Vec<T>::V]) {
+  constexpr int V = Vec<T>::V;
+  typedef typename SlopeOf<T>::type S;
+  const T* dy = static_cast<const T*>(a.dy) + m * a.lddy + n;
+  const S* sl = a.slope == nullptr ? nullptr : static_cast<const S*>(a.slope) + m * a.lds + n;
+  if (VEC) {
+    unpack16<T>(__ldg(reinterpret_cast<const uint4*>(dy)), v);
+    if (sl != nullptr) {
+      float s[V];
+      unpack16<S>(__ldg(reinterpret_cast<const uint4*>(sl)), s);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] *= s[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      v[e] = n + e < a.N ? to_float(dy[e]) : 0.f;
+      if (sl != nullptr && n + e < a.N) v[e] *= to_float(sl[e]);
+    }
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) grad_kernel(const GradArgs a) {
+  constexpr int V = Vec<T>::V;
+  __shared__ float red[3][64][V + 1];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int col = threadIdx.x & 63, grp = threadIdx.x >> 6;
+  const int n = (blockIdx.x * 64 + col) * V;
+  const int m1 = min(a.M, (int)(blockIdx.y + 1) * a.rows_per_slice);
+  float sum[V], top[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sum[e] = top[e] = 0.f;
+  if (n < a.N) {
+#pragma unroll 4
+    for (int m = blockIdx.y * a.rows_per_slice + grp; m < m1; m += 4) {
+      float v[V];
+      grad_values<T, VEC>(a, m, n, v);
+      const float back = a.x_inv != nullptr ? __ldg(a.x_inv + m) : 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        sum[e] += v[e];
+        top[e] = fmaxf(top[e], fabsf(v[e] * back));
+      }
+      if (a.d != nullptr) *reinterpret_cast<uint4*>(static_cast<T*>(a.d) + (long long)m * a.ldd + n) = pack16<T>(v);
+    }
+  }
+  for (int pass = 0; pass < (a.tops != nullptr ? 2 : 1); ++pass) {
+    float* out = pass == 0 ? a.sums : a.tops;
+    if (out == nullptr) continue;
+    __syncthreads();
+    if (grp > 0) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) red[grp - 1][col][e] = pass == 0 ? sum[e] : top[e];
     }
     __syncthreads();
+    if (grp == 0 && n < a.N) {
 #pragma unroll
-    for (int k = 0; k < DEPTH; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+      for (int e = 0; e < V; ++e) {
+        if (n + e >= a.N) continue;
+        const float r0 = red[0][col][e], r1 = red[1][col][e], r2 = red[2][col][e];
+        out[(long long)blockIdx.y * a.ldp + n + e] = pass == 0 ? ((sum[e] + r0) + r1) + r2 : fmaxf(fmaxf(top[e], r0), fmaxf(r1, r2));
+      }
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (m0 + ty * 4 + i < M && n0 + tx * 4 + j < N) store(m0 + ty * 4 + i, n0 + tx * 4 + j, acc[i][j]);
 }
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) linear_fwd_kernel(const b200gru_linear_args p) {
+// Joins the slices in order: db, and the scales of d's columns.  32 columns x 8 slices a CTA.
+template <typename T>
+__global__ void __launch_bounds__(256) grad_columns_kernel(const float* __restrict__ sums, const float* __restrict__ tops, int slices,
+                                                           long long ldp, int N, T* __restrict__ db, float* __restrict__ scale,
+                                                           float* __restrict__ back) {
+  __shared__ float rs[8][32], rt[8][32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int n = blockIdx.x * 32 + lane;
+  float s = 0.f, t = 0.f;
+  if (n < N) {
+#pragma unroll 4
+    for (int k = grp; k < slices; k += 8) {
+      if (sums != nullptr) s += sums[(long long)k * ldp + n];
+      if (tops != nullptr) t = fmaxf(t, tops[(long long)k * ldp + n]);
+    }
+  }
+  rs[grp][lane] = s;
+  rt[grp][lane] = t;
+  __syncthreads();
+  if (grp == 0 && n < N) {
+    for (int g = 1; g < 8; ++g) { s += rs[g][lane]; t = fmaxf(t, rt[g][lane]); }
+    if (db != nullptr) db[n] = from_float<T>(s);
+    if (tops != nullptr) pow2_row_scale(t, scale + n, back + n);
+  }
+}
+
+// fp32: d as two planes for dx (rows scaled, W's row scales folded in) and two for dW (columns scaled, x's row scales
+// folded in).  One warp per row.
+struct GradPlanesArgs {
+  GradArgs g;
+  const float* w_inv;
+  const float* col_scale;
+  __half* dx; float* dx_inv;            // NULL: not wanted
+  __half* dw;
+  long long ld, plane;
+};
+template <bool VEC>
+__global__ void __launch_bounds__(256) grad_planes_kernel(const GradPlanesArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= a.g.M) return;
+  auto value = [&](int c) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.g.N) grad_values<float, VEC>(a.g, row, c, v);
+    return make_float4(v[0], v[1], v[2], v[3]);
+  };
+  float scale = 1.f;
+  if (a.dx != nullptr) {
+    float mx = 0.f;
+#pragma unroll 4
+    for (int c = lane * 4; c < a.g.N; c += 128) mx = largest(times(value(c), four<false>(a.w_inv, c, a.g.N)), mx);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    float back;
+    pow2_row_scale(mx, &scale, &back);
+    if (lane == 0) a.dx_inv[row] = back;
+  }
+  const float x_inv = a.dw != nullptr ? __ldg(a.g.x_inv + row) : 0.f;
+#pragma unroll 2
+  for (int c = lane * 4; c < a.ld; c += 128) {
+    const float4 v = value(c);
+    const long long at = (long long)row * a.ld + c;
+    if (a.dx != nullptr) store_planes(a.dx + at, a.plane, times(times(v, four<false>(a.w_inv, c, a.g.N)), scale));
+    if (a.dw != nullptr) store_planes(a.dw + at, a.plane, times(times(v, x_inv), four<false>(a.col_scale, c, a.g.N)));
+  }
+}
+
+// ---- K slices ------------------------------------------------------------------------------------------
+// C = epilogue(sum of the slices, in their order).  Four columns a thread.
+struct FinishArgs {
+  int M, N, splits;
+  const float* partial; long long ldp, split_stride;
+  int activation, vec;
+  const void* bias;
+  const void* residual; long long ldr;
+  void* C; long long ldc;
+  void* slope; long long lds;
+};
+template <typename T> struct Four { T e[4]; };
+template <typename T> struct alignas(4 * sizeof(T)) Aligned { Four<T> f; };
+
+template <typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const FinishArgs a) {
+  typedef typename SlopeOf<T>::type S;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int quads = (int)(a.ldp / 4);
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)a.M * quads) return;
+  const int m = (int)(i / quads), n = (int)(i % quads) * 4;
+  const float* p = a.partial + (long long)m * a.ldp + n;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int z = 0; z < a.splits; ++z) {
+    const float4 f = __ldcs(reinterpret_cast<const float4*>(p + (long long)z * a.split_stride));
+    v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+  }
+  Four<T> y, r;
+  Four<S> sl;
+  const T* resp = static_cast<const T*>(a.residual) + (long long)m * a.ldr + n;
+  if (a.vec && a.residual != nullptr) r = reinterpret_cast<const Aligned<T>*>(resp)->f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (n + e < a.N) {
+      if (a.bias != nullptr) v[e] += to_float(static_cast<const T*>(a.bias)[n + e]);
+      if (a.activation != B200GRU_ACT_NONE) {
+        const Activated t = activate_as(a.activation, v[e]);
+        v[e] = t.y;
+        sl.e[e] = from_float<S>(t.slope);
+      }
+      if (a.residual != nullptr) v[e] += to_float(a.vec ? r.e[e] : resp[e]);
+    }
+    y.e[e] = from_float<T>(v[e]);
+  }
+  T* cp = static_cast<T*>(a.C) + (long long)m * a.ldc + n;
+  S* sp = static_cast<S*>(a.slope) + (long long)m * a.lds + n;
+  if (a.vec) {
+    reinterpret_cast<Aligned<T>*>(cp)->f = y;
+    if (a.slope != nullptr) reinterpret_cast<Aligned<S>*>(sp)->f = sl;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.N) {
+        cp[e] = y.e[e];
+        if (a.slope != nullptr) sp[e] = sl.e[e];
+      }
+  }
+}
+
+// ---- a few rows ----------------------------------------------------------------------------------------
+// Bound by one read of W.  A warp has NW rows of W and a slice of K; lanes take 16 bytes each, partial sums of the lanes are
+// added by a butterfly, those of the CTA's K slices in their order.  The assignment of k to lanes does not depend on alignment.
+constexpr int FEW = 8;
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void take(const T* p, int k, int K, float (&v)[Vec<T>::V]) {
+  constexpr int V = Vec<T>::V;
+  if (VEC) {
+    if (k < K) unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p + k)), v);
+    else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = k + e < K ? to_float(p[k + e]) : 0.f;
+  }
+}
+
+template <typename T, int MR, int NW, bool VEC>
+__global__ void __launch_bounds__(256) few_rows_kernel(const b200gru_linear_args p, int slices) {
+  constexpr int V = Vec<T>::V;
+  typedef typename SlopeOf<T>::type S;
+  __shared__ float part[8][MR * NW];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = 8 / slices, slice = warp % slices;
+  const int n0 = (blockIdx.x * groups + warp / slices) * NW;
+  const int m0 = blockIdx.y * MR;
   const T* x = static_cast<const T*>(p.x);
   const T* W = static_cast<const T*>(p.W);
-  tile_product(p.M, p.N, p.K, [&](int m, int k) { return to_float(x[(long long)m * p.ldx + k]); },
-               [&](int n, int k) { return to_float(W[(long long)n * p.ldw + k]); },
-               [&](int m, int n, float v) {
-                 if (p.bias != nullptr) v += to_float(static_cast<const T*>(p.bias)[n]);
-                 const Activated r = activate<ACT>(v);
-                 if (p.slope != nullptr)
-                   static_cast<typename SlopeOf<T>::type*>(p.slope)[(long long)m * p.lds + n] = from_float<typename SlopeOf<T>::type>(r.slope);
-                 float y = r.y;
-                 if (p.residual != nullptr) y += to_float(static_cast<const T*>(p.residual)[(long long)m * p.ldr + n]);
-                 static_cast<T*>(p.y)[(long long)m * p.ldy + n] = from_float<T>(y);
-               });
-}
-
-template <typename T>
-__device__ __forceinline__ float grad_at(const b200gru_linear_args& p, int m, int n) {
-  float d = to_float(static_cast<const T*>(p.dy)[(long long)m * p.lddy + n]);
-  if (p.slope != nullptr) d *= to_float(static_cast<const typename SlopeOf<T>::type*>(p.slope)[(long long)m * p.lds + n]);
-  return d;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) linear_dx_kernel(const b200gru_linear_args p) {
-  const T* W = static_cast<const T*>(p.W);
-  tile_product(p.M, p.K, p.N, [&](int m, int n) { return grad_at<T>(p, m, n); },
-               [&](int k, int n) { return to_float(W[(long long)n * p.ldw + k]); },
-               [&](int m, int k, float v) { static_cast<T*>(p.dx)[(long long)m * p.K + k] = from_float<T>(v); });
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) linear_dw_kernel(const b200gru_linear_args p) {
-  const T* x = static_cast<const T*>(p.x);
-  tile_product(p.N, p.K, p.M, [&](int n, int m) { return grad_at<T>(p, m, n); },
-               [&](int k, int m) { return to_float(x[(long long)m * p.ldx + k]); },
-               [&](int n, int k, float v) { static_cast<T*>(p.dW)[(long long)n * p.K + k] = from_float<T>(v); });
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) linear_db_kernel(const b200gru_linear_args p) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= p.N) return;
-  float s = 0.f;
-  for (int m = 0; m < p.M; ++m) s += grad_at<T>(p, m, n);
-  static_cast<T*>(p.db)[n] = from_float<T>(s);
-}
-
-template <typename T>
-int forward(const b200gru_linear_args& p, cudaStream_t st) {
-  const dim3 grid(cdiv(p.N, TILE), cdiv(p.M, TILE));
-  switch (p.activation) {
-    case B200GRU_ACT_NONE: linear_fwd_kernel<T, B200GRU_ACT_NONE><<<grid, 256, 0, st>>>(p); break;
-    case B200GRU_ACT_RELU: linear_fwd_kernel<T, B200GRU_ACT_RELU><<<grid, 256, 0, st>>>(p); break;
-    case B200GRU_ACT_SILU: linear_fwd_kernel<T, B200GRU_ACT_SILU><<<grid, 256, 0, st>>>(p); break;
-    case B200GRU_ACT_GELU: linear_fwd_kernel<T, B200GRU_ACT_GELU><<<grid, 256, 0, st>>>(p); break;
-    case B200GRU_ACT_SIGMOID: linear_fwd_kernel<T, B200GRU_ACT_SIGMOID><<<grid, 256, 0, st>>>(p); break;
-    case B200GRU_ACT_TANH: linear_fwd_kernel<T, B200GRU_ACT_TANH><<<grid, 256, 0, st>>>(p); break;
+  float acc[MR][NW];
+#pragma unroll
+  for (int i = 0; i < MR; ++i)
+#pragma unroll
+    for (int j = 0; j < NW; ++j) acc[i][j] = 0.f;
+  if (n0 < p.N) {
+#pragma unroll 2
+    for (int k = (slice * 32 + lane) * V; k < p.K; k += slices * 32 * V) {
+      float w[NW][V];
+#pragma unroll
+      for (int j = 0; j < NW; ++j) take<T, VEC>(W + (long long)min(n0 + j, p.N - 1) * p.ldw, k, p.K, w[j]);
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        float v[V];
+        take<T, VEC>(x + (long long)min(m0 + i, p.M - 1) * p.ldx, k, p.K, v);
+#pragma unroll
+        for (int j = 0; j < NW; ++j)
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[i][j] = fmaf(v[e], w[j][e], acc[i][j]);
+      }
+    }
   }
+  float mine = 0.f;                                       // result `lane` of the warp's MR x NW
+#pragma unroll
+  for (int i = 0; i < MR; ++i)
+#pragma unroll
+    for (int j = 0; j < NW; ++j) {
+      float s = acc[i][j];
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+      if (lane == i * NW + j) mine = s;
+    }
+  if (lane < MR * NW) part[warp][lane] = mine;
+  __syncthreads();
+  const int m = m0 + lane / NW, n = n0 + lane % NW;
+  if (slice != 0 || lane >= MR * NW || m >= p.M || n >= p.N) return;
+  float v = 0.f;
+  for (int k = 0; k < slices; ++k) v += part[warp + k][lane];
+  if (p.bias != nullptr) v += to_float(static_cast<const T*>(p.bias)[n]);
+  const Activated r = activate_as(p.activation, v);
+  if (p.slope != nullptr) static_cast<S*>(p.slope)[(long long)m * p.lds + n] = from_float<S>(r.slope);
+  v = r.y;
+  if (p.residual != nullptr) v += to_float(static_cast<const T*>(p.residual)[(long long)m * p.ldr + n]);
+  static_cast<T*>(p.y)[(long long)m * p.ldy + n] = from_float<T>(v);
+}
+
+template <typename T, int MR, int NW>
+int launch_few(const b200gru_linear_args& p, cudaStream_t st) {
+  const long long warps = cdiv(p.N, NW);
+  int slices = 1;                                         // K slices until every SM has a CTA, while a lane has work
+  while (slices < 8 && warps * slices < 8 * 148 && (long long)p.K > (long long)slices * 32 * Vec<T>::V) slices *= 2;
+  const dim3 grid((unsigned)((warps * slices + 7) / 8), (unsigned)cdiv(p.M, MR));
+  const bool vec = p.K % Vec<T>::V == 0 && on16(p.x, p.M > 1 ? p.ldx : 0, sizeof(T)) && on16(p.W, p.N > 1 ? p.ldw : 0, sizeof(T));
+  if (vec) few_rows_kernel<T, MR, NW, true><<<grid, 256, 0, st>>>(p, slices);
+  else few_rows_kernel<T, MR, NW, false><<<grid, 256, 0, st>>>(p, slices);
   note_launch();
-  return check_launch("linear_fwd_kernel");
+  return check_launch("few_rows_kernel");
+}
+template <typename T>
+int few_rows(const b200gru_linear_args& p, cudaStream_t st) {
+  if (p.M == 1) return launch_few<T, 1, 2>(p, st);
+  if (p.M == 2) return launch_few<T, 2, 2>(p, st);
+  if (p.M <= 4) return launch_few<T, 4, 2>(p, st);
+  return launch_few<T, 8, 2>(p, st);
 }
 
+// ---- who runs when ---------------------------------------------------------------------------------------
+// Hands out the workspace; without a base it only counts.
+struct Carver {
+  char* base;
+  size_t at;
+  template <typename T>
+  T* take(long long n) {
+    T* p = base == nullptr ? nullptr : reinterpret_cast<T*>(base + at);
+    at += align_up((size_t)n * sizeof(T), 256);
+    return p;
+  }
+};
+
+// A matrix as the product kernel reads it.
+struct Operand {
+  const void* p;
+  long long ld, plane;
+  float* inv;                  // fp32: what undoes the scale of a row
+};
+
 template <typename T>
-int backward(const b200gru_linear_args& p, cudaStream_t st) {
-  if (p.dx != nullptr) { linear_dx_kernel<T><<<dim3(cdiv(p.K, TILE), cdiv(p.M, TILE)), 256, 0, st>>>(p); note_launch(); }
-  if (p.dW != nullptr) { linear_dw_kernel<T><<<dim3(cdiv(p.K, TILE), cdiv(p.N, TILE)), 256, 0, st>>>(p); note_launch(); }
-  if (p.db != nullptr) { linear_db_kernel<T><<<cdiv(p.N, 256), 256, 0, st>>>(p); note_launch(); }
-  return check_launch("linear backward");
+struct Call {
+  const b200gru_linear_args& a;
+  Carver ws;
+  bool dry;                    // count the workspace only
+  cudaStream_t st;
+  int rc;
+
+  static constexpr bool F32 = std::is_same<T, float>::value;
+
+  void note(const char* what) {
+    note_launch();
+    if (rc == B200GRU_OK) rc = check_launch(what);
+  }
+
+  Operand operand(const void* src, long long ld, int rows, int cols) {
+    Operand o = {src, ld, 0, nullptr};
+    if (F32) {
+      o.ld = pad8(cols);
+      o.plane = (long long)rows * o.ld;
+      __half* d = ws.template take<__half>(2 * o.plane);
+      o.inv = ws.template take<float>(pad8(rows));
+      o.p = d;
+      if (!dry && rc == B200GRU_OK) {
+        const float* s = static_cast<const float*>(src);
+        const dim3 grid((unsigned)cdiv(rows, 8));
+        if (cols % 4 == 0 && on16(src, ld, 4)) launch_pdl(split_rows_kernel<true>, grid, dim3(256), 0, st, s, ld, d, o.ld, o.plane, rows, cols, o.inv);
+        else launch_pdl(split_rows_kernel<false>, grid, dim3(256), 0, st, s, ld, d, o.ld, o.plane, rows, cols, o.inv);
+        note("split_rows_kernel");
+      }
+      return o;
+    }
+    if (rows == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) { o.ld = pad8(cols); return o; }
+    if (ld >= cols && on16(src, ld, 2)) return o;
+    o.ld = pad8(cols);
+    unsigned short* d = ws.template take<unsigned short>((long long)rows * o.ld);
+    o.p = d;
+    if (!dry && rc == B200GRU_OK) {
+      launch_pdl(pack_rows_kernel, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, static_cast<const unsigned short*>(src), ld, d, o.ld, rows, cols);
+      note("pack_rows_kernel");
+    }
+    return o;
+  }
+
+  // The product of two operands, in K slices where that fills the GPU better.
+  void product(Gemm g) {
+    g.planes = F32 ? 2 : 1;
+    g.fp16 = F32 || std::is_same<T, __half>::value;
+    const Plan plan = plan_gemm(g.M, g.N, g.K, g.planes);
+    g.splits = plan.splits;
+    if (plan.splits == 1) {
+      if (!dry && rc == B200GRU_OK) rc = launch_gemm<T>(g, plan, st);
+      return;
+    }
+    FinishArgs f;
+    memset(&f, 0, sizeof(f));
+    f.M = g.M; f.N = g.N; f.splits = plan.splits;
+    g.ldp = f.ldp = pad8(g.N);
+    f.split_stride = (long long)g.M * g.ldp;
+    g.partial = ws.template take<float>(f.split_stride * plan.splits);
+    f.partial = g.partial;
+    f.activation = g.activation; f.bias = g.bias; f.residual = g.residual; f.ldr = g.ldr;
+    f.C = g.C; f.ldc = g.ldc; f.slope = g.slope; f.lds = g.lds;
+    f.vec = g.N % 4 == 0 && g.ldc % 4 == 0 && on16(g.C, 0, 1) && on16(g.slope, 0, 1) && g.lds % 4 == 0 && (g.residual == nullptr || (g.ldr % 4 == 0 && on16(g.residual, 0, 1)));
+    if (dry || rc != B200GRU_OK) return;
+    rc = launch_gemm<void>(g, plan, st);
+    if (rc != B200GRU_OK) return;
+    const long long quads = (long long)g.M * (g.ldp / 4);
+    launch_pdl(finish_kernel<T>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, f);
+    note("finish_kernel");
+  }
+
+  int forward() {
+    if (a.M <= FEW) {
+      if (!dry) rc = few_rows<T>(a, st);
+      return rc;
+    }
+    const Operand x = operand(a.x, a.ldx, a.M, a.K), W = operand(a.W, a.ldw, a.N, a.K);
+    Gemm g;
+    memset(&g, 0, sizeof(g));
+    g.M = a.M; g.N = a.N; g.K = a.K;
+    g.A = x.p; g.lda = x.ld; g.a_plane = x.plane; g.row_scale = x.inv;
+    g.B = W.p; g.ldb = W.ld; g.b_plane = W.plane; g.col_scale = W.inv;
+    g.activation = a.activation; g.bias = a.bias; g.residual = a.residual; g.ldr = a.ldr;
+    g.C = a.y; g.ldc = a.ldy; g.slope = a.slope; g.lds = a.lds;
+    product(g);
+    return rc;
+  }
+
+  int backward() {
+    const bool act = a.activation != B200GRU_ACT_NONE;
+    Operand x = {}, W = {}, dx = {}, dw = {};
+    if (a.dW != nullptr) x = operand(a.x, a.ldx, a.M, a.K);
+    if (a.dx != nullptr) W = operand(a.W, a.ldw, a.N, a.K);
+
+    GradArgs g;
+    memset(&g, 0, sizeof(g));
+    g.M = a.M; g.N = a.N; g.dy = a.dy; g.lddy = a.lddy; g.slope = act ? a.slope : nullptr; g.lds = a.lds;
+    g.ldd = pad8(a.N); g.ldp = pad8(a.N);
+    const bool vec = a.N % Vec<T>::V == 0 && on16(a.dy, a.lddy, sizeof(T)) && (!act || on16(a.slope, a.lds, sizeof(typename SlopeOf<T>::type)));
+    const bool products = a.dx != nullptr || a.dW != nullptr;
+    if (!F32 && products) {
+      if (act) {
+        T* d = ws.template take<T>((long long)a.M * g.ldd);
+        g.d = d;
+        dx.p = d; dx.ld = g.ldd;
+      } else {
+        dx = operand(a.dy, a.lddy, a.M, a.N);
+      }
+      dw = dx;
+    }
+    float* scale = nullptr;
+    float* back = nullptr;
+    const bool columns = F32 && a.dW != nullptr;
+    if (a.db != nullptr || columns || g.d != nullptr) {
+      const int across = cdiv(a.N, 64 * Vec<T>::V);
+      int slices = cdiv(4 * 148, across);                  // four CTAs to an SM, rows of 16 or more each
+      if (slices > cdiv(a.M, 16)) slices = cdiv(a.M, 16);
+      g.rows_per_slice = cdiv(cdiv(a.M, slices), 4) * 4;
+      slices = cdiv(a.M, g.rows_per_slice);
+      if (a.db != nullptr) g.sums = ws.template take<float>(slices * g.ldp);
+      if (columns) {
+        g.tops = ws.template take<float>(slices * g.ldp);
+        scale = ws.template take<float>(g.ldp);
+        back = ws.template take<float>(g.ldp);
+        g.x_inv = x.inv;
+      }
+      if (!dry && rc == B200GRU_OK) {
+        const dim3 grid((unsigned)across, (unsigned)slices);
+        if (vec) launch_pdl(grad_kernel<T, true>, grid, dim3(256), 0, st, g);
+        else launch_pdl(grad_kernel<T, false>, grid, dim3(256), 0, st, g);
+        note("grad_kernel");
+        if (a.db != nullptr || columns) {
+          launch_pdl(grad_columns_kernel<T>, dim3((unsigned)cdiv(a.N, 32)), dim3(256), 0, st, static_cast<const float*>(g.sums),
+                     static_cast<const float*>(g.tops), slices, g.ldp, a.N, static_cast<T*>(a.db), scale, back);
+          note("grad_columns_kernel");
+        }
+      }
+    }
+    if (F32 && products) {
+      GradPlanesArgs q;
+      memset(&q, 0, sizeof(q));
+      q.g = g; q.g.x_inv = x.inv;
+      q.w_inv = W.inv; q.col_scale = scale;
+      q.ld = pad8(a.N); q.plane = (long long)a.M * q.ld;
+      if (a.dx != nullptr) {
+        q.dx = ws.template take<__half>(2 * q.plane);
+        q.dx_inv = ws.template take<float>(pad8(a.M));
+        dx.p = q.dx; dx.ld = q.ld; dx.plane = q.plane; dx.inv = q.dx_inv;
+      }
+      if (a.dW != nullptr) {
+        q.dw = ws.template take<__half>(2 * q.plane);
+        dw.p = q.dw; dw.ld = q.ld; dw.plane = q.plane; dw.inv = back;
+      }
+      if (!dry && rc == B200GRU_OK) {
+        const dim3 grid((unsigned)cdiv(a.M, 8));
+        if (vec) launch_pdl(grad_planes_kernel<true>, grid, dim3(256), 0, st, q);
+        else launch_pdl(grad_planes_kernel<false>, grid, dim3(256), 0, st, q);
+        note("grad_planes_kernel");
+      }
+    }
+    Gemm m;
+    memset(&m, 0, sizeof(m));
+    if (a.dx != nullptr) {
+      m.M = a.M; m.N = a.K; m.K = a.N;
+      m.A = dx.p; m.lda = dx.ld; m.a_plane = dx.plane; m.row_scale = dx.inv;
+      m.B = W.p; m.ldb = W.ld; m.b_plane = W.plane; m.b_mn = true;
+      m.C = a.dx; m.ldc = a.K;
+      product(m);
+    }
+    if (a.dW != nullptr) {
+      memset(&m, 0, sizeof(m));
+      m.M = a.N; m.N = a.K; m.K = a.M;
+      m.A = dw.p; m.lda = dw.ld; m.a_plane = dw.plane; m.a_mn = true; m.row_scale = dw.inv;
+      m.B = x.p; m.ldb = x.ld; m.b_plane = x.plane; m.b_mn = true;
+      m.C = a.dW; m.ldc = a.K;
+      product(m);
+    }
+    return rc;
+  }
+};
+
+template <typename T>
+int run(const b200gru_linear_args& a, bool backward, bool dry, size_t* bytes, cudaStream_t st) {
+  Call<T> c = {a, {dry ? nullptr : static_cast<char*>(a.workspace), 0}, dry, st, B200GRU_OK};
+  const int rc = backward ? c.backward() : c.forward();
+  if (bytes != nullptr) *bytes = c.ws.at;
+  return rc;
+}
+
+int run_as(const b200gru_linear_args& a, bool backward, bool dry, size_t* bytes, cudaStream_t st) {
+  if (a.dtype == B200GRU_F32) return run<float>(a, backward, dry, bytes, st);
+  if (a.dtype == B200GRU_BF16) return run<__nv_bfloat16>(a, backward, dry, bytes, st);
+  return run<__half>(a, backward, dry, bytes, st);
 }
 
 bool bad(const b200gru_linear_args* p) {
-  return p == nullptr || p->M <= 0 || p->N <= 0 || p->K <= 0 || p->dtype < B200GRU_F32 || p->dtype > B200GRU_F16 ||
-         p->activation < B200GRU_ACT_NONE || p->activation > B200GRU_ACT_TANH || p->x == nullptr || p->W == nullptr ||
-         p->ldx < 0 || p->ldw < 0 || (p->slope != nullptr && p->lds < p->N);
+  return p == nullptr || p->M <= 0 || p->N <= 0 || p->K <= 0 || p->M > 0x7ffffff0 || p->N > 0x3ffffff0 || p->K > 0x3ffffff0 ||
+         p->dtype < B200GRU_F32 || p->dtype > B200GRU_F16 || p->activation < B200GRU_ACT_NONE ||
+         p->activation > B200GRU_ACT_TANH || p->x == nullptr || p->W == nullptr || p->ldx < 0 || p->ldw < 0 ||
+         (p->slope != nullptr && p->lds < p->N);
+}
+
+int checked(const b200gru_linear_args* p, bool backward, void* stream) {
+  size_t need = 0;
+  run_as(*p, backward, true, &need, nullptr);
+  if (need > 0 && (p->workspace == nullptr || (reinterpret_cast<uintptr_t>(p->workspace) & 255u))) return B200GRU_INVALID_ARGUMENT;
+  if (need > p->workspace_bytes) return B200GRU_WORKSPACE_TOO_SMALL;
+  return run_as(*p, backward, false, nullptr, static_cast<cudaStream_t>(stream));
 }
 
 }  // namespace
+
+// Cycles of a tile's k-block, of its start and end, of a launch that joins slices; the cheapest cut of the work.
+Plan plan_gemm(int M, int N, int K, int planes) {
+  const int kb = cdiv(K, 64);
+  const double products = planes == 2 ? 3.0 : 1.0;
+  Plan best = {1, 128, 1};
+  double best_cost = 1e30;
+  const struct { int ctas, m, n, units; double per_kb; } cuts[3] = {{2, 256, 256, 74, 560.0}, {1, 128, 128, 148, 330.0}, {1, 128, 64, 148, 260.0}};
+  for (const auto& c : cuts) {
+    const long long tiles = (long long)cdiv(M, c.m) * cdiv(N, c.n);
+    for (int want = 1; want <= 64 && want <= kb; ++want) {
+      const int per = cdiv(kb, want), splits = cdiv(kb, per);
+      if (splits != want || (splits > 1 && per < 4)) continue;
+      const double waves = (double)((tiles * splits + c.units - 1) / c.units);
+      double cost = waves * per * c.per_kb * products + 4000.0 + 2500.0 * (c.n / 128.0);
+      if (splits > 1) cost += 5000.0 + (double)splits * M * N * 8.0 / 3500.0;      // written and read again
+      if (cost < best_cost) { best_cost = cost; best = {c.ctas, c.n, splits}; }
+    }
+  }
+  return best;
+}
+
+int read_status(int reset) {
+  const int s[4] = {gemm_status<float>(reset), gemm_status<__nv_bfloat16>(reset), gemm_status<__half>(reset), gemm_status<void>(reset)};
+  int v = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (s[i] < 0) return -1;
+    v |= s[i];
+  }
+  return v;
+}
+
 }  // namespace lin
 }  // namespace b200gru
 
@@ -126,26 +663,28 @@ using namespace b200gru;
 
 extern "C" {
 
-size_t b200gru_linear_act_workspace_bytes(const b200gru_linear_args* p, int backward) {
-  (void)backward;
-  return lin::bad(p) ? (size_t)-1 : 0;
+size_t b200gru_linear_act_workspace_bytes(const b200gru_linear_args* p, int backward) try {
+  if (lin::bad(p)) return (size_t)-1;
+  size_t n = 0;
+  lin::run_as(*p, backward != 0, true, &n, nullptr);
+  return n;
+} catch (...) {
+  return (size_t)-1;
 }
 
-int b200gru_linear_act_forward(const b200gru_linear_args* p, void* stream) {
+int b200gru_linear_act_forward(const b200gru_linear_args* p, void* stream) try {
   if (lin::bad(p) || p->y == nullptr || p->ldy < p->N || (p->residual != nullptr && p->ldr < 0)) return B200GRU_INVALID_ARGUMENT;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p->dtype == B200GRU_F32) return lin::forward<float>(*p, st);
-  if (p->dtype == B200GRU_BF16) return lin::forward<__nv_bfloat16>(*p, st);
-  return lin::forward<__half>(*p, st);
+  return lin::checked(p, false, stream);
+} catch (...) {
+  return B200GRU_LAUNCH_FAILURE;
 }
 
-int b200gru_linear_act_backward(const b200gru_linear_args* p, void* stream) {
+int b200gru_linear_act_backward(const b200gru_linear_args* p, void* stream) try {
   if (lin::bad(p) || p->dy == nullptr || p->lddy < 0) return B200GRU_INVALID_ARGUMENT;
   if (p->activation != B200GRU_ACT_NONE && p->slope == nullptr) return B200GRU_INVALID_ARGUMENT;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p->dtype == B200GRU_F32) return lin::backward<float>(*p, st);
-  if (p->dtype == B200GRU_BF16) return lin::backward<__nv_bfloat16>(*p, st);
-  return lin::backward<__half>(*p, st);
+  return lin::checked(p, true, stream);
+} catch (...) {
+  return B200GRU_LAUNCH_FAILURE;
 }
 
 }  // extern "C"

@@ -1,0 +1,17 @@
+// Products of linear_act with results in __nv_bfloat16.
+#define B200GRU_LINEAR_GEMM_IMPL
+#include "linear_gemm.cuh"
+
+namespace b200gru {
+namespace lin {
+
+template <>
+int launch_gemm<__nv_bfloat16>(const Gemm& g, const Plan& plan, cudaStream_t st) {
+  return launch_plan<1, __nv_bfloat16>(g, plan, st);
+}
+
+template <>
+int gemm_status<__nv_bfloat16>(int reset) { return unit_status(reset); }
+
+}  // namespace lin
+}  // namespace b200gru

@@ -1,0 +1,17 @@
+// Products of linear_act with results in float.
+#define B200GRU_LINEAR_GEMM_IMPL
+#include "linear_gemm.cuh"
+
+namespace b200gru {
+namespace lin {
+
+template <>
+int launch_gemm<float>(const Gemm& g, const Plan& plan, cudaStream_t st) {
+  return launch_plan<2, float>(g, plan, st);
+}
+
+template <>
+int gemm_status<float>(int reset) { return unit_status(reset); }
+
+}  // namespace lin
+}  // namespace b200gru
