@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "approx.cuh"
 #include "common.cuh"
 
 namespace b200gru {
@@ -88,22 +89,6 @@ __device__ __forceinline__ P2 sub2(P2 a, P2 b) {
   return d;
 }
 __device__ __forceinline__ P2 both(float v) { return pair(v, v); }
-__device__ __forceinline__ float exp2_approx(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float rcp_approx(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-// The smaller one; NaN if either is.
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 // The constants of the packed instructions, which take registers alone.  Behind a volatile move they stay in theirs; the
 // compiler would otherwise build each pair anew at each use, seven moves beside the 24 instructions of an element.
 struct Constants {

@@ -5,8 +5,8 @@
 //
 // Operands: one plane of bf16 or fp16, or (fp32) two row-scaled fp16 planes, of which low x high, high x low and high x high
 // are summed in that order.  Either operand K-major (rows of K) or MN-major (rows of M or N, one per k).  The tensor core's
-// fp32 accumulator truncates, so sums are built in chunks (32 steps for planes; 256 for 16-bit types, whose results are rounded
-// to 2^-9 or 2^-12) in one of two tensor-memory buffers and added to register totals with round-to-nearest.
+// fp32 accumulator truncates, so sums are built in chunks (24 steps for planes; 512 for 16-bit types: 512 losses of 2^-23 stay
+// a quarter of half a step of fp16) in one of two tensor-memory buffers and added to register totals with round-to-nearest.
 //
 // Roles of a CTA's ten warps: 0 loads k-blocks by TMA, 1 issues tcgen05.mma, 2-9 drain the accumulator (32 rows and half the
 // columns each), turn it through a transpose buffer so that rows leave in whole sectors, and apply the epilogue there.  The
@@ -57,17 +57,6 @@ int launch_gemm(const Gemm& g, const Plan& plan, cudaStream_t st);
 template <typename T>
 int gemm_status(int reset);
 
-__device__ __forceinline__ Activated activate_as(int act, float v) {
-  switch (act) {
-    case B200GRU_ACT_RELU: return activate<B200GRU_ACT_RELU>(v);
-    case B200GRU_ACT_SILU: return activate<B200GRU_ACT_SILU>(v);
-    case B200GRU_ACT_GELU: return activate<B200GRU_ACT_GELU>(v);
-    case B200GRU_ACT_SIGMOID: return activate<B200GRU_ACT_SIGMOID>(v);
-    case B200GRU_ACT_TANH: return activate<B200GRU_ACT_TANH>(v);
-  }
-  return activate<B200GRU_ACT_NONE>(v);
-}
-
 // Rows that start on 16-byte boundaries.
 inline bool on16(const void* p, long long ld, size_t es) {
   return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * (long long)es) % 16 == 0);
@@ -114,7 +103,6 @@ struct Params {
   unsigned ab_format;
   const float* row_scale;
   const float* col_scale;
-  int activation;
   const void* bias;
   const void* residual; long long ldr;
   void* C; long long ldc;
@@ -174,8 +162,177 @@ template <typename T> constexpr int STEP = 4 * Vec<T>::V;
 template <typename T> constexpr int TR_LD = STEP<T> + 4;      // floats per row of the transpose buffer
 template <typename T> constexpr int TR_BYTES = EPI_WARPS * 32 * TR_LD<T> * 4;
 
+// 32 lanes x 32 consecutive columns back into tensor memory.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+        "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// First row and column of a warp's part of a tile, and its K slice.
+struct Corner {
+  int row, col, z;
+};
+
+// The residual of 32 rows and the lane's V columns from n on, four rows a lane.
+template <typename T>
+__device__ __forceinline__ void request_residual(const Params& p, const Corner& at, int n, int lane, uint4 (&res)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int m = at.row + k * 8 + (lane >> 2);
+    res[k] = make_uint4(0, 0, 0, 0);
+    if (m < p.M && n < p.N) res[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + (long long)m * p.ldr + n));
+  }
+}
+
+// STEP columns from column j of the warp's part on, which lie in the transpose buffer as rows: scales, bias, activation,
+// residual, and out.
+template <int ACT, int PL, typename Out>
+__device__ __forceinline__ void store_step(const Params& p, const float* tr, const Corner& at, int j, int lane, const uint4 (&res)[4]) {
+  typedef typename Turn<Out>::T T;
+  typedef typename SlopeOf<T>::type S;
+  constexpr bool PARTIAL = std::is_void<Out>::value;
+  constexpr int V = Vec<T>::V, ST = STEP<T>, LD = TR_LD<T>;
+  if (p.vec) {
+    const int rsub = lane >> 2, csub = (lane & 3) * V, n = at.col + j + csub;
+    if (n >= p.N) return;                                  // N is a multiple of V
+    float cs[V], bs[V];
+    if (PL == 2) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) cs[e] = p.col_scale != nullptr ? __ldg(p.col_scale + n + e) : 1.f;
+    }
+    if (!PARTIAL) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) bs[e] = 0.f;
+      if (p.bias != nullptr) unpack16<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.bias) + n)), bs);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int m = at.row + k * 8 + rsub;
+      if (m >= p.M) continue;
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; e += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(tr + (k * 8 + rsub) * LD + csub + e);
+        v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
+      }
+      if (PL == 2) {
+        const float rs = p.row_scale != nullptr ? __ldg(p.row_scale + m) : 1.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = v[e] * rs * cs[e];
+      }
+      if (PARTIAL) {
+        *reinterpret_cast<float4*>(p.partial + (long long)at.z * p.split_stride + (long long)m * p.ldp + n) = make_float4(v[0], v[1], v[2], v[3]);
+        continue;
+      }
+      float sl[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const Activated r = activate<ACT>(v[e] + bs[e]);
+        v[e] = r.y;
+        sl[e] = r.slope;
+      }
+      if (ACT != B200GRU_ACT_NONE && p.slope != nullptr)
+        *reinterpret_cast<uint4*>(static_cast<S*>(p.slope) + (long long)m * p.lds + n) = pack16<S>(sl);
+      if (p.residual != nullptr) {
+        float rv[V];
+        unpack16<T>(res[k], rv);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += rv[e];
+      }
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.C) + (long long)m * p.ldc + n) = pack16<T>(v);
+    }
+  } else {
+    // rows that lie on no boundary: a column per lane
+    const int cl = lane % ST, n = at.col + j + cl;
+    if (n >= p.N) return;
+    const float cs = p.col_scale != nullptr ? __ldg(p.col_scale + n) : 1.f;
+    const float bs = (!PARTIAL && p.bias != nullptr) ? to_float(static_cast<const T*>(p.bias)[n]) : 0.f;
+#pragma unroll 4
+    for (int r = lane / ST; r < 32; r += 32 / ST) {
+      const int m = at.row + r;
+      if (m >= p.M) break;
+      float v = tr[r * LD + cl];
+      if (PL == 2) v = v * (p.row_scale != nullptr ? __ldg(p.row_scale + m) : 1.f) * cs;
+      if (PARTIAL) {
+        p.partial[(long long)at.z * p.split_stride + (long long)m * p.ldp + n] = v;
+        continue;
+      }
+      const Activated a = activate<ACT>(v + bs);
+      v = a.y;
+      if (ACT != B200GRU_ACT_NONE && p.slope != nullptr) static_cast<S*>(p.slope)[(long long)m * p.lds + n] = from_float<S>(a.slope);
+      if (p.residual != nullptr) v += to_float(static_cast<const T*>(p.residual)[(long long)m * p.ldr + n]);
+      static_cast<T*>(p.C)[(long long)m * p.ldc + n] = from_float<T>(v);
+    }
+  }
+}
+
+// The tail of a tile from tensor memory: 32 columns at a time, the next ones requested before these are finished.
+template <int ACT, int PL, int NC, typename Out>
+__device__ __forceinline__ void from_tmem(const Params& p, float* tr, uint32_t src, const Corner& at, int lane) {
+  typedef typename Turn<Out>::T T;
+  constexpr int ST = STEP<T>, LD = TR_LD<T>, V = Vec<T>::V;
+  const bool ahead = !std::is_void<Out>::value && p.vec && p.residual != nullptr;
+  uint4 res[4];
+  if (ahead) request_residual<T>(p, at, at.col + (lane & 3) * V, lane, res);
+#pragma unroll 1
+  for (int c0 = 0; c0 < NC; c0 += 32) {
+    if (at.col + c0 >= p.N) break;                         // warp-uniform
+    uint32_t v[32];
+    tc::tmem_ld32(src + (uint32_t)c0, v);
+    tc::tmem_ld_wait();
+#pragma unroll
+    for (int s = 0; s < 32; s += ST) {
+      if (at.col + c0 + s >= p.N) break;
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < ST; e += 4)
+        *reinterpret_cast<uint4*>(tr + lane * LD + e) = make_uint4(v[s + e], v[s + e + 1], v[s + e + 2], v[s + e + 3]);
+      __syncwarp();
+      uint4 now[4];
+      if (ahead) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) now[k] = res[k];
+        if (c0 + s + ST < NC) request_residual<T>(p, at, at.col + c0 + s + ST + (lane & 3) * V, lane, res);
+      }
+      store_step<ACT, PL, Out>(p, tr, at, c0 + s, lane, now);
+    }
+  }
+}
+// The same from totals in registers.
+template <int ACT, int PL, int NC, typename Out>
+__device__ __forceinline__ void from_registers(const Params& p, float* tr, const float (&acc)[NC], const Corner& at, int lane) {
+  typedef typename Turn<Out>::T T;
+  constexpr int ST = STEP<T>, LD = TR_LD<T>, V = Vec<T>::V;
+  const bool ahead = !std::is_void<Out>::value && p.vec && p.residual != nullptr;
+  uint4 res[4];
+  if (ahead) request_residual<T>(p, at, at.col + (lane & 3) * V, lane, res);
+#pragma unroll
+  for (int j = 0; j < NC; j += ST) {
+    if (at.col + j >= p.N) break;                          // warp-uniform
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < ST; e += 4)
+      *reinterpret_cast<float4*>(tr + lane * LD + e) = make_float4(acc[j + e], acc[j + e + 1], acc[j + e + 2], acc[j + e + 3]);
+    __syncwarp();
+    uint4 now[4];
+    if (ahead) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) now[k] = res[k];
+      if (j + ST < NC) request_residual<T>(p, at, at.col + j + ST + (lane & 3) * V, lane, res);
+    }
+    store_step<ACT, PL, Out>(p, tr, at, j, lane, now);
+  }
+}
+
 // Out = void: partial sums in fp32.
-template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, typename Out>
+template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out>
 __global__ void __launch_bounds__(THREADS, 1)
 lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
   typedef typename Turn<Out>::T T;
@@ -328,55 +485,22 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
   } else {
     // ---- epilogue: warp w reads lanes 32 (w % 4) .. of this CTA's accumulator, one half of the columns
-    constexpr int ST = STEP<T>, LD = TR_LD<T>;
+    constexpr int LD = TR_LD<T>;
     const int q = warp & 3, half = (warp - 2) >> 2;
     float* tr = reinterpret_cast<float*>(smem + p.stages * STAGE) + (warp - 2) * 32 * LD;
-    const int rsub = lane >> 2, csub = (lane & 3) * V;
-    const T* resp = static_cast<const T*>(p.residual);
-    typedef typename SlopeOf<T>::type S;
     int c = 0;
     bool ok = __all_sync(0xffffffffu, *deadp == 0);
     for (int t = unit; t < p.tiles && ok; t += units) {
       int m0, n0, z, kb0, nkb;
       locate(t, m0, n0, z, kb0, nkb);
-      const int row_base = m0 + q * 32, col_base = n0 + half * NC;
-      uint4 res[4];
-      const bool prefetch = !PARTIAL && p.vec && resp != nullptr;
-      auto request = [&](int j) {                         // the residual of columns col_base + j ..
-        const int n = col_base + j + csub;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int m = row_base + k * 8 + rsub;
-          res[k] = make_uint4(0, 0, 0, 0);
-          if (m < p.M && n < p.N) res[k] = __ldg(reinterpret_cast<const uint4*>(resp + (long long)m * p.ldr + n));
-        }
-      };
-      if (prefetch) request(0);
-      float rs[4] = {1.f, 1.f, 1.f, 1.f};
-      if (p.row_scale != nullptr) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int m = row_base + k * 8 + rsub;
-          if (m < p.M) rs[k] = __ldg(p.row_scale + m);
-        }
-      }
-      float acc[NC];
-#pragma unroll
-      for (int j = 0; j < NC; ++j) acc[j] = 0.f;
-      for (int i0 = 0; i0 < nkb; i0 += p.chunk_kb, ++c) {
-        const int buf = c & 1;
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&bar_acc_full[buf]), (c >> 1) & 1, deadp, status));
-        if (!ok) break;
+      Corner at = {m0 + q * 32, n0 + half * NC, z};
+      const int chunks = (nkb + p.chunk_kb - 1) / p.chunk_kb;
+      auto landed = [&](int buf) {
+        const bool there = __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&bar_acc_full[buf]), (c >> 1) & 1, deadp, status));
         tc::tc_fence_after();
-        const uint32_t tsrc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * NC);
-#pragma unroll
-        for (int c0 = 0; c0 < NC; c0 += 32) {
-          uint32_t v[32];
-          tc::tmem_ld32(tsrc + (uint32_t)c0, v);
-          tc::tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c0 + j] += __uint_as_float(v[j]);
-        }
+        return there;
+      };
+      auto release = [&](int buf) {
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -384,100 +508,58 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           if (CTAS == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_leader(own)) : "memory");
           else tc::mbar_arrive(own);
         }
+      };
+      auto source = [&](int buf) { return tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * NC); };
+      if (PL == 1 && chunks == 1) {
+        // one chunk: results go from tensor memory to the transpose buffer, 32 columns at a time
+        const int buf = c & 1;
+        ok = landed(buf);
+        if (!ok) break;
+        from_tmem<ACT, PL, NC, Out>(p, tr, source(buf), at, lane);
+        release(buf);
+        ++c;
+        continue;
       }
-      if (!ok) break;
+      float acc[NC];
 #pragma unroll
-      for (int j = 0; j < NC; j += ST) {
-        if (col_base + j >= p.N) break;                    // warp-uniform
-        __syncwarp();
+      for (int j = 0; j < NC; ++j) acc[j] = 0.f;
+      for (int i = 0; i < chunks; ++i, ++c) {
+        const int buf = c & 1;
+        ok = landed(buf);
+        if (!ok) break;
+        if (PL == 2) {
 #pragma unroll
-        for (int e = 0; e < ST; e += 4)
-          *reinterpret_cast<float4*>(tr + lane * LD + e) = make_float4(acc[j + e], acc[j + e + 1], acc[j + e + 2], acc[j + e + 3]);
-        __syncwarp();
-        if (p.vec) {
-          const int n = col_base + j + csub;
-          uint4 now[4];
+          for (int c0 = 0; c0 < NC; c0 += 16) {
+            uint32_t v[16];
+            tc::tmem_ld16(source(buf) + (uint32_t)c0, v);
+            tc::tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 4; ++k) now[k] = res[k];
-          if (prefetch && j + ST < NC) request(j + ST);
-          if (n < p.N) {                                   // N is a multiple of V
-            float cs[V], bs[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) { cs[e] = 1.f; bs[e] = 0.f; }
-            if (p.col_scale != nullptr) {
-#pragma unroll
-              for (int e = 0; e < V; ++e) cs[e] = __ldg(p.col_scale + n + e);
-            }
-            if (!PARTIAL && p.bias != nullptr) unpack16<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.bias) + n)), bs);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int m = row_base + k * 8 + rsub;
-              if (m < p.M) {
-                float v[V];
-#pragma unroll
-                for (int e = 0; e < V; e += 4) {
-                  const float4 f = *reinterpret_cast<const float4*>(tr + (k * 8 + rsub) * LD + csub + e);
-                  v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
-                }
-                if (PL == 2) {
-#pragma unroll
-                  for (int e = 0; e < V; ++e) v[e] = v[e] * rs[k] * cs[e];
-                }
-                if (PARTIAL) {
-                  *reinterpret_cast<float4*>(p.partial + (long long)z * p.split_stride + (long long)m * p.ldp + n) = make_float4(v[0], v[1], v[2], v[3]);
-                } else {
-#pragma unroll
-                  for (int e = 0; e < V; ++e) v[e] += bs[e];
-                  if (p.activation != B200GRU_ACT_NONE) {
-                    float sl[V];
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                      const Activated r = activate_as(p.activation, v[e]);
-                      v[e] = r.y;
-                      sl[e] = r.slope;
-                    }
-                    if (p.slope != nullptr)
-                      *reinterpret_cast<uint4*>(static_cast<S*>(p.slope) + (long long)m * p.lds + n) = pack16<S>(sl);
-                  }
-                  if (resp != nullptr) {
-                    float rv[V];
-                    unpack16<T>(now[k], rv);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) v[e] += rv[e];
-                  }
-                  *reinterpret_cast<uint4*>(static_cast<T*>(p.C) + (long long)m * p.ldc + n) = pack16<T>(v);
-                }
-              }
-            }
+            for (int j = 0; j < 16; ++j) acc[c0 + j] += __uint_as_float(v[j]);
           }
         } else {
-          // rows that lie on no boundary: a column per lane
-          const int cl = lane % ST, n = col_base + j + cl;
-          if (n < p.N) {
-            const float cs = p.col_scale != nullptr ? __ldg(p.col_scale + n) : 1.f;
-            const float bs = (!PARTIAL && p.bias != nullptr) ? to_float(static_cast<const T*>(p.bias)[n]) : 0.f;
-#pragma unroll 4
-            for (int r = lane / ST; r < 32; r += 32 / ST) {
-              const int m = row_base + r;
-              if (m >= p.M) break;
-              float v = tr[r * LD + cl];
-              if (PL == 2) v = v * (p.row_scale != nullptr ? __ldg(p.row_scale + m) : 1.f) * cs;
-              if (PARTIAL) {
-                p.partial[(long long)z * p.split_stride + (long long)m * p.ldp + n] = v;
-              } else {
-                v += bs;
-                if (p.activation != B200GRU_ACT_NONE) {
-                  const Activated a = activate_as(p.activation, v);
-                  v = a.y;
-                  if (p.slope != nullptr) static_cast<S*>(p.slope)[(long long)m * p.lds + n] = from_float<S>(a.slope);
-                }
-                if (resp != nullptr) v += to_float(resp[(long long)m * p.ldr + n]);
-                static_cast<T*>(p.C)[(long long)m * p.ldc + n] = from_float<T>(v);
-              }
+#pragma unroll
+          for (int c0 = 0; c0 < NC; c0 += 32) {
+            uint32_t v[32];
+            tc::tmem_ld32(source(buf) + (uint32_t)c0, v);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[c0 + j] += __uint_as_float(v[j]);
+            if (i == chunks - 1) {                        // the totals go back: the tail is the same as above
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(acc[c0 + j]);
+              tmem_st32(source(buf) + (uint32_t)c0, v);
             }
           }
         }
+        if (PL == 1 && i == chunks - 1) {
+          tmem_st_wait();
+          from_tmem<ACT, PL, NC, Out>(p, tr, source(buf), at, lane);
+        }
+        release(buf);
       }
+      if (!ok) break;
+      // planes: chunks are short, so the totals stay in registers and the buffer is free at once
+      if (PL == 2) from_registers<ACT, PL, NC, Out>(p, tr, acc, at, lane);
     }
   }
 
@@ -525,10 +607,10 @@ int units_on_device(const void* fn, size_t smem, int ctas) {
   return n;
 }
 
-template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, typename Out>
+template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out>
 int launch_variant(const Gemm& g, Params p, const CUtensorMap& ta, const CUtensorMap& tb, cudaStream_t st) {
   typedef typename Turn<Out>::T T;
-  auto kernel = lin_gemm_kernel<CTAS, BN, A_MN, B_MN, PL, Out>;
+  auto kernel = lin_gemm_kernel<CTAS, BN, A_MN, B_MN, PL, ACT, Out>;
   constexpr int BH = CTAS == 2 ? 128 : BN, stage = PL * (BM + BH) * 128;
   p.stages = (226 * 1024 - 1024 - TR_BYTES<T> - 512) / stage;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
@@ -562,9 +644,9 @@ int launch_tile(const Gemm& g, cudaStream_t st) {
   p.tiles = (int)tiles;
   p.kb_total = cdiv(g.K, 64);
   p.kb_per_split = cdiv(p.kb_total, g.splits);
-  p.chunk_kb = PL == 2 ? 2 : 64;
+  p.chunk_kb = PL == 2 ? 2 : 128;
   p.ab_format = g.fp16 ? 0u : 1u;
-  p.row_scale = g.row_scale; p.col_scale = g.col_scale; p.activation = g.activation; p.bias = g.bias;
+  p.row_scale = g.row_scale; p.col_scale = g.col_scale; p.bias = g.bias;
   p.residual = g.residual; p.ldr = g.ldr; p.C = g.C; p.ldc = g.ldc; p.slope = g.slope; p.lds = g.lds;
   p.partial = g.partial; p.ldp = g.ldp; p.split_stride = (long long)g.M * g.ldp;
   if (std::is_void<Out>::value) p.vec = 1;                // partial rows are padded to 16 bytes
@@ -582,10 +664,20 @@ int launch_tile(const Gemm& g, cudaStream_t st) {
   if (rc) return rc;
   rc = tc::make_tensor_map_3d(&tb, dt, g.B, g.b_mn ? g.N : g.K, b_rows, PL, (unsigned long long)g.ldb * 2, b_pl, 64, g.b_mn ? 64 : BH);
   if (rc) return rc;
-  if (!g.a_mn && !g.b_mn) return launch_variant<CTAS, BN, false, false, PL, Out>(g, p, ta, tb, st);
-  if (!g.a_mn && g.b_mn) return launch_variant<CTAS, BN, false, true, PL, Out>(g, p, ta, tb, st);
-  if (g.a_mn && g.b_mn) return launch_variant<CTAS, BN, true, true, PL, Out>(g, p, ta, tb, st);
-  return B200GRU_UNSUPPORTED;
+  constexpr int NONE = B200GRU_ACT_NONE;
+  if (g.a_mn && g.b_mn) return launch_variant<CTAS, BN, true, true, PL, NONE, Out>(g, p, ta, tb, st);
+  if (!g.a_mn && g.b_mn) return launch_variant<CTAS, BN, false, true, PL, NONE, Out>(g, p, ta, tb, st);
+  if (g.a_mn) return B200GRU_UNSUPPORTED;
+  if constexpr (!std::is_void<Out>::value) {              // one kernel for each activation: chosen once an element, it cost 30 products
+    switch (g.activation) {
+      case B200GRU_ACT_RELU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_RELU, Out>(g, p, ta, tb, st);
+      case B200GRU_ACT_SILU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_SILU, Out>(g, p, ta, tb, st);
+      case B200GRU_ACT_GELU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_GELU, Out>(g, p, ta, tb, st);
+      case B200GRU_ACT_SIGMOID: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_SIGMOID, Out>(g, p, ta, tb, st);
+      case B200GRU_ACT_TANH: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_TANH, Out>(g, p, ta, tb, st);
+    }
+  }
+  return launch_variant<CTAS, BN, false, false, PL, NONE, Out>(g, p, ta, tb, st);
 }
 
 template <int PL, typename Out>
