@@ -1,4 +1,5 @@
-// Single instructions of the special-function unit and NaN-keeping minima, shared by the kernels of scan_gated and linear_act.
+// Arithmetic shared by the kernels of scan_gated and linear_act: single instructions of the special-function unit, NaN-keeping
+// minima, packed fp32.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -28,5 +29,41 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+
+// Two values in one 64-bit register, as the packed fp32 instructions of sm_100 take them: one issue for both.
+struct P2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ P2 pair(float x, float y) {
+  P2 p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float2 split(P2 p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+  return f;
+}
+__device__ __forceinline__ P2 fma2(P2 a, P2 b, P2 c) {
+  P2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ P2 mul2(P2 a, P2 b) {
+  P2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ P2 add2(P2 a, P2 b) {
+  P2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ P2 sub2(P2 a, P2 b) {
+  P2 d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ P2 both(float v) { return pair(v, v); }
 
 }  // namespace b200gru

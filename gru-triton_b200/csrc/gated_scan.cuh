@@ -52,43 +52,6 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// ---- two units at a time: the packed fp32 instructions of sm_100 --------------------------------------
-// Both values in one 64-bit register, as the instructions take them.  (As a pair of floats, put together for each
-// instruction, the compiler spent ten moves beside 60 instructions of a pair.)
-struct P2 {
-  unsigned long long v;
-};
-__device__ __forceinline__ P2 pair(float x, float y) {
-  P2 p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
-  return p;
-}
-__device__ __forceinline__ float2 split(P2 p) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
-  return f;
-}
-__device__ __forceinline__ P2 fma2(P2 a, P2 b, P2 c) {
-  P2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
-}
-__device__ __forceinline__ P2 mul2(P2 a, P2 b) {
-  P2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ P2 add2(P2 a, P2 b) {
-  P2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ P2 sub2(P2 a, P2 b) {
-  P2 d;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ P2 both(float v) { return pair(v, v); }
 // The constants of the packed instructions, which take registers alone.  Behind a volatile move they stay in theirs; the
 // compiler would otherwise build each pair anew at each use, seven moves beside the 24 instructions of an element.
 struct Constants {

@@ -19,16 +19,18 @@ namespace {
 inline long long pad8(long long n) { return (n + 7) / 8 * 8; }
 
 // ---- operands ------------------------------------------------------------------------------------------
-// 16-bit rows that TMA cannot read where they lie (odd widths, bases or strides): copied to padded rows.
-__global__ void __launch_bounds__(256) pack_rows_kernel(const unsigned short* __restrict__ src, long long ld, unsigned short* __restrict__ dst,
-                                                        long long dld, int rows, int cols) {
+// Rows that TMA cannot reach where they lie (odd widths, bases or strides) are copied to padded rows, and back.
+template <typename T>
+__global__ void __launch_bounds__(256) copy_rows_kernel(const T* __restrict__ src, long long ld, T* __restrict__ dst, long long dld,
+                                                        int rows, int cols) {
   pdl_launch_dependents();
   pdl_wait();
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= rows) return;
-  const unsigned short* s = src + (long long)row * ld;
-  unsigned short* d = dst + (long long)row * dld;
-  for (int c = lane; c < dld; c += 32) d[c] = c < cols ? s[c] : (unsigned short)0;
+  const T* s = src + (long long)row * ld;
+  T* d = dst + (long long)row * dld;
+#pragma unroll 4
+  for (int c = lane; c < cols; c += 32) d[c] = s[c];
 }
 
 struct HiLo { __half hi, lo; };
@@ -267,17 +269,21 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishArgs a) {
   Four<S> sl;
   const T* resp = static_cast<const T*>(a.residual) + (long long)m * a.ldr + n;
   if (a.vec && a.residual != nullptr) r = reinterpret_cast<const Aligned<T>*>(resp)->f;
+  if (a.bias != nullptr) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.N) v[e] += to_float(static_cast<const T*>(a.bias)[n + e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e += 2) {
+    const Activated2 t = activate_as(a.activation, pair(v[e], v[e + 1]));
+    const float2 f = split(t.y), g = split(t.slope);
+    v[e] = f.x; v[e + 1] = f.y;
+    sl.e[e] = from_float<S>(g.x); sl.e[e + 1] = from_float<S>(g.y);
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if (n + e < a.N) {
-      if (a.bias != nullptr) v[e] += to_float(static_cast<const T*>(a.bias)[n + e]);
-      if (a.activation != B200GRU_ACT_NONE) {
-        const Activated t = activate_as(a.activation, v[e]);
-        v[e] = t.y;
-        sl.e[e] = from_float<S>(t.slope);
-      }
-      if (a.residual != nullptr) v[e] += to_float(a.vec ? r.e[e] : resp[e]);
-    }
+    if (a.residual != nullptr && n + e < a.N) v[e] += to_float(a.vec ? r.e[e] : resp[e]);
     y.e[e] = from_float<T>(v[e]);
   }
   T* cp = static_cast<T*>(a.C) + (long long)m * a.ldc + n;
@@ -365,9 +371,9 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const b200gru_linear_args
   float v = 0.f;
   for (int k = 0; k < slices; ++k) v += part[warp + k][lane];
   if (p.bias != nullptr) v += to_float(static_cast<const T*>(p.bias)[n]);
-  const Activated r = activate_as(p.activation, v);
-  if (p.slope != nullptr) static_cast<S*>(p.slope)[(long long)m * p.lds + n] = from_float<S>(r.slope);
-  v = r.y;
+  const Activated2 r = activate_as(p.activation, pair(v, 0.f));
+  if (p.slope != nullptr) static_cast<S*>(p.slope)[(long long)m * p.lds + n] = from_float<S>(split(r.slope).x);
+  v = split(r.y).x;
   if (p.residual != nullptr) v += to_float(static_cast<const T*>(p.residual)[(long long)m * p.ldr + n]);
   static_cast<T*>(p.y)[(long long)m * p.ldy + n] = from_float<T>(v);
 }
@@ -447,13 +453,16 @@ struct Call {
     if (rows == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) { o.ld = pad8(cols); return o; }
     if (ld >= cols && on16(src, ld, 2)) return o;
     o.ld = pad8(cols);
-    unsigned short* d = ws.template take<unsigned short>((long long)rows * o.ld);
+    T* d = ws.template take<T>((long long)rows * o.ld);
     o.p = d;
-    if (!dry && rc == B200GRU_OK) {
-      launch_pdl(pack_rows_kernel, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, static_cast<const unsigned short*>(src), ld, d, o.ld, rows, cols);
-      note("pack_rows_kernel");
-    }
+    copy_rows(static_cast<const T*>(src), ld, d, o.ld, rows, cols);
     return o;
+  }
+
+  void copy_rows(const T* src, long long ld, T* dst, long long dld, int rows, int cols) {
+    if (dry || rc != B200GRU_OK) return;
+    launch_pdl(copy_rows_kernel<T>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, src, ld, dst, dld, rows, cols);
+    note("copy_rows_kernel");
   }
 
   // The product of two operands, in K slices where that fills the GPU better.
@@ -463,7 +472,18 @@ struct Call {
     const Plan plan = plan_gemm(g.M, g.N, g.K, g.planes);
     g.splits = plan.splits;
     if (plan.splits == 1) {
+      const long long ld = pad8(g.N);
+      if (g.residual != nullptr && (g.ldr < g.N || !on16(g.residual, g.ldr, sizeof(T)))) {
+        T* r = ws.template take<T>(g.M * ld);
+        copy_rows(static_cast<const T*>(g.residual), g.ldr, r, ld, g.M, g.N);
+        g.residual = r; g.ldr = ld;
+      }
+      T* out = static_cast<T*>(g.C);
+      const long long ldc = g.ldc;
+      const bool apart = !on16(g.C, g.ldc, sizeof(T));
+      if (apart) { g.C = ws.template take<T>(g.M * ld); g.ldc = ld; }
       if (!dry && rc == B200GRU_OK) rc = launch_gemm<T>(g, plan, st);
+      if (apart) copy_rows(static_cast<const T*>(g.C), ld, out, ldc, g.M, g.N);
       return;
     }
     FinishArgs f;

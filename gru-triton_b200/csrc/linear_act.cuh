@@ -24,58 +24,69 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 template <typename T> struct SlopeOf { typedef __half type; };
 template <> struct SlopeOf<float> { typedef float type; };
 
-struct Activated { float y, slope; };
+// Two values behind the activation, and its slopes there.
+struct Activated2 {
+  P2 y, slope;
+};
 
-// sigmoid: e = exp(-v), s = 1 / (1 + e), 1 - s = e s; above e = 2^127 s and e s are zero.
-// silu: v s, slope s (1 + v (1 - s)); v held inside [-100, 100] where an infinite one would meet a zero.
+// sigmoid: e = exp(-v), s = 1 / (1 + e), 1 - s = e s.  silu: v s, slope s (1 + v (1 - s)).
 // tanh: f = exp(-2|v|): (1 - f) / (1 + f) with v's sign, slope 4 f / (1 + f)^2; below |v| = 1/8, where 1 - f cancels, the series
 //   v - v^3/3 + 2 v^5/15 (next term 2e-7 of v at most).
 // gelu: v Phi(v), slope Phi(v) + v phi(v), with Phi by formula 7.1.26 of Abramowitz and Stegun's handbook:
 //   erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x), |error| <= 1.5e-7: half of that in Phi, a unit in the
 //   last place of 1; exp(-v^2 / 2) serves phi as well.
+// Values far out reach the limits without an infinity times zero (e above 2^126 counts as 2^126 in e s).
 template <int ACT>
-__device__ __forceinline__ Activated activate(float v) {
+__device__ __forceinline__ Activated2 activate(P2 v) {
   constexpr float LOG2E = 1.44269504f;
-  Activated r;
+  Activated2 r;
+  const float2 at = split(v);
+  const P2 one = both(1.f);
   if (ACT == B200GRU_ACT_RELU) {
-    r.y = max_nan(v, 0.f);
-    r.slope = v > 0.f ? 1.f : 0.f;
+    r.y = pair(max_nan(at.x, 0.f), max_nan(at.y, 0.f));
+    r.slope = pair(at.x > 0.f ? 1.f : 0.f, at.y > 0.f ? 1.f : 0.f);
   } else if (ACT == B200GRU_ACT_SILU || ACT == B200GRU_ACT_SIGMOID) {
-    const float e = exp2_approx(min_nan(v * -LOG2E, 127.5f));
-    const float s = rcp_approx(1.f + e), o = e * s;
+    const float2 e = make_float2(exp2_approx(at.x * -LOG2E), exp2_approx(at.y * -LOG2E));
+    const P2 s = pair(rcp_approx(1.f + e.x), rcp_approx(1.f + e.y));
+    const P2 o = mul2(pair(min_nan(e.x, 8.507059e37f), min_nan(e.y, 8.507059e37f)), s);
     if (ACT == B200GRU_ACT_SIGMOID) {
       r.y = s;
-      r.slope = s * o;
+      r.slope = mul2(s, o);
     } else {
-      const float w = max_nan(v, -100.f);
-      r.y = w * s;
-      r.slope = s * fmaf(min_nan(w, 100.f), o, 1.f);
+      r.y = mul2(v, s);
+      r.slope = mul2(s, fma2(v, o, one));
     }
   } else if (ACT == B200GRU_ACT_TANH) {
-    const float f = exp2_approx(fabsf(v) * (-2.f * LOG2E)), q = rcp_approx(1.f + f);
-    const float v2 = v * v, near0 = fmaf(fmaf(v2, 2.f / 15.f, -1.f / 3.f) * v2, v, v);
-    r.y = fabsf(v) < 0.125f ? near0 : copysignf((1.f - f) * q, v);
-    r.slope = 4.f * f * q * q;
+    const P2 f = pair(exp2_approx(fabsf(at.x) * (-2.f * LOG2E)), exp2_approx(fabsf(at.y) * (-2.f * LOG2E)));
+    const float2 d = split(add2(one, f));
+    const P2 q = pair(rcp_approx(d.x), rcp_approx(d.y));
+    const P2 v2 = mul2(v, v);
+    const float2 near0 = split(fma2(mul2(fma2(v2, both(2.f / 15.f), both(-1.f / 3.f)), v2), v, v));
+    const float2 far = split(mul2(sub2(one, f), q));
+    r.y = pair(fabsf(at.x) < 0.125f ? near0.x : copysignf(far.x, at.x), fabsf(at.y) < 0.125f ? near0.y : copysignf(far.y, at.y));
+    r.slope = mul2(mul2(mul2(f, q), q), both(4.f));
   } else if (ACT == B200GRU_ACT_GELU) {
-    const float w = max_nan(v, -100.f), c = min_nan(w, 100.f);
-    const float E = exp2_approx(c * c * (-0.5f * LOG2E));
-    const float t = rcp_approx(fmaf(fabsf(c), 0.3275911f * 0.70710678f, 1.f));
-    float poly = fmaf(t, 1.061405429f, -1.453152027f);
-    poly = fmaf(poly, t, 1.421413741f);
-    poly = fmaf(poly, t, -0.284496736f);
-    poly = fmaf(poly, t, 0.254829592f);
-    const float tail = poly * t * (0.5f * E);                // 1 - Phi(|v|)
-    const float cdf = c >= 0.f ? 1.f - tail : tail;
-    r.y = w * cdf;
-    r.slope = fmaf(c, 0.39894228f * E, cdf);
+    const float2 h = split(mul2(mul2(v, v), both(-0.5f * LOG2E)));
+    const P2 E = pair(exp2_approx(h.x), exp2_approx(h.y));
+    const P2 t = pair(rcp_approx(fmaf(fabsf(at.x), 0.3275911f * 0.70710678f, 1.f)),
+                      rcp_approx(fmaf(fabsf(at.y), 0.3275911f * 0.70710678f, 1.f)));
+    P2 poly = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+    poly = fma2(poly, t, both(0.5f * 1.421413741f));
+    poly = fma2(poly, t, both(0.5f * -0.284496736f));
+    poly = fma2(poly, t, both(0.5f * 0.254829592f));
+    const P2 tail = mul2(mul2(poly, t), E);                  // 1 - Phi(|v|)
+    const float2 lo = split(tail), hi = split(sub2(one, tail));
+    const P2 cdf = pair(at.x >= 0.f ? hi.x : lo.x, at.y >= 0.f ? hi.y : lo.y);
+    r.y = mul2(v, cdf);
+    r.slope = fma2(v, mul2(E, both(0.39894228f)), cdf);
   } else {
     r.y = v;
-    r.slope = 1.f;
+    r.slope = one;
   }
   return r;
 }
 
-__device__ __forceinline__ Activated activate_as(int act, float v) {
+__device__ __forceinline__ Activated2 activate_as(int act, P2 v) {
   switch (act) {
     case B200GRU_ACT_RELU: return activate<B200GRU_ACT_RELU>(v);
     case B200GRU_ACT_SILU: return activate<B200GRU_ACT_SILU>(v);

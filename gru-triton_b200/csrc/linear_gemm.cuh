@@ -9,8 +9,9 @@
 // a quarter of half a step of fp16) in one of two tensor-memory buffers and added to register totals with round-to-nearest.
 //
 // Roles of a CTA's ten warps: 0 loads k-blocks by TMA, 1 issues tcgen05.mma, 2-9 drain the accumulator (32 rows and half the
-// columns each), turn it through a transpose buffer so that rows leave in whole sectors, and apply the epilogue there.  The
-// residual of the next columns is requested before the present ones are finished.
+// columns each; a lane has a row).  Results, slopes and residual move as TMA tiles of 32 rows x 128 bytes through swizzled
+// shared memory of the warp's own: the residual of the next columns lands while these are computed, and results are added
+// in its place.  (Rows turned through shared memory and stored by the warp cost as many instructions again as the activation.)
 #pragma once
 
 #include <cstring>
@@ -99,15 +100,11 @@ struct Params {
   int tiles_m, tiles_n, tiles;               // tiles of the K slices included
   int kb_total, kb_per_split;
   int stages, chunk_kb;
-  int vec;                                   // rows of every epilogue tensor on 16-byte boundaries, N a multiple of V
+  int with_residual, with_slope;
   unsigned ab_format;
   const float* row_scale;
   const float* col_scale;
   const void* bias;
-  const void* residual; long long ldr;
-  void* C; long long ldc;
-  void* slope; long long lds;
-  float* partial; long long ldp, split_stride;
 };
 
 __device__ __forceinline__ uint32_t cta_rank() {
@@ -155,12 +152,20 @@ __device__ __forceinline__ void commit(uint32_t bar) {
   }
 }
 
-// Columns that a warp turns at a time: 64 bytes of a row for every type.
-template <typename Out> struct Turn { typedef Out T; };
-template <> struct Turn<void> { typedef float T; };
-template <typename T> constexpr int STEP = 4 * Vec<T>::V;
-template <typename T> constexpr int TR_LD = STEP<T> + 4;      // floats per row of the transpose buffer
-template <typename T> constexpr int TR_BYTES = EPI_WARPS * 32 * TR_LD<T> * 4;
+// How a warp's results leave: groups of 32 rows x 128 bytes (64 for a 64-wide tile of a 16-bit type).
+template <typename Out> struct Leaves { typedef Out T; };
+template <> struct Leaves<void> { typedef float T; };
+template <typename T, int NC>
+struct Group {
+  static constexpr int COLS = 128 / (int)sizeof(T) < NC ? 128 / (int)sizeof(T) : NC;
+  static constexpr int ROW_BYTES = COLS * (int)sizeof(T), BYTES = 32 * ROW_BYTES, COUNT = NC / COLS;
+  // Byte of 16-byte piece c of row r: the swizzle of TMA tiles this wide.
+  static __device__ __forceinline__ uint32_t piece(int r, int c) {
+    return (uint32_t)(r * ROW_BYTES + ((c ^ (ROW_BYTES == 128 ? r & 7 : (r >> 1) & 3)) << 4));
+  }
+};
+constexpr int WARP_OUT = 4096;               // bytes of a warp's tile buffer
+constexpr int WARP_COEF = 128 * 8;           // its columns' bias and scale
 
 // 32 lanes x 32 consecutive columns back into tensor memory.
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
@@ -174,179 +179,125 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
         "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// At most N of this thread's latest tile stores may still be reading shared memory.
+template <int N>
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 
-// First row and column of a warp's part of a tile, and its K slice.
-struct Corner {
-  int row, col, z;
+// A warp's shared memory, and how many groups it has sent: group i uses buffer i & 1.
+struct Lane {
+  unsigned char* out;                        // two tile buffers
+  unsigned char* slopes;                     // one
+  float* coef;                               // bias[NC], scale[NC]
+  uint32_t bar[2];                           // the residual of a buffer has landed
+  int lane;
+  int sent;
 };
+struct Corner { int row, col, z; };          // first row and column of the warp's part of a tile, its K slice
 
-// The residual of 32 rows and the lane's V columns from n on, four rows a lane.
-template <typename T>
-__device__ __forceinline__ void request_residual(const Params& p, const Corner& at, int n, int lane, uint4 (&res)[4]) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int m = at.row + k * 8 + (lane >> 2);
-    res[k] = make_uint4(0, 0, 0, 0);
-    if (m < p.M && n < p.N) res[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + (long long)m * p.ldr + n));
+template <typename T, int COLS>
+__device__ __forceinline__ void fetch_residual(const Params& p, const CUtensorMap* map, const Lane& w, int i, int row, int col) {
+  if (w.lane == 0) {
+    tc::mbar_expect_tx(w.bar[i & 1], 32 * COLS * sizeof(T));
+    tc::tma_load_3d(tc::smem_u32(w.out + (i & 1) * WARP_OUT), map, col, row, 0, w.bar[i & 1]);
   }
 }
 
-// STEP columns from column j of the warp's part on, which lie in the transpose buffer as rows: scales, bias, activation,
-// residual, and out.
-template <int ACT, int PL, typename Out>
-__device__ __forceinline__ void store_step(const Params& p, const float* tr, const Corner& at, int j, int lane, const uint4 (&res)[4]) {
-  typedef typename Turn<Out>::T T;
+// 32 columns from column c of the group on: scales, bias, activation, residual; into the buffers.
+template <int ACT, int PL, typename Out, int NC>
+__device__ __forceinline__ void finish_columns(const Params& p, const Lane& w, unsigned char* out, const uint32_t (&v)[32], float rs, int col, int c) {
+  typedef typename Leaves<Out>::T T;
   typedef typename SlopeOf<T>::type S;
-  constexpr bool PARTIAL = std::is_void<Out>::value;
-  constexpr int V = Vec<T>::V, ST = STEP<T>, LD = TR_LD<T>;
-  if (p.vec) {
-    const int rsub = lane >> 2, csub = (lane & 3) * V, n = at.col + j + csub;
-    if (n >= p.N) return;                                  // N is a multiple of V
-    float cs[V], bs[V];
-    if (PL == 2) {
+  typedef Group<T, NC> G;
+  constexpr int V = Vec<T>::V;
+  const bool add = !std::is_void<Out>::value && p.with_residual, keep = ACT != B200GRU_ACT_NONE && p.with_slope;
 #pragma unroll
-      for (int e = 0; e < V; ++e) cs[e] = p.col_scale != nullptr ? __ldg(p.col_scale + n + e) : 1.f;
-    }
-    if (!PARTIAL) {
+  for (int e = 0; e < 32; e += V) {
+    P2 x[V / 2], sl[V / 2];
 #pragma unroll
-      for (int e = 0; e < V; ++e) bs[e] = 0.f;
-      if (p.bias != nullptr) unpack16<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.bias) + n)), bs);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int m = at.row + k * 8 + rsub;
-      if (m >= p.M) continue;
-      float v[V];
-#pragma unroll
-      for (int e = 0; e < V; e += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(tr + (k * 8 + rsub) * LD + csub + e);
-        v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
-      }
+    for (int k = 0; k < V / 2; ++k) {
+      x[k] = pair(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1]));
       if (PL == 2) {
-        const float rs = p.row_scale != nullptr ? __ldg(p.row_scale + m) : 1.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = v[e] * rs * cs[e];
+        const float2 cs = *reinterpret_cast<const float2*>(w.coef + NC + col + e + 2 * k);
+        x[k] = mul2(mul2(x[k], both(rs)), pair(cs.x, cs.y));
       }
-      if (PARTIAL) {
-        *reinterpret_cast<float4*>(p.partial + (long long)at.z * p.split_stride + (long long)m * p.ldp + n) = make_float4(v[0], v[1], v[2], v[3]);
-        continue;
-      }
-      float sl[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const Activated r = activate<ACT>(v[e] + bs[e]);
-        v[e] = r.y;
-        sl[e] = r.slope;
-      }
-      if (ACT != B200GRU_ACT_NONE && p.slope != nullptr)
-        *reinterpret_cast<uint4*>(static_cast<S*>(p.slope) + (long long)m * p.lds + n) = pack16<S>(sl);
-      if (p.residual != nullptr) {
-        float rv[V];
-        unpack16<T>(res[k], rv);
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] += rv[e];
-      }
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.C) + (long long)m * p.ldc + n) = pack16<T>(v);
     }
-  } else {
-    // rows that lie on no boundary: a column per lane
-    const int cl = lane % ST, n = at.col + j + cl;
-    if (n >= p.N) return;
-    const float cs = p.col_scale != nullptr ? __ldg(p.col_scale + n) : 1.f;
-    const float bs = (!PARTIAL && p.bias != nullptr) ? to_float(static_cast<const T*>(p.bias)[n]) : 0.f;
-#pragma unroll 4
-    for (int r = lane / ST; r < 32; r += 32 / ST) {
-      const int m = at.row + r;
-      if (m >= p.M) break;
-      float v = tr[r * LD + cl];
-      if (PL == 2) v = v * (p.row_scale != nullptr ? __ldg(p.row_scale + m) : 1.f) * cs;
-      if (PARTIAL) {
-        p.partial[(long long)at.z * p.split_stride + (long long)m * p.ldp + n] = v;
-        continue;
+    if (!std::is_void<Out>::value) {
+#pragma unroll
+      for (int k = 0; k < V / 2; k += 2) {
+        const float4 b = *reinterpret_cast<const float4*>(w.coef + col + e + 2 * k);
+        const Activated2 r0 = activate<ACT>(add2(x[k], pair(b.x, b.y))), r1 = activate<ACT>(add2(x[k + 1], pair(b.z, b.w)));
+        x[k] = r0.y; x[k + 1] = r1.y;
+        sl[k] = r0.slope; sl[k + 1] = r1.slope;
       }
-      const Activated a = activate<ACT>(v + bs);
-      v = a.y;
-      if (ACT != B200GRU_ACT_NONE && p.slope != nullptr) static_cast<S*>(p.slope)[(long long)m * p.lds + n] = from_float<S>(a.slope);
-      if (p.residual != nullptr) v += to_float(static_cast<const T*>(p.residual)[(long long)m * p.ldr + n]);
-      static_cast<T*>(p.C)[(long long)m * p.ldc + n] = from_float<T>(v);
     }
+    const uint32_t at = G::piece(w.lane, (c + e) / V);
+    if (keep) {
+      float f[V];
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) { const float2 s = split(sl[k]); f[2 * k] = s.x; f[2 * k + 1] = s.y; }
+      *reinterpret_cast<uint4*>(w.slopes + at) = pack16<S>(f);
+    }
+    if (add) {
+      float f[V];
+      unpack16<T>(*reinterpret_cast<const uint4*>(out + at), f);
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) x[k] = add2(x[k], pair(f[2 * k], f[2 * k + 1]));
+    }
+    float f[V];
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) { const float2 y = split(x[k]); f[2 * k] = y.x; f[2 * k + 1] = y.y; }
+    *reinterpret_cast<uint4*>(out + at) = pack16<T>(f);
   }
 }
 
-// The tail of a tile from tensor memory: 32 columns at a time, the next ones requested before these are finished.
-template <int ACT, int PL, int NC, typename Out>
-__device__ __forceinline__ void from_tmem(const Params& p, float* tr, uint32_t src, const Corner& at, int lane) {
-  typedef typename Turn<Out>::T T;
-  constexpr int ST = STEP<T>, LD = TR_LD<T>, V = Vec<T>::V;
-  const bool ahead = !std::is_void<Out>::value && p.vec && p.residual != nullptr;
-  uint4 res[4];
-  if (ahead) request_residual<T>(p, at, at.col + (lane & 3) * V, lane, res);
-#pragma unroll 1
-  for (int c0 = 0; c0 < NC; c0 += 32) {
-    if (at.col + c0 >= p.N) break;                         // warp-uniform
-    uint32_t v[32];
-    tc::tmem_ld32(src + (uint32_t)c0, v);
-    tc::tmem_ld_wait();
-#pragma unroll
-    for (int s = 0; s < 32; s += ST) {
-      if (at.col + c0 + s >= p.N) break;
-      __syncwarp();
-#pragma unroll
-      for (int e = 0; e < ST; e += 4)
-        *reinterpret_cast<uint4*>(tr + lane * LD + e) = make_uint4(v[s + e], v[s + e + 1], v[s + e + 2], v[s + e + 3]);
-      __syncwarp();
-      uint4 now[4];
-      if (ahead) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) now[k] = res[k];
-        if (c0 + s + ST < NC) request_residual<T>(p, at, at.col + c0 + s + ST + (lane & 3) * V, lane, res);
-      }
-      store_step<ACT, PL, Out>(p, tr, at, c0 + s, lane, now);
-    }
+// Before a group's columns are written: its buffer is free, its residual there, the next group's requested.
+template <typename Out, int NC>
+__device__ __forceinline__ bool open_group(const Params& p, const CUtensorMap* tmR, Lane& w, const Corner& next, bool more, volatile int* dead, int* status) {
+  typedef typename Leaves<Out>::T T;
+  typedef Group<T, NC> G;
+  if (!std::is_void<Out>::value && p.with_residual) {
+    if (w.lane == 0) stores_read<0>();
+    __syncwarp();
+    if (more) fetch_residual<T, G::COLS>(p, tmR, w, w.sent + 1, next.row, next.col);
+    return __all_sync(0xffffffffu, tc::mbar_wait(w.bar[w.sent & 1], (uint32_t)(w.sent >> 1) & 1u, dead, status));
   }
+  if (w.lane == 0) {
+    if (p.with_slope) stores_read<0>();
+    else stores_read<1>();
+  }
+  __syncwarp();
+  return true;
 }
-// The same from totals in registers.
-template <int ACT, int PL, int NC, typename Out>
-__device__ __forceinline__ void from_registers(const Params& p, float* tr, const float (&acc)[NC], const Corner& at, int lane) {
-  typedef typename Turn<Out>::T T;
-  constexpr int ST = STEP<T>, LD = TR_LD<T>, V = Vec<T>::V;
-  const bool ahead = !std::is_void<Out>::value && p.vec && p.residual != nullptr;
-  uint4 res[4];
-  if (ahead) request_residual<T>(p, at, at.col + (lane & 3) * V, lane, res);
-#pragma unroll
-  for (int j = 0; j < NC; j += ST) {
-    if (at.col + j >= p.N) break;                          // warp-uniform
-    __syncwarp();
-#pragma unroll
-    for (int e = 0; e < ST; e += 4)
-      *reinterpret_cast<float4*>(tr + lane * LD + e) = make_float4(acc[j + e], acc[j + e + 1], acc[j + e + 2], acc[j + e + 3]);
-    __syncwarp();
-    uint4 now[4];
-    if (ahead) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) now[k] = res[k];
-      if (j + ST < NC) request_residual<T>(p, at, at.col + j + ST + (lane & 3) * V, lane, res);
-    }
-    store_step<ACT, PL, Out>(p, tr, at, j, lane, now);
+// The group's results (and slopes) start on their way.
+template <typename Out, int NC>
+__device__ __forceinline__ void close_group(const Params& p, const CUtensorMap* tmC, const CUtensorMap* tmS, Lane& w, const Corner& at, int col) {
+  tc::fence_async_smem();
+  __syncwarp();
+  if (w.lane == 0) {
+    tc::tma_store_3d(tmC, at.col + col, at.row, at.z, tc::smem_u32(w.out + (w.sent & 1) * WARP_OUT));
+    if (!std::is_void<Out>::value && p.with_slope) tc::tma_store_3d(tmS, at.col + col, at.row, 0, tc::smem_u32(w.slopes));
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
+  ++w.sent;
 }
 
 // Out = void: partial sums in fp32.
 template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out>
 __global__ void __launch_bounds__(THREADS, 1)
-lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
-  typedef typename Turn<Out>::T T;
-  constexpr bool PARTIAL = std::is_void<Out>::value;
-  constexpr int V = Vec<T>::V;
+lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmS,
+                const __grid_constant__ CUtensorMap tmR, const Params p) {
+  typedef typename Leaves<Out>::T T;
   constexpr int BH = CTAS == 2 ? 128 : BN;               // rows of B per CTA
   constexpr int A_PLANE = BM * 128, B_PLANE = BH * 128, STAGE = PL * (A_PLANE + B_PLANE);
   constexpr int UMMA_K = 16, NC = BN / 2;                // accumulator columns per epilogue thread
+  constexpr bool PARTIAL = std::is_void<Out>::value;
   const uint32_t IDESC = tc::umma_idesc(false, A_MN, B_MN, CTAS * BM, BN, p.ab_format);
 
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) unsigned long long bar_full[MAX_STAGES], bar_empty[MAX_STAGES];
-  __shared__ __align__(8) unsigned long long bar_acc_full[2], bar_acc_empty[2];
+  __shared__ __align__(8) unsigned long long bar_acc_full[2], bar_acc_empty[2], bar_res[EPI_WARPS][2];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
 
@@ -366,6 +317,7 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     for (int b = 0; b < 2; ++b) {
       tc::mbar_init(tc::smem_u32(&bar_acc_full[b]), 1);
       tc::mbar_init(tc::smem_u32(&bar_acc_empty[b]), CTAS * EPI_WARPS);
+      for (int w = 0; w < EPI_WARPS; ++w) tc::mbar_init(tc::smem_u32(&bar_res[w][b]), 1);
     }
     tc::mbar_fence_init();
     tc::tma_prefetch_map(&tmA);
@@ -485,16 +437,46 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
   } else {
     // ---- epilogue: warp w reads lanes 32 (w % 4) .. of this CTA's accumulator, one half of the columns
-    constexpr int LD = TR_LD<T>;
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    float* tr = reinterpret_cast<float*>(smem + p.stages * STAGE) + (warp - 2) * 32 * LD;
+    typedef Group<T, NC> G;
+    const int q = warp & 3, half = (warp - 2) >> 2, me = warp - 2;
+    unsigned char* tail = smem + p.stages * STAGE;           // buffers of the warps, 1024-byte aligned
+    Lane w;
+    w.out = tail + me * 2 * WARP_OUT;
+    w.slopes = tail + EPI_WARPS * 2 * WARP_OUT + me * WARP_OUT;
+    w.coef = reinterpret_cast<float*>(tail + EPI_WARPS * (p.with_slope ? 3 : 2) * WARP_OUT + me * WARP_COEF);
+    w.bar[0] = tc::smem_u32(&bar_res[me][0]); w.bar[1] = tc::smem_u32(&bar_res[me][1]);
+    w.lane = lane; w.sent = 0;
     int c = 0;
     bool ok = __all_sync(0xffffffffu, *deadp == 0);
+    // the next tile from t on in which this warp has columns (a narrow matrix ends before its half of the tile)
+    auto next_tile = [&](int t, Corner& at) {
+      for (; t < p.tiles; t += units) {
+        int m0, n0, z, kb0, nkb;
+        locate(t, m0, n0, z, kb0, nkb);
+        at = Corner{m0 + q * 32, n0 + half * NC, z};
+        if (at.col < p.N) return true;
+      }
+      return false;
+    };
+    Corner then = {0, 0, 0};
+    if (!PARTIAL && p.with_residual && ok && next_tile(unit, then)) fetch_residual<T, G::COLS>(p, &tmR, w, 0, then.row, then.col);
     for (int t = unit; t < p.tiles && ok; t += units) {
       int m0, n0, z, kb0, nkb;
       locate(t, m0, n0, z, kb0, nkb);
-      Corner at = {m0 + q * 32, n0 + half * NC, z};
+      const Corner at = {m0 + q * 32, n0 + half * NC, z};
+      bool last = true;
+      if (!PARTIAL && p.with_residual) last = !next_tile(t + units, then);
       const int chunks = (nkb + p.chunk_kb - 1) / p.chunk_kb;
+      // bias and scales of the columns; the row's scale
+      __syncwarp();
+      for (int j = lane; j < NC; j += 32) {
+        const int n = at.col + j;
+        if (!PARTIAL) w.coef[j] = (p.bias != nullptr && n < p.N) ? to_float(static_cast<const T*>(p.bias)[n]) : 0.f;
+        if (PL == 2) w.coef[NC + j] = (p.col_scale != nullptr && n < p.N) ? __ldg(p.col_scale + n) : 1.f;
+      }
+      __syncwarp();
+      float rs = 1.f;
+      if (PL == 2 && p.row_scale != nullptr && at.row + lane < p.M) rs = __ldg(p.row_scale + at.row + lane);
       auto landed = [&](int buf) {
         const bool there = __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&bar_acc_full[buf]), (c >> 1) & 1, deadp, status));
         tc::tc_fence_after();
@@ -505,29 +487,74 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         __syncwarp();
         if (lane == 0) {
           const uint32_t own = tc::smem_u32(&bar_acc_empty[buf]);
-          if (CTAS == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_leader(own)) : "memory");
+          // relaxed: a release would wait for results on their way to memory
+          if (CTAS == 2) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_leader(own)) : "memory");
           else tc::mbar_arrive(own);
         }
       };
       auto source = [&](int buf) { return tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * NC); };
-      if (PL == 1 && chunks == 1) {
-        // one chunk: results go from tensor memory to the transpose buffer, 32 columns at a time
-        const int buf = c & 1;
-        ok = landed(buf);
+      auto open = [&](int g) {
+        const bool here = g + 1 < G::COUNT && at.col + (g + 1) * G::COLS < p.N;
+        return open_group<Out, NC>(p, &tmR, w, here ? Corner{at.row, at.col + (g + 1) * G::COLS, 0} : then, here || !last, deadp, status);
+      };
+      auto close = [&](int g) { close_group<Out, NC>(p, &tmC, &tmS, w, at, g * G::COLS); };
+      if (PL == 1) {
+        // Totals of more than one chunk are summed in registers and put back, so that the way out is one: from tensor memory, the
+        // next 32 columns requested before these are finished.
+        const int buf0 = c & 1;
+        ok = landed(buf0);
         if (!ok) break;
-        from_tmem<ACT, PL, NC, Out>(p, tr, source(buf), at, lane);
+        int buf = buf0;
+        for (int i = 1; i < chunks; ++i) {                   // add this buffer's sums to the next one's
+          ++c;
+          ok = landed(buf ^ 1);
+          if (!ok) break;
+#pragma unroll 1
+          for (int c0 = 0; c0 < NC; c0 += 32) {
+            uint32_t v[32], u[32];
+            tc::tmem_ld32(source(buf) + (uint32_t)c0, v);
+            tc::tmem_ld32(source(buf ^ 1) + (uint32_t)c0, u);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) u[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u[j]));
+            tmem_st32(source(buf ^ 1) + (uint32_t)c0, u);
+          }
+          tmem_st_wait();
+          release(buf);
+          buf ^= 1;
+        }
+        if (!ok) break;
+        uint32_t v[32];
+        tc::tmem_ld32(source(buf), v);
+#pragma unroll 1
+        for (int g = 0; g < G::COUNT; ++g) {
+          if (at.col + g * G::COLS >= p.N) break;            // warp-uniform
+          ok = open(g);
+          unsigned char* out = w.out + (w.sent & 1) * WARP_OUT;
+#pragma unroll
+          for (int c0 = 0; c0 < G::COLS; c0 += 32) {
+            const int col = g * G::COLS + c0;
+            tc::tmem_ld_wait();
+            uint32_t x[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = v[j];
+            if (col + 32 < NC) tc::tmem_ld32(source(buf) + (uint32_t)(col + 32), v);
+            finish_columns<ACT, PL, Out, NC>(p, w, out, x, rs, col, c0);
+          }
+          close(g);
+        }
+        tc::tmem_ld_wait();
         release(buf);
         ++c;
-        continue;
-      }
-      float acc[NC];
+      } else {
+        // planes: chunks are short, so the totals stay in registers and a buffer is free at once
+        float acc[NC];
 #pragma unroll
-      for (int j = 0; j < NC; ++j) acc[j] = 0.f;
-      for (int i = 0; i < chunks; ++i, ++c) {
-        const int buf = c & 1;
-        ok = landed(buf);
-        if (!ok) break;
-        if (PL == 2) {
+        for (int j = 0; j < NC; ++j) acc[j] = 0.f;
+        for (int i = 0; i < chunks; ++i, ++c) {
+          const int buf = c & 1;
+          ok = landed(buf);
+          if (!ok) break;
 #pragma unroll
           for (int c0 = 0; c0 < NC; c0 += 16) {
             uint32_t v[16];
@@ -536,31 +563,24 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[c0 + j] += __uint_as_float(v[j]);
           }
-        } else {
-#pragma unroll
-          for (int c0 = 0; c0 < NC; c0 += 32) {
-            uint32_t v[32];
-            tc::tmem_ld32(source(buf) + (uint32_t)c0, v);
-            tc::tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) acc[c0 + j] += __uint_as_float(v[j]);
-            if (i == chunks - 1) {                        // the totals go back: the tail is the same as above
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(acc[c0 + j]);
-              tmem_st32(source(buf) + (uint32_t)c0, v);
-            }
-          }
+          release(buf);
         }
-        if (PL == 1 && i == chunks - 1) {
-          tmem_st_wait();
-          from_tmem<ACT, PL, NC, Out>(p, tr, source(buf), at, lane);
+        if (!ok) break;
+#pragma unroll
+        for (int g = 0; g < G::COUNT; ++g) {
+          if (at.col + g * G::COLS >= p.N) break;            // warp-uniform
+          if (ok) ok = open(g);
+          unsigned char* out = w.out + (w.sent & 1) * WARP_OUT;
+          uint32_t x[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(acc[g * G::COLS + j]);
+          finish_columns<ACT, PL, Out, NC>(p, w, out, x, rs, g * G::COLS, 0);
+          close(g);
         }
-        release(buf);
       }
-      if (!ok) break;
-      // planes: chunks are short, so the totals stay in registers and the buffer is free at once
-      if (PL == 2) from_registers<ACT, PL, NC, Out>(p, tr, acc, at, lane);
     }
+    // shared memory is read, and results are in memory, before the CTA ends; a residual that nobody took has landed
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   if (warp == 0 && lane == 0 && *deadp) {                 // a CTA that gave up: let tile copies in flight land
@@ -607,14 +627,18 @@ int units_on_device(const void* fn, size_t smem, int ctas) {
   return n;
 }
 
+struct Maps {
+  alignas(64) CUtensorMap a, b, c, slope, residual;
+};
+
 template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out>
-int launch_variant(const Gemm& g, Params p, const CUtensorMap& ta, const CUtensorMap& tb, cudaStream_t st) {
-  typedef typename Turn<Out>::T T;
+int launch_variant(Params p, const Maps& m, cudaStream_t st) {
   auto kernel = lin_gemm_kernel<CTAS, BN, A_MN, B_MN, PL, ACT, Out>;
   constexpr int BH = CTAS == 2 ? 128 : BN, stage = PL * (BM + BH) * 128;
-  p.stages = (226 * 1024 - 1024 - TR_BYTES<T> - 512) / stage;
+  const int tail = EPI_WARPS * ((p.with_slope ? 3 : 2) * WARP_OUT + WARP_COEF);
+  p.stages = (227 * 1024 - 1024 - 512 - tail) / stage;       // 512: barriers
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-  const size_t smem = (size_t)p.stages * stage + TR_BYTES<T> + 1024;
+  const size_t smem = (size_t)p.stages * stage + tail + 1024;
   const int units = units_on_device(reinterpret_cast<const void*>(kernel), smem, CTAS);
   if (units <= 0) return B200GRU_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
@@ -626,15 +650,22 @@ int launch_variant(const Gemm& g, Params p, const CUtensorMap& ta, const CUtenso
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = CTAS; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
   cfg.attrs = at; cfg.numAttrs = CTAS == 2 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+  cudaLaunchKernelEx(&cfg, kernel, m.a, m.b, m.c, m.slope, m.residual, p);
   note_launch();
   return check_launch("lin_gemm_kernel");
 }
 
+template <typename T> struct MapType;
+template <> struct MapType<float> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_FLOAT32; };
+template <> struct MapType<__nv_bfloat16> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; };
+template <> struct MapType<__half> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_FLOAT16; };
+
 template <int CTAS, int BN, int PL, typename Out>
 int launch_tile(const Gemm& g, cudaStream_t st) {
-  typedef typename Turn<Out>::T T;
+  typedef typename Leaves<Out>::T T;
   typedef typename SlopeOf<T>::type S;
+  typedef Group<T, BN / 2> G;
+  constexpr bool PARTIAL = std::is_void<Out>::value;
   Params p;
   memset(&p, 0, sizeof(p));
   p.M = g.M; p.N = g.N;
@@ -647,37 +678,42 @@ int launch_tile(const Gemm& g, cudaStream_t st) {
   p.chunk_kb = PL == 2 ? 2 : 128;
   p.ab_format = g.fp16 ? 0u : 1u;
   p.row_scale = g.row_scale; p.col_scale = g.col_scale; p.bias = g.bias;
-  p.residual = g.residual; p.ldr = g.ldr; p.C = g.C; p.ldc = g.ldc; p.slope = g.slope; p.lds = g.lds;
-  p.partial = g.partial; p.ldp = g.ldp; p.split_stride = (long long)g.M * g.ldp;
-  if (std::is_void<Out>::value) p.vec = 1;                // partial rows are padded to 16 bytes
-  else p.vec = g.N % Vec<T>::V == 0 && on16(g.C, g.ldc, sizeof(T)) && on16(g.residual, g.ldr, sizeof(T)) &&
-               on16(g.bias, 0, sizeof(T)) && on16(g.slope, g.lds, sizeof(S));
-  if (std::is_void<Out>::value) p.N = (int)g.ldp;         // and written to their padded end
+  p.with_residual = !PARTIAL && g.residual != nullptr;
+  p.with_slope = !PARTIAL && g.slope != nullptr && g.activation != B200GRU_ACT_NONE;
 
   constexpr int BH = CTAS == 2 ? 128 : BN;
   const CUtensorMapDataType dt = g.fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  alignas(64) CUtensorMap ta, tb;
+  Maps m;
+  memset(&m, 0, sizeof(m));
   const unsigned long long a_rows = g.a_mn ? g.K : g.M, b_rows = g.b_mn ? g.K : g.N;
   const unsigned long long a_pl = PL > 1 ? (unsigned long long)g.a_plane * 2 : a_rows * g.lda * 2;
   const unsigned long long b_pl = PL > 1 ? (unsigned long long)g.b_plane * 2 : b_rows * g.ldb * 2;
-  int rc = tc::make_tensor_map_3d(&ta, dt, g.A, g.a_mn ? g.M : g.K, a_rows, PL, (unsigned long long)g.lda * 2, a_pl, 64, g.a_mn ? 64 : BM);
-  if (rc) return rc;
-  rc = tc::make_tensor_map_3d(&tb, dt, g.B, g.b_mn ? g.N : g.K, b_rows, PL, (unsigned long long)g.ldb * 2, b_pl, 64, g.b_mn ? 64 : BH);
-  if (rc) return rc;
+  int rc = tc::make_tensor_map_3d(&m.a, dt, g.A, g.a_mn ? g.M : g.K, a_rows, PL, (unsigned long long)g.lda * 2, a_pl, 64, g.a_mn ? 64 : BM);
+  if (rc == B200GRU_OK) rc = tc::make_tensor_map_3d(&m.b, dt, g.B, g.b_mn ? g.N : g.K, b_rows, PL, (unsigned long long)g.ldb * 2, b_pl, 64, g.b_mn ? 64 : BH);
+  // rows of results; partial sums to the padded end of their rows
+  auto rows_map = [&](CUtensorMap* map, CUtensorMapDataType type, const void* base, long long cols, int slices, long long ld, size_t es) {
+    return tc::make_tensor_map_out(map, type, base, cols, g.M, slices, (unsigned long long)ld * es, (unsigned long long)g.M * ld * es,
+                                   G::COLS, 32, G::ROW_BYTES);
+  };
+  if (rc == B200GRU_OK) rc = PARTIAL ? rows_map(&m.c, MapType<T>::value, g.partial, g.N, g.splits, g.ldp, sizeof(T))
+                                     : rows_map(&m.c, MapType<T>::value, g.C, g.N, 1, g.ldc, sizeof(T));
+  if (rc == B200GRU_OK && p.with_slope) rc = rows_map(&m.slope, MapType<S>::value, g.slope, g.N, 1, g.lds, sizeof(S));
+  if (rc == B200GRU_OK && p.with_residual) rc = rows_map(&m.residual, MapType<T>::value, g.residual, g.N, 1, g.ldr, sizeof(T));
+  if (rc != B200GRU_OK) return rc;
   constexpr int NONE = B200GRU_ACT_NONE;
-  if (g.a_mn && g.b_mn) return launch_variant<CTAS, BN, true, true, PL, NONE, Out>(g, p, ta, tb, st);
-  if (!g.a_mn && g.b_mn) return launch_variant<CTAS, BN, false, true, PL, NONE, Out>(g, p, ta, tb, st);
+  if (g.a_mn && g.b_mn) return launch_variant<CTAS, BN, true, true, PL, NONE, Out>(p, m, st);
+  if (!g.a_mn && g.b_mn) return launch_variant<CTAS, BN, false, true, PL, NONE, Out>(p, m, st);
   if (g.a_mn) return B200GRU_UNSUPPORTED;
-  if constexpr (!std::is_void<Out>::value) {              // one kernel for each activation: chosen once an element, it cost 30 products
+  if constexpr (!PARTIAL) {                               // one kernel for each activation: chosen once an element, it cost 30 products
     switch (g.activation) {
-      case B200GRU_ACT_RELU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_RELU, Out>(g, p, ta, tb, st);
-      case B200GRU_ACT_SILU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_SILU, Out>(g, p, ta, tb, st);
-      case B200GRU_ACT_GELU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_GELU, Out>(g, p, ta, tb, st);
-      case B200GRU_ACT_SIGMOID: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_SIGMOID, Out>(g, p, ta, tb, st);
-      case B200GRU_ACT_TANH: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_TANH, Out>(g, p, ta, tb, st);
+      case B200GRU_ACT_RELU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_RELU, Out>(p, m, st);
+      case B200GRU_ACT_SILU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_SILU, Out>(p, m, st);
+      case B200GRU_ACT_GELU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_GELU, Out>(p, m, st);
+      case B200GRU_ACT_SIGMOID: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_SIGMOID, Out>(p, m, st);
+      case B200GRU_ACT_TANH: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_TANH, Out>(p, m, st);
     }
   }
-  return launch_variant<CTAS, BN, false, false, PL, NONE, Out>(g, p, ta, tb, st);
+  return launch_variant<CTAS, BN, false, false, PL, NONE, Out>(p, m, st);
 }
 
 template <int PL, typename Out>

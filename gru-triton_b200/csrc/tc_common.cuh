@@ -180,6 +180,11 @@ int make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* 
                        unsigned long long d1, unsigned long long d2, unsigned long long stride1_bytes,
                        unsigned long long stride2_bytes, unsigned box0, unsigned box1);
 
+// The same for boxes whose rows are 128 or 64 bytes, each with the swizzle of its width.
+int make_tensor_map_out(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, unsigned long long d0,
+                        unsigned long long d1, unsigned long long d2, unsigned long long stride1_bytes,
+                        unsigned long long stride2_bytes, unsigned box0, unsigned box1, int row_bytes);
+
 // The same without swizzle, for boxes of box0 x 1 x box2 elements (rows of the middle index, box0 wide, one after the other).
 int make_tensor_map_rows(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, unsigned long long d0,
                          unsigned long long d1, unsigned long long d2, unsigned long long stride1_bytes,

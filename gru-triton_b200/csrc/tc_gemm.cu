@@ -531,6 +531,13 @@ int make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* 
   return encode_3d(map, dtype, base, d0, d1, d2, stride1_bytes, stride2_bytes, box0, box1, 1, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+int make_tensor_map_out(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, unsigned long long d0,
+                        unsigned long long d1, unsigned long long d2, unsigned long long stride1_bytes,
+                        unsigned long long stride2_bytes, unsigned box0, unsigned box1, int row_bytes) {
+  return encode_3d(map, dtype, base, d0, d1, d2, stride1_bytes, stride2_bytes, box0, box1, 1,
+                   row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 int make_tensor_map_rows(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, unsigned long long d0,
                          unsigned long long d1, unsigned long long d2, unsigned long long stride1_bytes,
                          unsigned long long stride2_bytes, unsigned box0, unsigned box2) {
