@@ -165,12 +165,12 @@ __global__ void __launch_bounds__(256) grad_kernel(const GradArgs a) {
   }
 }
 
-// Joins the slices in order: db, and the scales of d's columns.  32 columns x 8 slices a CTA.
+// Joins the slices in order: db, and the scales of d's columns.  32 columns x 32 groups of slices a CTA.
 template <typename T>
-__global__ void __launch_bounds__(256) grad_columns_kernel(const float* __restrict__ sums, const float* __restrict__ tops, int slices,
-                                                           long long ldp, int N, T* __restrict__ db, float* __restrict__ scale,
-                                                           float* __restrict__ back) {
-  __shared__ float rs[8][32], rt[8][32];
+__global__ void __launch_bounds__(1024) grad_columns_kernel(const float* __restrict__ sums, const float* __restrict__ tops, int slices,
+                                                            long long ldp, int N, T* __restrict__ db, float* __restrict__ scale,
+                                                            float* __restrict__ back) {
+  __shared__ float rs[32][33], rt[32][33];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(256) grad_columns_kernel(const float* __restri
   float s = 0.f, t = 0.f;
   if (n < N) {
 #pragma unroll 4
-    for (int k = grp; k < slices; k += 8) {
+    for (int k = grp; k < slices; k += 32) {
       if (sums != nullptr) s += sums[(long long)k * ldp + n];
       if (tops != nullptr) t = fmaxf(t, tops[(long long)k * ldp + n]);
     }
@@ -186,10 +186,17 @@ __global__ void __launch_bounds__(256) grad_columns_kernel(const float* __restri
   rs[grp][lane] = s;
   rt[grp][lane] = t;
   __syncthreads();
-  if (grp == 0 && n < N) {
-    for (int g = 1; g < 8; ++g) { s += rs[g][lane]; t = fmaxf(t, rt[g][lane]); }
-    if (db != nullptr) db[n] = from_float<T>(s);
-    if (tops != nullptr) pow2_row_scale(t, scale + n, back + n);
+  s = rs[lane][grp];                                       // warp `grp` adds column `grp`
+  t = rt[lane][grp];
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, off);
+    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, off));
+  }
+  const int c = blockIdx.x * 32 + grp;
+  if (lane == 0 && c < N) {
+    if (db != nullptr) db[c] = from_float<T>(s);
+    if (tops != nullptr) pow2_row_scale(t, scale + c, back + c);
   }
 }
 
@@ -218,7 +225,7 @@ __global__ void __launch_bounds__(256) grad_planes_kernel(const GradPlanesArgs a
   if (a.dx != nullptr) {
     float mx = 0.f;
 #pragma unroll 4
-    for (int c = lane * 4; c < a.g.N; c += 128) mx = largest(times(value(c), four<false>(a.w_inv, c, a.g.N)), mx);
+    for (int c = lane * 4; c < a.g.N; c += 128) mx = largest(times(value(c), *reinterpret_cast<const float4*>(a.w_inv + c)), mx);
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
     float back;
@@ -230,8 +237,8 @@ __global__ void __launch_bounds__(256) grad_planes_kernel(const GradPlanesArgs a
   for (int c = lane * 4; c < a.ld; c += 128) {
     const float4 v = value(c);
     const long long at = (long long)row * a.ld + c;
-    if (a.dx != nullptr) store_planes(a.dx + at, a.plane, times(times(v, four<false>(a.w_inv, c, a.g.N)), scale));
-    if (a.dw != nullptr) store_planes(a.dw + at, a.plane, times(times(v, x_inv), four<false>(a.col_scale, c, a.g.N)));
+    if (a.dx != nullptr) store_planes(a.dx + at, a.plane, times(times(v, c < a.g.N ? *reinterpret_cast<const float4*>(a.w_inv + c) : v), scale));
+    if (a.dw != nullptr) store_planes(a.dw + at, a.plane, times(times(v, x_inv), c < a.g.N ? *reinterpret_cast<const float4*>(a.col_scale + c) : v));
   }
 }
 
@@ -548,7 +555,7 @@ struct Call {
     const bool columns = F32 && a.dW != nullptr;
     if (a.db != nullptr || columns || g.d != nullptr) {
       const int across = cdiv(a.N, 64 * Vec<T>::V);
-      int slices = cdiv(4 * 148, across);                  // four CTAs to an SM, rows of 16 or more each
+      int slices = cdiv(2 * 148, across);                  // two CTAs to an SM, 16 rows or more each
       if (slices > cdiv(a.M, 16)) slices = cdiv(a.M, 16);
       g.rows_per_slice = cdiv(cdiv(a.M, slices), 4) * 4;
       slices = cdiv(a.M, g.rows_per_slice);
@@ -565,7 +572,7 @@ struct Call {
         else launch_pdl(grad_kernel<T, false>, grid, dim3(256), 0, st, g);
         note("grad_kernel");
         if (a.db != nullptr || columns) {
-          launch_pdl(grad_columns_kernel<T>, dim3((unsigned)cdiv(a.N, 32)), dim3(256), 0, st, static_cast<const float*>(g.sums),
+          launch_pdl(grad_columns_kernel<T>, dim3((unsigned)cdiv(a.N, 32)), dim3(1024), 0, st, static_cast<const float*>(g.sums),
                      static_cast<const float*>(g.tops), slices, g.ldp, a.N, static_cast<T*>(a.db), scale, back);
           note("grad_columns_kernel");
         }
@@ -638,8 +645,8 @@ bool bad(const b200gru_linear_args* p) {
 int checked(const b200gru_linear_args* p, bool backward, void* stream) {
   size_t need = 0;
   run_as(*p, backward, true, &need, nullptr);
-  if (need > 0 && (p->workspace == nullptr || (reinterpret_cast<uintptr_t>(p->workspace) & 255u))) return B200GRU_INVALID_ARGUMENT;
   if (need > p->workspace_bytes) return B200GRU_WORKSPACE_TOO_SMALL;
+  if (need > 0 && (p->workspace == nullptr || (reinterpret_cast<uintptr_t>(p->workspace) & 255u))) return B200GRU_INVALID_ARGUMENT;
   return run_as(*p, backward, false, nullptr, static_cast<cudaStream_t>(stream));
 }
 

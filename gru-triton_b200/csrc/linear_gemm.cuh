@@ -101,6 +101,7 @@ struct Params {
   int kb_total, kb_per_split;
   int stages, chunk_kb;
   int with_residual, with_slope;
+  int out_mask;                              // 1: two result buffers a warp in turn, 0: one (beside one for slopes)
   unsigned ab_format;
   const float* row_scale;
   const float* col_scale;
@@ -185,8 +186,8 @@ __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait
 
 // A warp's shared memory, and how many groups it has sent: group i uses buffer i & 1.
 struct Lane {
-  unsigned char* out;                        // two tile buffers
-  unsigned char* slopes;                     // one
+  unsigned char* out;                        // result tiles
+  unsigned char* slopes;                     // slope tile
   float* coef;                               // bias[NC], scale[NC]
   uint32_t bar[2];                           // the residual of a buffer has landed
   int lane;
@@ -274,7 +275,7 @@ __device__ __forceinline__ void close_group(const Params& p, const CUtensorMap* 
   tc::fence_async_smem();
   __syncwarp();
   if (w.lane == 0) {
-    tc::tma_store_3d(tmC, at.col + col, at.row, at.z, tc::smem_u32(w.out + (w.sent & 1) * WARP_OUT));
+    tc::tma_store_3d(tmC, at.col + col, at.row, at.z, tc::smem_u32(w.out + (w.sent & p.out_mask) * WARP_OUT));
     if (!std::is_void<Out>::value && p.with_slope) tc::tma_store_3d(tmS, at.col + col, at.row, 0, tc::smem_u32(w.slopes));
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
@@ -441,9 +442,10 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int q = warp & 3, half = (warp - 2) >> 2, me = warp - 2;
     unsigned char* tail = smem + p.stages * STAGE;           // buffers of the warps, 1024-byte aligned
     Lane w;
-    w.out = tail + me * 2 * WARP_OUT;
-    w.slopes = tail + EPI_WARPS * 2 * WARP_OUT + me * WARP_OUT;
-    w.coef = reinterpret_cast<float*>(tail + EPI_WARPS * (p.with_slope ? 3 : 2) * WARP_OUT + me * WARP_COEF);
+    const int buffers = 1 + p.out_mask + p.with_slope;
+    w.out = tail + me * buffers * WARP_OUT;
+    w.slopes = w.out + (1 + p.out_mask) * WARP_OUT;
+    w.coef = reinterpret_cast<float*>(tail + EPI_WARPS * buffers * WARP_OUT + me * WARP_COEF);
     w.bar[0] = tc::smem_u32(&bar_res[me][0]); w.bar[1] = tc::smem_u32(&bar_res[me][1]);
     w.lane = lane; w.sent = 0;
     int c = 0;
@@ -530,7 +532,7 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         for (int g = 0; g < G::COUNT; ++g) {
           if (at.col + g * G::COLS >= p.N) break;            // warp-uniform
           ok = open(g);
-          unsigned char* out = w.out + (w.sent & 1) * WARP_OUT;
+          unsigned char* out = w.out + (w.sent & p.out_mask) * WARP_OUT;
 #pragma unroll
           for (int c0 = 0; c0 < G::COLS; c0 += 32) {
             const int col = g * G::COLS + c0;
@@ -570,7 +572,7 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         for (int g = 0; g < G::COUNT; ++g) {
           if (at.col + g * G::COLS >= p.N) break;            // warp-uniform
           if (ok) ok = open(g);
-          unsigned char* out = w.out + (w.sent & 1) * WARP_OUT;
+          unsigned char* out = w.out + (w.sent & p.out_mask) * WARP_OUT;
           uint32_t x[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(acc[g * G::COLS + j]);
@@ -635,7 +637,7 @@ template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out>
 int launch_variant(Params p, const Maps& m, cudaStream_t st) {
   auto kernel = lin_gemm_kernel<CTAS, BN, A_MN, B_MN, PL, ACT, Out>;
   constexpr int BH = CTAS == 2 ? 128 : BN, stage = PL * (BM + BH) * 128;
-  const int tail = EPI_WARPS * ((p.with_slope ? 3 : 2) * WARP_OUT + WARP_COEF);
+  const int tail = EPI_WARPS * ((1 + p.out_mask + p.with_slope) * WARP_OUT + WARP_COEF);
   p.stages = (227 * 1024 - 1024 - 512 - tail) / stage;       // 512: barriers
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   const size_t smem = (size_t)p.stages * stage + tail + 1024;
@@ -680,6 +682,7 @@ int launch_tile(const Gemm& g, cudaStream_t st) {
   p.row_scale = g.row_scale; p.col_scale = g.col_scale; p.bias = g.bias;
   p.with_residual = !PARTIAL && g.residual != nullptr;
   p.with_slope = !PARTIAL && g.slope != nullptr && g.activation != B200GRU_ACT_NONE;
+  p.out_mask = p.with_slope && !p.with_residual ? 0 : 1;    // shared memory for a fourth stage of operands
 
   constexpr int BH = CTAS == 2 ? 128 : BN;
   const CUtensorMapDataType dt = g.fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

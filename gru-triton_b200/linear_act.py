@@ -23,7 +23,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._scan_common import require_cuda
-from .scan_gated import DTYPES, on_device, rows_contiguous, stream_of
+from .scan_gated import DTYPES, call_on, rows_contiguous
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4, "tanh": 5}
 
@@ -31,30 +31,34 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4, "tanh":
 def _check(x, W, bias, residual, activation):
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}; got {activation!r}")
-    given = {k: v for k, v in (("x", x), ("W", W), ("bias", bias), ("residual", residual)) if v is not None}
-    if x.dtype not in DTYPES:
-        raise ValueError(f"x dtype must be float32, bfloat16 or float16; got {x.dtype}")
-    for name, t in given.items():
-        if t.dtype != x.dtype:
-            raise ValueError(f"{name} dtype must be x's, {x.dtype}; got {t.dtype}")
-    if W.dim() != 2 or x.dim() < 1 or x.shape[-1] != W.shape[1]:
-        raise ValueError(f"linear_act needs x[..., K] and W[N, K]; got {tuple(x.shape)} and {tuple(W.shape)}")
-    N, K = W.shape
+    dtype = x.dtype
+    if dtype not in DTYPES:
+        raise ValueError(f"x dtype must be float32, bfloat16 or float16; got {dtype}")
+    for name, t in (("W", W), ("bias", bias), ("residual", residual)):
+        if t is not None and t.dtype != dtype:
+            raise ValueError(f"{name} dtype must be x's, {dtype}; got {t.dtype}")
+    lead, w = x.shape, W.shape
+    if len(w) != 2 or len(lead) < 1 or lead[-1] != w[1]:
+        raise ValueError(f"linear_act needs x[..., K] and W[N, K]; got {tuple(lead)} and {tuple(w)}")
+    N, K = w
     if N == 0 or K == 0:
         raise ValueError(f"N and K must be > 0; got N={N}, K={K}")
-    if bias is not None and tuple(bias.shape) != (N,):
+    if bias is not None and bias.shape != (N,):
         raise ValueError(f"bias shape must be (N,)=({N},); got {tuple(bias.shape)}")
-    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
-        raise ValueError(f"residual shape must be {(*x.shape[:-1], N)}; got {tuple(residual.shape)}")
-    require_cuda(**given)
-    for name, t in given.items():
-        if t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    if residual is not None and residual.shape != (*lead[:-1], N):
+        raise ValueError(f"residual shape must be {(*lead[:-1], N)}; got {tuple(residual.shape)}")
+    device = x.device
+    if not x.is_cuda or any(t is not None and t.device != device for t in (W, bias, residual)):
+        given = {k: v for k, v in (("x", x), ("W", W), ("bias", bias), ("residual", residual)) if v is not None}
+        require_cuda(**given)
+        for name, t in given.items():
+            if t.device != device:
+                raise ValueError(f"{name} is on {t.device}, x on {device}")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as a matrix of rows, in place where its strides allow it."""
-    return rows_contiguous(t.reshape(-1, t.shape[-1]))
+    return rows_contiguous(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
 
 
 def _fill(x, W, activation) -> _lib.CLinearArgs:
@@ -66,17 +70,19 @@ def _fill(x, W, activation) -> _lib.CLinearArgs:
     return a
 
 
+_WORKSPACE_TOO_SMALL = 4
+
+
 def _run(a, backward: bool, device) -> None:
     lib = _lib.load()
-    n = lib.b200gru_linear_act_workspace_bytes(ctypes.byref(a), int(backward))
-    if n == ctypes.c_size_t(-1).value:
-        raise RuntimeError("linear_act: shape not supported")
-    if n:
+    call = lib.b200gru_linear_act_backward if backward else lib.b200gru_linear_act_forward
+    ref = ctypes.byref(a)
+    rc = call_on(device, call, ref)
+    if rc == _WORKSPACE_TOO_SMALL:                     # 16-bit tensors in the common layout need none
+        n = lib.b200gru_linear_act_workspace_bytes(ref, int(backward))
         ws = torch.empty(n, dtype=torch.uint8, device=device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), n
-    call = lib.b200gru_linear_act_backward if backward else lib.b200gru_linear_act_forward
-    with on_device(device):
-        rc = call(ctypes.byref(a), stream_of(device))
+        rc = call_on(device, call, ref)
     if rc:
         _lib._raise(rc, "linear_act backward" if backward else "linear_act")
     _lib._after_call()
@@ -104,7 +110,7 @@ def _forward(x, W, bias, residual, activation, want_slope: bool):
         if slope is not None:
             a.slope, a.lds = slope.data_ptr(), slope.stride(0)
         _run(a, False, x.device)
-    return y.reshape(*lead, N), slope
+    return (y if len(lead) == 1 else y.reshape(*lead, N)), slope
 
 
 class LinearActFunction(torch.autograd.Function):
@@ -131,7 +137,9 @@ class LinearActFunction(torch.autograd.Function):
             a.dy, a.lddy = dy2.data_ptr(), dy2.stride(0)
             if slope:
                 a.slope, a.lds = slope[0].data_ptr(), slope[0].stride(0)
-            a.dx, a.dW, a.db = (None if t is None else t.data_ptr() for t in (dx, dW, db))
+            for name, t in (("dx", dx), ("dW", dW), ("db", db)):
+                if t is not None:
+                    setattr(a, name, t.data_ptr())
             _run(a, True, x.device)
         return dx, dW, db, (dy if need_r else None), None
 

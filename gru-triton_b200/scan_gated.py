@@ -17,7 +17,6 @@ counterpart in the reference, whose recurrences all have hidden weights (scan_di
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Any, Optional, Tuple
 
@@ -29,16 +28,16 @@ from ._scan_common import require_cuda
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _CANDIDATES = {"identity": 0, "tanh": 1}
-_HERE = contextlib.nullcontext()
 
 
-def on_device(device: torch.device):
-    """The device's context where it is not the current one."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def stream_of(device: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def call_on(device: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` on the device's current stream, with that device current.  (The raw handles: a token's call
+    takes longer on the host than on the GPU, and the stream object alone was a sixth of it.)"""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(device):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def rows_contiguous(t: torch.Tensor) -> torch.Tensor:
@@ -46,45 +45,48 @@ def rows_contiguous(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _check_common(gi, candidate, dims, layout):
+def _check_common(gi, candidate, dims, layout) -> Tuple[int, ...]:
     if not isinstance(gi, torch.Tensor):
         raise ValueError("gi must be a tensor")
     if candidate not in _CANDIDATES:
         raise ValueError(f"candidate must be 'tanh' or 'identity'; got {candidate!r}")
     if gi.dtype not in DTYPES:
         raise ValueError(f"gi dtype must be float32, bfloat16 or float16; got {gi.dtype}")
-    if gi.dim() != dims or gi.shape[-1] % 2 != 0:
-        raise ValueError(f"gi must be {layout}; got {tuple(gi.shape)}")
+    shape = gi.shape
+    if len(shape) != dims or shape[-1] % 2 != 0:
+        raise ValueError(f"gi must be {layout}; got {tuple(shape)}")
+    return shape
 
 
 def _check_state(name, h, B, H):
     if h.dtype != torch.float32:
         raise ValueError(f"{name} dtype must be float32; got {h.dtype}")
-    if tuple(h.shape) != (B, H):
+    if h.shape != (B, H):
         raise ValueError(f"{name} shape must be (B, H)=({B}, {H}); got {tuple(h.shape)}")
 
 
-def _check_devices(gi, others):
-    require_cuda(gi=gi, **others)
-    for name, t in others.items():
-        if t.device != gi.device:
-            raise ValueError(f"{name} is on {t.device}, gi on {gi.device}")
+def _check_devices(gi, names, others):
+    if not gi.is_cuda or any(t is not None and t.device != gi.device for t in others):
+        given = {n: t for n, t in zip(names, others) if t is not None}
+        require_cuda(gi=gi, **given)
+        for name, t in given.items():
+            if t.device != gi.device:
+                raise ValueError(f"{name} is on {t.device}, gi on {gi.device}")
 
 
 def _check_scan(gi, h0, lengths, candidate) -> None:
-    _check_common(gi, candidate, 3, "[T, B, 2H]")
-    T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
+    T, B, two_h = _check_common(gi, candidate, 3, "[T, B, 2H]")
+    H = two_h // 2
     if T == 0 or B == 0 or H == 0:
         raise ValueError(f"T, B and H must be > 0; got T={T}, B={B}, H={H}")
-    given = {k: v for k, v in (("h0", h0), ("lengths", lengths)) if v is not None}
     if h0 is not None:
         _check_state("h0", h0, B, H)
     if lengths is not None:
         if lengths.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"lengths dtype must be int32 or int64; got {lengths.dtype}")
-        if tuple(lengths.shape) != (B,):
+        if lengths.shape != (B,):
             raise ValueError(f"lengths shape must be (B,)=({B},); got {tuple(lengths.shape)}")
-    _check_devices(gi, given)
+    _check_devices(gi, ("h0", "lengths"), (h0, lengths))
 
 
 def _empty_like_rows(gi: torch.Tensor, cols: int) -> torch.Tensor:
@@ -97,10 +99,11 @@ def _empty_like_rows(gi: torch.Tensor, cols: int) -> torch.Tensor:
 
 def _fill(gi, h0, lengths, candidate) -> _lib.CGatedArgs:
     a = _lib.CGatedArgs()
-    a.T, a.B = gi.shape[0], gi.shape[1]
-    a.H = gi.shape[2] // 2
+    a.T, a.B, two_h = gi.shape
+    a.H = two_h // 2
     a.dtype, a.candidate_tanh = DTYPES[gi.dtype], _CANDIDATES[candidate]
-    a.gi, a.gi_t, a.gi_b = gi.data_ptr(), gi.stride(0), gi.stride(1)
+    a.gi = gi.data_ptr()
+    a.gi_t, a.gi_b, _ = gi.stride()
     if h0 is not None:
         a.h0, a.h0_b = h0.data_ptr(), h0.stride(0)
     if lengths is not None:
@@ -120,10 +123,11 @@ def _forward(gi, h0, lengths, candidate, want_states: bool):
     if want_states:
         states = torch.empty((lib.b200gru_gated_states_bytes(T, B, H) // 4,), device=gi.device, dtype=torch.float32)
     a = _fill(gi, h0, lengths, candidate)
-    a.out, a.out_t, a.out_b, a.h_T = out.data_ptr(), out.stride(0), out.stride(1), h_T.data_ptr()
-    a.states = None if states is None else states.data_ptr()
-    with on_device(gi.device):
-        rc = lib.b200gru_gated_scan_forward(ctypes.byref(a), stream_of(gi.device))
+    a.out, a.h_T = out.data_ptr(), h_T.data_ptr()
+    a.out_t, a.out_b, _ = out.stride()
+    if states is not None:
+        a.states = states.data_ptr()
+    rc = call_on(gi.device, lib.b200gru_gated_scan_forward, ctypes.byref(a))
     if rc:
         _lib._raise(rc, "gated scan forward")
     _lib._after_call()
@@ -140,14 +144,16 @@ def _backward(gi, h0, lengths, candidate, states, dout, dh_T, want_h0: bool):
     a.states = states.data_ptr()
     if dout is not None:
         dout = rows_contiguous(dout)
-        a.dout, a.dout_t, a.dout_b = dout.data_ptr(), dout.stride(0), dout.stride(1)
+        a.dout = dout.data_ptr()
+        a.dout_t, a.dout_b, _ = dout.stride()
     if dh_T is not None:
         dh_T = rows_contiguous(dh_T)
         a.dh_T, a.dh_b = dh_T.data_ptr(), dh_T.stride(0)
-    a.dgi, a.dgi_t, a.dgi_b = dgi.data_ptr(), dgi.stride(0), dgi.stride(1)
-    a.dh0 = None if dh0 is None else dh0.data_ptr()
-    with on_device(gi.device):
-        rc = lib.b200gru_gated_scan_backward(ctypes.byref(a), stream_of(gi.device))
+    a.dgi = dgi.data_ptr()
+    a.dgi_t, a.dgi_b, _ = dgi.stride()
+    if dh0 is not None:
+        a.dh0 = dh0.data_ptr()
+    rc = call_on(gi.device, lib.b200gru_gated_scan_backward, ctypes.byref(a))
     if rc:
         _lib._raise(rc, "gated scan backward")
     _lib._after_call()
@@ -192,22 +198,20 @@ def gated_step(gi: torch.Tensor, h: torch.Tensor, *, candidate: str = "tanh",
 
     The new state goes into ``out_state`` where given, which may be ``h`` itself (update in place).  Serving only: it has
     no gradients; ``gated_scan`` of one step has."""
-    _check_common(gi, candidate, 2, "[B, 2H]")
-    B, H = gi.shape[0], gi.shape[1] // 2
+    B, two_h = _check_common(gi, candidate, 2, "[B, 2H]")
+    H = two_h // 2
     if B == 0 or H == 0:
         raise ValueError(f"B and H must be > 0; got B={B}, H={H}")
     _check_state("h", h, B, H)
-    given = {"h": h}
     if out_state is not None:
         _check_state("out_state", out_state, B, H)
-        given["out_state"] = out_state
-    _check_devices(gi, given)
+    _check_devices(gi, ("h", "out_state"), (h, out_state))
     if torch.is_grad_enabled() and (gi.requires_grad or h.requires_grad):
         raise ValueError("gated_step has no gradients: call it under torch.no_grad(), or gated_scan on gi[None]")
-    gi = rows_contiguous(gi)
+    gi, device = rows_contiguous(gi), gi.device
     if out_state is None:
         h = rows_contiguous(h)
-        new = torch.empty((B, H), device=gi.device, dtype=torch.float32)
+        new = torch.empty((B, H), device=device, dtype=torch.float32)
     else:
         new = out_state
         if (new.stride(1) != 1 and H > 1) or (B > 1 and new.stride(0) < H):
@@ -218,11 +222,9 @@ def gated_step(gi: torch.Tensor, h: torch.Tensor, *, candidate: str = "tanh",
         if _overlap(new, gi):
             raise ValueError("out_state must not overlap gi")
         h = h if same else rows_contiguous(h)
-    out = torch.empty((B, H), device=gi.device, dtype=gi.dtype)
-    with on_device(gi.device):
-        rc = _lib.load().b200gru_gated_step(DTYPES[gi.dtype], _CANDIDATES[candidate], B, H, gi.data_ptr(), gi.stride(0),
-                                            h.data_ptr(), h.stride(0), out.data_ptr(), new.data_ptr(),
-                                            max(new.stride(0), H), stream_of(gi.device))
+    out = torch.empty((B, H), device=device, dtype=gi.dtype)
+    rc = call_on(device, _lib.load().b200gru_gated_step, DTYPES[gi.dtype], _CANDIDATES[candidate], B, H, gi.data_ptr(),
+                 gi.stride(0), h.data_ptr(), h.stride(0), out.data_ptr(), new.data_ptr(), max(new.stride(0), H))
     if rc:
         _lib._raise(rc, "gated step")
     return out, new
