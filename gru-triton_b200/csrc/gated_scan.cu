@@ -3,8 +3,8 @@
 //   z = sigmoid(x)   n = tanh(c) or c   h_t = z h_{t-1} + (1 - z) n        gi[t,b,:] = (x[H], c[H])
 //
 // Each (row, unit) is a chain of its own whose steps are affine maps h -> z h + u.  Maps compose,
-// (A2, b2) o (A1, b1) = (A2 A1, A2 b1 + b2), so time is cut: a thread folds eight steps of two units, a CTA a tile (64 steps
-// of 64 units, or 128 of 32), and a cluster of up to 8 CTAs takes that many tiles of the same units at once.  Maps are joined in
+// (A2, b2) o (A1, b1) = (A2 A1, A2 b1 + b2), so time is cut: a thread folds 8 or 16 steps of two units, a CTA a tile (64 steps
+// of 64 units; where rows are few 128), and a cluster of up to 8 CTAs takes that many tiles of the same units at once.  Maps are joined in
 // the order of time at every level (through shared memory, then through the cluster's), never in the order of arrival.
 // The backward pass is the same scan in the other direction, G_t = z_t (dout_t + G_{t+1}), with the same products of z; it
 // recomputes the states of a tile from the one that the forward kept, so `out` is not read again.
@@ -24,15 +24,22 @@ __device__ int g_gated_status;
 
 namespace {
 
-constexpr int THREADS = 256;
 constexpr int MAX_CLUSTER = 8;
 constexpr int STAGES_MAX = 4;
 
-// LANES threads side by side have a row's units of the tile (two each), THREADS / LANES of them one behind the other its steps.
-template <int LANES>
+// L threads side by side have the units of a tile (two each), P of them one behind the other its steps (S each).
+template <int L, int P, int S>
 struct Tile {
-  static constexpr int UNITS = 2 * LANES, PARTS = THREADS / LANES, STEPS = PARTS * SEG;
+  static constexpr int LANES = L, PARTS = P, SEG = S, THREADS = L * P, UNITS = 2 * L, STEPS = P * S, WARPS = THREADS / 32;
 };
+// Forward: 16 steps a thread, which halves what a round costs beside its elements (2048 x 64 x 1024, bf16: 197 -> 175 us against
+// 8); the backward has no registers for more than 8.
+typedef Tile<32, 4, 16> Forward;
+typedef Tile<32, 8, 8> Backward;
+// Few rows: 128 steps of 32 units, which makes twice as many CTAs (32768 x 1 x 1024: 87 us against 165 with 64 units and half the
+// CTAs); a warp has two parts, one behind the other.
+typedef Tile<16, 16, 8> Narrow;
+static_assert(Forward::STEPS == Backward::STEPS, "states lie between tiles of both directions");
 
 // ---- element access: FAST = two adjacent units per lane (aligned), else units `lane` and `lane + LANES`
 template <typename T> struct Pair;
@@ -89,6 +96,7 @@ struct __align__(16) Map {
 // The map `m` after the map `first`.
 __device__ __forceinline__ Map after(const Map& m, const Map& first) { return {mul2(m.A, first.A), fma2(m.A, first.b, m.b)}; }
 __device__ __forceinline__ P2 apply(const Map& m, P2 h) { return fma2(m.A, h, m.b); }
+__device__ __forceinline__ P2 from_other_half(P2 v) { return P2{__shfl_xor_sync(0xffffffffu, v.v, 16)}; }
 
 // ---- cluster exchange ----------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -111,10 +119,10 @@ __device__ __forceinline__ void send16(uint32_t dst, const Map& m, uint32_t bar)
                ::"r"(dst), "l"(m.A.v), "l"(m.b.v), "r"(bar) : "memory");
 }
 
-template <int LANES>
+template <typename Cut>
 struct Shared {
-  Map part[2][Tile<LANES>::PARTS][LANES];      // maps of the threads
-  P2 carry[2][LANES];                          // what enters the round
+  Map part[2][Cut::WARPS][Cut::LANES];         // maps of the warps
+  P2 carry[2][Cut::LANES];                     // what enters the round
   unsigned long long full[STAGES_MAX];       // a stage of inputs has landed
   unsigned long long joined[2];              // maps of all ranks have landed
   int dead;
@@ -140,8 +148,9 @@ __device__ __forceinline__ Place place_of(const Args& a, int ranks) {
   return w;
 }
 
-template <int LANES>
-__device__ __forceinline__ void set_up(Shared<LANES>& s, int stages, int ranks) {
+template <typename Cut>
+__device__ __forceinline__ void set_up(Shared<Cut>& s, int stages, int ranks) {
+  constexpr int LANES = Cut::LANES;
   if (threadIdx.x == 0) {
     s.dead = 0;
     for (int i = 0; i < stages; ++i) tc::mbar_init(tc::smem_u32(&s.full[i]), 1);
@@ -156,16 +165,18 @@ __device__ __forceinline__ void set_up(Shared<LANES>& s, int stages, int ranks) 
 
 // One part of the threads (all of a CTA's units) sends the CTA's map to every rank.  A slot is used again two rounds later: a
 // peer sends its map of the round between only after all its threads have read this round's, so two slots are enough.
-template <int LANES>
-__device__ __forceinline__ void send_map(Shared<LANES>& s, Map* peers, const Place& w, int round, Map all, int lane) {
+template <typename Cut>
+__device__ __forceinline__ void send_map(Shared<Cut>& s, Map* peers, const Place& w, int round, Map all, int lane) {
+  constexpr int LANES = Cut::LANES;
   const int slot = round & 1;
   const uint32_t to = tc::smem_u32(peers + (slot * w.ranks + w.rank) * LANES + lane), bar = tc::smem_u32(&s.joined[slot]);
   for (int r = 0; r < w.ranks; ++r) send16(at_rank(to, (uint32_t)r), all, at_rank(bar, (uint32_t)r));
 }
 // What enters this CTA's tile: the round's carry through the maps of the ranks before it.  Part 1 folds on through all of
 // them, which is what the next round starts from.
-template <int LANES>
-__device__ __forceinline__ P2 join(Shared<LANES>& s, const Map* peers, const Place& w, int round, int part, int lane) {
+template <typename Cut>
+__device__ __forceinline__ P2 join(Shared<Cut>& s, const Map* peers, const Place& w, int round, int part, int lane) {
+  constexpr int LANES = Cut::LANES;
   const int slot = round & 1;
   tc::mbar_wait(tc::smem_u32(&s.joined[slot]), (uint32_t)(round >> 1) & 1u, &s.dead, &g_gated_status);
   if (threadIdx.x == 0) tc::mbar_expect_tx(tc::smem_u32(&s.joined[slot]), (uint32_t)(w.ranks * LANES * sizeof(Map)));
@@ -176,6 +187,20 @@ __device__ __forceinline__ P2 join(Shared<LANES>& s, const Map* peers, const Pla
     P2 end = h;
     for (int r = w.rank; r < w.ranks; ++r) end = apply(m[r * LANES], end);
     s.carry[slot ^ 1][lane] = end;
+  }
+  return h;
+}
+
+// What enters this warp: h through the maps of the warps before it (v = 0 .. warp - 1, or the last .. warp + 1 where BACK).
+template <bool BACK, int WARPS, int LANES>
+__device__ __forceinline__ P2 through(const Map* m, int warp, P2 h) {
+  Map all[WARPS];
+#pragma unroll
+  for (int v = 0; v < WARPS; ++v) all[v] = m[v * LANES];
+#pragma unroll
+  for (int i = 0; i < WARPS - 1; ++i) {
+    const int v = BACK ? WARPS - 1 - i : i;
+    if (BACK ? v > warp : v < warp) h = apply(all[v], h);
   }
   return h;
 }
@@ -200,18 +225,19 @@ __device__ __forceinline__ void tear_down(const volatile int* dead, int ranks) {
 }
 
 // ---- forward -------------------------------------------------------------------------------------
-// A round's phases: gates and maps of the threads | barrier | the state that enters, the results.  CLUSTERED: the gates of the next
-// round are computed while the maps of this one travel (two sets of registers, two CTAs to an SM); otherwise a third CTA
-// covers for the barrier.
-template <typename T, int LANES, bool FAST, bool TANH, bool CLUSTERED>
-__global__ void __launch_bounds__(THREADS, CLUSTERED ? 2 : 3)
+// A round's phases: gates and maps of the threads | barrier | the state that enters, the results.  AHEAD: the gates of the next
+// round are computed while the maps of this one travel through the cluster (two sets of registers: where rows are few, a CTA
+// or two to an SM are all there are); otherwise other CTAs of the SM cover for the barrier.
+template <typename T, typename Cut, bool FAST, bool TANH, bool CLUSTERED, bool AHEAD>
+__global__ void __launch_bounds__(Cut::THREADS, AHEAD ? 2 : 512 / Cut::THREADS)
 gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int ranks, int stages) {
-  constexpr int UNITS = Tile<LANES>::UNITS, PARTS = Tile<LANES>::PARTS, STEPS = Tile<LANES>::STEPS;
+  constexpr int UNITS = Cut::UNITS, PARTS = Cut::PARTS, STEPS = Cut::STEPS, LANES = Cut::LANES, SEG = Cut::SEG, WARPS = Cut::WARPS;
   extern __shared__ __align__(128) unsigned char raw[];
-  __shared__ Shared<LANES> s;
+  __shared__ Shared<Cut> s;
   T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c][STEPS][UNITS]
   Map* peers = reinterpret_cast<Map*>(raw + (size_t)stages * 2 * STEPS * UNITS * sizeof(T));
-  const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES, warp = tc::uniform_warp();
+  const bool second = LANES == 16 && (threadIdx.x & 16) != 0;  // the later of the warp's two parts
   if (!CLUSTERED) ranks = 1;
   const Place w = place_of<UNITS>(a, ranks);
   const int len = row_length(a, w.b);
@@ -243,7 +269,7 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
   Ring at = {0, 0};
 
   // gates of a round into z and u, the thread's map into shared memory
-  auto open_gates = [&](int round, P2 (&z)[SEG], P2 (&u)[SEG]) {
+  auto open_gates = [&](int round, P2 (&z)[SEG], P2 (&u)[SEG], Map& first) {
     const int tile = round * ranks + w.rank;
     const int t0 = tile * STEPS + part * SEG;
     const int n = len - t0;                                   // steps left from here
@@ -279,16 +305,24 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
         b = fma2(z[k], b, u[k]);
       }
     }
-    s.part[round & 1][part][lane] = Map{A, b};
+    first = Map{A, b};
+    if (LANES == 16) {                                        // `first`: the earlier part's map, in both
+      const Map other = {from_other_half(A), from_other_half(b)};
+      const Map later = second ? first : other;
+      if (second) first = other;
+      A = mul2(later.A, first.A);
+      b = fma2(later.A, first.b, later.b);
+    }
+    if (!second) s.part[round & 1][warp][lane] = Map{A, b};
   };
   // results of a round from the state that enters its tile
-  auto walk = [&](int round, P2 h, const P2 (&z)[SEG], const P2 (&u)[SEG]) {
+  auto walk = [&](int round, P2 h, const P2 (&z)[SEG], const P2 (&u)[SEG], const Map& first) {
     const int tile = round * ranks + w.rank;
     if (tile >= tiles) return;
     if (a.states != nullptr && part == 0)
       store_state<FAST, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left, h);
-    const Map* m = &s.part[round & 1][0][lane];
-    for (int v = 0; v < part; ++v) h = apply(m[v * LANES], h);
+    h = through<false, WARPS, LANES>(&s.part[round & 1][0][lane], warp, h);
+    if (second) h = apply(first, h);
     const int t0 = tile * STEPS + part * SEG, n = len - t0;
     T* o = op + (long long)t0 * a.out_t;
     if (n >= SEG) {
@@ -308,34 +342,38 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
     if (!CLUSTERED && part == PARTS - 1) s.carry[(round & 1) ^ 1][lane] = h;
   };
 
-  if (CLUSTERED) {
-    auto round_of = [&](int round, const P2 (&z)[SEG], const P2 (&u)[SEG], P2 (&zn)[SEG], P2 (&un)[SEG]) {
-      __syncthreads();                                        // the stage is read, the threads' maps are there
-      if (part == 0) {
-        Map all = s.part[round & 1][0][lane];
+  auto send = [&](int round) {                                // part 0: the CTA's map to every rank
+    Map all = s.part[round & 1][0][lane];
 #pragma unroll
-        for (int v = 1; v < PARTS; ++v) all = after(s.part[round & 1][v][lane], all);
-        send_map(s, peers, w, round, all, lane);
-      }
+    for (int v = 1; v < WARPS; ++v) all = after(s.part[round & 1][v][lane], all);
+    send_map(s, peers, w, round, all, lane);
+  };
+  if (AHEAD) {
+    auto round_of = [&](int round, const P2 (&z)[SEG], const P2 (&u)[SEG], const Map& m, P2 (&zn)[SEG], P2 (&un)[SEG], Map& mn) {
+      __syncthreads();                                        // the stage is read, the threads' maps are there
+      if (part == 0) send(round);
       if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
       at.next(stages);
-      if (round + 1 < rounds) open_gates(round + 1, zn, un);
-      walk(round, join(s, peers, w, round, part, lane), z, u);
+      if (round + 1 < rounds) open_gates(round + 1, zn, un, mn);
+      walk(round, join(s, peers, w, round, part, lane), z, u, m);
     };
     P2 za[SEG], ua[SEG], zb[SEG], ub[SEG];
-    if (rounds > 0) open_gates(0, za, ua);
+    Map ma, mb;
+    if (rounds > 0) open_gates(0, za, ua, ma);
     for (int round = 0; round < rounds; round += 2) {
-      round_of(round, za, ua, zb, ub);
-      if (round + 1 < rounds) round_of(round + 1, zb, ub, za, ua);
+      round_of(round, za, ua, ma, zb, ub, mb);
+      if (round + 1 < rounds) round_of(round + 1, zb, ub, mb, za, ua, ma);
     }
   } else {
     for (int round = 0; round < rounds; ++round) {
       P2 z[SEG], u[SEG];
-      open_gates(round, z, u);
+      Map first;
+      open_gates(round, z, u, first);
       __syncthreads();
+      if (CLUSTERED && part == 0) send(round);
       if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
       at.next(stages);
-      walk(round, s.carry[round & 1][lane], z, u);
+      walk(round, CLUSTERED ? join(s, peers, w, round, part, lane) : s.carry[round & 1][lane], z, u, first);
     }
   }
 
@@ -351,17 +389,18 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
 // ---- backward ------------------------------------------------------------------------------------
 // Tiles from the last to the first; rank 0 of a round has the latest.  `front` joins the states inside a tile forwards, `part`
 // the gradients backwards, both with the same products of z.
-template <typename T, int LANES, bool FAST, bool TANH, bool CLUSTERED>
-__global__ void __launch_bounds__(THREADS, 2)
+template <typename T, typename Cut, bool FAST, bool TANH, bool CLUSTERED>
+__global__ void __launch_bounds__(Cut::THREADS, 2)
 gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap dmap, const Args a, int ranks,
                  int stages) {
-  constexpr int UNITS = Tile<LANES>::UNITS, PARTS = Tile<LANES>::PARTS, STEPS = Tile<LANES>::STEPS;
+  constexpr int UNITS = Cut::UNITS, PARTS = Cut::PARTS, STEPS = Cut::STEPS, LANES = Cut::LANES, SEG = Cut::SEG, WARPS = Cut::WARPS;
   extern __shared__ __align__(128) unsigned char raw[];
-  __shared__ Shared<LANES> s;
-  __shared__ P2 front[2][PARTS][LANES];
+  __shared__ Shared<Cut> s;
+  __shared__ P2 front[2][WARPS][LANES];
   T* ring = reinterpret_cast<T*>(raw);                        // [stages][x, c, dout][STEPS][UNITS]
   Map* peers = reinterpret_cast<Map*>(raw + (size_t)stages * 3 * STEPS * UNITS * sizeof(T));
-  const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const int part = threadIdx.x / LANES, lane = threadIdx.x % LANES, warp = tc::uniform_warp();
+  const bool second = LANES == 16 && (threadIdx.x & 16) != 0;  // the later of the warp's two parts
   if (!CLUSTERED) ranks = 1;
   const Place w = place_of<UNITS>(a, ranks);
   const int len = row_length(a, w.b);
@@ -441,19 +480,35 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
       for (int k = SEG - 1; k >= 0; --k) r = mul2(z[k], add2(d[k], r));
     }
     const int slot = round & 1;
-    s.part[slot][part][lane] = Map{A, r};
-    front[slot][part][lane] = f;
+    Map back = {A, r};                                        // gradients: from the later part to the earlier one
+    P2 A0 = A, f0 = f;                                        // states: the earlier part's
+    if (LANES == 16) {
+      const P2 oA = from_other_half(A), orr = from_other_half(r), of = from_other_half(f);
+      const Map early = second ? Map{oA, orr} : back, late = second ? back : Map{oA, orr};
+      A0 = early.A;
+      f0 = second ? of : f;
+      const P2 f1 = second ? f : of;
+      back = late;                                            // for the earlier part
+      if (!second) {
+        s.part[slot][warp][lane] = after(early, late);
+        front[slot][warp][lane] = fma2(late.A, f0, f1);
+      }
+    } else {
+      s.part[slot][warp][lane] = back;
+      front[slot][warp][lane] = f;
+    }
     __syncthreads();
     const Map* m = &s.part[slot][0][lane];
     if (CLUSTERED && part == 0) {
-      Map all = m[(PARTS - 1) * LANES];
+      Map all = m[(WARPS - 1) * LANES];
 #pragma unroll
-      for (int v = PARTS - 2; v >= 0; --v) all = after(m[v * LANES], all);
+      for (int v = WARPS - 2; v >= 0; --v) all = after(m[v * LANES], all);
       send_map(s, peers, w, round, all, lane);
     }
     if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
     at.next(stages);
-    for (int v = 0; v < part; ++v) h = fma2(m[v * LANES].A, h, front[slot][v][lane]);
+    for (int v = 0; v < warp; ++v) h = fma2(m[v * LANES].A, h, front[slot][v][lane]);
+    if (second) h = fma2(A0, h, f0);
     if (tile >= 0) {
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
@@ -463,7 +518,8 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     }
     P2 G = CLUSTERED ? join(s, peers, w, round, part, lane) : s.carry[slot][lane];
     if (tile >= 0) {
-      for (int v = PARTS - 1; v > part; --v) G = apply(m[v * LANES], G);
+      G = through<true, WARPS, LANES>(m, warp, G);
+      if (LANES == 16 && !second) G = apply(back, G);
       T* o = qp + (long long)t0 * a.dgi_t;
 #pragma unroll
       for (int k = SEG - 1; k >= 0; --k) {
@@ -489,7 +545,9 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
 }
 
 // ---- a few steps -----------------------------------------------------------------------------------
-// At most SEG steps: a warp has 64 units of a row and all their steps, nothing to join.
+constexpr int SHORT = 8;
+
+// At most SHORT steps: a warp has 64 units of a row and all their steps, nothing to join.
 template <typename T, bool FAST, bool TANH>
 __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
   const int lane = threadIdx.x & 31, columns = (a.H + 63) / 64;
@@ -503,15 +561,15 @@ __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
   if (a.h0 != nullptr) h = load_state<FAST, 32>(a.h0 + (long long)b * a.h0_b + unit, lane, left);
   if (a.states != nullptr) store_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left, h);
   const Constants K = constants();
-  P2 x[SEG], c[SEG];
+  P2 x[SHORT], c[SHORT];
 #pragma unroll
-  for (int k = 0; k < SEG; ++k)
+  for (int k = 0; k < SHORT; ++k)
     if (k < len) {
       x[k] = load_units<FAST, 32>(gp + (long long)k * a.gi_t, lane, left);
       c[k] = load_units<FAST, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
     }
 #pragma unroll
-  for (int k = 0; k < SEG; ++k)
+  for (int k = 0; k < SHORT; ++k)
     if (k < a.T) {
       P2 o = both(0.f);
       if (k < len) {
@@ -538,9 +596,9 @@ __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
   if (a.dh_T != nullptr) G = load_state<FAST, 32>(a.dh_T + (long long)b * a.dh_b + unit, lane, left);
   P2 h = load_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left);
   const Constants K = constants();
-  P2 z[SEG], p[SEG], q[SEG], d[SEG];
+  P2 z[SHORT], p[SHORT], q[SHORT], d[SHORT];
 #pragma unroll
-  for (int k = 0; k < SEG; ++k) {
+  for (int k = 0; k < SHORT; ++k) {
     d[k] = both(0.f);
     if (k < len) {
       const P2 x = load_units<FAST, 32>(gp + (long long)k * a.gi_t, lane, left);
@@ -554,7 +612,7 @@ __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
     }
   }
 #pragma unroll
-  for (int k = SEG - 1; k >= 0; --k)
+  for (int k = SHORT - 1; k >= 0; --k)
     if (k < a.T) {
       P2 dx = both(0.f), dc = dx;
       if (k < len) {
@@ -600,32 +658,32 @@ template <typename T>
 bool paired(const void* p, long long st, long long sb) {
   return (reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1)) == 0 && st % 2 == 0 && sb % 2 == 0;
 }
-template <typename T, int LANES>
+template <typename T, typename Cut>
 int tile_map(CUtensorMap* map, const void* p, long long units, const Args& a, long long st, long long sb) {
   const unsigned long long row = a.B == 1 ? 16 : (unsigned long long)sb * sizeof(T);
   return tc::make_tensor_map_rows(map, MapType<T>::value, p, units, a.B, a.T, row, (unsigned long long)st * sizeof(T),
-                                  Tile<LANES>::UNITS, Tile<LANES>::STEPS);
+                                  Cut::UNITS, Cut::STEPS);
 }
 
-// Tiles of 32 units where 64 leave most of the GPU idle even with full clusters.
-bool narrow(int T, int B, int H) { return T > Tile<32>::STEPS && (long long)B * cdiv(H, Tile<32>::UNITS) * MAX_CLUSTER < 2 * 148; }
+// Few rows: full clusters of 64-unit tiles would leave SMs without work.
+bool narrow(int T, int B, int H) { return T > Forward::STEPS && (long long)B * cdiv(H, Forward::UNITS) * MAX_CLUSTER < 2 * 148; }
 
 // CTAs of a row's units: one, or as many as it takes to fill the GPU, up to the row's tiles.
-template <int LANES>
+template <typename Cut>
 int ranks_for(const Args& a, int ctas) {
-  const long long base = (long long)a.B * cdiv(a.H, Tile<LANES>::UNITS);
-  const int tiles = cdiv(a.T, Tile<LANES>::STEPS);
+  const long long base = (long long)a.B * cdiv(a.H, Cut::UNITS);
+  const int tiles = cdiv(a.T, Cut::STEPS);
   int ranks = 1;
   while (ranks < MAX_CLUSTER && ranks < tiles && base * ranks < ctas) ranks *= 2;
   return ranks;
 }
 
 template <typename... KArgs, typename... CArgs>
-int launch_tiles(void (*kernel)(KArgs...), long long blocks, int ranks, size_t smem, cudaStream_t st, CArgs... args) {
+int launch_tiles(void (*kernel)(KArgs...), long long blocks, int threads, int ranks, size_t smem, cudaStream_t st, CArgs... args) {
   if (allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem) != B200GRU_OK) return B200GRU_UNSUPPORTED;
   if (blocks > 0x7fffffffll) return B200GRU_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)blocks); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
@@ -636,56 +694,62 @@ int launch_tiles(void (*kernel)(KArgs...), long long blocks, int ranks, size_t s
 }
 
 // Stages of `stage` bytes that fit beside the rest where `ctas` CTAs share an SM's 227 KB.
-template <int LANES>
-int stages_for(size_t stage, size_t fixed, int ranks, int ctas) {
-  const size_t room = 227 * 1024 / ctas - 1024 - fixed - peer_bytes<LANES>(ranks);
+int stages_for(size_t stage, size_t fixed, int ctas) {
+  const size_t room = 227 * 1024 / ctas - 1024 - fixed;
   const int n = (int)(room / stage);
   return n < 1 ? 1 : (n > STAGES_MAX ? STAGES_MAX : n);
 }
 
-template <typename T, int LANES, bool TANH>
+template <typename T, typename Cut, bool FAST, bool TANH>
+int forward_cut(const Args& a, const CUtensorMap& map, int ranks, int stages, cudaStream_t st) {
+  constexpr bool AHEAD = Cut::STEPS == Narrow::STEPS;
+  const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS) * ranks;
+  const size_t smem = (size_t)stages * 2 * Cut::STEPS * Cut::UNITS * sizeof(T) + peer_bytes<Cut::LANES>(ranks);
+  return ranks > 1 ? launch_tiles(gated_fwd_kernel<T, Cut, FAST, TANH, true, AHEAD>, blocks, Cut::THREADS, ranks, smem, st, map, a, ranks, stages)
+                   : launch_tiles(gated_fwd_kernel<T, Cut, FAST, TANH, false, false>, blocks, Cut::THREADS, 1, smem, st, map, a, 1, stages);
+}
+template <typename T, typename Cut, bool TANH>
 int forward_tiles(const Args& a, cudaStream_t st) {
-  const int ranks = ranks_for<LANES>(a, 3 * 148);
-  const long long blocks = (long long)a.B * cdiv(a.H, Tile<LANES>::UNITS) * ranks;
-  const size_t peers = peer_bytes<LANES>(ranks);
+  const int share = Cut::STEPS == Narrow::STEPS ? 2 : 512 / Cut::THREADS;       // CTAs to an SM
+  const int ranks = ranks_for<Cut>(a, share * 148);
   alignas(64) CUtensorMap map;
   memset(&map, 0, sizeof(map));
   if (paired<T>(a.out, a.out_t, a.out_b) && a.H * sizeof(T) % 16 == 0 && tileable<T>(a.gi, a.gi_t, a.gi_b, a.B) &&
-      tile_map<T, LANES>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK) {
-    const size_t stage = (size_t)2 * Tile<LANES>::STEPS * Tile<LANES>::UNITS * sizeof(T);
-    const int stages = stages_for<LANES>(stage, sizeof(Shared<LANES>), ranks, ranks > 1 ? 2 : 3);
-    return ranks > 1 ? launch_tiles(gated_fwd_kernel<T, LANES, true, TANH, true>, blocks, ranks, stages * stage + peers, st, map, a, ranks, stages)
-                     : launch_tiles(gated_fwd_kernel<T, LANES, true, TANH, false>, blocks, 1, stages * stage, st, map, a, 1, stages);
+      tile_map<T, Cut>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK) {
+    const size_t stage = (size_t)2 * Cut::STEPS * Cut::UNITS * sizeof(T);
+    const int stages = stages_for(stage, sizeof(Shared<Cut>) + peer_bytes<Cut::LANES>(ranks), share);
+    return forward_cut<T, Cut, true, TANH>(a, map, ranks, stages, st);
   }
-  return ranks > 1 ? launch_tiles(gated_fwd_kernel<T, LANES, false, TANH, true>, blocks, ranks, peers, st, map, a, ranks, 0)
-                   : launch_tiles(gated_fwd_kernel<T, LANES, false, TANH, false>, blocks, 1, 0, st, map, a, 1, 0);
+  return forward_cut<T, Cut, false, TANH>(a, map, ranks, 0, st);
 }
 
-template <typename T, int LANES, bool TANH>
+template <typename T, typename Cut, bool FAST, bool TANH>
+int backward_cut(const Args& a, const CUtensorMap& map, const CUtensorMap& dmap, int ranks, int stages, cudaStream_t st) {
+  const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS) * ranks;
+  const size_t smem = (size_t)stages * 3 * Cut::STEPS * Cut::UNITS * sizeof(T) + peer_bytes<Cut::LANES>(ranks);
+  return ranks > 1 ? launch_tiles(gated_bwd_kernel<T, Cut, FAST, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, dmap, a, ranks, stages)
+                   : launch_tiles(gated_bwd_kernel<T, Cut, FAST, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, dmap, a, 1, stages);
+}
+template <typename T, typename Cut, bool TANH>
 int backward_tiles(const Args& a, cudaStream_t st) {
-  const int ranks = ranks_for<LANES>(a, 2 * 148);
-  const long long blocks = (long long)a.B * cdiv(a.H, Tile<LANES>::UNITS) * ranks;
-  const size_t peers = peer_bytes<LANES>(ranks);
+  const int ranks = ranks_for<Cut>(a, 2 * 148);
   alignas(64) CUtensorMap map, dmap;
   memset(&map, 0, sizeof(map));
   memset(&dmap, 0, sizeof(dmap));
   if (paired<T>(a.dgi, a.dgi_t, a.dgi_b) && a.H * sizeof(T) % 16 == 0 && tileable<T>(a.gi, a.gi_t, a.gi_b, a.B) &&
-      tile_map<T, LANES>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK &&
+      tile_map<T, Cut>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK &&
       (a.dout == nullptr || (tileable<T>(a.dout, a.dout_t, a.dout_b, a.B) &&
-                             tile_map<T, LANES>(&dmap, a.dout, a.H, a, a.dout_t, a.dout_b) == B200GRU_OK))) {
-    const size_t stage = (size_t)3 * Tile<LANES>::STEPS * Tile<LANES>::UNITS * sizeof(T);
-    const size_t fixed = sizeof(Shared<LANES>) + 2 * THREADS * sizeof(P2);
-    const int stages = stages_for<LANES>(stage, fixed, ranks, 2);
-    return ranks > 1 ? launch_tiles(gated_bwd_kernel<T, LANES, true, TANH, true>, blocks, ranks, stages * stage + peers, st, map, dmap, a, ranks, stages)
-                     : launch_tiles(gated_bwd_kernel<T, LANES, true, TANH, false>, blocks, 1, stages * stage, st, map, dmap, a, 1, stages);
+                             tile_map<T, Cut>(&dmap, a.dout, a.H, a, a.dout_t, a.dout_b) == B200GRU_OK))) {
+    const size_t stage = (size_t)3 * Cut::STEPS * Cut::UNITS * sizeof(T);
+    const int stages = stages_for(stage, sizeof(Shared<Cut>) + 2 * Cut::THREADS * sizeof(P2) + peer_bytes<Cut::LANES>(ranks), 2);
+    return backward_cut<T, Cut, true, TANH>(a, map, dmap, ranks, stages, st);
   }
-  return ranks > 1 ? launch_tiles(gated_bwd_kernel<T, LANES, false, TANH, true>, blocks, ranks, peers, st, map, dmap, a, ranks, 0)
-                   : launch_tiles(gated_bwd_kernel<T, LANES, false, TANH, false>, blocks, 1, 0, st, map, dmap, a, 1, 0);
+  return backward_cut<T, Cut, false, TANH>(a, map, dmap, ranks, 0, st);
 }
 
 template <typename T, bool TANH>
 int forward(const Args& a, cudaStream_t st) {
-  if (a.T > SEG) return narrow(a.T, a.B, a.H) ? forward_tiles<T, 16, TANH>(a, st) : forward_tiles<T, 32, TANH>(a, st);
+  if (a.T > SHORT) return narrow(a.T, a.B, a.H) ? forward_tiles<T, Narrow, TANH>(a, st) : forward_tiles<T, Forward, TANH>(a, st);
   const unsigned blocks = (unsigned)(((long long)a.B * cdiv(a.H, 64) + 3) / 4);
   if (a.H % 2 == 0 && paired<T>(a.out, a.out_t, a.out_b) && paired<T>(a.gi, a.gi_t, a.gi_b))
     gated_short_fwd_kernel<T, true, TANH><<<blocks, 128, 0, st>>>(a);
@@ -697,7 +761,7 @@ int forward(const Args& a, cudaStream_t st) {
 
 template <typename T, bool TANH>
 int backward(const Args& a, cudaStream_t st) {
-  if (a.T > SEG) return narrow(a.T, a.B, a.H) ? backward_tiles<T, 16, TANH>(a, st) : backward_tiles<T, 32, TANH>(a, st);
+  if (a.T > SHORT) return narrow(a.T, a.B, a.H) ? backward_tiles<T, Narrow, TANH>(a, st) : backward_tiles<T, Backward, TANH>(a, st);
   const unsigned blocks = (unsigned)(((long long)a.B * cdiv(a.H, 64) + 3) / 4);
   if (a.H % 2 == 0 && paired<T>(a.dgi, a.dgi_t, a.dgi_b) && paired<T>(a.gi, a.gi_t, a.gi_b) &&
       (a.dout == nullptr || paired<T>(a.dout, a.dout_t, a.dout_b)))
@@ -719,7 +783,7 @@ int step(const StepArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-int tile_steps(int T, int B, int H) { return narrow(T, B, H) ? Tile<16>::STEPS : Tile<32>::STEPS; }
+int tile_steps(int T, int B, int H) { return narrow(T, B, H) ? Narrow::STEPS : Forward::STEPS; }
 
 int launch_forward(const Args& a, int dtype, cudaStream_t st) {
   if (dtype == B200GRU_F32) return a.tanh ? forward<float, true>(a, st) : forward<float, false>(a, st);

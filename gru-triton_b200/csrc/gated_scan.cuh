@@ -10,8 +10,6 @@
 namespace b200gru {
 namespace gated {
 
-constexpr int SEG = 8;         // steps that a thread folds
-
 // Strides in elements; the units of a row are contiguous.  h0, dout, dh_T: NULL = zeros.
 struct Args {
   int T, B, H;
