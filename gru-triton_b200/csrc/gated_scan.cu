@@ -13,6 +13,7 @@
 // registers between the fold and the results; inputs arrive by TMA a few tiles ahead.
 
 #include <cstring>
+#include <type_traits>
 
 #include "gated_scan.cuh"
 #include "tc_common.cuh"
@@ -225,11 +226,11 @@ __device__ __forceinline__ void tear_down(const volatile int* dead, int ranks) {
 }
 
 // ---- forward -------------------------------------------------------------------------------------
-// A round's phases: gates and maps of the threads | barrier | the state that enters, the results.  AHEAD: the gates of the next
-// round are computed while the maps of this one travel through the cluster (two sets of registers: where rows are few, a CTA
-// or two to an SM are all there are); otherwise other CTAs of the SM cover for the barrier.
-template <typename T, typename Cut, bool FAST, bool TANH, bool CLUSTERED, bool AHEAD>
-__global__ void __launch_bounds__(Cut::THREADS, AHEAD ? 2 : 512 / Cut::THREADS)
+// A round's phases: gates and maps of the threads | barrier | the state that enters, the results.  CLUSTERED: the gates of the next
+// round are computed while the maps of this one travel (two sets of registers); otherwise other CTAs of the SM cover for the
+// barrier.
+template <typename T, typename Cut, bool FAST, bool TANH, bool CLUSTERED>
+__global__ void __launch_bounds__(Cut::THREADS, 512 / Cut::THREADS)
 gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int ranks, int stages) {
   constexpr int UNITS = Cut::UNITS, PARTS = Cut::PARTS, STEPS = Cut::STEPS, LANES = Cut::LANES, SEG = Cut::SEG, WARPS = Cut::WARPS;
   extern __shared__ __align__(128) unsigned char raw[];
@@ -348,7 +349,7 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
     for (int v = 1; v < WARPS; ++v) all = after(s.part[round & 1][v][lane], all);
     send_map(s, peers, w, round, all, lane);
   };
-  if (AHEAD) {
+  if (CLUSTERED) {
     auto round_of = [&](int round, const P2 (&z)[SEG], const P2 (&u)[SEG], const Map& m, P2 (&zn)[SEG], P2 (&un)[SEG], Map& mn) {
       __syncthreads();                                        // the stage is read, the threads' maps are there
       if (part == 0) send(round);
@@ -370,10 +371,9 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
       Map first;
       open_gates(round, z, u, first);
       __syncthreads();
-      if (CLUSTERED && part == 0) send(round);
       if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
       at.next(stages);
-      walk(round, CLUSTERED ? join(s, peers, w, round, part, lane) : s.carry[round & 1][lane], z, u, first);
+      walk(round, s.carry[round & 1][lane], z, u, first);
     }
   }
 
@@ -665,16 +665,19 @@ int tile_map(CUtensorMap* map, const void* p, long long units, const Args& a, lo
                                   Cut::UNITS, Cut::STEPS);
 }
 
-// Few rows: full clusters of 64-unit tiles would leave SMs without work.
-bool narrow(int T, int B, int H) { return T > Forward::STEPS && (long long)B * cdiv(H, Forward::UNITS) * MAX_CLUSTER < 2 * 148; }
+// Few rows: less than 256 CTAs of 64 units.  Measured on both sides (forward / backward, us): 128 CTAs of 64 units over 3000 steps
+// 78 / 102, as 256 narrow ones 51 / 82; 160 over 600 steps 27 / 37 and 23 / 35; 256 over 400 steps 23 / 29 and 25 / 35.
+bool narrow(int T, int B, int H) { return T > Forward::STEPS && (long long)B * cdiv(H, Forward::UNITS) < 256; }
 
-// CTAs of a row's units: one, or as many as it takes to fill the GPU, up to the row's tiles.
-template <typename Cut>
-int ranks_for(const Args& a, int ctas) {
-  const long long base = (long long)a.B * cdiv(a.H, Cut::UNITS);
-  const int tiles = cdiv(a.T, Cut::STEPS);
+// CTAs of a row's units: a cluster of them where that makes at most 256 CTAs, up to the row's tiles.  An exchange costs about
+// what a tile does, so more pay only where SMs have nothing else (64 narrow CTAs over 2000 steps: 27 / 41 us alone, 18 / 25 in
+// clusters of 4, 23 / 29 of 8).
+int ranks_for(const Args& a) {
+  if (!narrow(a.T, a.B, a.H)) return 1;
+  const long long base = (long long)a.B * cdiv(a.H, Narrow::UNITS);
+  const int tiles = cdiv(a.T, Narrow::STEPS);
   int ranks = 1;
-  while (ranks < MAX_CLUSTER && ranks < tiles && base * ranks < ctas) ranks *= 2;
+  while (ranks < MAX_CLUSTER && ranks < tiles && base * ranks * 2 <= 256) ranks *= 2;
   return ranks;
 }
 
@@ -702,22 +705,22 @@ int stages_for(size_t stage, size_t fixed, int ctas) {
 
 template <typename T, typename Cut, bool FAST, bool TANH>
 int forward_cut(const Args& a, const CUtensorMap& map, int ranks, int stages, cudaStream_t st) {
-  constexpr bool AHEAD = Cut::STEPS == Narrow::STEPS;
   const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS) * ranks;
   const size_t smem = (size_t)stages * 2 * Cut::STEPS * Cut::UNITS * sizeof(T) + peer_bytes<Cut::LANES>(ranks);
-  return ranks > 1 ? launch_tiles(gated_fwd_kernel<T, Cut, FAST, TANH, true, AHEAD>, blocks, Cut::THREADS, ranks, smem, st, map, a, ranks, stages)
-                   : launch_tiles(gated_fwd_kernel<T, Cut, FAST, TANH, false, false>, blocks, Cut::THREADS, 1, smem, st, map, a, 1, stages);
+  if constexpr (std::is_same<Cut, Narrow>::value) {
+    if (ranks > 1) return launch_tiles(gated_fwd_kernel<T, Cut, FAST, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, a, ranks, stages);
+  }
+  return launch_tiles(gated_fwd_kernel<T, Cut, FAST, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, a, 1, stages);
 }
 template <typename T, typename Cut, bool TANH>
 int forward_tiles(const Args& a, cudaStream_t st) {
-  const int share = Cut::STEPS == Narrow::STEPS ? 2 : 512 / Cut::THREADS;       // CTAs to an SM
-  const int ranks = ranks_for<Cut>(a, share * 148);
+  const int ranks = ranks_for(a);
   alignas(64) CUtensorMap map;
   memset(&map, 0, sizeof(map));
   if (paired<T>(a.out, a.out_t, a.out_b) && a.H * sizeof(T) % 16 == 0 && tileable<T>(a.gi, a.gi_t, a.gi_b, a.B) &&
       tile_map<T, Cut>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK) {
     const size_t stage = (size_t)2 * Cut::STEPS * Cut::UNITS * sizeof(T);
-    const int stages = stages_for(stage, sizeof(Shared<Cut>) + peer_bytes<Cut::LANES>(ranks), share);
+    const int stages = stages_for(stage, sizeof(Shared<Cut>) + peer_bytes<Cut::LANES>(ranks), 512 / Cut::THREADS);
     return forward_cut<T, Cut, true, TANH>(a, map, ranks, stages, st);
   }
   return forward_cut<T, Cut, false, TANH>(a, map, ranks, 0, st);
@@ -727,12 +730,14 @@ template <typename T, typename Cut, bool FAST, bool TANH>
 int backward_cut(const Args& a, const CUtensorMap& map, const CUtensorMap& dmap, int ranks, int stages, cudaStream_t st) {
   const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS) * ranks;
   const size_t smem = (size_t)stages * 3 * Cut::STEPS * Cut::UNITS * sizeof(T) + peer_bytes<Cut::LANES>(ranks);
-  return ranks > 1 ? launch_tiles(gated_bwd_kernel<T, Cut, FAST, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, dmap, a, ranks, stages)
-                   : launch_tiles(gated_bwd_kernel<T, Cut, FAST, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, dmap, a, 1, stages);
+  if constexpr (std::is_same<Cut, Narrow>::value) {
+    if (ranks > 1) return launch_tiles(gated_bwd_kernel<T, Cut, FAST, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, dmap, a, ranks, stages);
+  }
+  return launch_tiles(gated_bwd_kernel<T, Cut, FAST, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, dmap, a, 1, stages);
 }
 template <typename T, typename Cut, bool TANH>
 int backward_tiles(const Args& a, cudaStream_t st) {
-  const int ranks = ranks_for<Cut>(a, 2 * 148);
+  const int ranks = ranks_for(a);
   alignas(64) CUtensorMap map, dmap;
   memset(&map, 0, sizeof(map));
   memset(&dmap, 0, sizeof(dmap));
