@@ -42,7 +42,7 @@ typedef Tile<32, 8, 8> Backward;
 typedef Tile<16, 16, 8> Narrow;
 static_assert(Forward::STEPS == Backward::STEPS, "states lie between tiles of both directions");
 
-// ---- element access: FAST = two adjacent units per lane (aligned), else units `lane` and `lane + LANES`
+// ---- element access: PAIRS = two adjacent units per lane (aligned), else units `lane` and `lane + LANES`
 template <typename T> struct Pair;
 template <> struct Pair<float> { typedef float2 type; };
 template <> struct Pair<__nv_bfloat16> { typedef __nv_bfloat162 type; };
@@ -60,15 +60,15 @@ template <> __device__ __forceinline__ __nv_bfloat162 pack<__nv_bfloat16>(float2
 template <> __device__ __forceinline__ __half2 pack<__half>(float2 v) { return __float22half2_rn(v); }
 
 // The lane's two units of a row that starts at p (unit 0 of the CTA); `left`: units of the row from there on.
-template <bool FAST, int LANES, typename T>
+template <bool PAIRS, int LANES, typename T>
 __device__ __forceinline__ P2 load_units(const T* p, int lane, int left) {
-  if (FAST) return 2 * lane < left ? unpack(*reinterpret_cast<const typename Pair<T>::type*>(p + 2 * lane)) : both(0.f);
+  if (PAIRS) return 2 * lane < left ? unpack(*reinterpret_cast<const typename Pair<T>::type*>(p + 2 * lane)) : both(0.f);
   return pair(lane < left ? to_float(p[lane]) : 0.f, lane + LANES < left ? to_float(p[lane + LANES]) : 0.f);
 }
-template <bool FAST, int LANES, typename T>
+template <bool PAIRS, int LANES, typename T>
 __device__ __forceinline__ void store_units(T* p, int lane, int left, P2 pv) {
   const float2 v = split(pv);
-  if (FAST) {
+  if (PAIRS) {
     if (2 * lane < left) *reinterpret_cast<typename Pair<T>::type*>(p + 2 * lane) = pack<T>(v);
   } else {
     if (lane < left) p[lane] = from_float<T>(v.x);
@@ -77,15 +77,15 @@ __device__ __forceinline__ void store_units(T* p, int lane, int left, P2 pv) {
 }
 
 // fp32 states of the lane's units; rows of any alignment.
-template <bool FAST, int LANES>
+template <bool PAIRS, int LANES>
 __device__ __forceinline__ P2 load_state(const float* p, int lane, int left) {
-  const int i = FAST ? 2 * lane : lane, j = FAST ? 2 * lane + 1 : lane + LANES;
+  const int i = PAIRS ? 2 * lane : lane, j = PAIRS ? 2 * lane + 1 : lane + LANES;
   return pair(i < left ? p[i] : 0.f, j < left ? p[j] : 0.f);
 }
-template <bool FAST, int LANES>
+template <bool PAIRS, int LANES>
 __device__ __forceinline__ void store_state(float* p, int lane, int left, P2 pv) {
   const float2 v = split(pv);
-  const int i = FAST ? 2 * lane : lane, j = FAST ? 2 * lane + 1 : lane + LANES;
+  const int i = PAIRS ? 2 * lane : lane, j = PAIRS ? 2 * lane + 1 : lane + LANES;
   if (i < left) p[i] = v.x;
   if (j < left) p[j] = v.y;
 }
@@ -206,6 +206,34 @@ __device__ __forceinline__ P2 through(const Map* m, int warp, P2 h) {
   return h;
 }
 
+// How inputs come: as TMA tiles (rows on 16-byte boundaries); by asynchronous copies of two units, each thread its own; by
+// such copies of single fp32 units; or, 16-bit units on odd boundaries, by loads of the threads.
+enum { BY_TMA = 0, BY_PAIRS = 1, BY_UNITS = 2 };
+template <int MODE> constexpr bool PAIRED = MODE != BY_UNITS;        // a lane has units 2 i and 2 i + 1, not i and i + LANES
+template <int MODE, typename T> constexpr bool OWN_COPIES = MODE == BY_PAIRS || (MODE == BY_UNITS && sizeof(T) == 4);
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+}
+// A thread's SEG rows of its two units into its own places of a stage; behind the row's end the last step again.
+template <int MODE, int SEG, int LANES, typename T>
+__device__ __forceinline__ void copy_own(T* st, const T* p, long long stride, int t0, int len, int lane, int left) {
+#pragma unroll
+  for (int k = 0; k < SEG; ++k) {
+    const T* row = p + (long long)min(t0 + k, len - 1) * stride;
+    T* dst = st + k * 2 * LANES;
+    if (MODE == BY_PAIRS) {
+      if (2 * lane < left) copy_async<2 * sizeof(T)>(dst + 2 * lane, row + 2 * lane);
+    } else {
+      if (lane < left) copy_async<4>(dst + lane, row + lane);
+      if (lane + LANES < left) copy_async<4>(dst + lane + LANES, row + lane + LANES);
+    }
+  }
+}
+__device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_landed_but_last() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
 // Stage of the ring and the phase of its barrier, moved on once a round (a division of the round would cost as much as eight
 // elements).
 struct Ring {
@@ -229,7 +257,7 @@ __device__ __forceinline__ void tear_down(const volatile int* dead, int ranks) {
 // A round's phases: gates and maps of the threads | barrier | the state that enters, the results.  CLUSTERED: the gates of the next
 // round are computed while the maps of this one travel (two sets of registers); otherwise other CTAs of the SM cover for the
 // barrier.
-template <typename T, typename Cut, bool FAST, bool TANH, bool CLUSTERED>
+template <typename T, typename Cut, int MODE, bool TANH, bool CLUSTERED>
 __global__ void __launch_bounds__(Cut::THREADS, 512 / Cut::THREADS)
 gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int ranks, int stages) {
   constexpr int UNITS = Cut::UNITS, PARTS = Cut::PARTS, STEPS = Cut::STEPS, LANES = Cut::LANES, SEG = Cut::SEG, WARPS = Cut::WARPS;
@@ -255,19 +283,31 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
     tc::tma_load_3d(tc::smem_u32(dst), &map, w.unit, w.b, tile * STEPS, bar);
     tc::tma_load_3d(tc::smem_u32(dst + STEPS * UNITS), &map, a.H + w.unit, w.b, tile * STEPS, bar);
   };
-  if (FAST && threadIdx.x == 0)
+  if (MODE == BY_TMA && threadIdx.x == 0)
     for (int r = 0; r < stages; ++r) fetch(r, r);
 
   const T* gp = static_cast<const T*>(a.gi) + (long long)w.b * a.gi_b + w.unit;
   T* op = static_cast<T*>(a.out) + (long long)w.b * a.out_b + w.unit;
   if (part == 0) {
     P2 h = both(0.f);
-    if (a.h0 != nullptr) h = load_state<FAST, LANES>(a.h0 + (long long)w.b * a.h0_b + w.unit, lane, w.left);
+    if (a.h0 != nullptr) h = load_state<PAIRED<MODE>, LANES>(a.h0 + (long long)w.b * a.h0_b + w.unit, lane, w.left);
     s.carry[0][lane] = h;
   }
   const Constants K = constants();
 
   Ring at = {0, 0};
+
+  // a thread's own copies: the next round's are sent before this one's are waited for
+  auto copy_round = [&](int round, int stage) {
+    const int tile = round * ranks + w.rank;
+    if (round < rounds && tile < tiles) {
+      T* st = ring + (size_t)stage * 2 * STEPS * UNITS + part * SEG * UNITS;
+      copy_own<MODE, SEG, LANES>(st, gp, a.gi_t, tile * STEPS + part * SEG, len, lane, w.left);
+      copy_own<MODE, SEG, LANES>(st + STEPS * UNITS, gp + a.H, a.gi_t, tile * STEPS + part * SEG, len, lane, w.left);
+    }
+    copies_sent();
+  };
+  if (OWN_COPIES<MODE, T>) copy_round(0, 0);
 
   // gates of a round into z and u, the thread's map into shared memory
   auto open_gates = [&](int round, P2 (&z)[SEG], P2 (&u)[SEG], Map& first) {
@@ -275,17 +315,19 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
     const int t0 = tile * STEPS + part * SEG;
     const int n = len - t0;                                   // steps left from here
     P2 A = both(1.f), b = both(0.f);
+    if (OWN_COPIES<MODE, T>) copy_round(round + 1, at.stage ^ 1);
     if (tile < tiles) {
-      if (FAST) tc::mbar_wait(tc::smem_u32(&s.full[at.stage]), (uint32_t)at.phase, &s.dead, &g_gated_status);
+      if (MODE == BY_TMA) tc::mbar_wait(tc::smem_u32(&s.full[at.stage]), (uint32_t)at.phase, &s.dead, &g_gated_status);
+      if (OWN_COPIES<MODE, T>) copies_landed_but_last();
       const T* st = ring + (size_t)at.stage * 2 * STEPS * UNITS + part * SEG * UNITS;
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
         P2 x = both(0.f), c = x;
-        if (FAST) {
-          x = load_units<true, LANES>(st + k * UNITS, lane, UNITS);
-          c = load_units<true, LANES>(st + (STEPS + k) * UNITS, lane, UNITS);
-        } else if (k < n) {
-          const T* p = gp + (long long)(t0 + k) * a.gi_t;
+        if (MODE == BY_TMA || OWN_COPIES<MODE, T>) {
+          x = load_units<PAIRED<MODE>, LANES>(st + k * UNITS, lane, UNITS);
+          c = load_units<PAIRED<MODE>, LANES>(st + (STEPS + k) * UNITS, lane, UNITS);
+        } else {                                              // behind the end the last row again: no branch between loads
+          const T* p = gp + (long long)min(t0 + k, len - 1) * a.gi_t;
           x = load_units<false, LANES>(p, lane, w.left);
           c = load_units<false, LANES>(p + a.H, lane, w.left);
         }
@@ -321,7 +363,7 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
     const int tile = round * ranks + w.rank;
     if (tile >= tiles) return;
     if (a.states != nullptr && part == 0)
-      store_state<FAST, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left, h);
+      store_state<PAIRED<MODE>, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left, h);
     h = through<false, WARPS, LANES>(&s.part[round & 1][0][lane], warp, h);
     if (second) h = apply(first, h);
     const int t0 = tile * STEPS + part * SEG, n = len - t0;
@@ -330,14 +372,14 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
         h = fma2(z[k], h, u[k]);
-        store_units<FAST, LANES>(o, lane, w.left, h);
+        store_units<PAIRED<MODE>, LANES>(o, lane, w.left, h);
         o += a.out_t;
       }
     } else {
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
         h = fma2(z[k], h, u[k]);
-        if (k < n) store_units<FAST, LANES>(o + (long long)k * a.out_t, lane, w.left, h);
+        if (k < n) store_units<PAIRED<MODE>, LANES>(o + (long long)k * a.out_t, lane, w.left, h);
       }
     }
     if (!CLUSTERED && part == PARTS - 1) s.carry[(round & 1) ^ 1][lane] = h;
@@ -353,7 +395,7 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
     auto round_of = [&](int round, const P2 (&z)[SEG], const P2 (&u)[SEG], const Map& m, P2 (&zn)[SEG], P2 (&un)[SEG], Map& mn) {
       __syncthreads();                                        // the stage is read, the threads' maps are there
       if (part == 0) send(round);
-      if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
+      if (MODE == BY_TMA && threadIdx.x == 0) fetch(round + stages, at.stage);
       at.next(stages);
       if (round + 1 < rounds) open_gates(round + 1, zn, un, mn);
       walk(round, join(s, peers, w, round, part, lane), z, u, m);
@@ -371,7 +413,7 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
       Map first;
       open_gates(round, z, u, first);
       __syncthreads();
-      if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
+      if (MODE == BY_TMA && threadIdx.x == 0) fetch(round + stages, at.stage);
       at.next(stages);
       walk(round, s.carry[round & 1][lane], z, u, first);
     }
@@ -379,17 +421,17 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
 
   // steps behind the row's last, and the state after it
   for (int t = len + w.rank * PARTS + part; t < a.T; t += ranks * PARTS)
-    store_units<FAST, LANES>(op + (long long)t * a.out_t, lane, w.left, both(0.f));
+    store_units<PAIRED<MODE>, LANES>(op + (long long)t * a.out_t, lane, w.left, both(0.f));
   __syncthreads();
   if (w.rank == 0 && part == 0)
-    store_state<FAST, LANES>(a.h_T + (long long)w.b * a.H + w.unit, lane, w.left, s.carry[rounds & 1][lane]);
+    store_state<PAIRED<MODE>, LANES>(a.h_T + (long long)w.b * a.H + w.unit, lane, w.left, s.carry[rounds & 1][lane]);
   tear_down(&s.dead, ranks);
 }
 
 // ---- backward ------------------------------------------------------------------------------------
 // Tiles from the last to the first; rank 0 of a round has the latest.  `front` joins the states inside a tile forwards, `part`
 // the gradients backwards, both with the same products of z.
-template <typename T, typename Cut, bool FAST, bool TANH, bool CLUSTERED>
+template <typename T, typename Cut, int MODE, bool TANH, bool CLUSTERED>
 __global__ void __launch_bounds__(Cut::THREADS, 2)
 gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap dmap, const Args a, int ranks,
                  int stages) {
@@ -419,7 +461,7 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     tc::tma_load_3d(tc::smem_u32(dst + STEPS * UNITS), &map, a.H + w.unit, w.b, tile * STEPS, bar);
     if (with_dout) tc::tma_load_3d(tc::smem_u32(dst + 2 * STEPS * UNITS), &dmap, w.unit, w.b, tile * STEPS, bar);
   };
-  if (FAST && threadIdx.x == 0)
+  if (MODE == BY_TMA && threadIdx.x == 0)
     for (int r = 0; r < stages; ++r) fetch(r, r);
 
   const T* gp = static_cast<const T*>(a.gi) + (long long)w.b * a.gi_b + w.unit;
@@ -427,13 +469,26 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
   T* qp = static_cast<T*>(a.dgi) + (long long)w.b * a.dgi_b + w.unit;
   if (part == 0) {
     P2 G = both(0.f);
-    if (a.dh_T != nullptr) G = load_state<FAST, LANES>(a.dh_T + (long long)w.b * a.dh_b + w.unit, lane, w.left);
+    if (a.dh_T != nullptr) G = load_state<PAIRED<MODE>, LANES>(a.dh_T + (long long)w.b * a.dh_b + w.unit, lane, w.left);
     s.carry[0][lane] = G;
   }
   const Constants K = constants();
 
   Ring at = {0, 0};
+  auto copy_round = [&](int round, int stage) {
+    const int tile = tiles - 1 - (round * ranks + w.rank);
+    if (round < rounds && tile >= 0) {
+      T* st = ring + (size_t)stage * 3 * STEPS * UNITS + part * SEG * UNITS;
+      const int t0 = tile * STEPS + part * SEG;
+      copy_own<MODE, SEG, LANES>(st, gp, a.gi_t, t0, len, lane, w.left);
+      copy_own<MODE, SEG, LANES>(st + STEPS * UNITS, gp + a.H, a.gi_t, t0, len, lane, w.left);
+      if (with_dout) copy_own<MODE, SEG, LANES>(st + 2 * STEPS * UNITS, dp, a.dout_t, t0, len, lane, w.left);
+    }
+    copies_sent();
+  };
+  if (OWN_COPIES<MODE, T>) copy_round(0, 0);
   for (int round = 0; round < rounds; ++round) {
+    if (OWN_COPIES<MODE, T>) copy_round(round + 1, at.stage ^ 1);
     const int tile = tiles - 1 - (round * ranks + w.rank);
     const int t0 = tile * STEPS + part * SEG;
     const int n = len - t0;                                   // steps left from here
@@ -442,22 +497,24 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     P2 A = both(1.f), f = both(0.f), r = f;
     P2 zk[SEG];
     if (tile >= 0) {
-      h = load_state<FAST, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left);
-      if (FAST) tc::mbar_wait(tc::smem_u32(&s.full[at.stage]), (uint32_t)at.phase, &s.dead, &g_gated_status);
+      h = load_state<PAIRED<MODE>, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left);
+      if (MODE == BY_TMA) tc::mbar_wait(tc::smem_u32(&s.full[at.stage]), (uint32_t)at.phase, &s.dead, &g_gated_status);
+      if (OWN_COPIES<MODE, T>) copies_landed_but_last();
       const T* st = ring + (size_t)at.stage * 3 * STEPS * UNITS + part * SEG * UNITS;
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
         P2 x = both(0.f), c = x;
         d[k] = x;
-        if (FAST) {
-          x = load_units<true, LANES>(st + k * UNITS, lane, UNITS);
-          c = load_units<true, LANES>(st + (STEPS + k) * UNITS, lane, UNITS);
-          if (with_dout) d[k] = load_units<true, LANES>(st + (2 * STEPS + k) * UNITS, lane, UNITS);
-        } else if (k < n) {
-          const T* row = gp + (long long)(t0 + k) * a.gi_t;
+        if (MODE == BY_TMA || OWN_COPIES<MODE, T>) {
+          x = load_units<PAIRED<MODE>, LANES>(st + k * UNITS, lane, UNITS);
+          c = load_units<PAIRED<MODE>, LANES>(st + (STEPS + k) * UNITS, lane, UNITS);
+          if (with_dout) d[k] = load_units<PAIRED<MODE>, LANES>(st + (2 * STEPS + k) * UNITS, lane, UNITS);
+        } else {                                              // behind the end the last row again: no branch between loads
+          const long long t = min(t0 + k, len - 1);
+          const T* row = gp + t * a.gi_t;
           x = load_units<false, LANES>(row, lane, w.left);
           c = load_units<false, LANES>(row + a.H, lane, w.left);
-          if (with_dout) d[k] = load_units<false, LANES>(dp + (long long)(t0 + k) * a.dout_t, lane, w.left);
+          if (with_dout) d[k] = load_units<false, LANES>(dp + t * a.dout_t, lane, w.left);
         }
         const Gates g = gates<TANH, true>(x, c, K);
         z[k] = g.z;
@@ -505,7 +562,7 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
       for (int v = WARPS - 2; v >= 0; --v) all = after(m[v * LANES], all);
       send_map(s, peers, w, round, all, lane);
     }
-    if (FAST && threadIdx.x == 0) fetch(round + stages, at.stage);
+    if (MODE == BY_TMA && threadIdx.x == 0) fetch(round + stages, at.stage);
     at.next(stages);
     for (int v = 0; v < warp; ++v) h = fma2(m[v * LANES].A, h, front[slot][v][lane]);
     if (second) h = fma2(A0, h, f0);
@@ -526,8 +583,8 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
         const P2 g = add2(G, d[k]);
         G = mul2(z[k], g);
         if (k < n) {
-          store_units<FAST, LANES>(o + (long long)k * a.dgi_t, lane, w.left, mul2(g, p[k]));
-          store_units<FAST, LANES>(o + (long long)k * a.dgi_t + a.H, lane, w.left, mul2(g, q[k]));
+          store_units<PAIRED<MODE>, LANES>(o + (long long)k * a.dgi_t, lane, w.left, mul2(g, p[k]));
+          store_units<PAIRED<MODE>, LANES>(o + (long long)k * a.dgi_t + a.H, lane, w.left, mul2(g, q[k]));
         }
       }
       if (!CLUSTERED && part == 0) s.carry[slot ^ 1][lane] = G;
@@ -535,12 +592,12 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
   }
 
   for (int t = len + w.rank * PARTS + part; t < a.T; t += ranks * PARTS) {
-    store_units<FAST, LANES>(qp + (long long)t * a.dgi_t, lane, w.left, both(0.f));
-    store_units<FAST, LANES>(qp + (long long)t * a.dgi_t + a.H, lane, w.left, both(0.f));
+    store_units<PAIRED<MODE>, LANES>(qp + (long long)t * a.dgi_t, lane, w.left, both(0.f));
+    store_units<PAIRED<MODE>, LANES>(qp + (long long)t * a.dgi_t + a.H, lane, w.left, both(0.f));
   }
   __syncthreads();
   if (a.dh0 != nullptr && w.rank == 0 && part == 0)
-    store_state<FAST, LANES>(a.dh0 + (long long)w.b * a.H + w.unit, lane, w.left, s.carry[rounds & 1][lane]);
+    store_state<PAIRED<MODE>, LANES>(a.dh0 + (long long)w.b * a.H + w.unit, lane, w.left, s.carry[rounds & 1][lane]);
   tear_down(&s.dead, ranks);
 }
 
@@ -548,7 +605,7 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
 constexpr int SHORT = 8;
 
 // At most SHORT steps: a warp has 64 units of a row and all their steps, nothing to join.
-template <typename T, bool FAST, bool TANH>
+template <typename T, bool PAIRS, bool TANH>
 __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
   const int lane = threadIdx.x & 31, columns = (a.H + 63) / 64;
   const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -558,15 +615,15 @@ __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
   const T* gp = static_cast<const T*>(a.gi) + (long long)b * a.gi_b + unit;
   T* op = static_cast<T*>(a.out) + (long long)b * a.out_b + unit;
   P2 h = both(0.f);
-  if (a.h0 != nullptr) h = load_state<FAST, 32>(a.h0 + (long long)b * a.h0_b + unit, lane, left);
-  if (a.states != nullptr) store_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left, h);
+  if (a.h0 != nullptr) h = load_state<PAIRS, 32>(a.h0 + (long long)b * a.h0_b + unit, lane, left);
+  if (a.states != nullptr) store_state<PAIRS, 32>(a.states + (long long)b * a.H + unit, lane, left, h);
   const Constants K = constants();
   P2 x[SHORT], c[SHORT];
 #pragma unroll
   for (int k = 0; k < SHORT; ++k)
     if (k < len) {
-      x[k] = load_units<FAST, 32>(gp + (long long)k * a.gi_t, lane, left);
-      c[k] = load_units<FAST, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
+      x[k] = load_units<PAIRS, 32>(gp + (long long)k * a.gi_t, lane, left);
+      c[k] = load_units<PAIRS, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
     }
 #pragma unroll
   for (int k = 0; k < SHORT; ++k)
@@ -577,12 +634,12 @@ __global__ void __launch_bounds__(128) gated_short_fwd_kernel(const Args a) {
         h = fma2(g.z, h, mul2(g.keep, g.n));
         o = h;
       }
-      store_units<FAST, 32>(op + (long long)k * a.out_t, lane, left, o);
+      store_units<PAIRS, 32>(op + (long long)k * a.out_t, lane, left, o);
     }
-  store_state<FAST, 32>(a.h_T + (long long)b * a.H + unit, lane, left, h);
+  store_state<PAIRS, 32>(a.h_T + (long long)b * a.H + unit, lane, left, h);
 }
 
-template <typename T, bool FAST, bool TANH>
+template <typename T, bool PAIRS, bool TANH>
 __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
   const int lane = threadIdx.x & 31, columns = (a.H + 63) / 64;
   const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -593,17 +650,17 @@ __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
   const T* dp = a.dout != nullptr ? static_cast<const T*>(a.dout) + (long long)b * a.dout_b + unit : nullptr;
   T* qp = static_cast<T*>(a.dgi) + (long long)b * a.dgi_b + unit;
   P2 G = both(0.f);
-  if (a.dh_T != nullptr) G = load_state<FAST, 32>(a.dh_T + (long long)b * a.dh_b + unit, lane, left);
-  P2 h = load_state<FAST, 32>(a.states + (long long)b * a.H + unit, lane, left);
+  if (a.dh_T != nullptr) G = load_state<PAIRS, 32>(a.dh_T + (long long)b * a.dh_b + unit, lane, left);
+  P2 h = load_state<PAIRS, 32>(a.states + (long long)b * a.H + unit, lane, left);
   const Constants K = constants();
   P2 z[SHORT], p[SHORT], q[SHORT], d[SHORT];
 #pragma unroll
   for (int k = 0; k < SHORT; ++k) {
     d[k] = both(0.f);
     if (k < len) {
-      const P2 x = load_units<FAST, 32>(gp + (long long)k * a.gi_t, lane, left);
-      const P2 c = load_units<FAST, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
-      if (dp != nullptr) d[k] = load_units<FAST, 32>(dp + (long long)k * a.dout_t, lane, left);
+      const P2 x = load_units<PAIRS, 32>(gp + (long long)k * a.gi_t, lane, left);
+      const P2 c = load_units<PAIRS, 32>(gp + (long long)k * a.gi_t + a.H, lane, left);
+      if (dp != nullptr) d[k] = load_units<PAIRS, 32>(dp + (long long)k * a.dout_t, lane, left);
       const Gates g = gates<TANH, true>(x, c, K);
       z[k] = g.z;
       p[k] = mul2(sub2(h, g.n), mul2(g.open, g.keep));
@@ -621,25 +678,25 @@ __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
         dx = mul2(g, p[k]);
         dc = mul2(g, q[k]);
       }
-      store_units<FAST, 32>(qp + (long long)k * a.dgi_t, lane, left, dx);
-      store_units<FAST, 32>(qp + (long long)k * a.dgi_t + a.H, lane, left, dc);
+      store_units<PAIRS, 32>(qp + (long long)k * a.dgi_t, lane, left, dx);
+      store_units<PAIRS, 32>(qp + (long long)k * a.dgi_t + a.H, lane, left, dc);
     }
-  if (a.dh0 != nullptr) store_state<FAST, 32>(a.dh0 + (long long)b * a.H + unit, lane, left, G);
+  if (a.dh0 != nullptr) store_state<PAIRS, 32>(a.dh0 + (long long)b * a.H + unit, lane, left, G);
 }
 
-template <typename T, bool FAST, bool TANH>
+template <typename T, bool PAIRS, bool TANH>
 __global__ void __launch_bounds__(128) gated_step_kernel(const StepArgs a) {
   const int lane = threadIdx.x & 31, columns = (a.H + 63) / 64;
   const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (i >= (long long)a.B * columns) return;
   const int b = (int)(i / columns), unit = (int)(i % columns) * 64, left = a.H - unit;
   const T* gp = static_cast<const T*>(a.gi) + (long long)b * a.gi_b + unit;
-  const P2 x = load_units<FAST, 32>(gp, lane, left), c = load_units<FAST, 32>(gp + a.H, lane, left);
-  P2 h = load_state<FAST, 32>(a.h + (long long)b * a.h_b + unit, lane, left);
+  const P2 x = load_units<PAIRS, 32>(gp, lane, left), c = load_units<PAIRS, 32>(gp + a.H, lane, left);
+  P2 h = load_state<PAIRS, 32>(a.h + (long long)b * a.h_b + unit, lane, left);
   const Gates g = gates<TANH, false>(x, c, constants());
   h = fma2(g.z, h, mul2(g.keep, g.n));
-  store_state<FAST, 32>(a.h_new + (long long)b * a.hn_b + unit, lane, left, h);
-  store_units<FAST, 32>(static_cast<T*>(a.out) + (long long)b * a.H + unit, lane, left, h);
+  store_state<PAIRS, 32>(a.h_new + (long long)b * a.hn_b + unit, lane, left, h);
+  store_units<PAIRS, 32>(static_cast<T*>(a.out) + (long long)b * a.H + unit, lane, left, h);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -703,14 +760,14 @@ int stages_for(size_t stage, size_t fixed, int ctas) {
   return n < 1 ? 1 : (n > STAGES_MAX ? STAGES_MAX : n);
 }
 
-template <typename T, typename Cut, bool FAST, bool TANH>
+template <typename T, typename Cut, int MODE, bool TANH>
 int forward_cut(const Args& a, const CUtensorMap& map, int ranks, int stages, cudaStream_t st) {
   const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS) * ranks;
   const size_t smem = (size_t)stages * 2 * Cut::STEPS * Cut::UNITS * sizeof(T) + peer_bytes<Cut::LANES>(ranks);
   if constexpr (std::is_same<Cut, Narrow>::value) {
-    if (ranks > 1) return launch_tiles(gated_fwd_kernel<T, Cut, FAST, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, a, ranks, stages);
+    if (ranks > 1) return launch_tiles(gated_fwd_kernel<T, Cut, MODE, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, a, ranks, stages);
   }
-  return launch_tiles(gated_fwd_kernel<T, Cut, FAST, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, a, 1, stages);
+  return launch_tiles(gated_fwd_kernel<T, Cut, MODE, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, a, 1, stages);
 }
 template <typename T, typename Cut, bool TANH>
 int forward_tiles(const Args& a, cudaStream_t st) {
@@ -721,19 +778,21 @@ int forward_tiles(const Args& a, cudaStream_t st) {
       tile_map<T, Cut>(&map, a.gi, 2ll * a.H, a, a.gi_t, a.gi_b) == B200GRU_OK) {
     const size_t stage = (size_t)2 * Cut::STEPS * Cut::UNITS * sizeof(T);
     const int stages = stages_for(stage, sizeof(Shared<Cut>) + peer_bytes<Cut::LANES>(ranks), 512 / Cut::THREADS);
-    return forward_cut<T, Cut, true, TANH>(a, map, ranks, stages, st);
+    return forward_cut<T, Cut, BY_TMA, TANH>(a, map, ranks, stages, st);
   }
-  return forward_cut<T, Cut, false, TANH>(a, map, ranks, 0, st);
+  if (a.H % 2 == 0 && paired<T>(a.out, a.out_t, a.out_b) && paired<T>(a.gi, a.gi_t, a.gi_b))
+    return forward_cut<T, Cut, BY_PAIRS, TANH>(a, map, ranks, 2, st);
+  return forward_cut<T, Cut, BY_UNITS, TANH>(a, map, ranks, sizeof(T) == 4 ? 2 : 0, st);
 }
 
-template <typename T, typename Cut, bool FAST, bool TANH>
+template <typename T, typename Cut, int MODE, bool TANH>
 int backward_cut(const Args& a, const CUtensorMap& map, const CUtensorMap& dmap, int ranks, int stages, cudaStream_t st) {
   const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS) * ranks;
   const size_t smem = (size_t)stages * 3 * Cut::STEPS * Cut::UNITS * sizeof(T) + peer_bytes<Cut::LANES>(ranks);
   if constexpr (std::is_same<Cut, Narrow>::value) {
-    if (ranks > 1) return launch_tiles(gated_bwd_kernel<T, Cut, FAST, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, dmap, a, ranks, stages);
+    if (ranks > 1) return launch_tiles(gated_bwd_kernel<T, Cut, MODE, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, dmap, a, ranks, stages);
   }
-  return launch_tiles(gated_bwd_kernel<T, Cut, FAST, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, dmap, a, 1, stages);
+  return launch_tiles(gated_bwd_kernel<T, Cut, MODE, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, dmap, a, 1, stages);
 }
 template <typename T, typename Cut, bool TANH>
 int backward_tiles(const Args& a, cudaStream_t st) {
@@ -747,9 +806,12 @@ int backward_tiles(const Args& a, cudaStream_t st) {
                              tile_map<T, Cut>(&dmap, a.dout, a.H, a, a.dout_t, a.dout_b) == B200GRU_OK))) {
     const size_t stage = (size_t)3 * Cut::STEPS * Cut::UNITS * sizeof(T);
     const int stages = stages_for(stage, sizeof(Shared<Cut>) + 2 * Cut::THREADS * sizeof(P2) + peer_bytes<Cut::LANES>(ranks), 2);
-    return backward_cut<T, Cut, true, TANH>(a, map, dmap, ranks, stages, st);
+    return backward_cut<T, Cut, BY_TMA, TANH>(a, map, dmap, ranks, stages, st);
   }
-  return backward_cut<T, Cut, false, TANH>(a, map, dmap, ranks, 0, st);
+  if (a.H % 2 == 0 && paired<T>(a.dgi, a.dgi_t, a.dgi_b) && paired<T>(a.gi, a.gi_t, a.gi_b) &&
+      (a.dout == nullptr || paired<T>(a.dout, a.dout_t, a.dout_b)))
+    return backward_cut<T, Cut, BY_PAIRS, TANH>(a, map, dmap, ranks, 2, st);
+  return backward_cut<T, Cut, BY_UNITS, TANH>(a, map, dmap, ranks, sizeof(T) == 4 ? 2 : 0, st);
 }
 
 template <typename T, bool TANH>
