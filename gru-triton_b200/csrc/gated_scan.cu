@@ -212,24 +212,31 @@ enum { BY_TMA = 0, BY_PAIRS = 1, BY_UNITS = 2 };
 template <int MODE> constexpr bool PAIRED = MODE != BY_UNITS;        // a lane has units 2 i and 2 i + 1, not i and i + LANES
 template <int MODE, typename T> constexpr bool OWN_COPIES = MODE == BY_PAIRS || (MODE == BY_UNITS && sizeof(T) == 4);
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+template <int BYTES, int TO, int FROM>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0 + %2], [%1 + %3], %4;" ::"r"(dst), "l"(src), "n"(TO), "n"(FROM), "n"(BYTES) : "memory");
 }
-// A thread's SEG rows of its two units into its own places of a stage; behind the row's end the last step again.
+// A thread's rows K .. SEG - 1 of its two units into its own places of a stage; behind the row's end (not ALL) the last step again.
+template <bool ALL, int MODE, int SEG, int LANES, typename T, int K = 0>
+__device__ __forceinline__ void copy_rows(uint32_t dst, const T* row, long long stride, int left_steps, bool first, bool second) {
+  if constexpr (K < SEG) {
+    constexpr int TO = K * 2 * LANES * (int)sizeof(T);
+    if (MODE == BY_PAIRS) {
+      if (first) copy_async<2 * sizeof(T), TO, 0>(dst, row);
+    } else {
+      if (first) copy_async<4, TO, 0>(dst, row);
+      if (second) copy_async<4, TO + LANES * (int)sizeof(T), LANES * (int)sizeof(T)>(dst, row);
+    }
+    copy_rows<ALL, MODE, SEG, LANES, T, K + 1>(dst, row + (ALL || K + 1 < left_steps ? stride : 0), stride, left_steps, first, second);
+  }
+}
 template <int MODE, int SEG, int LANES, typename T>
 __device__ __forceinline__ void copy_own(T* st, const T* p, long long stride, int t0, int len, int lane, int left) {
-#pragma unroll
-  for (int k = 0; k < SEG; ++k) {
-    const T* row = p + (long long)min(t0 + k, len - 1) * stride;
-    T* dst = st + k * 2 * LANES;
-    if (MODE == BY_PAIRS) {
-      if (2 * lane < left) copy_async<2 * sizeof(T)>(dst + 2 * lane, row + 2 * lane);
-    } else {
-      if (lane < left) copy_async<4>(dst + lane, row + lane);
-      if (lane + LANES < left) copy_async<4>(dst + lane + LANES, row + lane + LANES);
-    }
-  }
+  const int unit = MODE == BY_PAIRS ? 2 * lane : lane;
+  const uint32_t dst = tc::smem_u32(st + unit);
+  const T* row = p + (long long)min(t0, len - 1) * stride + unit;
+  if (len - t0 >= SEG) copy_rows<true, MODE, SEG, LANES>(dst, row, stride, SEG, unit < left, lane + LANES < left);
+  else copy_rows<false, MODE, SEG, LANES>(dst, row, stride, len - t0, unit < left, lane + LANES < left);
 }
 __device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copies_landed_but_last() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
@@ -367,19 +374,20 @@ gated_fwd_kernel(const __grid_constant__ CUtensorMap map, const Args a, int rank
     h = through<false, WARPS, LANES>(&s.part[round & 1][0][lane], warp, h);
     if (second) h = apply(first, h);
     const int t0 = tile * STEPS + part * SEG, n = len - t0;
-    T* o = op + (long long)t0 * a.out_t;
+    char* o = reinterpret_cast<char*>(op + (long long)t0 * a.out_t);
     if (n >= SEG) {
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
         h = fma2(z[k], h, u[k]);
-        store_units<PAIRED<MODE>, LANES>(o, lane, w.left, h);
-        o += a.out_t;
+        store_units<PAIRED<MODE>, LANES>(reinterpret_cast<T*>(o), lane, w.left, h);
+        o += a.out_step;
       }
     } else {
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
         h = fma2(z[k], h, u[k]);
-        if (k < n) store_units<PAIRED<MODE>, LANES>(o + (long long)k * a.out_t, lane, w.left, h);
+        if (k < n) store_units<PAIRED<MODE>, LANES>(reinterpret_cast<T*>(o), lane, w.left, h);
+        o += a.out_step;
       }
     }
     if (!CLUSTERED && part == PARTS - 1) s.carry[(round & 1) ^ 1][lane] = h;
@@ -493,9 +501,10 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     const int t0 = tile * STEPS + part * SEG;
     const int n = len - t0;                                   // steps left from here
     P2 h = both(0.f);
-    P2 z[SEG], u[SEG], p[SEG], q[SEG], d[SEG];            // p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'
+    // keep: 1 - z, then z;  p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'.  Five values a step: with a sixth the
+    // compiler computes addresses over and over for want of registers (60 instructions an element against 69).
+    P2 keep[SEG], open[SEG], p[SEG], q[SEG], d[SEG];
     P2 A = both(1.f), f = both(0.f), r = f;
-    P2 zk[SEG];
     if (tile >= 0) {
       h = load_state<PAIRED<MODE>, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left);
       if (MODE == BY_TMA) tc::mbar_wait(tc::smem_u32(&s.full[at.stage]), (uint32_t)at.phase, &s.dead, &g_gated_status);
@@ -517,24 +526,24 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
           if (with_dout) d[k] = load_units<false, LANES>(dp + t * a.dout_t, lane, w.left);
         }
         const Gates g = gates<TANH, true>(x, c, K);
-        z[k] = g.z;
-        u[k] = mul2(g.keep, g.n);
+        keep[k] = g.keep;
+        open[k] = g.open;
         p[k] = g.n;
         q[k] = mul2(g.keep, g.slope);
-        zk[k] = mul2(g.open, g.keep);
       }
       if (n < SEG) {
 #pragma unroll
         for (int k = 0; k < SEG; ++k)
-          if (k >= n) { z[k] = both(1.f); u[k] = d[k] = both(0.f); }
+          if (k >= n) keep[k] = p[k] = d[k] = both(0.f);
       }
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
-        A = mul2(z[k], A);
-        f = fma2(z[k], f, u[k]);
+        const P2 z = sub2(K.one, keep[k]);
+        A = mul2(z, A);
+        f = fma2(z, f, mul2(keep[k], p[k]));
       }
 #pragma unroll
-      for (int k = SEG - 1; k >= 0; --k) r = mul2(z[k], add2(d[k], r));
+      for (int k = SEG - 1; k >= 0; --k) r = mul2(sub2(K.one, keep[k]), add2(d[k], r));
     }
     const int slot = round & 1;
     Map back = {A, r};                                        // gradients: from the later part to the earlier one
@@ -569,23 +578,26 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     if (tile >= 0) {
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
-        p[k] = mul2(sub2(h, p[k]), zk[k]);
-        h = fma2(z[k], h, u[k]);
+        const P2 z = sub2(K.one, keep[k]), n = p[k];
+        p[k] = mul2(sub2(h, n), mul2(open[k], keep[k]));
+        h = fma2(z, h, mul2(keep[k], n));
+        keep[k] = z;
       }
     }
     P2 G = CLUSTERED ? join(s, peers, w, round, part, lane) : s.carry[slot][lane];
     if (tile >= 0) {
       G = through<true, WARPS, LANES>(m, warp, G);
       if (LANES == 16 && !second) G = apply(back, G);
-      T* o = qp + (long long)t0 * a.dgi_t;
+      char* o = reinterpret_cast<char*>(qp + (long long)(t0 + SEG - 1) * a.dgi_t);
 #pragma unroll
       for (int k = SEG - 1; k >= 0; --k) {
         const P2 g = add2(G, d[k]);
-        G = mul2(z[k], g);
+        G = mul2(keep[k], g);
         if (k < n) {
-          store_units<PAIRED<MODE>, LANES>(o + (long long)k * a.dgi_t, lane, w.left, mul2(g, p[k]));
-          store_units<PAIRED<MODE>, LANES>(o + (long long)k * a.dgi_t + a.H, lane, w.left, mul2(g, q[k]));
+          store_units<PAIRED<MODE>, LANES>(reinterpret_cast<T*>(o), lane, w.left, mul2(g, p[k]));
+          store_units<PAIRED<MODE>, LANES>(reinterpret_cast<T*>(o + a.half), lane, w.left, mul2(g, q[k]));
         }
+        o -= a.dgi_step;
       }
       if (!CLUSTERED && part == 0) s.carry[slot ^ 1][lane] = G;
     }
@@ -906,6 +918,8 @@ gated::Args to_args(const b200gru_gated_args* p) {
   a.out = p->out; a.out_t = p->out_t; a.out_b = p->out_b; a.h_T = p->h_T; a.states = p->states;
   a.dout = p->dout; a.dout_t = p->dout_t; a.dout_b = p->dout_b; a.dh_T = p->dh_T; a.dh_b = p->dh_b;
   a.dgi = p->dgi; a.dgi_t = p->dgi_t; a.dgi_b = p->dgi_b; a.dh0 = p->dh0;
+  const long long size = p->dtype == B200GRU_F32 ? 4 : 2;
+  a.out_step = p->out_t * size; a.dgi_step = p->dgi_t * size; a.half = p->H * size;
   return a;
 }
 
