@@ -210,7 +210,8 @@ struct GradPlanesArgs {
   __half* dw;
   long long ld, plane;
 };
-template <bool VEC>
+// HELD: rows of at most 128 * HELD columns stay in registers between the row's maximum and its planes (0: read twice).
+template <bool VEC, int HELD>
 __global__ void __launch_bounds__(256) grad_planes_kernel(const GradPlanesArgs a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -221,25 +222,52 @@ __global__ void __launch_bounds__(256) grad_planes_kernel(const GradPlanesArgs a
     if (c < a.g.N) grad_values<float, VEC>(a.g, row, c, v);
     return make_float4(v[0], v[1], v[2], v[3]);
   };
+  float4 held[HELD > 0 ? HELD : 1];
+  if (HELD > 0) {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) held[i] = value(lane * 4 + i * 128);
+  }
+  const float x_inv = a.dw != nullptr ? __ldg(a.g.x_inv + row) : 0.f;
   float scale = 1.f;
   if (a.dx != nullptr) {
     float mx = 0.f;
+    auto take = [&](int c, float4 v) {
+      if (c < a.g.N) mx = largest(times(v, __ldg(reinterpret_cast<const float4*>(a.w_inv + c))), mx);
+    };
+    if (HELD > 0) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) take(lane * 4 + i * 128, held[i]);
+    } else {
 #pragma unroll 4
-    for (int c = lane * 4; c < a.g.N; c += 128) mx = largest(times(value(c), *reinterpret_cast<const float4*>(a.w_inv + c)), mx);
+      for (int c = lane * 4; c < a.g.N; c += 128) take(c, value(c));
+    }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
     float back;
     pow2_row_scale(mx, &scale, &back);
     if (lane == 0) a.dx_inv[row] = back;
   }
-  const float x_inv = a.dw != nullptr ? __ldg(a.g.x_inv + row) : 0.f;
-#pragma unroll 2
-  for (int c = lane * 4; c < a.ld; c += 128) {
-    const float4 v = value(c);
+  auto put = [&](int c, float4 v) {
+    if (c >= a.ld) return;
     const long long at = (long long)row * a.ld + c;
-    if (a.dx != nullptr) store_planes(a.dx + at, a.plane, times(times(v, c < a.g.N ? *reinterpret_cast<const float4*>(a.w_inv + c) : v), scale));
-    if (a.dw != nullptr) store_planes(a.dw + at, a.plane, times(times(v, x_inv), c < a.g.N ? *reinterpret_cast<const float4*>(a.col_scale + c) : v));
+    const bool inside = c < a.g.N;
+    if (a.dx != nullptr) store_planes(a.dx + at, a.plane, times(times(v, inside ? __ldg(reinterpret_cast<const float4*>(a.w_inv + c)) : v), scale));
+    if (a.dw != nullptr) store_planes(a.dw + at, a.plane, times(times(v, x_inv), inside ? __ldg(reinterpret_cast<const float4*>(a.col_scale + c)) : v));
+  };
+  if (HELD > 0) {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) put(lane * 4 + i * 128, held[i]);
+  } else {
+#pragma unroll 2
+    for (int c = lane * 4; c < a.ld; c += 128) put(c, value(c));
   }
+}
+template <bool VEC>
+void launch_grad_planes(const GradPlanesArgs& q, cudaStream_t st) {
+  const dim3 grid((unsigned)cdiv(q.g.M, 8));
+  if (q.ld <= 512) launch_pdl(grad_planes_kernel<VEC, 4>, grid, dim3(256), 0, st, q);
+  else if (q.ld <= 1024) launch_pdl(grad_planes_kernel<VEC, 8>, grid, dim3(256), 0, st, q);
+  else launch_pdl(grad_planes_kernel<VEC, 0>, grid, dim3(256), 0, st, q);
 }
 
 // ---- K slices ------------------------------------------------------------------------------------------
@@ -555,7 +583,7 @@ struct Call {
     const bool columns = F32 && a.dW != nullptr;
     if (a.db != nullptr || columns || g.d != nullptr) {
       const int across = cdiv(a.N, 64 * Vec<T>::V);
-      int slices = cdiv(2 * 148, across);                  // two CTAs to an SM, 16 rows or more each
+      int slices = cdiv(8 * 148, across);                  // as many CTAs as an SM holds, 16 rows or more each
       if (slices > cdiv(a.M, 16)) slices = cdiv(a.M, 16);
       g.rows_per_slice = cdiv(cdiv(a.M, slices), 4) * 4;
       slices = cdiv(a.M, g.rows_per_slice);
@@ -594,9 +622,8 @@ struct Call {
         dw.p = q.dw; dw.ld = q.ld; dw.plane = q.plane; dw.inv = back;
       }
       if (!dry && rc == B200GRU_OK) {
-        const dim3 grid((unsigned)cdiv(a.M, 8));
-        if (vec) launch_pdl(grad_planes_kernel<true>, grid, dim3(256), 0, st, q);
-        else launch_pdl(grad_planes_kernel<false>, grid, dim3(256), 0, st, q);
+        if (vec) launch_grad_planes<true>(q, st);
+        else launch_grad_planes<false>(q, st);
         note("grad_planes_kernel");
       }
     }
@@ -658,7 +685,7 @@ Plan plan_gemm(int M, int N, int K, int planes) {
   const double products = planes == 2 ? 3.0 : 1.0;
   Plan best = {1, 128, 1};
   double best_cost = 1e30;
-  const struct { int ctas, m, n, units; double per_kb; } cuts[3] = {{2, 256, 256, 74, 560.0}, {1, 128, 128, 148, 330.0}, {1, 128, 64, 148, 260.0}};
+  const struct { int ctas, m, n, units; double per_kb; } cuts[3] = {{2, 256, 256, 74, 560.0}, {1, 128, 128, 148, 370.0}, {1, 128, 64, 148, 270.0}};
   for (const auto& c : cuts) {
     const long long tiles = (long long)cdiv(M, c.m) * cdiv(N, c.n);
     for (int want = 1; want <= 64 && want <= kb; ++want) {

@@ -339,12 +339,17 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   const uint32_t tmem = tmem_slot;
   pdl_wait();
 
-  // tile index -> K slice, row panel, column panel (columns fastest: neighbours share the rows of A)
+  // tile index -> K slice, row panel, column panel.  Tiles run down bands of eight row panels, column by column: what runs at
+  // a time is about as high as wide, and reads the least of A and B (8192^3 bf16, where a row of tiles would draw all of B
+  // through L2: 929 -> 855 us).
   auto locate = [&](int t, int& m0, int& n0, int& z, int& kb0, int& nkb) {
-    n0 = (t % p.tiles_n) * BN;
-    const int r = t / p.tiles_n;
-    m0 = (r % p.tiles_m) * CTAS * BM + (int)rank * BM;
-    z = r / p.tiles_m;
+    constexpr int BAND = 8;
+    const int plane = p.tiles_m * p.tiles_n;
+    z = t / plane;
+    const int r = t - z * plane, band = r / (BAND * p.tiles_n), first = band * BAND;
+    const int high = min(BAND, p.tiles_m - first), i = r - band * BAND * p.tiles_n;
+    n0 = (i / high) * BN;
+    m0 = (first + i % high) * CTAS * BM + (int)rank * BM;
     kb0 = z * p.kb_per_split;
     nkb = max(0, min(p.kb_total, kb0 + p.kb_per_split) - kb0);
   };
