@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256) grad_kernel(const GradArgs a) {
 #pragma unroll
   for (int e = 0; e < V; ++e) sum[e] = top[e] = 0.f;
   if (n < a.N) {
-#pragma unroll 4
+#pragma unroll 8
     for (int m = blockIdx.y * a.rows_per_slice + grp; m < m1; m += 4) {
       float v[V];
       grad_values<T, VEC>(a, m, n, v);
@@ -583,7 +583,7 @@ struct Call {
     const bool columns = F32 && a.dW != nullptr;
     if (a.db != nullptr || columns || g.d != nullptr) {
       const int across = cdiv(a.N, 64 * Vec<T>::V);
-      int slices = cdiv(8 * 148, across);                  // as many CTAs as an SM holds, 16 rows or more each
+      int slices = cdiv(4 * 148, across);                  // four CTAs to an SM (two or eight took longer), 16 rows or more each
       if (slices > cdiv(a.M, 16)) slices = cdiv(a.M, 16);
       g.rows_per_slice = cdiv(cdiv(a.M, slices), 4) * 4;
       slices = cdiv(a.M, g.rows_per_slice);

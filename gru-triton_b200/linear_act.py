@@ -9,7 +9,8 @@ quantised weights: float32 alone, no activation or residual.
 Element types float32, bfloat16 and float16, one for all tensors of a call; sums are float32.  float32 operands run as
 two row-scaled fp16 planes in three tensor-core products (22 significant bits, as ``tc.linear``'s).  What the backward
 needs of the activation is its slope, kept by the forward in float32 or, for the 16-bit types, in float16.  The
-same call repeats its bits.  CUDA tensors only; there is no fallback.  The reference's counterpart is ``F.linear``
+same call repeats its bits.  A float32 row of x, or of the gradient, that holds an infinity gives NaN in its row (its
+two planes cannot hold one).  CUDA tensors only; there is no fallback.  The reference's counterpart is ``F.linear``
 (src/gru_qat/gru_cell.py:410-435), without activation and residual.
 """
 
@@ -43,6 +44,8 @@ def _check(x, W, bias, residual, activation):
     N, K = w
     if N == 0 or K == 0:
         raise ValueError(f"N and K must be > 0; got N={N}, K={K}")
+    if x.numel() // K > 2 ** 31 - 16 or N > 2 ** 30 - 16 or K > 2 ** 30 - 16:
+        raise ValueError(f"at most 2^31 - 16 rows and 2^30 - 16 columns; got x {tuple(lead)}, W {tuple(w)}")
     if bias is not None and bias.shape != (N,):
         raise ValueError(f"bias shape must be (N,)=({N},); got {tuple(bias.shape)}")
     if residual is not None and residual.shape != (*lead[:-1], N):

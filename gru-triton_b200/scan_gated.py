@@ -65,6 +65,11 @@ def _check_state(name, h, B, H):
         raise ValueError(f"{name} shape must be (B, H)=({B}, {H}); got {tuple(h.shape)}")
 
 
+def _check_size(T, B, H):
+    if T > 2 ** 30 or B * H > 2 ** 31 - 1:
+        raise ValueError(f"at most 2^30 steps and 2^31 - 1 states; got T={T}, B={B}, H={H}")
+
+
 def _check_devices(gi, names, others):
     if not gi.is_cuda or any(t is not None and t.device != gi.device for t in others):
         given = {n: t for n, t in zip(names, others) if t is not None}
@@ -79,6 +84,7 @@ def _check_scan(gi, h0, lengths, candidate) -> None:
     H = two_h // 2
     if T == 0 or B == 0 or H == 0:
         raise ValueError(f"T, B and H must be > 0; got T={T}, B={B}, H={H}")
+    _check_size(T, B, H)
     if h0 is not None:
         _check_state("h0", h0, B, H)
     if lengths is not None:
@@ -202,6 +208,7 @@ def gated_step(gi: torch.Tensor, h: torch.Tensor, *, candidate: str = "tanh",
     H = two_h // 2
     if B == 0 or H == 0:
         raise ValueError(f"B and H must be > 0; got B={B}, H={H}")
+    _check_size(1, B, H)
     _check_state("h", h, B, H)
     if out_state is not None:
         _check_state("out_state", out_state, B, H)

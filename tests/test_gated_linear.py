@@ -120,7 +120,7 @@ def check_scan(gi, h0, lengths, candidate, dout, dh):
     return out, h_T, grads
 
 
-SCAN_SIZES = [(1, 1, 1), (1, 3, 33), (2, 1, 8), (7, 2, 64), (16, 40, 72), (17, 2, 64), (63, 2, 64), (64, 5, 40), (65, 3, 96),
+SCAN_SIZES = [(40, 3, 34), (200, 2, 1030), (600, 1, 130), (70, 260, 66), (9, 1, 8), (128, 1, 32), (129, 9, 2048), (1, 1, 1), (1, 3, 33), (2, 1, 8), (7, 2, 64), (16, 40, 72), (17, 2, 64), (63, 2, 64), (64, 5, 40), (65, 3, 96),
               (130, 1, 512), (300, 2, 72), (257, 19, 607), (1000, 1, 1024), (200, 64, 256), (2100, 1, 24)]
 
 
@@ -676,6 +676,11 @@ def test_scan_refusals():
             gated_step(*bad)
     with pytest.raises(ValueError, match="out_state"):
         gated_step(gi[0], h0, out_state=h0.half())
+    # sizes that the 32-bit counts of the library do not hold
+    with pytest.raises(ValueError, match="2\\^30"):
+        gated_scan(torch.zeros(1, 1, 2).expand(2 ** 32 + 4, 1, 2))
+    with pytest.raises(ValueError, match="2\\^30"):
+        gated_step(torch.zeros(1, 16).expand(2 ** 29, 16), torch.zeros(1, 8).expand(2 ** 29, 8))
 
 
 def test_linear_refusals():
@@ -686,6 +691,8 @@ def test_linear_refusals():
                             ((x, W, b.half()), {}, "bias dtype"), ((x[:, :0], W[:, :0]), {}, "K=0")]:
         with pytest.raises(ValueError, match=match):
             linear_act(*args, **kw)
+    with pytest.raises(ValueError, match="rows"):
+        linear_act(torch.zeros(1, 16).expand(2 ** 32 + 4, 16), W)
 
 
 def test_library_refuses_bad_arguments():
