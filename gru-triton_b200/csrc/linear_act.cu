@@ -59,27 +59,40 @@ __device__ __forceinline__ float largest(float4 v, float m) {
 __device__ __forceinline__ float4 times(float4 v, float s) { return make_float4(v.x * s, v.y * s, v.z * s, v.w * s); }
 __device__ __forceinline__ float4 times(float4 v, float4 s) { return make_float4(v.x * s.x, v.y * s.y, v.z * s.z, v.w * s.w); }
 
-// A row into two fp16 planes, scaled so that its largest element lies in [2^14, 2^15): 22 significant bits of all elements down
-// to 2^-17 of it.  One warp per row; the second read of the row comes from L1.
+// Rows into two fp16 planes each, scaled so that a row's largest element lies in [2^14, 2^15): 22 significant bits of all elements
+// down to 2^-17 of it.  One warp per row; the second read of the row comes from L1.  Up to two matrices in a launch.
+struct SplitArgs {
+  const float* src; long long ld;
+  __half* dst; long long dld, plane;
+  int rows, cols, vec;
+  float* inv;
+};
 template <bool VEC>
-__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, long long ld, __half* __restrict__ dst, long long dld,
-                                                         long long plane, int rows, int cols, float* __restrict__ inv) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  const float* s = src + (long long)row * ld;
+__device__ __forceinline__ void split_row(const SplitArgs& a, int row, int lane) {
+  const float* s = a.src + (long long)row * a.ld;
   float mx = 0.f;
 #pragma unroll 4
-  for (int c = lane * 4; c < cols; c += 128) mx = largest(four<VEC>(s, c, cols), mx);
+  for (int c = lane * 4; c < a.cols; c += 128) mx = largest(four<VEC>(s, c, a.cols), mx);
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
   float scale, back;
   pow2_row_scale(mx, &scale, &back);
-  if (lane == 0) inv[row] = back;
-  __half* d = dst + (long long)row * dld;
+  if (lane == 0) a.inv[row] = back;
+  __half* d = a.dst + (long long)row * a.dld;
 #pragma unroll 4
-  for (int c = lane * 4; c < dld; c += 128) store_planes(d + c, plane, times(four<VEC>(s, c, cols), scale));
+  for (int c = lane * 4; c < a.dld; c += 128) store_planes(d + c, a.plane, times(four<VEC>(s, c, a.cols), scale));
+}
+__global__ void __launch_bounds__(256) split_rows_kernel(const SplitArgs one, const SplitArgs two) {
+  pdl_launch_dependents();
+  pdl_wait();
+  long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const bool first = row < one.rows;
+  const SplitArgs& a = first ? one : two;
+  if (!first) row -= one.rows;
+  if (row >= a.rows) return;
+  if (a.vec) split_row<true>(a, (int)row, lane);
+  else split_row<false>(a, (int)row, lane);
 }
 
 // ---- the gradient behind the activation ------------------------------------------------------------------
@@ -468,23 +481,9 @@ struct Call {
     if (rc == B200GRU_OK) rc = check_launch(what);
   }
 
+  // 16-bit rows where they lie, if TMA can read them there.
   Operand operand(const void* src, long long ld, int rows, int cols) {
     Operand o = {src, ld, 0, nullptr};
-    if (F32) {
-      o.ld = pad8(cols);
-      o.plane = (long long)rows * o.ld;
-      __half* d = ws.template take<__half>(2 * o.plane);
-      o.inv = ws.template take<float>(pad8(rows));
-      o.p = d;
-      if (!dry && rc == B200GRU_OK) {
-        const float* s = static_cast<const float*>(src);
-        const dim3 grid((unsigned)cdiv(rows, 8));
-        if (cols % 4 == 0 && on16(src, ld, 4)) launch_pdl(split_rows_kernel<true>, grid, dim3(256), 0, st, s, ld, d, o.ld, o.plane, rows, cols, o.inv);
-        else launch_pdl(split_rows_kernel<false>, grid, dim3(256), 0, st, s, ld, d, o.ld, o.plane, rows, cols, o.inv);
-        note("split_rows_kernel");
-      }
-      return o;
-    }
     if (rows == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) { o.ld = pad8(cols); return o; }
     if (ld >= cols && on16(src, ld, 2)) return o;
     o.ld = pad8(cols);
@@ -492,6 +491,35 @@ struct Call {
     o.p = d;
     copy_rows(static_cast<const T*>(src), ld, d, o.ld, rows, cols);
     return o;
+  }
+  // fp32 rows as planes; the launch follows in split().
+  Operand planes(const void* src, long long ld, int rows, int cols, SplitArgs* s) {
+    Operand o = {nullptr, pad8(cols), (long long)rows * pad8(cols), nullptr};
+    __half* d = ws.template take<__half>(2 * o.plane);
+    o.inv = ws.template take<float>(pad8(rows));
+    o.p = d;
+    *s = {static_cast<const float*>(src), ld, d, o.ld, o.plane, rows, cols, cols % 4 == 0 && on16(src, ld, 4) ? 1 : 0, o.inv};
+    return o;
+  }
+  void split(const SplitArgs& one, const SplitArgs& two) {
+    const long long rows = (long long)one.rows + two.rows;
+    if (dry || rc != B200GRU_OK || rows == 0) return;
+    launch_pdl(split_rows_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, one, two);
+    note("split_rows_kernel");
+  }
+  // x and W as the products read them (either may not be wanted).
+  void operands(bool want_x, bool want_w, Operand* x, Operand* W) {
+    if (F32) {
+      SplitArgs one, two;
+      memset(&one, 0, sizeof(one));
+      memset(&two, 0, sizeof(two));
+      if (want_x) *x = planes(a.x, a.ldx, a.M, a.K, &one);
+      if (want_w) *W = planes(a.W, a.ldw, a.N, a.K, &two);
+      split(one, two);
+    } else {
+      if (want_x) *x = operand(a.x, a.ldx, a.M, a.K);
+      if (want_w) *W = operand(a.W, a.ldw, a.N, a.K);
+    }
   }
 
   void copy_rows(const T* src, long long ld, T* dst, long long dld, int rows, int cols) {
@@ -544,7 +572,8 @@ struct Call {
       if (!dry) rc = few_rows<T>(a, st);
       return rc;
     }
-    const Operand x = operand(a.x, a.ldx, a.M, a.K), W = operand(a.W, a.ldw, a.N, a.K);
+    Operand x = {}, W = {};
+    operands(true, true, &x, &W);
     Gemm g;
     memset(&g, 0, sizeof(g));
     g.M = a.M; g.N = a.N; g.K = a.K;
@@ -559,8 +588,7 @@ struct Call {
   int backward() {
     const bool act = a.activation != B200GRU_ACT_NONE;
     Operand x = {}, W = {}, dx = {}, dw = {};
-    if (a.dW != nullptr) x = operand(a.x, a.ldx, a.M, a.K);
-    if (a.dx != nullptr) W = operand(a.W, a.ldw, a.N, a.K);
+    operands(a.dW != nullptr, a.dx != nullptr, &x, &W);
 
     GradArgs g;
     memset(&g, 0, sizeof(g));

@@ -18,10 +18,18 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// The slope act'(pre) that the backward multiplies with is kept in fp32 for fp32 and in fp16 for the 16-bit types: it lies
-// in [-0.13, 1.13] for every activation, so fp16 holds it to 11 bits (below 6e-5 to 3e-8 absolute) where bf16 would add an
-// error as large as that of the output's own rounding.
-template <typename T> struct SlopeOf { typedef __half type; };
+// The slope act'(pre) that the backward multiplies with is kept in fp32 for fp32.  For the 16-bit types it is a fixed-point number:
+// it lies in [-0.13, 1.13] for every activation, so 16 bits hold it to 2^-16, and zero and one exactly.  (As fp16 it was off by
+// up to 2^-12 at one, which doubled the error of an fp16 gradient.)  0xffff: NaN.
+struct Slope16 { unsigned short u; };
+__device__ __forceinline__ float to_float(Slope16 s) {
+  const float v = fmaf(__uint_as_float(0x4b000000u | s.u), 1.f / 32768.f, -256.5f);      // (2^23 + u) 2^-15 - 256.5 = u 2^-15 - 0.5
+  return s.u == 0xffffu ? __uint_as_float(0x7fffffffu) : v;
+}
+template <> __device__ __forceinline__ Slope16 from_float<Slope16>(float v) {            // the low bits of 2^23 + 2^14 + v 2^15
+  return Slope16{(unsigned short)(__float_as_uint(fmaf(v, 32768.f, 8404992.f)) & 0xffffu)};
+}
+template <typename T> struct SlopeOf { typedef Slope16 type; };
 template <> struct SlopeOf<float> { typedef float type; };
 
 // Two values behind the activation, and its slopes there.

@@ -100,7 +100,7 @@ def _forward(x, W, bias, residual, activation, want_slope: bool):
     slope = None
     if want_slope and activation != "none":
         # rows padded to eight elements: 16-byte accesses at any width
-        slope = torch.empty((M, -(-N // 8) * 8), device=x.device, dtype=torch.float32 if x.dtype == torch.float32 else torch.float16)
+        slope = torch.empty((M, -(-N // 8) * 8), device=x.device, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16)
     if M:
         a = _fill(x, W, activation)
         if bias is not None:

@@ -10,7 +10,8 @@ Tolerances (u = 2^-24, half a step of float32; ``half(t)`` = eps / 2 of an outpu
 * product: S = sum |x| |W| of a result.  Operands of two fp16 planes are off by 2^-23 each, their dropped product by 2^-24;
   the tensor core truncates each of at most 32 steps of a chunk by 2 u, chunks of 64 or more terms add with u each:
   u S (80 + K / 64).  An activation adds its own 8 u of its value, and multiplies by a slope below 1.2.
-* 16-bit gradients: d = dy * slope is rounded to the type, its slope to fp16: S_d (half(t) + 2^-11 + u (80 + K / 64)).
+* 16-bit gradients: d = dy * slope is rounded to the type, its slope to steps of 2^-15, half a step off at most:
+  S_d (half(t) + u (80 + K / 64)) + S_dy 2^-16.
 * every result: half(t) of itself, and half the step of the smallest numbers of its type.
 """
 
@@ -390,12 +391,12 @@ def check_linear(x, W, bias, residual, activation, dy):
     S = x64.abs() @ W64.abs().t() + (0 if bias is None else bias.double().abs())
     off_pre = U * S * (80 + K / 64)
     close(y.detach(), ref, 1.2 * off_pre + 8 * U * (a.abs() + pre.abs() + ref.abs()) + rounding(ref, dtype))
-    # the slope's own error: |act''| <= 1 of the error of pre, a few units of itself; fp16 behind 16-bit types
+    # the slope's own error: |act''| <= 1 of the error of pre, a few units of itself; fixed point behind 16-bit types
     off_d = dy64.abs() * (off_pre + 16 * U)
     if activation == "relu":
         off_d = dy64.abs() * (pre.abs() <= off_pre) + 0 * d      # the sign of pre decides
-    if dtype != torch.float32:
-        off_d = off_d + d.abs() * (2.0 ** -11 if activation != "none" else 0.0) + dy64.abs() * 2.0 ** -24
+    if dtype != torch.float32 and activation != "none":
+        off_d = off_d + dy64.abs() * 2.0 ** -16
     in_product = off_d + (half(dtype) * d.abs() if dtype != torch.float32 and activation != "none" else 0.0)
     refs = [d @ W64, d.t() @ x64]
     sums = [d.abs() @ W64.abs(), d.abs().t() @ x64.abs()]
@@ -506,6 +507,19 @@ def test_linear_no_rows_some_gradients_and_special_values(M):
         g, = torch.autograd.grad(y, leaf, torch.ones_like(y))
         assert bool((y[:, 1] == lo).all()) and (hi is None or bool((y[:, 0] == hi).all())) and bool((y[:, 0] > 0).all())
         assert bool((g == (1.0 if hi is None else 0.0)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid", "tanh"])
+@pytest.mark.parametrize("M", [5, 200])
+def test_linear_gradient_of_a_nan_row_is_nan_and_stays_there(dtype, activation, M):
+    x, W, bias, _, dy = linear_problem(dtype, M, 64, 48)
+    x[3] = float("nan")
+    leaf = x.requires_grad_(True)
+    dx, = torch.autograd.grad(linear_act(leaf, W, bias, activation=activation), leaf, dy)
+    rest = [m for m in range(M) if m != 3]
+    assert bool(dx[3].isnan().all()) and bool(torch.isfinite(dx[rest]).all())
 
 
 @pytest.mark.gpu
