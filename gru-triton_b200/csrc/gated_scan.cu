@@ -4,7 +4,7 @@
 //
 // Each (row, unit) is a chain of its own whose steps are affine maps h -> z h + u.  Maps compose,
 // (A2, b2) o (A1, b1) = (A2 A1, A2 b1 + b2), so time is cut: a thread folds 8 or 16 steps of two units, a CTA a tile (64 steps
-// of 64 units; where rows are few 128), and a cluster of up to 8 CTAs takes that many tiles of the same units at once.  Maps are joined in
+// of 64 units; where rows are few 128), and a cluster of up to 16 CTAs takes that many tiles of the same units at once.  Maps are joined in
 // the order of time at every level (through shared memory, then through the cluster's), never in the order of arrival.
 // The backward pass is the same scan in the other direction, G_t = z_t (dout_t + G_{t+1}), with the same products of z; it
 // recomputes the states of a tile from the one that the forward kept, so `out` is not read again.
@@ -25,7 +25,6 @@ __device__ int g_gated_status;
 
 namespace {
 
-constexpr int MAX_CLUSTER = 8;
 constexpr int STAGES_MAX = 4;
 
 // L threads side by side have the units of a tile (two each), P of them one behind the other its steps (S each).
@@ -740,19 +739,25 @@ bool narrow(int T, int B, int H) { return T > Forward::STEPS && (long long)B * c
 
 // CTAs of a row's units: a cluster of them where that makes at most 256 CTAs, up to the row's tiles.  An exchange costs about
 // what a tile does, so more pay only where SMs have nothing else (64 narrow CTAs over 2000 steps: 27 / 41 us alone, 18 / 25 in
-// clusters of 4, 23 / 29 of 8).
+// clusters of 4, 23 / 29 of 8).  Clusters above 8 find room only while there are few of them: 16 columns over 20000 steps 54 / 82 us
+// with 8, 41 / 63 with 12, 53 / 74 with 16; 8 columns 41 / 61, 39 / 59, 33 / 47; 32 columns over 32768 steps 84 / 133 with 8,
+// 115 / 176 with 12.
 int ranks_for(const Args& a) {
   if (!narrow(a.T, a.B, a.H)) return 1;
   const long long base = (long long)a.B * cdiv(a.H, Narrow::UNITS);
   const int tiles = cdiv(a.T, Narrow::STEPS);
   int ranks = 1;
-  while (ranks < MAX_CLUSTER && ranks < tiles && base * ranks * 2 <= 256) ranks *= 2;
-  return ranks;
+  while (ranks < 8 && base * ranks * 2 <= 256) ranks *= 2;
+  if (base <= 16) ranks = base <= 8 ? 16 : 12;
+  return ranks < tiles ? ranks : tiles;
 }
 
 template <typename... KArgs, typename... CArgs>
 int launch_tiles(void (*kernel)(KArgs...), long long blocks, int threads, int ranks, size_t smem, cudaStream_t st, CArgs... args) {
-  if (allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem) != B200GRU_OK) return B200GRU_UNSUPPORTED;
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  if (allow_dynamic_smem(fn, smem) != B200GRU_OK) return B200GRU_UNSUPPORTED;
+  if (ranks > 8 && cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return check_launch("cudaFuncSetAttribute(gated scan)");
   if (blocks > 0x7fffffffll) return B200GRU_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;

@@ -80,8 +80,8 @@ def _run(a, backward: bool, device) -> None:
     lib = _lib.load()
     call = lib.b200gru_linear_act_backward if backward else lib.b200gru_linear_act_forward
     ref = ctypes.byref(a)
-    rc = call_on(device, call, ref)
-    if rc == _WORKSPACE_TOO_SMALL:                     # 16-bit tensors in the common layout need none
+    rc = _WORKSPACE_TOO_SMALL if a.dtype == 0 and a.M > 8 else call_on(device, call, ref)
+    if rc == _WORKSPACE_TOO_SMALL:                     # 16-bit tensors in the common layout need none, planes of fp32 always
         n = lib.b200gru_linear_act_workspace_bytes(ref, int(backward))
         ws = torch.empty(n, dtype=torch.uint8, device=device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), n

@@ -121,7 +121,7 @@ def check_scan(gi, h0, lengths, candidate, dout, dh):
     return out, h_T, grads
 
 
-SCAN_SIZES = [(40, 3, 34), (200, 2, 1030), (600, 1, 130), (70, 260, 66), (9, 1, 8), (128, 1, 32), (129, 9, 2048), (1, 1, 1), (1, 3, 33), (2, 1, 8), (7, 2, 64), (16, 40, 72), (17, 2, 64), (63, 2, 64), (64, 5, 40), (65, 3, 96),
+SCAN_SIZES = [(40, 3, 34), (200, 2, 1030), (600, 1, 130), (70, 260, 66), (9, 1, 8), (128, 1, 32), (129, 9, 2048), (1700, 1, 300), (2300, 2, 256), (1, 1, 1), (1, 3, 33), (2, 1, 8), (7, 2, 64), (16, 40, 72), (17, 2, 64), (63, 2, 64), (64, 5, 40), (65, 3, 96),
               (130, 1, 512), (300, 2, 72), (257, 19, 607), (1000, 1, 1024), (200, 64, 256), (2100, 1, 24)]
 
 
