@@ -76,14 +76,15 @@ def _fill(x, W, activation) -> _lib.CLinearArgs:
 _WORKSPACE_TOO_SMALL = 4
 
 
-def _run(a, backward: bool, device) -> None:
+def _run(a, backward: bool, x) -> None:
+    device = x.device
     lib = _lib.load()
     call = lib.b200gru_linear_act_backward if backward else lib.b200gru_linear_act_forward
     ref = ctypes.byref(a)
     rc = _WORKSPACE_TOO_SMALL if a.dtype == 0 and a.M > 8 else call_on(device, call, ref)
     if rc == _WORKSPACE_TOO_SMALL:                     # 16-bit tensors in the common layout need none, planes of fp32 always
         n = lib.b200gru_linear_act_workspace_bytes(ref, int(backward))
-        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        ws = x.new_empty(n, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), n
         rc = call_on(device, call, ref)
     if rc:
@@ -96,11 +97,11 @@ def _forward(x, W, bias, residual, activation, want_slope: bool):
     lead, N = x.shape[:-1], W.shape[0]
     x, W = _rows(x), rows_contiguous(W)
     M = x.shape[0]
-    y = torch.empty((M, N), device=x.device, dtype=x.dtype)
+    y = x.new_empty((M, N))
     slope = None
     if want_slope and activation != "none":
         # rows padded to eight elements: 16-byte accesses at any width
-        slope = torch.empty((M, -(-N // 8) * 8), device=x.device, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16)
+        slope = x.new_empty((M, -(-N // 8) * 8), dtype=torch.float32 if x.dtype == torch.float32 else torch.int16)
     if M:
         a = _fill(x, W, activation)
         if bias is not None:
@@ -112,7 +113,7 @@ def _forward(x, W, bias, residual, activation, want_slope: bool):
         a.y, a.ldy = y.data_ptr(), N
         if slope is not None:
             a.slope, a.lds = slope.data_ptr(), slope.stride(0)
-        _run(a, False, x.device)
+        _run(a, False, x)
     return (y if len(lead) == 1 else y.reshape(*lead, N)), slope
 
 
@@ -129,11 +130,11 @@ class LinearActFunction(torch.autograd.Function):
     def backward(ctx: Any, dy):
         x, W, *slope = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+        dx = x.new_empty(x.shape) if need_x else None
         M, (N, K) = x.numel() // x.shape[-1], W.shape
-        fresh = torch.empty if M else torch.zeros
-        dW = fresh((N, K), device=x.device, dtype=x.dtype) if need_w else None
-        db = fresh((N,), device=x.device, dtype=x.dtype) if need_b else None
+        fresh = x.new_empty if M else x.new_zeros
+        dW = fresh((N, K)) if need_w else None
+        db = fresh((N,)) if need_b else None
         if M and (need_x or need_w or need_b):
             x2, W2, dy2 = _rows(x), rows_contiguous(W), _rows(dy)
             a = _fill(x2, W2, ctx.activation)
@@ -143,7 +144,7 @@ class LinearActFunction(torch.autograd.Function):
             for name, t in (("dx", dx), ("dW", dW), ("db", db)):
                 if t is not None:
                     setattr(a, name, t.data_ptr())
-            _run(a, True, x.device)
+            _run(a, True, x)
         return dx, dW, db, (dy if need_r else None), None
 
 

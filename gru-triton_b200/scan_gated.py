@@ -99,8 +99,8 @@ def _empty_like_rows(gi: torch.Tensor, cols: int) -> torch.Tensor:
     """``[T, B, cols]`` in gi's order of axes (a batch-first view stays one)."""
     T, B, _ = gi.shape
     if gi.stride(0) < gi.stride(1):
-        return torch.empty((B, T, cols), device=gi.device, dtype=gi.dtype).transpose(0, 1)
-    return torch.empty((T, B, cols), device=gi.device, dtype=gi.dtype)
+        return gi.new_empty((B, T, cols)).transpose(0, 1)
+    return gi.new_empty((T, B, cols))
 
 
 def _fill(gi, h0, lengths, candidate) -> _lib.CGatedArgs:
@@ -124,10 +124,10 @@ def _forward(gi, h0, lengths, candidate, want_states: bool):
     lengths = None if lengths is None else lengths.contiguous()
     T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
     out = _empty_like_rows(gi, H)
-    h_T = torch.empty((B, H), device=gi.device, dtype=torch.float32)
+    h_T = gi.new_empty((B, H), dtype=torch.float32)
     states = None
     if want_states:
-        states = torch.empty((lib.b200gru_gated_states_bytes(T, B, H) // 4,), device=gi.device, dtype=torch.float32)
+        states = gi.new_empty(lib.b200gru_gated_states_bytes(T, B, H) // 4, dtype=torch.float32)
     a = _fill(gi, h0, lengths, candidate)
     a.out, a.h_T = out.data_ptr(), h_T.data_ptr()
     a.out_t, a.out_b, _ = out.stride()
@@ -145,7 +145,7 @@ def _backward(gi, h0, lengths, candidate, states, dout, dh_T, want_h0: bool):
     gi = rows_contiguous(gi)
     lengths = None if lengths is None else lengths.contiguous()
     dgi = _empty_like_rows(gi, gi.shape[2])
-    dh0 = torch.empty((gi.shape[1], gi.shape[2] // 2), device=gi.device, dtype=torch.float32) if want_h0 else None
+    dh0 = gi.new_empty((gi.shape[1], gi.shape[2] // 2), dtype=torch.float32) if want_h0 else None
     a = _fill(gi, None, lengths, candidate)
     a.states = states.data_ptr()
     if dout is not None:
@@ -218,7 +218,7 @@ def gated_step(gi: torch.Tensor, h: torch.Tensor, *, candidate: str = "tanh",
     gi, device = rows_contiguous(gi), gi.device
     if out_state is None:
         h = rows_contiguous(h)
-        new = torch.empty((B, H), device=device, dtype=torch.float32)
+        new = gi.new_empty((B, H), dtype=torch.float32)
     else:
         new = out_state
         if (new.stride(1) != 1 and H > 1) or (B > 1 and new.stride(0) < H):
@@ -229,7 +229,7 @@ def gated_step(gi: torch.Tensor, h: torch.Tensor, *, candidate: str = "tanh",
         if _overlap(new, gi):
             raise ValueError("out_state must not overlap gi")
         h = h if same else rows_contiguous(h)
-    out = torch.empty((B, H), device=device, dtype=gi.dtype)
+    out = gi.new_empty((B, H))
     rc = call_on(device, _lib.load().b200gru_gated_step, DTYPES[gi.dtype], _CANDIDATES[candidate], B, H, gi.data_ptr(),
                  gi.stride(0), h.data_ptr(), h.stride(0), out.data_ptr(), new.data_ptr(), max(new.stride(0), H))
     if rc:
