@@ -4,8 +4,9 @@
 //
 // Each (row, unit) is a chain of its own whose steps are affine maps h -> z h + u.  Maps compose,
 // (A2, b2) o (A1, b1) = (A2 A1, A2 b1 + b2), so time is cut: a thread folds 8 or 16 steps of two units, a CTA a tile (64 steps
-// of 64 units; where rows are few 128), and a cluster of up to 16 CTAs takes that many tiles of the same units at once.  Maps are joined in
-// the order of time at every level (through shared memory, then through the cluster's), never in the order of arrival.
+// of 64 units; where rows are few 128 of 32), and a cluster of up to 16 CTAs takes that many tiles of the same units at once.
+// Maps are joined in the order of time at every level (through shared memory, then through the cluster's), never in the order
+// of arrival.
 // The backward pass is the same scan in the other direction, G_t = z_t (dout_t + G_{t+1}), with the same products of z; it
 // recomputes the states of a tile from the one that the forward kept, so `out` is not read again.
 //
@@ -251,6 +252,7 @@ struct Ring {
 
 // Nobody leaves while a peer may still write here; a CTA that gave up waits for what is in flight.
 __device__ __forceinline__ void tear_down(const volatile int* dead, int ranks) {
+  __syncwarp();                                            // the barrier is a whole warp's instruction
   if (ranks > 1) cluster_barrier();
   if (*dead) {
     const long long start = clock64();
@@ -500,8 +502,8 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     const int t0 = tile * STEPS + part * SEG;
     const int n = len - t0;                                   // steps left from here
     P2 h = both(0.f);
-    // keep: 1 - z, then z;  p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'.  Five values a step: with a sixth the
-    // compiler computes addresses over and over for want of registers (60 instructions an element against 69).
+    // keep: 1 - z, then z;  p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'.  Five values a step: a sixth, open * keep,
+    // would save a multiplication and cost 16 registers (501 x 19 x 607, fp32: 51 us against 48).
     P2 keep[SEG], open[SEG], p[SEG], q[SEG], d[SEG];
     P2 A = both(1.f), f = both(0.f), r = f;
     if (tile >= 0) {

@@ -24,7 +24,7 @@ struct Args {
   const float* dh_T; long long dh_b;
   void* dgi; long long dgi_t, dgi_b;
   float* dh0;                  // [B][H] or NULL
-  // in bytes, ready to be added to an address (scaled in the loop, for want of registers, they cost 11 instructions of 70)
+  // in bytes, ready to be added to an address (scaled in the loop, for want of registers, they cost ten instructions of 70)
   long long out_step, dgi_step, half;          // a step of out, of dgi; from x's to c's half of a row
 };
 

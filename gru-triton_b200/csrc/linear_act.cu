@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(256) grad_kernel(const GradArgs a) {
   pdl_wait();
   const int col = threadIdx.x & 63, grp = threadIdx.x >> 6;
   const int n = (blockIdx.x * 64 + col) * V;
-  const int m1 = min(a.M, (int)(blockIdx.y + 1) * a.rows_per_slice);
+  const int m1 = (int)min((long long)a.M, (long long)(blockIdx.y + 1) * a.rows_per_slice);
   float sum[V], top[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sum[e] = top[e] = 0.f;

@@ -624,6 +624,59 @@ def test_block_trains_and_serves(dtype, T, B, K, H):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("activation", list(ACTIVATIONS))
+@pytest.mark.parametrize("M", [6, 90])
+def test_linear_gradient_against_differences(activation, M):
+    x, W, bias, residual, dy = linear_problem(torch.float32, M, 72, 40, seed=21)
+    leaves = [t.detach().requires_grad_(True) for t in (x, W, bias, residual)]
+    got = torch.autograd.grad(linear_act(*leaves[:3], activation=activation, residual=leaves[3]), leaves, dy)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    step = 1e-6
+    for which in range(4):
+        base = [t.double() for t in (x, W, bias, residual)]
+        way = torch.randn(base[which].shape, device="cuda", generator=gen, dtype=torch.float64)
+        ends = []
+        for sign in (1, -1):
+            at = list(base)
+            at[which] = at[which] + sign * step * way
+            ends.append(float(((act64(at[0] @ at[1].t() + at[2], activation) + at[3]) * dy.double()).sum()))
+        slope = (ends[0] - ends[1]) / (2 * step)
+        terms = (got[which].double() * way)
+        # step^2 times a third derivative and 2^-53 of the sums over step, the gradient's own error as above; a kink of relu
+        # within step of a value moves the difference by that value's share
+        assert abs(slope - float(terms.sum())) <= 2e-5 * float(terms.abs().sum())
+
+
+@pytest.mark.gpu
+def test_operators_from_two_threads():
+    """Two host threads, each training a block on a stream of its own."""
+    import threading
+    sets = [block_problem(torch.float32, 90, 4, 64, 128, seed=s) for s in (1, 2)]
+    want = []
+    for tensors, dy in sets:
+        leaves = [t.detach().requires_grad_(True) for t in tensors]
+        want.append(torch.autograd.grad(block(*leaves)[0], leaves, dy))
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(k):
+        tensors, dy = sets[k]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                leaves = [t.detach().requires_grad_(True) for t in tensors]
+                got[k] = torch.autograd.grad(block(*leaves)[0], leaves, dy)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in (0, 1):
+        assert all(torch.equal(a, b) for a, b in zip(got[k], want[k]))
+
+
+@pytest.mark.gpu
 def test_operators_on_another_stream():
     tensors, dy = block_problem(torch.bfloat16, 90, 4, 64, 128)
     ref = [t.detach().requires_grad_(True) for t in tensors]
