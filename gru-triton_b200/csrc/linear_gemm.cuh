@@ -6,7 +6,8 @@
 // Operands: one plane of bf16 or fp16, or (fp32) two row-scaled fp16 planes, of which low x high, high x low and high x high
 // are summed in that order.  Either operand K-major (rows of K) or MN-major (rows of M or N, one per k).  The tensor core's
 // fp32 accumulator truncates, so sums are built in chunks (24 steps for planes; 512 for 16-bit types: 512 losses of 2^-23 stay
-// a quarter of half a step of fp16) in one of two tensor-memory buffers and added to register totals with round-to-nearest.
+// a quarter of half a step of fp16) in one of two tensor-memory buffers and added with round-to-nearest (planes: in registers; 16-bit types, whose chunks are
+// long: into the next buffer).
 //
 // Roles of a CTA's ten warps: 0 loads k-blocks by TMA, 1 issues tcgen05.mma, 2-9 drain the accumulator (32 rows and half the
 // columns each; a lane has a row).  Results, slopes and residual move as TMA tiles of 32 rows x 128 bytes through swizzled
@@ -204,14 +205,14 @@ __device__ __forceinline__ void fetch_residual(const Params& p, const CUtensorMa
   }
 }
 
-// 32 columns from column c of the group on: scales, bias, activation, residual; into the buffers.
-template <int ACT, int PL, typename Out, int NC>
-__device__ __forceinline__ void finish_columns(const Params& p, const Lane& w, unsigned char* out, const uint32_t (&v)[32], float rs, int col, int c) {
+// 32 columns from column c of the group on: scales, bias, activation, residual; into the buffers.  KEEP: slopes too.
+template <int ACT, int PL, typename Out, int NC, bool KEEP>
+__device__ __forceinline__ void finish_some(const Params& p, const Lane& w, unsigned char* out, const uint32_t (&v)[32], float rs, int col, int c) {
   typedef typename Leaves<Out>::T T;
   typedef typename SlopeOf<T>::type S;
   typedef Group<T, NC> G;
   constexpr int V = Vec<T>::V;
-  const bool add = !std::is_void<Out>::value && p.with_residual, keep = ACT != B200GRU_ACT_NONE && p.with_slope;
+  const bool add = !std::is_void<Out>::value && p.with_residual;
 #pragma unroll
   for (int e = 0; e < 32; e += V) {
     P2 x[V / 2], sl[V / 2];
@@ -233,7 +234,7 @@ __device__ __forceinline__ void finish_columns(const Params& p, const Lane& w, u
       }
     }
     const uint32_t at = G::piece(w.lane, (c + e) / V);
-    if (keep) {
+    if (KEEP) {
       float f[V];
 #pragma unroll
       for (int k = 0; k < V / 2; ++k) { const float2 s = split(sl[k]); f[2 * k] = s.x; f[2 * k + 1] = s.y; }
@@ -250,6 +251,12 @@ __device__ __forceinline__ void finish_columns(const Params& p, const Lane& w, u
     for (int k = 0; k < V / 2; ++k) { const float2 y = split(x[k]); f[2 * k] = y.x; f[2 * k + 1] = y.y; }
     *reinterpret_cast<uint4*>(out + at) = pack16<T>(f);
   }
+}
+
+template <int ACT, int PL, typename Out, int NC>
+__device__ __forceinline__ void finish_columns(const Params& p, const Lane& w, unsigned char* out, const uint32_t (&v)[32], float rs, int col, int c) {
+  if (ACT != B200GRU_ACT_NONE && p.with_slope) finish_some<ACT, PL, Out, NC, true>(p, w, out, v, rs, col, c);
+  else finish_some<ACT, PL, Out, NC, false>(p, w, out, v, rs, col, c);
 }
 
 // Before a group's columns are written: its buffer is free, its residual there, the next group's requested.
@@ -270,14 +277,27 @@ __device__ __forceinline__ bool open_group(const Params& p, const CUtensorMap* t
   __syncwarp();
   return true;
 }
+// Tile store whose lines leave L2 before others: results pass through, the operands are read again (32768 x 2048 -> 4096, gelu:
+// 371 -> 348 us, with slopes 444 -> 402).
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, int c0, int c1, int c2, uint32_t src, uint64_t policy) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%1, %2, %3}], [%4], %5;"
+               ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(src), "l"(policy) : "memory");
+}
 // The group's results (and slopes) start on their way.
 template <typename Out, int NC>
 __device__ __forceinline__ void close_group(const Params& p, const CUtensorMap* tmC, const CUtensorMap* tmS, Lane& w, const Corner& at, int col) {
   tc::fence_async_smem();
   __syncwarp();
   if (w.lane == 0) {
-    tc::tma_store_3d(tmC, at.col + col, at.row, at.z, tc::smem_u32(w.out + (w.sent & p.out_mask) * WARP_OUT));
-    if (!std::is_void<Out>::value && p.with_slope) tc::tma_store_3d(tmS, at.col + col, at.row, 0, tc::smem_u32(w.slopes));
+    const uint32_t from = tc::smem_u32(w.out + (w.sent & p.out_mask) * WARP_OUT);
+    if (std::is_void<Out>::value) {
+      tc::tma_store_3d(tmC, at.col + col, at.row, at.z, from);       // read again at once
+    } else {
+      uint64_t policy;
+      asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+      store_tile(tmC, at.col + col, at.row, 0, from, policy);
+      if (p.with_slope) store_tile(tmS, at.col + col, at.row, 0, tc::smem_u32(w.slopes), policy);
+    }
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
   ++w.sent;
@@ -714,7 +734,7 @@ int launch_tile(const Gemm& g, cudaStream_t st) {
   if (g.a_mn && g.b_mn) return launch_variant<CTAS, BN, true, true, PL, NONE, Out>(p, m, st);
   if (!g.a_mn && g.b_mn) return launch_variant<CTAS, BN, false, true, PL, NONE, Out>(p, m, st);
   if (g.a_mn) return B200GRU_UNSUPPORTED;
-  if constexpr (!PARTIAL) {                               // one kernel for each activation: chosen once an element, it cost 30 products
+  if constexpr (!PARTIAL) {                               // one kernel for each activation: chosen once an element, it cost ten products
     switch (g.activation) {
       case B200GRU_ACT_RELU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_RELU, Out>(p, m, st);
       case B200GRU_ACT_SILU: return launch_variant<CTAS, BN, false, false, PL, B200GRU_ACT_SILU, Out>(p, m, st);
