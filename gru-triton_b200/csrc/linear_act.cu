@@ -350,9 +350,16 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishArgs a) {
 }
 
 // ---- a few rows ----------------------------------------------------------------------------------------
-// Bound by one read of W.  A warp has NW rows of W and a slice of K; lanes take 16 bytes each, partial sums of the lanes are
+// Bound by one read of W (for each eight rows of x).  A warp has NW rows of W and a slice of K; lanes take 16 bytes each, partial sums of the lanes are
 // added by a butterfly, those of the CTA's K slices in their order.  The assignment of k to lanes does not depend on alignment.
-constexpr int FEW = 8;
+// Where it runs (us in a graph, it / the tensor-core products): bf16 1024 -> 4096 2 rows 4.5 / 7.3, 4 rows 6.9 / 7.3, 8 rows
+// 10.1 / 7.3; 4096 -> 4096 2 rows 9.7 / 10.3, 4 rows 19.7 / 10.3.  fp32 (whose products need a pass for their planes) 4096 -> 4096
+// 8 rows 45 / 65, 512 -> 512 8 rows 3.2 / 9.7.
+bool few_rows_apply(int M, int N, int K, bool f32) {
+  const double work = (double)M * N * K;
+  if (f32) return M <= 8 || (M <= 32 && work <= 8.4e6);
+  return M <= 2 || (M <= 8 && work <= 16.8e6);
+}
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void take(const T* p, int k, int K, float (&v)[Vec<T>::V]) {
@@ -568,7 +575,7 @@ struct Call {
   }
 
   int forward() {
-    if (a.M <= FEW) {
+    if (few_rows_apply(a.M, a.N, a.K, F32)) {
       if (!dry) rc = few_rows<T>(a, st);
       return rc;
     }
@@ -707,20 +714,23 @@ int checked(const b200gru_linear_args* p, bool backward, void* stream) {
 
 }  // namespace
 
-// Cycles of a tile's k-block, of its start and end, of a launch that joins slices; the cheapest cut of the work.
+// Cycles of a tile's k-block and tail, of a launch's start and end, of one that joins slices; the cheapest cut of the work.
+// Fitted to 16 .. 16384 rows, 120 .. 8192 columns in both types: within 16 % of the best of 30 cuts.
 Plan plan_gemm(int M, int N, int K, int planes) {
   const int kb = cdiv(K, 64);
   const double products = planes == 2 ? 3.0 : 1.0;
   Plan best = {1, 128, 1};
   double best_cost = 1e30;
-  const struct { int ctas, m, n, units; double per_kb; } cuts[3] = {{2, 256, 256, 74, 560.0}, {1, 128, 128, 148, 370.0}, {1, 128, 64, 148, 270.0}};
+  const struct { int ctas, m, n, units; double per_kb, tail; } cuts[3] = {
+      {2, 256, 256, 74, 560.0, 4500.0}, {1, 128, 128, 148, 370.0, 2500.0}, {1, 128, 64, 148, 270.0, 1500.0}};
   for (const auto& c : cuts) {
     const long long tiles = (long long)cdiv(M, c.m) * cdiv(N, c.n);
     for (int want = 1; want <= 64 && want <= kb; ++want) {
       const int per = cdiv(kb, want), splits = cdiv(kb, per);
       if (splits != want || (splits > 1 && per < 4)) continue;
       const double waves = (double)((tiles * splits + c.units - 1) / c.units);
-      double cost = waves * per * c.per_kb * products + 4000.0 + 2500.0 * (c.n / 128.0);
+      const double loop = per * c.per_kb * products;       // a tile's tail hides under the next one's products, if those last
+      double cost = waves * (loop > c.tail ? loop : c.tail) + 4000.0 + 2500.0 * (c.n / 128.0);
       if (splits > 1) cost += 5000.0 + (double)splits * M * N * 8.0 / 3500.0;      // written and read again
       if (cost < best_cost) { best_cost = cost; best = {c.ctas, c.n, splits}; }
     }

@@ -311,7 +311,8 @@ int b200gru_gated_step(int dtype, int candidate_tanh, int B, int H, const void* 
  * All of `dtype`; row strides ld* in elements (inputs may have stride 0), rows contiguous; dx, dW and db are packed.
  * bias, residual, dx, dW, db may be NULL.  slope: [M][lds], written by a forward that a backward follows (4 bytes each
  * for fp32, else 2) and read by it; NULL in inference and where there is no activation.  workspace: 256-byte aligned,
- * b200gru_linear_act_workspace_bytes of the same arguments ((size_t)-1: invalid).  No reference counterpart (its
+ * b200gru_linear_act_workspace_bytes of the same arguments ((size_t)-1: invalid).  Results repeat their bits; those of a row
+ * depend on M to rounding.  No reference counterpart (its
  * projections are F.linear, src/gru_qat/gru_cell.py:410-435). */
 enum { B200GRU_ACT_NONE = 0, B200GRU_ACT_RELU = 1, B200GRU_ACT_SILU = 2, B200GRU_ACT_GELU = 3, B200GRU_ACT_SIGMOID = 4,
        B200GRU_ACT_TANH = 5 };
