@@ -121,7 +121,7 @@ def check_scan(gi, h0, lengths, candidate, dout, dh):
     return out, h_T, grads
 
 
-SCAN_SIZES = [(40, 3, 34), (200, 2, 1030), (600, 1, 130), (70, 260, 66), (9, 1, 8), (128, 1, 32), (129, 9, 2048), (1700, 1, 300), (2300, 2, 256), (1, 1, 1), (1, 3, 33), (2, 1, 8), (7, 2, 64), (16, 40, 72), (17, 2, 64), (63, 2, 64), (64, 5, 40), (65, 3, 96),
+SCAN_SIZES = [(12, 70001, 8), (3, 70001, 5), (20, 1, 70002), (40, 3, 34), (200, 2, 1030), (600, 1, 130), (70, 260, 66), (9, 1, 8), (128, 1, 32), (129, 9, 2048), (1700, 1, 300), (2300, 2, 256), (1, 1, 1), (1, 3, 33), (2, 1, 8), (7, 2, 64), (16, 40, 72), (17, 2, 64), (63, 2, 64), (64, 5, 40), (65, 3, 96),
               (130, 1, 512), (300, 2, 72), (257, 19, 607), (1000, 1, 1024), (200, 64, 256), (2100, 1, 24)]
 
 
@@ -411,7 +411,7 @@ def check_linear(x, W, bias, residual, activation, dy):
     return y, got
 
 
-LINEAR_SIZES = [(5, 2048, 2048), (2, 1024, 1024), (17, 96, 130), (32, 200, 64), (1, 1, 1), (1, 64, 64), (2, 100, 7), (3, 129, 250), (8, 512, 1024), (9, 256, 96), (16, 65, 33), (33, 1024, 512),
+LINEAR_SIZES = [(300, 70000, 1), (40, 1, 70000), (70000, 1, 3), (70000, 3, 9), (1, 70000, 2), (5, 2048, 2048), (2, 1024, 1024), (17, 96, 130), (32, 200, 64), (1, 1, 1), (1, 64, 64), (2, 100, 7), (3, 129, 250), (8, 512, 1024), (9, 256, 96), (16, 65, 33), (33, 1024, 512),
                 (64, 96, 260), (127, 63, 127), (128, 128, 128), (129, 72, 257), (300, 1000, 136), (1000, 120, 608), (2048, 512, 1024),
                 (700, 2050, 70), (5000, 40, 24), (4100, 136, 1032)]
 
