@@ -474,6 +474,23 @@ def test_linear_reads_any_layout(dtype, M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("activation", ["none", "gelu"])
+@pytest.mark.parametrize("M, K, N", [(4, 64, 1), (40, 1, 1), (300, 128, 1), (300, 1, 72), (300, 200, 72)])
+def test_linear_rows_of_stride_zero(dtype, activation, M, K, N):
+    x, W, bias, residual, dy = linear_problem(dtype, M, K, N, seed=5)
+    same = [x[:1].expand(M, K), W[:1].expand(N, K), bias[:1].expand(N), residual[:1, :1].expand(M, N)]
+    every = dy[:1, :1].expand(M, N)
+    results = []
+    for form in (lambda t: t, lambda t: t.clone(memory_format=torch.contiguous_format)):
+        leaves = [form(t).detach().requires_grad_(True) for t in same]
+        out = linear_act(*leaves[:3], activation=activation, residual=leaves[3])
+        results.append((out, *torch.autograd.grad(out, leaves, form(every))))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [5, 200])
 def test_linear_no_rows_some_gradients_and_special_values(M):
     x, W, bias, residual, dy = linear_problem(torch.float32, M, 64, 48)
