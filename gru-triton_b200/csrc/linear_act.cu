@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishArgs a) {
   typedef typename SlopeOf<T>::type S;
   pdl_launch_dependents();
   pdl_wait();
-  const int quads = (int)(a.ldp / 4);
+  const int quads = cdiv(a.N, 4);                          // not ldp / 4: rows of C may end four columns before the padded ones do
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= (long long)a.M * quads) return;
   const int m = (int)(i / quads), n = (int)(i % quads) * 4;
@@ -569,7 +569,7 @@ struct Call {
     if (dry || rc != B200GRU_OK) return;
     rc = launch_gemm<void>(g, plan, st);
     if (rc != B200GRU_OK) return;
-    const long long quads = (long long)g.M * (g.ldp / 4);
+    const long long quads = (long long)g.M * cdiv(g.N, 4);
     launch_pdl(finish_kernel<T>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, f);
     note("finish_kernel");
   }

@@ -411,7 +411,7 @@ def check_linear(x, W, bias, residual, activation, dy):
     return y, got
 
 
-LINEAR_SIZES = [(300, 70000, 1), (40, 1, 70000), (70000, 1, 3), (70000, 3, 9), (1, 70000, 2), (5, 2048, 2048), (2, 1024, 1024), (17, 96, 130), (32, 200, 64), (1, 1, 1), (1, 64, 64), (2, 100, 7), (3, 129, 250), (8, 512, 1024), (9, 256, 96), (16, 65, 33), (33, 1024, 512),
+LINEAR_SIZES = [(40, 2048, 132), (1000, 132, 60), (5310, 804, 423), (300, 70000, 1), (40, 1, 70000), (70000, 1, 3), (70000, 3, 9), (1, 70000, 2), (5, 2048, 2048), (2, 1024, 1024), (17, 96, 130), (32, 200, 64), (1, 1, 1), (1, 64, 64), (2, 100, 7), (3, 129, 250), (8, 512, 1024), (9, 256, 96), (16, 65, 33), (33, 1024, 512),
                 (64, 96, 260), (127, 63, 127), (128, 128, 128), (129, 72, 257), (300, 1000, 136), (1000, 120, 608), (2048, 512, 1024),
                 (700, 2050, 70), (5000, 40, 24), (4100, 136, 1032)]
 
