@@ -17,6 +17,7 @@ Tolerances (u = 2^-24, half a step of float32; ``half(t)`` = eps / 2 of an outpu
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -121,8 +122,10 @@ def check_scan(gi, h0, lengths, candidate, dout, dh):
     return out, h_T, grads
 
 
-SCAN_SIZES = [(12, 70001, 8), (3, 70001, 5), (20, 1, 70002), (40, 3, 34), (200, 2, 1030), (600, 1, 130), (70, 260, 66), (9, 1, 8), (128, 1, 32), (129, 9, 2048), (1700, 1, 300), (2300, 2, 256), (1, 1, 1), (1, 3, 33), (2, 1, 8), (7, 2, 64), (16, 40, 72), (17, 2, 64), (63, 2, 64), (64, 5, 40), (65, 3, 96),
-              (130, 1, 512), (300, 2, 72), (257, 19, 607), (1000, 1, 1024), (200, 64, 256), (2100, 1, 24)]
+SCAN_SIZES = [(12, 70001, 8), (3, 70001, 5), (20, 1, 70002), (40, 3, 34), (200, 2, 1030), (600, 1, 130), (70, 260, 66),
+              (9, 1, 8), (128, 1, 32), (129, 9, 2048), (1700, 1, 300), (2300, 2, 256), (1, 1, 1), (1, 3, 33), (2, 1, 8),
+              (7, 2, 64), (16, 40, 72), (17, 2, 64), (63, 2, 64), (64, 5, 40), (65, 3, 96), (130, 1, 512), (300, 2, 72),
+              (257, 19, 607), (1000, 1, 1024), (200, 64, 256), (2100, 1, 24)]
 
 
 @pytest.mark.gpu
@@ -397,7 +400,9 @@ def check_linear(x, W, bias, residual, activation, dy):
         off_d = dy64.abs() * (pre.abs() <= off_pre) + 0 * d      # the sign of pre decides
     if dtype != torch.float32 and activation != "none":
         off_d = off_d + dy64.abs() * 2.0 ** -16
-    in_product = off_d + (half(dtype) * d.abs() if dtype != torch.float32 and activation != "none" else 0.0)
+    # the products take d in the type: half a step of its value, or of fp16's smallest, 2^-24, where d is that small (a
+    # product of one term, M or N of 1, has no larger ones beside it)
+    in_product = off_d + (rounding(d, dtype) if dtype != torch.float32 and activation != "none" else 0.0)
     refs = [d @ W64, d.t() @ x64]
     sums = [d.abs() @ W64.abs(), d.abs().t() @ x64.abs()]
     carried = [in_product @ W64.abs(), in_product.t() @ x64.abs()]
@@ -411,9 +416,11 @@ def check_linear(x, W, bias, residual, activation, dy):
     return y, got
 
 
-LINEAR_SIZES = [(40, 2048, 132), (1000, 132, 60), (5310, 804, 423), (300, 70000, 1), (40, 1, 70000), (70000, 1, 3), (70000, 3, 9), (1, 70000, 2), (5, 2048, 2048), (2, 1024, 1024), (17, 96, 130), (32, 200, 64), (1, 1, 1), (1, 64, 64), (2, 100, 7), (3, 129, 250), (8, 512, 1024), (9, 256, 96), (16, 65, 33), (33, 1024, 512),
-                (64, 96, 260), (127, 63, 127), (128, 128, 128), (129, 72, 257), (300, 1000, 136), (1000, 120, 608), (2048, 512, 1024),
-                (700, 2050, 70), (5000, 40, 24), (4100, 136, 1032)]
+LINEAR_SIZES = [(40, 2048, 132), (1000, 132, 60), (5310, 804, 423), (300, 70000, 1), (40, 1, 70000), (70000, 1, 3),
+                (70000, 3, 9), (1, 70000, 2), (5, 2048, 2048), (2, 1024, 1024), (17, 96, 130), (32, 200, 64), (1, 1, 1),
+                (1, 64, 64), (2, 100, 7), (3, 129, 250), (8, 512, 1024), (9, 256, 96), (16, 65, 33), (33, 1024, 512),
+                (64, 96, 260), (127, 63, 127), (128, 128, 128), (129, 72, 257), (300, 1000, 136), (1000, 120, 608),
+                (2048, 512, 1024), (700, 2050, 70), (5000, 40, 24), (4100, 136, 1032)]
 
 
 @pytest.mark.gpu
@@ -488,6 +495,43 @@ def test_linear_rows_of_stride_zero(dtype, activation, M, K, N):
         results.append((out, *torch.autograd.grad(out, leaves, form(every))))
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M, K, N", [(40, 2048, 132), (1000, 132, 60), (40, 2048, 130), (300, 100, 135), (2, 60, 36)])
+def test_linear_writes_inside_its_results(dtype, M, K, N):
+    x, W, bias, residual, dy = linear_problem(dtype, M, K, N, seed=6)
+    size, margin, lds = dtype.itemsize, 4096, (N + 7) // 8 * 8
+    lib, stream = _lib.load(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def guarded(count):
+        return torch.full((count + 2 * margin,), 0x5A, dtype=torch.uint8, device="cuda")
+
+    def args(**buffers):
+        a = _lib.CLinearArgs()
+        a.M, a.K, a.N, a.dtype, a.activation = M, K, N, DTYPES.index(dtype), ACTIVATIONS["gelu"]
+        a.x, a.ldx, a.W, a.ldw, a.lds = x.data_ptr(), K, W.data_ptr(), K, lds
+        for name, t in buffers.items():
+            setattr(a, name, t.data_ptr() + margin)
+        return a
+
+    def call(fn, backward, a, buffers):
+        n = lib.b200gru_linear_act_workspace_bytes(ctypes.byref(a), backward)
+        buffers = dict(buffers, workspace=guarded(n))
+        a.workspace, a.workspace_bytes = buffers["workspace"].data_ptr() + margin, n
+        assert fn(ctypes.byref(a), stream) == 0
+        for name, t in buffers.items():
+            assert bool((t[:margin] == 0x5A).all()) and bool((t[t.numel() - margin:] == 0x5A).all()), name
+
+    out = dict(y=guarded(M * N * size), slope=guarded(M * lds * max(2, size)))
+    a = args(**out)
+    a.bias, a.residual, a.ldr, a.ldy = bias.data_ptr(), residual.data_ptr(), N, N
+    call(lib.b200gru_linear_act_forward, 0, a, out)
+    grads = dict(dx=guarded(M * K * size), dW=guarded(N * K * size), db=guarded(N * size))
+    a = args(slope=out["slope"], **grads)
+    a.dy, a.lddy = dy.data_ptr(), N
+    call(lib.b200gru_linear_act_backward, 1, a, grads)
 
 
 @pytest.mark.gpu
