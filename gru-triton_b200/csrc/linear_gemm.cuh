@@ -4,10 +4,15 @@
 //   C[M,N] = epilogue( row_scale[m] col_scale[n] sum_p A_p[M,K] B_p[N,K]^T )
 //
 // Operands: one plane of bf16 or fp16, or (fp32) two row-scaled fp16 planes, of which low x high, high x low and high x high
-// are summed in that order.  Either operand K-major (rows of K) or MN-major (rows of M or N, one per k).  The tensor core's
-// fp32 accumulator truncates, so sums are built in chunks (24 steps for planes; 512 for 16-bit types: 512 losses of 2^-23 stay
-// a quarter of half a step of fp16) in one of two tensor-memory buffers and added with round-to-nearest (planes: in registers; 16-bit types, whose chunks are
-// long: into the next buffer).
+// are summed in that order.  Either operand K-major (rows of K) or MN-major (rows of M or N, one per k).
+//
+// The tensor core's fp32 accumulator truncates: a sum of K terms loses up to 2^-23 of itself at each of its K / 16 steps, always
+// towards zero.  So sums are built in chunks, in one of two tensor-memory buffers, and the chunks added with round-to-nearest.
+// Planes: 24 steps.  16-bit types without an activation (gates of a recurrence, whose fp32 state carries every rounding of a
+// gate on; gradients): 8 steps where K is at most 512, else 16, added in registers.  With an activation 64 steps, added into the
+// next buffer: its epilogue is long, and reading chunks between would hold the products up (32768 x 1024 -> 4096 bf16, gelu: 196 us;
+// 241 with 32 steps, 304 with 16; none: 198 us with 16, 177 with one chunk).  Share of bf16 results that are not the rounding of the exact
+// sum, K 512 / 1024 / 4096: 1.0 / 1.8 / 2.0e-4 (one chunk: 2.8 / 5.6 / 23e-4; fp32 multiply-adds: 1.2 / 1.7 / 3.7e-4).
 //
 // Roles of a CTA's ten warps: 0 loads k-blocks by TMA, 1 issues tcgen05.mma, 2-9 drain the accumulator (32 rows and half the
 // columns each; a lane has a row).  Results, slopes and residual move as TMA tiles of 32 rows x 128 bytes through swizzled
@@ -207,7 +212,7 @@ __device__ __forceinline__ void fetch_residual(const Params& p, const CUtensorMa
 
 // 32 columns from column c of the group on: scales, bias, activation, residual; into the buffers.  KEEP: slopes too.
 template <int ACT, int PL, typename Out, int NC, bool KEEP>
-__device__ __forceinline__ void finish_some(const Params& p, const Lane& w, unsigned char* out, const uint32_t (&v)[32], float rs, int col, int c) {
+__device__ __forceinline__ void finish_some(const Params& p, const Lane& w, unsigned char* out, const P2* v, float rs, int col, int c) {
   typedef typename Leaves<Out>::T T;
   typedef typename SlopeOf<T>::type S;
   typedef Group<T, NC> G;
@@ -218,7 +223,7 @@ __device__ __forceinline__ void finish_some(const Params& p, const Lane& w, unsi
     P2 x[V / 2], sl[V / 2];
 #pragma unroll
     for (int k = 0; k < V / 2; ++k) {
-      x[k] = pair(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1]));
+      x[k] = v[e / 2 + k];
       if (PL == 2) {
         const float2 cs = *reinterpret_cast<const float2*>(w.coef + NC + col + e + 2 * k);
         x[k] = mul2(mul2(x[k], both(rs)), pair(cs.x, cs.y));
@@ -254,7 +259,7 @@ __device__ __forceinline__ void finish_some(const Params& p, const Lane& w, unsi
 }
 
 template <int ACT, int PL, typename Out, int NC>
-__device__ __forceinline__ void finish_columns(const Params& p, const Lane& w, unsigned char* out, const uint32_t (&v)[32], float rs, int col, int c) {
+__device__ __forceinline__ void finish_columns(const Params& p, const Lane& w, unsigned char* out, const P2* v, float rs, int col, int c) {
   if (ACT != B200GRU_ACT_NONE && p.with_slope) finish_some<ACT, PL, Out, NC, true>(p, w, out, v, rs, col, c);
   else finish_some<ACT, PL, Out, NC, false>(p, w, out, v, rs, col, c);
 }
@@ -526,9 +531,9 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         return open_group<Out, NC>(p, &tmR, w, here ? Corner{at.row, at.col + (g + 1) * G::COLS, 0} : then, here || !last, deadp, status);
       };
       auto close = [&](int g) { close_group<Out, NC>(p, &tmC, &tmS, w, at, g * G::COLS); };
-      if (PL == 1) {
-        // Totals of more than one chunk are summed in registers and put back, so that the way out is one: from tensor memory, the
-        // next 32 columns requested before these are finished.
+      if (PL == 1 && ACT != B200GRU_ACT_NONE) {
+        // Long chunks, usually one: a total of more is summed in registers and put back, so that the way out is one: from tensor
+        // memory, the next 32 columns requested before these are finished.
         const int buf0 = c & 1;
         ok = landed(buf0);
         if (!ok) break;
@@ -563,9 +568,9 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           for (int c0 = 0; c0 < G::COLS; c0 += 32) {
             const int col = g * G::COLS + c0;
             tc::tmem_ld_wait();
-            uint32_t x[32];
+            P2 x[16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] = v[j];
+            for (int j = 0; j < 16; ++j) x[j] = pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
             if (col + 32 < NC) tc::tmem_ld32(source(buf) + (uint32_t)(col + 32), v);
             finish_columns<ACT, PL, Out, NC>(p, w, out, x, rs, col, c0);
           }
@@ -575,10 +580,10 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         release(buf);
         ++c;
       } else {
-        // planes: chunks are short, so the totals stay in registers and a buffer is free at once
-        float acc[NC];
+        // chunks are short, so the totals stay in registers and a buffer is free at once
+        P2 acc[NC / 2];
 #pragma unroll
-        for (int j = 0; j < NC; ++j) acc[j] = 0.f;
+        for (int j = 0; j < NC / 2; ++j) acc[j] = both(0.f);
         for (int i = 0; i < chunks; ++i, ++c) {
           const int buf = c & 1;
           ok = landed(buf);
@@ -589,7 +594,8 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             tc::tmem_ld16(source(buf) + (uint32_t)c0, v);
             tc::tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) acc[c0 + j] += __uint_as_float(v[j]);
+            for (int j = 0; j < 16; j += 2)
+              acc[(c0 + j) / 2] = add2(acc[(c0 + j) / 2], pair(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
           }
           release(buf);
         }
@@ -599,10 +605,9 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           if (at.col + g * G::COLS >= p.N) break;            // warp-uniform
           if (ok) ok = open(g);
           unsigned char* out = w.out + (w.sent & p.out_mask) * WARP_OUT;
-          uint32_t x[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(acc[g * G::COLS + j]);
-          finish_columns<ACT, PL, Out, NC>(p, w, out, x, rs, g * G::COLS, 0);
+          for (int c0 = 0; c0 < G::COLS; c0 += 32)
+            finish_columns<ACT, PL, Out, NC>(p, w, out, acc + (g * G::COLS + c0) / 2, rs, g * G::COLS + c0, c0);
           close(g);
         }
       }
@@ -704,7 +709,8 @@ int launch_tile(const Gemm& g, cudaStream_t st) {
   p.tiles = (int)tiles;
   p.kb_total = cdiv(g.K, 64);
   p.kb_per_split = cdiv(p.kb_total, g.splits);
-  p.chunk_kb = PL == 2 ? 2 : 128;
+  if (PL == 1 && !PARTIAL && g.activation != B200GRU_ACT_NONE) p.chunk_kb = 16;
+  else p.chunk_kb = PL == 2 || p.kb_per_split <= 8 ? 2 : 4;
   p.ab_format = g.fp16 ? 0u : 1u;
   p.row_scale = g.row_scale; p.col_scale = g.col_scale; p.bias = g.bias;
   p.with_residual = !PARTIAL && g.residual != nullptr;

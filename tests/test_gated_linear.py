@@ -630,6 +630,48 @@ def test_linear_offsets_past_32_bits():
     start = (M - 2048) // 2048 * 2048
     assert torch.equal(y[start:start + 2048], ref) and torch.equal(y[-37:], ref[:37])
 
+def rounding_share(x, W, dtype, steps):
+    """Of the results of a 16-bit product above 1/4 in size, the share that its sums round to another number than the exact sum does.
+    A step of 16 terms that truncates loses half a unit in the last place on average, u of the running sum at most; adding a
+    chunk is off by u / 2 of the total on average; the losses of different chunks add up like random signs (their sums have
+    any sign).  A sum that is off by e lies on the other side of a border of its type with probability e / step."""
+    parts = torch.einsum("msk,nsk->mns", x.double().unflatten(1, (-1, 16)), W.double().unflatten(1, (-1, 16)))
+    total = parts.cumsum(2)
+    lost = U * parts.unflatten(2, (-1, steps)).cumsum(3).abs().sum(3)
+    off = (lost.square().sum(2) + (U / 2 * total[..., steps - 1::steps]).square().sum(2)).sqrt()
+    ref = total[..., -1]
+    step = torch.finfo(dtype).eps * torch.exp2(torch.floor(torch.log2(ref.abs().clamp(min=0.25))))
+    return float((off / step)[ref.abs() >= 0.25].mean())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("activation,K,steps", [("none", 512, 8), ("none", 1024, 16), ("none", 4096, 16), ("relu", 4096, 64)])
+def test_linear_16_bit_sums_are_built_in_short_chunks(dtype, activation, K, steps):
+    """The share of results that are not the rounding of the exact sum (the tensor core truncates at every step: one chunk of
+    all of K would leave eight times as many at K = 4096)."""
+    x, W, _, _, _ = linear_problem(dtype, 8192, K, 1024, seed=K)
+    y = linear_act(x, W, activation=activation)
+    ref = act64(x.double() @ W.double().t(), activation)
+    here = ref.abs() >= 0.25
+    n, share = int(here.sum()), rounding_share(x[:128], W, dtype, steps)
+    assert int((y != ref.to(dtype))[here].sum()) <= n * share + 6 * math.sqrt(n * share)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_block_state_is_float32_of_its_gates(dtype):
+    """The state behind 16-bit gates is that of these gates to float32 accuracy.  (That of other sums for the same gates is not: a gate
+    on the border of two of its type's numbers may be rounded to either.)"""
+    T, B, K, H = 100, 17, 512, 512
+    (x, Wi, bi, _, _, h0), _ = block_problem(dtype, T, B, K, H)
+    gi = linear_act(x, Wi, bi)
+    _, h_T = gated_scan(gi, h0)
+    ref = scan64(gi, h0, None, "tanh")[1]
+    close(h_T, ref, scan_tolerance(gi, h0, T, "tanh")[1] + rounding(ref, torch.float32))
+    # relative to the norm: errors of a step, about 3 u, add up over memories of ten steps
+    assert float((h_T.double() - ref).norm() / ref.norm()) <= 30 * U
+
 
 # ---- streams, graphs, the two together ---------------------------------------------------------------
 
