@@ -9,6 +9,12 @@ import torch
 from . import _lib
 
 
+def transformed() -> bool:
+    """Function transforms, forward-mode AD and tracing look at every operation: not for a call past autograd."""
+    return (torch._C._functorch.peek_interpreter_stack() is not None or
+            torch.autograd.forward_ad._current_level >= 0 or torch.jit.is_tracing())
+
+
 def require_cuda(**tensors) -> None:
     bad = {k: v.device for k, v in tensors.items() if not v.is_cuda}
     if bad:

@@ -18,6 +18,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
+from ._scan_common import transformed
 from .quantizers import FakeQuantizePerChannel, FakeQuantizePerGroup, FakeQuantizePerTensor, Identity
 
 _INTS = ctypes.c_int * 10
@@ -71,12 +72,6 @@ def _observed(module) -> bool:
 def _plain(t, shape, device):
     return ((type(t) is torch.nn.Parameter or type(t) is torch.Tensor) and t.dtype is torch.float32 and
             t.device == device and t.shape == shape and t.is_contiguous())
-
-
-def _transformed() -> bool:
-    """Function transforms, forward-mode AD and tracing look at every operation: not for one opaque call."""
-    return (torch._C._functorch.peek_interpreter_stack() is not None or
-            torch.autograd.forward_ad._current_level >= 0 or torch.jit.is_tracing() or torch.compiler.is_compiling())
 
 
 def _parameters(cell, kind, device, I, H):
@@ -240,7 +235,8 @@ def forward(layer, x, h0):
     I, H = cell.input_size, cell.hidden_size
     device = x.device
     if (not cell._input_dense or I % 8 or H % 8 or not _plain_input(x, device) or not _plain_input(h0, device) or
-            x.shape[2] != I or h0.dim() != 2 or h0.shape[0] != x.shape[1] or h0.shape[1] != H or _transformed()):
+            x.shape[2] != I or h0.dim() != 2 or h0.shape[0] != x.shape[1] or h0.shape[1] != H or transformed() or
+            torch.compiler.is_compiling()):
         return None
     mods = cell._modules
     quant_x, quant_wi, quant_wh = mods["quant_x"], [mods["quant_W_i" + g] for g in _GATES], [mods["quant_W_h" + g] for g in _GATES]

@@ -23,7 +23,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._scan_common import require_cuda
+from ._scan_common import require_cuda, transformed
 from .scan_gated import DTYPES, call_on, rows_contiguous
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4, "tanh": 5}
@@ -153,8 +153,9 @@ def linear_act(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = 
     """``act(x[..., K] @ W[N, K]^T + bias[N]) + residual[..., N]`` in x's type; differentiable in all four tensors.
 
     ``activation``: none, relu, silu, gelu (the error-function form), sigmoid or tanh.  Rows may have any stride; a
-    residual has the result's shape (``expand`` a broadcast one)."""
+    residual has the result's shape (``expand`` a broadcast one).  Reverse mode only: forward-mode AD and ``torch.func``
+    transforms raise an error."""
     _check(x, W, bias, residual, activation)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, W, bias, residual)):
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, W, bias, residual))) or transformed():
         return LinearActFunction.apply(x, W, bias, residual, activation)
     return _forward(x, W, bias, residual, activation, False)[0]

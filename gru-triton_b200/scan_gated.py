@@ -24,7 +24,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._scan_common import require_cuda
+from ._scan_common import require_cuda, transformed
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _CANDIDATES = {"identity": 0, "tanh": 1}
@@ -191,9 +191,10 @@ def gated_scan(gi: torch.Tensor, h0: Optional[torch.Tensor] = None, *, lengths: 
     """``(out[T, B, H], h_T[B, H])`` of ``gi[T, B, 2H]`` from ``h0`` (zeros where None); differentiable in ``gi`` and ``h0``.
 
     ``gi`` may have any strides over time and batch (a transposed batch-first tensor is read where it lies, and ``out``
-    comes in the same order of axes).  ``lengths``: int32 or int64 ``[B]`` on the same device, read there."""
+    comes in the same order of axes).  ``lengths``: int32 or int64 ``[B]`` on the same device, read there.  Reverse mode only:
+    forward-mode AD and ``torch.func`` transforms raise an error."""
     _check_scan(gi, h0, lengths, candidate)
-    if torch.is_grad_enabled() and (gi.requires_grad or (h0 is not None and h0.requires_grad)):
+    if (torch.is_grad_enabled() and (gi.requires_grad or (h0 is not None and h0.requires_grad))) or transformed():
         return GatedScanFunction.apply(gi, h0, lengths, candidate)
     return _forward(gi, h0, lengths, candidate, False)[:2]
 
@@ -213,6 +214,8 @@ def gated_step(gi: torch.Tensor, h: torch.Tensor, *, candidate: str = "tanh",
     if out_state is not None:
         _check_state("out_state", out_state, B, H)
     _check_devices(gi, ("h", "out_state"), (h, out_state))
+    if transformed():
+        raise ValueError("gated_step is one opaque call: not for function transforms, forward-mode AD or tracing")
     if torch.is_grad_enabled() and (gi.requires_grad or h.requires_grad):
         raise ValueError("gated_step has no gradients: call it under torch.no_grad(), or gated_scan on gi[None]")
     gi, device = rows_contiguous(gi), gi.device

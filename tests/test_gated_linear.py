@@ -891,3 +891,62 @@ def test_library_refuses_bad_arguments():
     assert lib.b200gru_linear_act_backward(ctypes.byref(p), None) == 1                  # no dy
     p.dy, p.lddy, p.activation = 256, 8, 2
     assert lib.b200gru_linear_act_backward(ctypes.byref(p), None) == 1                  # no slope
+
+
+# ---- calls that look past autograd (no GPU) ------------------------------------------------------------
+
+@pytest.fixture
+def opaque(monkeypatch):
+    """The operators with their library calls replaced by memory that nobody wrote, on CPU tensors."""
+    from gru_triton_b200 import linear_act as linear, scan_gated as scan
+
+    def fake_scan(gi, h0, lengths, candidate, want_states):
+        T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
+        return gi.new_zeros((T, B, H)), gi.new_zeros((B, H)), gi.new_zeros(1)
+
+    def fake_linear(x, W, bias, residual, activation, want_slope):
+        return x.new_zeros((*x.shape[:-1], W.shape[0])), None
+
+    monkeypatch.setattr(scan, "_check_devices", lambda *a: None)
+    monkeypatch.setattr(scan, "_forward", fake_scan)
+    monkeypatch.setattr(linear, "_check", lambda *a: None)
+    monkeypatch.setattr(linear, "_forward", fake_linear)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(opaque, grad):
+    from torch.autograd import forward_ad as fwad
+    gi, W = torch.randn(3, 2, 8), torch.randn(5, 8)
+    for call in (lambda t: gated_scan(t), lambda t: linear_act(t, W), lambda t: linear_act(W, t[0]), lambda t: gated_step(t[0], torch.zeros(2, 4))):
+        with torch.set_grad_enabled(grad), fwad.dual_level():
+            with pytest.raises((RuntimeError, NotImplementedError, ValueError)):
+                call(fwad.make_dual(gi, torch.ones_like(gi)))
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.jvp(lambda t: call(t), (gi,), (torch.ones_like(gi),))
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.vmap(lambda t: call(t))(torch.stack([gi, gi]))
+
+
+def test_traces_hold_the_operators(opaque):
+    gi, W = torch.randn(3, 2, 8), torch.randn(5, 8)
+    for call, t in ((lambda t: gated_scan(t), gi), (lambda t: linear_act(t, W), gi)):
+        with torch.no_grad():
+            graph = torch.jit.trace(call, (t,), check_trace=False).graph
+        assert any(n.kind() == "prim::PythonOp" for n in graph.nodes()) and "empty" not in str(graph) and "zeros" not in str(graph)
+    with pytest.raises(ValueError, match="tracing"):
+        torch.jit.trace(lambda t: gated_step(t, torch.zeros(2, 4)), (gi[0],), check_trace=False)
+
+
+@pytest.mark.gpu
+def test_traced_calls_run_the_operators():
+    gi, h0, _, _ = problem(torch.float32, 40, 3, 32, seed=2)
+    W = torch.randn(24, 32, device="cuda")
+
+    def step(gi):
+        out, h_T = gated_scan(gi)
+        return linear_act(out, W, activation="silu"), h_T
+
+    with torch.no_grad():
+        traced = torch.jit.trace(step, (torch.zeros_like(gi),), check_trace=False)
+        for a, b in zip(traced(gi), step(gi)):
+            assert torch.equal(a, b)
