@@ -216,7 +216,7 @@ def gated_step(gi: torch.Tensor, h: torch.Tensor, *, candidate: str = "tanh",
     _check_devices(gi, ("h", "out_state"), (h, out_state))
     if transformed():
         raise ValueError("gated_step is one opaque call: not for function transforms, forward-mode AD or tracing")
-    if torch.is_grad_enabled() and (gi.requires_grad or h.requires_grad):
+    if torch.is_grad_enabled() and (gi.requires_grad or h.requires_grad or (out_state is not None and out_state.requires_grad)):
         raise ValueError("gated_step has no gradients: call it under torch.no_grad(), or gated_scan on gi[None]")
     gi, device = rows_contiguous(gi), gi.device
     if out_state is None:
@@ -237,6 +237,8 @@ def gated_step(gi: torch.Tensor, h: torch.Tensor, *, candidate: str = "tanh",
                  gi.stride(0), h.data_ptr(), h.stride(0), out.data_ptr(), new.data_ptr(), max(new.stride(0), H))
     if rc:
         _lib._raise(rc, "gated step")
+    if out_state is not None:
+        torch.autograd.graph.increment_version(new)      # autograd refuses what it saved of the old state, as after any in-place write
     return out, new
 
 

@@ -950,3 +950,29 @@ def test_traced_calls_run_the_operators():
         traced = torch.jit.trace(step, (torch.zeros_like(gi),), check_trace=False)
         for a, b in zip(traced(gi), step(gi)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("same", [True, False])
+def test_step_tells_autograd_that_it_wrote_a_state(opaque, monkeypatch, same):
+    from gru_triton_b200 import scan_gated as scan
+    monkeypatch.setattr(scan, "call_on", lambda *a: 0)
+    gi, w = torch.randn(2, 8), torch.ones(2, 4, requires_grad=True)
+    state = torch.zeros(2, 4)
+    loss = (w * state).sum()
+    table = torch.zeros(4, 4)
+    other = (w * table[:2]).sum()
+    gated_step(gi, state if same else torch.zeros(2, 4), out_state=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    gated_step(gi, state, out_state=table[2:])           # a view: its base counts
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        other.backward()
+    version = state._version
+    gated_step(gi, state)
+    assert state._version == version
+    with pytest.raises(ValueError, match="gradients"):
+        gated_step(gi, state, out_state=torch.zeros(2, 4, requires_grad=True))
+    with torch.no_grad():
+        gated_step(gi, state, out_state=w)
+    with torch.inference_mode():
+        gated_step(gi, state.clone(), out_state=torch.zeros(2, 4))
