@@ -521,9 +521,9 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     const int t0 = tile * STEPS + part * SEG;
     const int n = len - t0;                                   // steps left from here
     P2 h = both(0.f);
-    // keep: 1 - z, then z;  p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'.  Five values a step: a sixth, open * keep,
-    // would save a multiplication and cost 16 registers (501 x 19 x 607, fp32: 51 us against 48).
-    P2 keep[SEG], open[SEG], p[SEG], q[SEG], d[SEG];
+    // p: candidate, then (h_{t-1} - n) z (1 - z);  q: (1 - z) n'.  Five values a step: a sixth, z (1 - z), would save a
+    // multiplication and cost 16 registers (501 x 19 x 607, fp32: 51 us against 48).
+    P2 z[SEG], keep[SEG], p[SEG], q[SEG], d[SEG];
     P2 A = both(1.f), f = both(0.f), r = f;
     if (tile >= 0) {
       h = load_state<PAIRED<MODE>, LANES>(a.states + ((long long)tile * a.B + w.b) * a.H + w.unit, lane, w.left);
@@ -550,24 +550,26 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
           if (with_dout) d[k] = unpack(rd[k]);
         }
         const Gates g = gates<TANH, true>(x, c, K);
+        z[k] = g.z;
         keep[k] = g.keep;
-        open[k] = g.open;
         p[k] = g.n;
         q[k] = mul2(g.keep, g.slope);
       }
       if (n < SEG) {
 #pragma unroll
         for (int k = 0; k < SEG; ++k)
-          if (k >= n) keep[k] = p[k] = d[k] = both(0.f);
+          if (k >= n) {
+            z[k] = both(1.f);
+            keep[k] = p[k] = d[k] = both(0.f);
+          }
       }
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
-        const P2 z = sub2(K.one, keep[k]);
-        A = mul2(z, A);
-        f = fma2(z, f, mul2(keep[k], p[k]));
+        A = mul2(z[k], A);
+        f = fma2(z[k], f, mul2(keep[k], p[k]));
       }
 #pragma unroll
-      for (int k = SEG - 1; k >= 0; --k) r = mul2(sub2(K.one, keep[k]), add2(d[k], r));
+      for (int k = SEG - 1; k >= 0; --k) r = mul2(z[k], add2(d[k], r));
     }
     const int slot = round & 1;
     Map back = {A, r};                                        // gradients: from the later part to the earlier one
@@ -602,10 +604,9 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
     if (tile >= 0) {
 #pragma unroll
       for (int k = 0; k < SEG; ++k) {
-        const P2 z = sub2(K.one, keep[k]), n = p[k];
-        p[k] = mul2(sub2(h, n), mul2(open[k], keep[k]));
-        h = fma2(z, h, mul2(keep[k], n));
-        keep[k] = z;
+        const P2 n = p[k];
+        p[k] = mul2(sub2(h, n), mul2(z[k], keep[k]));
+        h = fma2(z[k], h, mul2(keep[k], n));
       }
     }
     P2 G = CLUSTERED ? join(s, peers, w, round, part, lane) : s.carry[slot][lane];
@@ -616,7 +617,7 @@ gated_bwd_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant_
 #pragma unroll
       for (int k = SEG - 1; k >= 0; --k) {
         const P2 g = add2(G, d[k]);
-        G = mul2(keep[k], g);
+        G = mul2(z[k], g);
         if (k < n) {
           store_units<PAIRED<MODE>, LANES>(reinterpret_cast<T*>(o), lane, w.left, mul2(g, p[k]));
           store_units<PAIRED<MODE>, LANES>(reinterpret_cast<T*>(o + a.half), lane, w.left, mul2(g, q[k]));
@@ -699,7 +700,7 @@ __global__ void __launch_bounds__(128) gated_short_bwd_kernel(const Args a) {
       if (dp != nullptr) d[k] = load_units<PAIRS, 32>(dp + (long long)k * a.dout_t, lane, left);
       const Gates g = gates<TANH, true>(x, c, K);
       z[k] = g.z;
-      p[k] = mul2(sub2(h, g.n), mul2(g.open, g.keep));
+      p[k] = mul2(sub2(h, g.n), mul2(g.z, g.keep));
       q[k] = mul2(g.keep, g.slope);
       h = fma2(g.z, h, mul2(g.keep, g.n));
     }

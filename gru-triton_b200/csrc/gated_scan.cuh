@@ -55,67 +55,68 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 // The constants of the packed instructions, which take registers alone.  Behind a volatile move they stay in theirs; the
 // compiler would otherwise build each pair anew at each use, seven moves beside the 24 instructions of an element.
 struct Constants {
-  P2 one, to_e, to_2c, cubic, fifth;
+  P2 one, cubic, fifth;
 };
 __device__ __forceinline__ P2 pinned(float v) {
   P2 p;
   asm volatile("mov.b64 %0, {%1, %1};" : "=l"(p.v) : "f"(v));
   return p;
 }
-__device__ __forceinline__ Constants constants() {
-  constexpr float LOG2E = 1.44269504f;
-  return {pinned(1.f), pinned(-LOG2E), pinned(-2.f * LOG2E), pinned(-1.f / 3.f), pinned(2.f / 15.f)};
-}
+__device__ __forceinline__ Constants constants() { return {pinned(1.f), pinned(-1.f / 3.f), pinned(2.f / 15.f)}; }
 
-// 2^(v * scale), at most 2^60.
-__device__ __forceinline__ P2 power2(P2 v, P2 scale) {
-  const float2 t = split(mul2(v, scale));
-  return pair(exp2_approx(min_nan(t.x, 60.f)), exp2_approx(min_nan(t.y, 60.f)));
+// 2^(|v| * scale), scale < 0: in [0, 1].
+__device__ __forceinline__ P2 falling2(P2 v, float scale) {
+  const float2 t = split(v);
+  return pair(exp2_approx(fabsf(t.x) * scale), exp2_approx(fabsf(t.y) * scale));
 }
 __device__ __forceinline__ P2 reciprocal2(P2 v) {
   const float2 f = split(v);
   return pair(rcp_approx(f.x), rcp_approx(f.y));
 }
 
-// Gates of two units.  z = 1 - keep, so that the two add to one to a rounding and a state that holds for hundreds of steps
-// does not drift; `open` is the same gate to full relative precision, where its size matters (its slope).
+// Gates of two units: z, keep = 1 - z, n and its slope.
 struct Gates {
-  P2 z, open, keep, n, slope;
+  P2 z, keep, n, slope;
 };
 
-// With e = exp(-x) and f = exp(-2c):  open = 1 / (1 + e), keep = e open, tanh c = (1 - f) / (1 + f), dn/dc = 4 f / (1 + f)^2.
-// Both quotients come from one reciprocal, of (1 + e)(1 + f): three special-function values instead of four, of which an SM
+// With e = exp(-|x|) and f = exp(-2|c|): the smaller of z and 1 - z is e / (1 + e), the larger one minus that.  So both have full
+// relative precision, a closed gate (z of 1e-10) as well as an open one, and the two add to one to a rounding, so that a state
+// which holds for hundreds of steps does not drift.  tanh |c| = (1 - f) / (1 + f), dn/dc = 4 f / (1 + f)^2.
+// Both quotients come from one reciprocal, of (1 + e)(1 + f) <= 4: three special-function values instead of four, of which an SM
 // has 16 a cycle.  APART: a NaN of c stays out of x's gate (in the forward both make the state NaN from there on; in the
 // backward the gate alone carries the gradient to earlier steps).  Below |c| = 1/8, where 1 - f cancels, the series
 // c - c^3/3 + 2 c^5/15 (next term 17/315 c^7: 2e-7 of c at most).
 template <bool TANH, bool APART>
 __device__ __forceinline__ Gates gates(P2 x, P2 c, const Constants& k) {
+  constexpr float LOG2E = 1.44269504f;
   Gates g;
-  const P2 e = power2(x, k.to_e);
+  const P2 e = falling2(x, -LOG2E);
   const P2 d = add2(k.one, e);
+  P2 s;
   if (TANH) {
-    const P2 f = power2(c, k.to_2c);
+    const P2 f = falling2(c, -2.f * LOG2E);
     P2 q = add2(k.one, f);
     if (APART) {
-      constexpr float MOST = 2305843009213693952.f;          // 2^61, above any 1 + f
-      const float2 s = split(q);
-      q = pair(fminf(s.x, MOST), fminf(s.y, MOST));
+      const float2 t = split(q);
+      q = pair(fminf(t.x, 2.f), fminf(t.y, 2.f));
     }
     const P2 r = reciprocal2(mul2(d, q));
-    g.open = mul2(r, q);
+    s = mul2(r, q);
     q = mul2(r, d);
     const P2 c2 = mul2(c, c);
     const float2 far = split(mul2(sub2(k.one, f), q)), near0 = split(fma2(mul2(fma2(c2, k.fifth, k.cubic), c2), c, c)), at = split(c);
-    g.n = pair(fabsf(at.x) < 0.125f ? near0.x : far.x, fabsf(at.y) < 0.125f ? near0.y : far.y);
+    g.n = pair(fabsf(at.x) < 0.125f ? near0.x : copysignf(far.x, at.x), fabsf(at.y) < 0.125f ? near0.y : copysignf(far.y, at.y));
     const P2 fq = mul2(mul2(f, q), q), twice = add2(fq, fq);
     g.slope = add2(twice, twice);
   } else {
-    g.open = reciprocal2(d);
+    s = reciprocal2(d);
     g.n = c;
     g.slope = k.one;
   }
-  g.keep = mul2(e, g.open);
-  g.z = sub2(k.one, g.keep);
+  const P2 small = mul2(e, s);
+  const float2 lo = split(small), hi = split(sub2(k.one, small)), at = split(x);
+  g.z = pair(at.x < 0.f ? lo.x : hi.x, at.y < 0.f ? lo.y : hi.y);
+  g.keep = pair(at.x < 0.f ? hi.x : lo.x, at.y < 0.f ? hi.y : lo.y);
   return g;
 }
 

@@ -210,6 +210,34 @@ def test_scan_small_candidates_keep_relative_precision():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("candidate", ["tanh", "identity"])
+@pytest.mark.parametrize("T,B,H", [(1, 2, 160), (6, 3, 33), (40, 2, 96), (100, 130, 160), (200, 3, 161), (1700, 1, 300), (100, 300, 72)])
+def test_scan_closed_gates_keep_relative_precision(dtype, candidate, T, B, H):
+    """One step with gates from e^-1 down to e^-80 among steps that hold: what is left of h0, and of its gradient, is exact to a
+    few units of itself.  e^-|x|: 2 u |x| of the exponent's two roundings, 4 u of the instruction; reciprocal and products 8 u."""
+    gi = torch.zeros(T, B, 2 * H, device="cuda")
+    gi[..., :H] = 60.0                                           # 1 - z = e^-60: lost beside one
+    gi[T // 2, :, :H] = -torch.linspace(1, 80, H, device="cuda")
+    gi = gi.to(dtype)
+    _, h0, _, dh = problem(torch.float32, 1, B, H, seed=T)
+    x = gi[T // 2, :, :H].double()
+    z = torch.sigmoid(x)
+    allowed = U * (12 + 2 * x.abs())
+    leaf, h = gi.requires_grad_(True), h0.requires_grad_(True)
+    out, h_T = gated_scan(leaf, h, candidate=candidate)
+    dgi, dh0 = torch.autograd.grad(h_T, (leaf, h), dh)
+    ref = z * h0.detach().double()
+    close(h_T.detach(), ref, allowed * ref.abs())
+    close(out[-1].detach(), ref, allowed * ref.abs() + rounding(ref, dtype))
+    close(dh0, z * dh.double(), allowed * (z * dh.double()).abs())
+    dx = dh.double() * ref * torch.sigmoid(-x)
+    close(dgi[T // 2, :, :H], dx, 2 * allowed * dx.abs() + rounding(dx, dtype))
+    _, new = gated_step(gi.detach()[T // 2], h0.detach(), candidate=candidate)
+    close(new, ref, allowed * ref.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("T", [3, 140])
 def test_scan_reads_any_layout(dtype, T):
     B, H = 3, 64
