@@ -13,24 +13,50 @@ namespace lin {
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_float(float v);
+template <typename T> __device__ __forceinline__ T from_float(float v) { return T::encode(v); }
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// The slope act'(pre) that the backward multiplies with is kept in fp32 for fp32.  For the 16-bit types it is a fixed-point number:
-// it lies in [-0.13, 1.13] for every activation, so 16 bits hold it to 2^-16, and zero and one exactly.  (As fp16 it was off by
-// up to 2^-12 at one, which doubled the error of an fp16 gradient.)  0xffff: NaN.
-struct Slope16 { unsigned short u; };
-__device__ __forceinline__ float to_float(Slope16 s) {
-  const float v = fmaf(__uint_as_float(0x4b000000u | s.u), 1.f / 32768.f, -256.5f);      // (2^23 + u) 2^-15 - 256.5 = u 2^-15 - 0.5
-  return s.u == 0xffffu ? __uint_as_float(0x7fffffffu) : v;
-}
-template <> __device__ __forceinline__ Slope16 from_float<Slope16>(float v) {            // the low bits of 2^23 + 2^14 + v 2^15
-  return Slope16{(unsigned short)(__float_as_uint(fmaf(v, 32768.f, 8404992.f)) & 0xffffu)};
-}
-template <typename T> struct SlopeOf { typedef Slope16 type; };
+// The slope act'(pre) that the backward multiplies with is kept in fp32 for fp32, in 16 bits for the 16-bit types.  It lies in
+// [-0.13, 1.13] for every activation, and a saturated unit's is tiny, so its numbers are even steps of 2^-15 down to
+// 2^(BITS - 15) and from there floating point with BITS bits behind the leading one, to 2^-LEAST, below which steps are even again.
+// Half a step is 2^-16 at most, and 2^-(BITS + 1) of the value: below the rounding of bf16 (BITS 8, down to 2^-55), one of
+// fp16 (BITS 9, down to 2^-30, where its gradients end).  Zero and one are exact.  (fp16 itself is off by up to 2^-12 at one, which doubled the
+// error of an fp16 gradient; steps of 2^-15 throughout lost units behind sigmoid(8) and tanh(5).)
+// Codes: 0 .. FIRST - 1 floating, from FIRST on even, 0xc000 added where negative; 0xffff: NaN.
+template <int BITS, int LEAST>
+struct Slope16 {
+  static constexpr int SHIFT = 23 - BITS, FIRST = (LEAST + BITS - 15) << BITS;
+  static constexpr uint32_t BASE = (uint32_t)(127 - LEAST) << 23;                        // 2^-LEAST
+  static constexpr float EVEN = 1.f / (float)(1 << (15 - BITS));                         // the smallest of the even steps
+  static_assert(FIRST - (1 << BITS) + 36995 < 0xc000 && FIRST - (1 << BITS) + 4227 < 0x3fff, "slopes in [-0.129, 1.129]");
+  unsigned short u;
+
+  static __device__ __forceinline__ Slope16 encode(float v) {
+    const float t = fabsf(v);
+    // the low bits of 2^23 + FIRST - 2^BITS + t 2^15
+    const uint32_t even = __float_as_uint(fmaf(t, 32768.f, 8388608.f + (float)(FIRST - (1 << BITS))));
+    const uint32_t floating = (__float_as_uint(t + __uint_as_float(BASE)) - BASE + (1u << (SHIFT - 1))) >> SHIFT;
+    uint32_t c = t >= EVEN ? even : floating;
+    c |= (uint32_t)(__float_as_int(v) >> 31) & 0xc000u;
+    return Slope16{(unsigned short)(v == v ? c & 0xffffu : 0xffffu)};
+  }
+  __device__ __forceinline__ float value() const {
+    const bool below = u >= 0xc000u;
+    const uint32_t c = below ? u - 0xc000u : u;
+    const float even = fmaf(__uint_as_float(0x4b000000u | c), 1.f / 32768.f, (float)(-256.0 - (FIRST - (1 << BITS)) / 32768.0));
+    const float floating = __uint_as_float((c << SHIFT) + BASE) - __uint_as_float(BASE);
+    const float t = c >= (uint32_t)FIRST ? even : floating;
+    return u == 0xffffu ? __uint_as_float(0x7fffffffu) : (below ? -t : t);
+  }
+};
+template <int BITS, int LEAST>
+__device__ __forceinline__ float to_float(Slope16<BITS, LEAST> s) { return s.value(); }
+template <typename T> struct SlopeOf;
 template <> struct SlopeOf<float> { typedef float type; };
+template <> struct SlopeOf<__nv_bfloat16> { typedef Slope16<8, 55> type; };
+template <> struct SlopeOf<__half> { typedef Slope16<9, 30> type; };
 
 // Two values behind the activation, and its slopes there.
 struct Activated2 {

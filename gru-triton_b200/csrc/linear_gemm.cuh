@@ -74,7 +74,7 @@ template <typename T> struct Vec;
 template <> struct Vec<float> { static constexpr int V = 4; };
 template <> struct Vec<__nv_bfloat16> { static constexpr int V = 8; };
 template <> struct Vec<__half> { static constexpr int V = 8; };
-template <> struct Vec<Slope16> { static constexpr int V = 8; };
+template <int B, int L> struct Vec<Slope16<B, L>> { static constexpr int V = 8; };
 
 template <typename T>
 __device__ __forceinline__ void unpack16(const uint4& w, float (&v)[Vec<T>::V]) {
@@ -692,7 +692,7 @@ template <typename T> struct MapType;
 template <> struct MapType<float> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_FLOAT32; };
 template <> struct MapType<__nv_bfloat16> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; };
 template <> struct MapType<__half> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_FLOAT16; };
-template <> struct MapType<Slope16> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_UINT16; };
+template <int B, int L> struct MapType<Slope16<B, L>> { static constexpr CUtensorMapDataType value = CU_TENSOR_MAP_DATA_TYPE_UINT16; };
 
 template <int CTAS, int BN, int PL, typename Out>
 int launch_tile(const Gemm& g, cudaStream_t st) {

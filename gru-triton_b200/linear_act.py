@@ -8,8 +8,8 @@ quantised weights: float32 alone, no activation or residual.
 
 Element types float32, bfloat16 and float16, one for all tensors of a call; sums are float32.  float32 operands run as
 two row-scaled fp16 planes in three tensor-core products (22 significant bits, as ``tc.linear``'s).  What the backward
-needs of the activation is its slope, kept by the forward in float32 or, for the 16-bit types, in steps of 2^-15.  The
-same call repeats its bits.  A float32 row of x, or of the gradient, that holds an infinity gives NaN in its row (its
+needs of the activation is its slope, kept by the forward in float32 or, for the 16-bit types, in 16 bits: to 2^-16, and to 2^-9
+of itself (float16: 2^-10) where it is small, so that saturated units keep their gradients.  The same call repeats its bits.  A float32 row of x, or of the gradient, that holds an infinity gives NaN in its row (its
 two planes cannot hold one).  CUDA tensors only; there is no fallback.  The reference's counterpart is ``F.linear``
 (src/gru_qat/gru_cell.py:410-435), without activation and residual.
 """

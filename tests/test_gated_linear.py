@@ -613,6 +613,39 @@ def test_linear_gradient_of_a_nan_row_is_nan_and_stays_there(dtype, activation, 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid", "tanh"])
+@pytest.mark.parametrize("M,K", [(2, 64), (7, 64), (161, 64), (40, 2048), (20000, 64)])
+def test_linear_gradient_of_saturated_units_keeps_relative_precision(dtype, activation, M, K):
+    """x -> x (W the identity, zeros beside it): the gradient of x is dy act'(x), down to slopes of e^-15 (fp16) and e^-35.
+
+    Off by: the rounding of d; the kept slope, 2^-10 (fp16) or 2^-9 (bf16) of itself, twice that at its lowest; 2 u |x| (tanh 4 u |x|) of
+    an exponential's argument and 16 u of the rest; gelu 2^-11 (Phi's formula against v phi(v) in the tail); where silu's and gelu's
+    slopes cross zero, 16 u absolute; fp32 gradients, a product of planes as above."""
+    N = 64
+    far = {"gelu": 4.5 if dtype == torch.float16 else 7.0, "tanh": 0.5 * (18 if dtype == torch.float16 else 37)}
+    far = far.get(activation, 18.0 if dtype == torch.float16 else 37.0)
+    x = torch.zeros(M, K, device="cuda")
+    x[:, :N] = torch.linspace(-far, far, M, device="cuda")[:, None]
+    x = x.to(dtype)
+    W = torch.eye(N, K, device="cuda").to(dtype)
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    dy = ((torch.rand(M, N, device="cuda", generator=gen) + 0.5) * (2.0 ** 8 if dtype == torch.float16 else 1.0)).to(dtype)
+    leaf = x.requires_grad_(True)
+    dx, = torch.autograd.grad(linear_act(leaf, W, activation=activation), leaf, dy)
+    pre = x.detach()[:, :N].double()
+    s, t = torch.sigmoid(pre), torch.sigmoid(-pre)               # written out: autograd's 1 - y loses the tails in 64 bits too
+    phi = torch.exp(-0.5 * pre * pre) / math.sqrt(2 * math.pi)
+    d = dy.double() * {"sigmoid": s * t, "tanh": torch.cosh(pre) ** -2, "silu": s * (1 + pre * t),
+                       "gelu": 0.5 * torch.erfc(-pre / math.sqrt(2.0)) + pre * phi}[activation]
+    kept = {torch.float32: U * (80 + N / 64), torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -9}[dtype]
+    own = U * (16 + 4 * pre.abs()) + (2.0 ** -11 if activation == "gelu" else 0.0)
+    zero = 16 * U * dy.double() * (pre.abs() < 3) * (activation in ("silu", "gelu"))
+    close(dx[:, :N], d, (kept + own) * d.abs() + zero + rounding(d, dtype))
+    assert not dx[:, N:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("M,K,N", [(4, 300, 50), (48, 512, 640), (520, 512, 640), (9000, 128, 264)])
 def test_linear_repeats_its_bits(dtype, M, K, N):
     x, W, bias, residual, dy = linear_problem(dtype, M, K, N)
