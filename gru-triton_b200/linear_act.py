@@ -9,9 +9,14 @@ quantised weights: float32 alone, no activation or residual.
 Element types float32, bfloat16 and float16, one for all tensors of a call; sums are float32.  float32 operands run as
 two row-scaled fp16 planes in three tensor-core products (22 significant bits, as ``tc.linear``'s).  What the backward
 needs of the activation is its slope, kept by the forward in float32 or, for the 16-bit types, in 16 bits: to 2^-16, and to 2^-9
-of itself (float16: 2^-10) where it is small, so that saturated units keep their gradients.  The same call repeats its bits.  A float32 row of x, or of the gradient, that holds an infinity gives NaN in its row (its
-two planes cannot hold one).  CUDA tensors only; there is no fallback.  The reference's counterpart is ``F.linear``
-(src/gru_qat/gru_cell.py:410-435), without activation and residual.
+of itself (float16: 2^-10) where it is small, so that saturated units keep their gradients.  The same call repeats its bits.
+
+The planes of a float32 row hold its elements down to 2^-17 of its largest in 22 bits, smaller ones to 2^-39 of the largest, and no
+infinity: where the tensor cores run (above a few rows) a row of x that holds one gives NaN in its row of the result, a row of W
+in its column, a row of the gradient in its row of x's gradient.  The 16-bit types keep infinities.
+
+CUDA tensors only; there is no fallback.  The reference's counterpart is ``F.linear`` (src/gru_qat/gru_cell.py:410-435), without
+activation and residual.
 """
 
 from __future__ import annotations

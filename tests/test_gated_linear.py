@@ -600,6 +600,25 @@ def test_linear_no_rows_some_gradients_and_special_values(M):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M", [2, 200])
+def test_linear_infinity_in_a_weight_stays_in_its_column(dtype, M):
+    x, W, bias, _, dy = linear_problem(dtype, M, 64, 48, seed=8)
+    bad = W.clone()
+    bad[5, 3] = float("inf")
+    y, ok = linear_act(x, bad, bias), linear_act(x, W, bias)
+    rest = [n for n in range(48) if n != 5]
+    assert torch.equal(y[:, rest], ok[:, rest])
+    if dtype == torch.float32 and M > 8:
+        assert bool(y[:, 5].isnan().all())                       # two planes hold no infinity
+    else:
+        assert torch.equal(y[:, 5], torch.where(x[:, 3] > 0, math.inf, -math.inf).to(dtype))
+    leaf = x.requires_grad_(True)
+    dx, = torch.autograd.grad(linear_act(leaf, bad, bias), leaf, dy)
+    assert not bool(torch.isfinite(dx[:, 3]).any()) and bool(torch.isfinite(dx[:, [k for k in range(64) if k != 3]]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid", "tanh"])
 @pytest.mark.parametrize("M", [5, 200])
 def test_linear_gradient_of_a_nan_row_is_nan_and_stays_there(dtype, activation, M):
