@@ -170,7 +170,8 @@ __device__ __forceinline__ GateGrad gru_gate_grads(float dh, float r, float z, f
 // ---- small host utilities --------------------------------------------------
 
 __host__ __device__ inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
-__host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
+// a >= 0; no sum that could pass 2^31
+__host__ __device__ inline int cdiv(int a, int b) { return a / b + (a % b != 0); }
 
 // Health flag of the diagonal kernels' bounded waits (diag_scan.cu); -1 on CUDA error.
 int diag_read_status(int reset);

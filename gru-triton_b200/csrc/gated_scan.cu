@@ -930,12 +930,15 @@ using namespace b200gru;
 
 namespace {
 
+// 2 H, and a tile's units behind it, are 32-bit coordinates.
+constexpr int MAX_UNITS = 0x40000000 - 64;
+
 // Sizes and pointers that both directions need; every stride is non-negative.
 int check_scan(const b200gru_gated_args* p) {
   if (p == nullptr || p->T <= 0 || p->B <= 0 || p->H <= 0 || p->gi == nullptr) return B200GRU_INVALID_ARGUMENT;
   if (p->dtype < B200GRU_F32 || p->dtype > B200GRU_F16) return B200GRU_INVALID_ARGUMENT;
   if (p->lengths != nullptr && p->length_bytes != 4 && p->length_bytes != 8) return B200GRU_INVALID_ARGUMENT;
-  if ((long long)p->B * p->H > 0x7fffffffll || p->T > 0x40000000) return B200GRU_UNSUPPORTED;
+  if ((long long)p->B * p->H > 0x7fffffffll || p->T > 0x40000000 || p->H > MAX_UNITS) return B200GRU_UNSUPPORTED;
   if (p->gi_t < 0 || p->gi_b < 0 || p->h0_b < 0) return B200GRU_INVALID_ARGUMENT;
   return B200GRU_OK;
 }
@@ -983,7 +986,7 @@ int b200gru_gated_step(int dtype, int candidate_tanh, int B, int H, const void* 
   if (dtype < B200GRU_F32 || dtype > B200GRU_F16 || B <= 0 || H <= 0) return B200GRU_INVALID_ARGUMENT;
   if (gi == nullptr || h == nullptr || out == nullptr || h_new == nullptr) return B200GRU_INVALID_ARGUMENT;
   if (gi_b < 0 || h_b < 0 || hn_b < H) return B200GRU_INVALID_ARGUMENT;
-  if ((long long)B * H > 0x7fffffffll) return B200GRU_UNSUPPORTED;
+  if ((long long)B * H > 0x7fffffffll || H > MAX_UNITS) return B200GRU_UNSUPPORTED;
   gated::StepArgs a;
   a.B = B; a.H = H; a.tanh = candidate_tanh != 0;
   a.gi = gi; a.gi_b = gi_b; a.h = h; a.h_b = h_b; a.out = out; a.h_new = h_new; a.hn_b = hn_b;

@@ -697,8 +697,9 @@ int run_as(const b200gru_linear_args& a, bool backward, bool dry, size_t* bytes,
   return run<__half>(a, backward, dry, bytes, st);
 }
 
+// M: a tile of 256 rows that begins inside the matrix ends below 2^31.
 bool bad(const b200gru_linear_args* p) {
-  return p == nullptr || p->M <= 0 || p->N <= 0 || p->K <= 0 || p->M > 0x7ffffff0 || p->N > 0x3ffffff0 || p->K > 0x3ffffff0 ||
+  return p == nullptr || p->M <= 0 || p->N <= 0 || p->K <= 0 || p->M > 0x7ffffe00 || p->N > 0x3ffffff0 || p->K > 0x3ffffff0 ||
          p->dtype < B200GRU_F32 || p->dtype > B200GRU_F16 || p->activation < B200GRU_ACT_NONE ||
          p->activation > B200GRU_ACT_TANH || p->x == nullptr || p->W == nullptr || p->ldx < 0 || p->ldw < 0 ||
          (p->slope != nullptr && p->lds < p->N);

@@ -49,8 +49,8 @@ def _check(x, W, bias, residual, activation):
     N, K = w
     if N == 0 or K == 0:
         raise ValueError(f"N and K must be > 0; got N={N}, K={K}")
-    if x.numel() // K > 2 ** 31 - 16 or N > 2 ** 30 - 16 or K > 2 ** 30 - 16:
-        raise ValueError(f"at most 2^31 - 16 rows and 2^30 - 16 columns; got x {tuple(lead)}, W {tuple(w)}")
+    if x.numel() // K > 2 ** 31 - 512 or N > 2 ** 30 - 16 or K > 2 ** 30 - 16:
+        raise ValueError(f"at most 2^31 - 512 rows and 2^30 - 16 columns; got x {tuple(lead)}, W {tuple(w)}")
     if bias is not None and bias.shape != (N,):
         raise ValueError(f"bias shape must be (N,)=({N},); got {tuple(bias.shape)}")
     if residual is not None and residual.shape != (*lead[:-1], N):

@@ -66,8 +66,8 @@ def _check_state(name, h, B, H):
 
 
 def _check_size(T, B, H):
-    if T > 2 ** 30 or B * H > 2 ** 31 - 1:
-        raise ValueError(f"at most 2^30 steps and 2^31 - 1 states; got T={T}, B={B}, H={H}")
+    if T > 2 ** 30 or H > 2 ** 30 - 64 or B * H > 2 ** 31 - 1:
+        raise ValueError(f"at most 2^30 steps, 2^30 - 64 units and 2^31 - 1 states; got T={T}, B={B}, H={H}")
 
 
 def _check_devices(gi, names, others):

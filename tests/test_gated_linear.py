@@ -1056,3 +1056,37 @@ def test_step_tells_autograd_that_it_wrote_a_state(opaque, monkeypatch, same):
         gated_step(gi, state, out_state=w)
     with torch.inference_mode():
         gated_step(gi, state.clone(), out_state=torch.zeros(2, 4))
+
+
+# ---- the largest sizes (no GPU) -------------------------------------------------------------------------
+
+def test_sizes_that_tiles_would_carry_past_32_bits_are_refused():
+    row, w = torch.zeros(1, 16), torch.zeros(8, 16)
+    with pytest.raises(ValueError, match="rows"):
+        linear_act(row.expand(2 ** 31 - 500, 16), w)
+    with pytest.raises(ValueError, match="CUDA"):                # the largest that is taken, stopped by its device
+        linear_act(row.expand(2 ** 31 - 512, 16), w)
+    one = torch.zeros(1, 1, 1)
+    with pytest.raises(ValueError, match="units"):
+        gated_scan(one.expand(1, 1, 2 ** 31))
+    with pytest.raises(ValueError, match="CUDA"):
+        gated_scan(one.expand(1, 1, 2 ** 31 - 128))
+    with pytest.raises(ValueError, match="units"):
+        gated_step(one[0].expand(1, 2 ** 31), one[0].expand(1, 2 ** 30))
+
+
+def test_library_refuses_sizes_past_32_bits():
+    lib = _lib.load()
+    p, none = _lib.CLinearArgs(), ctypes.c_size_t(-1).value
+    p.K, p.N, p.dtype, p.x, p.W, p.ldx, p.ldw = 8, 8, 1, 4096, 4096, 8, 8
+    for M, taken in ((2 ** 31 - 1, False), (2 ** 31 - 16, False), (2 ** 31 - 511, False), (2 ** 31 - 512, True)):
+        p.M = M
+        need = lib.b200gru_linear_act_workspace_bytes(ctypes.byref(p), 0)
+        assert need == (0 if taken else none)
+    a = _lib.CGatedArgs()
+    a.T, a.B, a.H = 1, 1, 2 ** 30 - 63
+    a.gi = a.out = a.h_T = a.states = a.dgi = 4096
+    a.gi_t = a.gi_b = a.out_t = a.out_b = a.dgi_t = a.dgi_b = 2 ** 31
+    unsupported = lib.b200gru_gated_scan_forward(ctypes.byref(a), None)
+    assert unsupported == lib.b200gru_gated_scan_backward(ctypes.byref(a), None) == 2
+    assert lib.b200gru_gated_step(0, 1, 1, 2 ** 30 - 63, 4096, 2 ** 31, 4096, 2 ** 31, 4096, 4096, 2 ** 31, None) == 2
