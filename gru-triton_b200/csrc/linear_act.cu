@@ -529,9 +529,10 @@ struct Call {
     }
   }
 
-  void copy_rows(const T* src, long long ld, T* dst, long long dld, int rows, int cols) {
+  template <typename U>
+  void copy_rows(const U* src, long long ld, U* dst, long long dld, int rows, int cols) {
     if (dry || rc != B200GRU_OK) return;
-    launch_pdl(copy_rows_kernel<T>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, src, ld, dst, dld, rows, cols);
+    launch_pdl(copy_rows_kernel<U>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, src, ld, dst, dld, rows, cols);
     note("copy_rows_kernel");
   }
 
@@ -552,8 +553,14 @@ struct Call {
       const long long ldc = g.ldc;
       const bool apart = !on16(g.C, g.ldc, sizeof(T));
       if (apart) { g.C = ws.template take<T>(g.M * ld); g.ldc = ld; }
+      typedef typename SlopeOf<T>::type S;
+      S* slope = static_cast<S*>(g.slope);
+      const long long lds = g.lds;
+      const bool slope_apart = !on16(g.slope, g.lds, sizeof(S)) && g.activation != B200GRU_ACT_NONE;
+      if (slope_apart) { g.slope = ws.template take<S>(g.M * ld); g.lds = ld; }
       if (!dry && rc == B200GRU_OK) rc = launch_gemm<T>(g, plan, st);
       if (apart) copy_rows(static_cast<const T*>(g.C), ld, out, ldc, g.M, g.N);
+      if (slope_apart) copy_rows(static_cast<const S*>(g.slope), ld, slope, lds, g.M, g.N);
       return;
     }
     FinishArgs f;

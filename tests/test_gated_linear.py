@@ -563,6 +563,44 @@ def test_linear_writes_inside_its_results(dtype, M, K, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M, K, N", [(2, 64, 130), (40, 2048, 130), (300, 128, 130), (300, 128, 132), (2100, 320, 516)])
+def test_linear_slopes_of_any_row_pitch(dtype, M, K, N):
+    """Slopes in rows without padding and off 16-byte boundaries, as a C caller may hold them: the same slopes and gradients."""
+    x, W, bias, residual, dy = linear_problem(dtype, M, K, N, seed=7)
+    lib, stream = _lib.load(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    kept = torch.float32 if dtype == torch.float32 else torch.int16
+
+    def call(fn, backward, a):
+        n = lib.b200gru_linear_act_workspace_bytes(ctypes.byref(a), backward)
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
+        assert fn(ctypes.byref(a), stream) == 0
+
+    def run(lds, offset):
+        slopes = torch.full((offset + M * lds + 8,), 77, dtype=kept, device="cuda")
+        y, dx, dW, db = (torch.empty_like(t) for t in (residual, x, W, bias))
+        a = _lib.CLinearArgs()
+        a.M, a.K, a.N, a.dtype, a.activation = M, K, N, DTYPES.index(dtype), ACTIVATIONS["silu"]
+        a.x, a.ldx, a.W, a.ldw, a.bias, a.residual, a.ldr = x.data_ptr(), K, W.data_ptr(), K, bias.data_ptr(), residual.data_ptr(), N
+        a.y, a.ldy, a.slope, a.lds = y.data_ptr(), N, slopes.data_ptr() + offset * slopes.element_size(), lds
+        call(lib.b200gru_linear_act_forward, 0, a)
+        a.dy, a.lddy, a.dx, a.dW, a.db = dy.data_ptr(), N, dx.data_ptr(), dW.data_ptr(), db.data_ptr()
+        call(lib.b200gru_linear_act_backward, 1, a)
+        rows = slopes[offset:offset + M * lds].view(M, lds)
+        outside = [slopes[:offset], slopes[offset + M * lds:]]
+        if lds > N and offset:
+            outside.append(rows[:, N:].reshape(-1))              # the padding of rows that are copied
+        assert all(bool((t == 77).all()) for t in outside)
+        return [rows[:, :N].contiguous(), y, dx, dW, db]
+
+    want = run((N + 7) // 8 * 8, 0)
+    for lds, offset in ((N, 0), (N, 1), (N + 3, 5)):
+        for a, b in zip(run(lds, offset), want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [5, 200])
 def test_linear_no_rows_some_gradients_and_special_values(M):
     x, W, bias, residual, dy = linear_problem(torch.float32, M, 64, 48)
