@@ -191,7 +191,8 @@ int read_status(int reset);          // products with bias, activation and resid
 // Test hook (b200gru_test_select_kernels): slot 0 != 0 -> butterfly launches use the register /
 // global-twiddle kernels on every shape; slot 1 != 0 -> the diagonal forward uses the register-ring
 // kernel on every shape.  Slot 2 (b200gru_test_select_dense_scan): 1 -> FP32 cluster kernels, 2 -> tensor-core
-// cluster scan wherever it applies.  Slot 3 (b200gru_test_select_gemm): 1 -> single CTAs, 2 -> CTA pairs.  Defaults 0: the dispatch is by shape only.
+// cluster scan wherever it applies.  Slot 3 (b200gru_test_select_gemm): 1 -> single CTAs, 2 -> CTA pairs.
+// Slot 4 (b200gru_test_limit_gated_clusters): the largest cluster of a gated scan.  Defaults 0: the dispatch is by shape only.
 int test_kernel_choice(int slot);
 
 // Launch bookkeeping shared by all translation units (defined in api.cu).

@@ -14,6 +14,9 @@
 // registers between the fold and the results; inputs arrive by TMA a few tiles ahead.
 
 #include <cstring>
+#include <map>
+#include <mutex>
+#include <tuple>
 #include <type_traits>
 
 #include "gated_scan.cuh"
@@ -767,7 +770,7 @@ bool narrow(int T, int B, int H) { return T > Forward::STEPS && (long long)B * c
 // what a tile does, so more pay only where SMs have nothing else (64 narrow CTAs over 2000 steps: 27 / 41 us alone, 18 / 25 in
 // clusters of 4, 23 / 29 of 8).  Clusters above 8 find room only while there are few of them: 16 columns over 20000 steps 54 / 82 us
 // with 8, 41 / 63 with 12, 53 / 74 with 16; 8 columns 41 / 61, 39 / 59, 33 / 47; 32 columns over 32768 steps 84 / 133 with 8,
-// 115 / 176 with 12.
+// 115 / 176 with 12.  A device that cannot place such a cluster gets 8 (states lie by tiles, so the two directions may differ).
 int ranks_for(const Args& a) {
   if (!narrow(a.T, a.B, a.H)) return 1;
   const long long base = (long long)a.B * cdiv(a.H, Narrow::UNITS);
@@ -778,10 +781,45 @@ int ranks_for(const Args& a) {
   return ranks < tiles ? ranks : tiles;
 }
 
+// The largest cluster that a test lets the device place; 0: what it can.
+bool too_large_for_test(int ranks) {
+  const int most = test_kernel_choice(4);
+  return most > 0 && ranks > most;
+}
+
+// Whether the device can place a cluster of `ranks` CTAs; above eight that depends on its SMs and on what a CTA holds.  Asked once
+// for each kernel and size.
+bool placeable(const void* fn, int threads, int ranks, size_t smem) {
+  static std::mutex mu;
+  static std::map<std::tuple<int, const void*, int, size_t>, bool> cache;
+  if (too_large_for_test(ranks)) return false;
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  std::lock_guard<std::mutex> lk(mu);
+  const auto key = std::make_tuple(dev, fn, ranks, smem);
+  const auto it = cache.find(key);
+  if (it != cache.end()) return it->second;
+  int n = 0;
+  if (allow_dynamic_smem(fn, smem) == B200GRU_OK &&
+      cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ranks); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+  } else {
+    cudaGetLastError();
+  }
+  cache[key] = n > 0;
+  return n > 0;
+}
+
 template <typename... KArgs, typename... CArgs>
 int launch_tiles(void (*kernel)(KArgs...), long long blocks, int threads, int ranks, size_t smem, cudaStream_t st, CArgs... args) {
   const void* fn = reinterpret_cast<const void*>(kernel);
-  if (allow_dynamic_smem(fn, smem) != B200GRU_OK) return B200GRU_UNSUPPORTED;
+  if (allow_dynamic_smem(fn, smem) != B200GRU_OK || too_large_for_test(ranks)) return B200GRU_UNSUPPORTED;
   if (ranks > 8 && cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
     return check_launch("cudaFuncSetAttribute(gated scan)");
   if (blocks > 0x7fffffffll) return B200GRU_UNSUPPORTED;
@@ -805,12 +843,14 @@ int stages_for(size_t stage, size_t fixed, int ctas) {
 
 template <typename T, typename Cut, int MODE, bool TANH>
 int forward_cut(const Args& a, const CUtensorMap& map, int ranks, int stages, cudaStream_t st) {
-  const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS) * ranks;
-  const size_t smem = (size_t)stages * 2 * Cut::STEPS * Cut::UNITS * sizeof(T) + peer_bytes<Cut::LANES>(ranks);
+  const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS);
+  const size_t ring = (size_t)stages * 2 * Cut::STEPS * Cut::UNITS * sizeof(T);
   if constexpr (std::is_same<Cut, Narrow>::value) {
-    if (ranks > 1) return launch_tiles(gated_fwd_kernel<T, Cut, MODE, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, a, ranks, stages);
+    auto kernel = gated_fwd_kernel<T, Cut, MODE, TANH, true>;
+    if (ranks > 8 && !placeable(reinterpret_cast<const void*>(kernel), Cut::THREADS, ranks, ring + peer_bytes<Cut::LANES>(ranks))) ranks = 8;
+    if (ranks > 1) return launch_tiles(kernel, blocks * ranks, Cut::THREADS, ranks, ring + peer_bytes<Cut::LANES>(ranks), st, map, a, ranks, stages);
   }
-  return launch_tiles(gated_fwd_kernel<T, Cut, MODE, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, a, 1, stages);
+  return launch_tiles(gated_fwd_kernel<T, Cut, MODE, TANH, false>, blocks, Cut::THREADS, 1, ring, st, map, a, 1, stages);
 }
 template <typename T, typename Cut, bool TANH>
 int forward_tiles(const Args& a, cudaStream_t st) {
@@ -830,12 +870,14 @@ int forward_tiles(const Args& a, cudaStream_t st) {
 
 template <typename T, typename Cut, int MODE, bool TANH>
 int backward_cut(const Args& a, const CUtensorMap& map, const CUtensorMap& dmap, int ranks, int stages, cudaStream_t st) {
-  const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS) * ranks;
-  const size_t smem = (size_t)stages * 3 * Cut::STEPS * Cut::UNITS * sizeof(T) + peer_bytes<Cut::LANES>(ranks);
+  const long long blocks = (long long)a.B * cdiv(a.H, Cut::UNITS);
+  const size_t ring = (size_t)stages * 3 * Cut::STEPS * Cut::UNITS * sizeof(T);
   if constexpr (std::is_same<Cut, Narrow>::value) {
-    if (ranks > 1) return launch_tiles(gated_bwd_kernel<T, Cut, MODE, TANH, true>, blocks, Cut::THREADS, ranks, smem, st, map, dmap, a, ranks, stages);
+    auto kernel = gated_bwd_kernel<T, Cut, MODE, TANH, true>;
+    if (ranks > 8 && !placeable(reinterpret_cast<const void*>(kernel), Cut::THREADS, ranks, ring + peer_bytes<Cut::LANES>(ranks))) ranks = 8;
+    if (ranks > 1) return launch_tiles(kernel, blocks * ranks, Cut::THREADS, ranks, ring + peer_bytes<Cut::LANES>(ranks), st, map, dmap, a, ranks, stages);
   }
-  return launch_tiles(gated_bwd_kernel<T, Cut, MODE, TANH, false>, blocks, Cut::THREADS, 1, smem, st, map, dmap, a, 1, stages);
+  return launch_tiles(gated_bwd_kernel<T, Cut, MODE, TANH, false>, blocks, Cut::THREADS, 1, ring, st, map, dmap, a, 1, stages);
 }
 template <typename T, typename Cut, bool TANH>
 int backward_tiles(const Args& a, cudaStream_t st) {

@@ -238,6 +238,27 @@ def test_scan_closed_gates_keep_relative_precision(dtype, candidate, T, B, H):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T,H,odd", [(2500, 256, 0), (2500, 512, 0), (2100, 255, 1)])
+def test_scan_where_large_clusters_cannot_be_placed(dtype, T, H, odd):
+    """A device without room for clusters of 12 or 16: the same sequences in clusters of eight, either direction by itself."""
+    gi, h0, dout, dh = problem(dtype, T, 1, H, seed=T)
+    lib = _lib.load()
+    try:
+        lib.b200gru_test_limit_gated_clusters(8)
+        check_scan(gi, h0, None, "tanh", dout, dh)
+        leaf = gi.detach().requires_grad_(True)
+        out, h_T = gated_scan(leaf, h0)
+        small, = torch.autograd.grad((out, h_T), leaf, (dout, dh), retain_graph=True)
+        lib.b200gru_test_limit_gated_clusters(0)
+        large, = torch.autograd.grad((out, h_T), leaf, (dout, dh))
+    finally:
+        lib.b200gru_test_limit_gated_clusters(0)
+    tol = 64 * U * float(dout.abs().max()) * 40                  # sums over memories of some ten steps, joined in another order
+    close(small, large.double(), tol + 2 * rounding(large.double(), dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("T", [3, 140])
 def test_scan_reads_any_layout(dtype, T):
     B, H = 3, 64
