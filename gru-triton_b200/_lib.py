@@ -120,6 +120,7 @@ SIGNATURES = {
     "b200gru_test_select_dense_scan": (None, [_I]),
     "b200gru_test_select_gemm": (None, [_I]),
     "b200gru_test_limit_gated_clusters": (None, [_I]),
+    "b200gru_test_linear_plan": (_I, [_I, _I, _I, _I, _I, _P]),
     "b200gru_test_wait_timeout": (_I, [_P]),
     "b200gru_launch_count": (ctypes.c_ulonglong, []),
     "b200gru_strerror": (ctypes.c_char_p, [_I]),

@@ -763,6 +763,15 @@ using namespace b200gru;
 
 extern "C" {
 
+int b200gru_test_linear_plan(int M, int N, int K, int planes, int activation, int* plan) {
+  if (M <= 0 || N <= 0 || K <= 0 || (planes != 1 && planes != 2) || plan == nullptr) return B200GRU_INVALID_ARGUMENT;
+  const lin::Plan p = lin::plan_gemm(M, N, K, planes);
+  const int per = cdiv(cdiv(K, 64), p.splits);
+  plan[0] = p.ctas; plan[1] = p.bn; plan[2] = p.splits; plan[3] = per;
+  plan[4] = lin::chunk_kblocks(planes, p.splits == 1 && activation != B200GRU_ACT_NONE, per);
+  return B200GRU_OK;
+}
+
 size_t b200gru_linear_act_workspace_bytes(const b200gru_linear_args* p, int backward) try {
   if (lin::bad(p)) return (size_t)-1;
   size_t n = 0;

@@ -58,6 +58,10 @@ struct Plan {
   int ctas, bn, splits;
 };
 Plan plan_gemm(int M, int N, int K, int planes);
+// K-blocks of 64 terms in a chunk (see above).
+inline int chunk_kblocks(int planes, bool activation, int kb_per_split) {
+  return planes == 1 && activation ? 16 : planes == 2 || kb_per_split <= 8 ? 2 : 4;
+}
 // T: element type of C (float, __nv_bfloat16, __half).
 template <typename T>
 int launch_gemm(const Gemm& g, const Plan& plan, cudaStream_t st);
@@ -709,8 +713,7 @@ int launch_tile(const Gemm& g, cudaStream_t st) {
   p.tiles = (int)tiles;
   p.kb_total = cdiv(g.K, 64);
   p.kb_per_split = cdiv(p.kb_total, g.splits);
-  if (PL == 1 && !PARTIAL && g.activation != B200GRU_ACT_NONE) p.chunk_kb = 16;
-  else p.chunk_kb = PL == 2 || p.kb_per_split <= 8 ? 2 : 4;
+  p.chunk_kb = chunk_kblocks(PL, !PARTIAL && g.activation != B200GRU_ACT_NONE, p.kb_per_split);
   p.ab_format = g.fp16 ? 0u : 1u;
   p.row_scale = g.row_scale; p.col_scale = g.col_scale; p.bias = g.bias;
   p.with_residual = !PARTIAL && g.residual != nullptr;
@@ -726,7 +729,7 @@ int launch_tile(const Gemm& g, cudaStream_t st) {
   const unsigned long long b_pl = PL > 1 ? (unsigned long long)g.b_plane * 2 : b_rows * g.ldb * 2;
   int rc = tc::make_tensor_map_3d(&m.a, dt, g.A, g.a_mn ? g.M : g.K, a_rows, PL, (unsigned long long)g.lda * 2, a_pl, 64, g.a_mn ? 64 : BM);
   if (rc == B200GRU_OK) rc = tc::make_tensor_map_3d(&m.b, dt, g.B, g.b_mn ? g.N : g.K, b_rows, PL, (unsigned long long)g.ldb * 2, b_pl, 64, g.b_mn ? 64 : BH);
-  // rows of results; partial sums to the padded end of their rows
+  // rows of results; partial sums end at N too, in rows padded for 16-byte alignment
   auto rows_map = [&](CUtensorMap* map, CUtensorMapDataType type, const void* base, long long cols, int slices, long long ld, size_t es) {
     return tc::make_tensor_map_out(map, type, base, cols, g.M, slices, (unsigned long long)ld * es, (unsigned long long)g.M * ld * es,
                                    G::COLS, 32, G::ROW_BYTES);

@@ -396,6 +396,8 @@ int b200gru_calibration_scan(const b200gru_shape* shape, const float* gi, const 
  * they do not apply); 0 the choice by shape.
  * b200gru_test_limit_gated_clusters: gated scans find, and launch, no cluster of more CTAs than this, as on a device that cannot
  * place one; 0 the device's own limit.
+ * b200gru_test_linear_plan: how a product of linear_act (1 plane of 16 bits, or 2 of fp32) is cut: plan[0] CTAs to a tile, [1] columns of a
+ * tile, [2] K slices, [3] blocks of 64 terms in a slice, [4] of them in a chunk.
  * b200gru_test_scan_plan: the kernel of a dense / block-diagonal scan as plan[0] (1 FP32 clusters, 2 tensor-core clusters,
  * 3 one product per step); for 2 its CTAs per cluster, row tile, rows per cluster, clusters and dynamic shared memory;
  * for 3 the tile width and K slices of the forward product.
@@ -409,6 +411,7 @@ int b200gru_test_set_scan_status(int value);
 void b200gru_test_select_dense_scan(int which);
 void b200gru_test_select_gemm(int which);
 void b200gru_test_limit_gated_clusters(int ranks);
+int b200gru_test_linear_plan(int M, int N, int K, int planes, int activation, int* plan);
 int b200gru_test_wait_timeout(void* stream);
 
 /* Human-readable text for a b200gru_status; plus the text of the last CUDA error

@@ -257,6 +257,72 @@ def test_scan_where_large_clusters_cannot_be_placed(dtype, T, H, odd):
     close(small, large.double(), tol + 2 * rounding(large.double(), dtype))
 
 
+def scan_errors(gi, h0, lengths, candidate, dout, dh):
+    """(h, dgi, dh0) in 64 bits, each with what every element may be off by: the recurrence applied to the errors of its steps.
+
+    A gate is off by u (12 + 2 |x|) of itself, a candidate by 30 u (identity: nothing) of itself, its slope by u (12 + 4 |c|).  Maps are
+    folded step by step and joined at three levels, so a position meets at most 8 roundings of sums whose terms add up to ``size``
+    (the recurrence of absolute values): E_t = z E_{t-1} + u ((12 + 2 |x|) (z size_{t-1} + (1 - z) |n|) + 30 (1 - z) |n| + 8 size_t), and
+    likewise for the gradients from behind."""
+    gi, dout, G = gi.double(), dout.double(), dh.double()
+    T, B, H = gi.shape[0], gi.shape[1], gi.shape[2] // 2
+    x, c = gi[..., :H], gi[..., H:]
+    z, keep = torch.sigmoid(x), torch.sigmoid(-x)
+    n, slope = (c.tanh(), c.cosh() ** -2) if candidate == "tanh" else (c, torch.ones_like(c))
+    own = 30.0 if candidate == "tanh" else 0.0
+    gate = 12 + 2 * x.abs()
+    on = (torch.arange(T, device=gi.device)[:, None] < (torch.full((B,), T, device=gi.device) if lengths is None else lengths))[..., None]
+    h = torch.zeros(B, H, dtype=torch.float64, device=gi.device) if h0 is None else h0.double()
+    size, E = h.abs(), torch.zeros_like(h)
+    hs, Es, ends = [h], [E], []
+    for t in range(T):
+        far = keep[t] * n[t].abs()
+        new = z[t] * size + far
+        E = torch.where(on[t], z[t] * E + U * (gate[t] * new + own * far + 8 * new), E)
+        size = torch.where(on[t], new, size)
+        h = torch.where(on[t], z[t] * h + keep[t] * n[t], h)
+        hs.append(h)
+        Es.append(E)
+        ends.append(size)
+    E, gabs = torch.zeros_like(G), G.abs()
+    dgi, off = torch.zeros_like(gi), torch.zeros_like(gi)
+    for t in reversed(range(T)):
+        g, gsize = G + dout[t], gabs + dout[t].abs()
+        E = E + U * gsize
+        left, both_gates = hs[t] - n[t], z[t] * keep[t]
+        dx, dc = g * left * both_gates, g * keep[t] * slope[t]
+        # h itself is computed anew from the tile's first state
+        wrong = Es[t + 1] + Es[t] + U * (own * n[t].abs() + left.abs())
+        ex = E * left.abs() * both_gates + gsize * wrong * both_gates + U * (8 + 2 * gate[t]) * dx.abs()
+        ec = E * keep[t] * slope[t] + U * (20 + gate[t] + 4 * c[t].abs()) * dc.abs()
+        dgi[t] = torch.where(on[t], torch.cat([dx, dc], 1), dgi[t])
+        off[t] = torch.where(on[t], torch.cat([ex, ec], 1), off[t])
+        G = torch.where(on[t], z[t] * g, G)
+        gabs = torch.where(on[t], z[t] * gsize, gabs)
+        E = torch.where(on[t], z[t] * E + U * (gate[t] + 8) * z[t] * gsize, E)
+    return (torch.stack(hs[1:]) * on, torch.stack(Es[1:]) * on), (hs[-1], Es[-1]), (dgi, off), (G, E)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("candidate", ["tanh", "identity"])
+@pytest.mark.parametrize("T,B,H,ragged", [(1, 3, 33, False), (8, 3, 64, False), (70, 2, 96, True), (257, 19, 607, False), (200, 64, 256, True),
+                                          (300, 300, 72, True), (600, 1, 130, False), (1000, 1, 1024, False), (1700, 1, 300, False),
+                                          (2100, 1, 24, False), (2300, 2, 256, True), (2300, 1, 513, False)])
+def test_scan_every_element_to_its_own_error(dtype, candidate, T, B, H, ragged):
+    """Bounds that follow the recurrence, far below the values they are for: a lost carry, map or tile shows at any length."""
+    gi, h0, dout, dh = problem(dtype, T, B, H, seed=T + B, lean=2.0)
+    gi[..., H + 3] *= 1e-6                                       # a column of tiny candidates, of tiny states where h0 is zero
+    h0[:, 3] = 0.0
+    lengths = torch.linspace(T, T // 2, B, device="cuda").long() if ragged else None
+    leaf, h = gi.detach().requires_grad_(True), h0.detach().requires_grad_(True)
+    out, h_T = gated_scan(leaf, h, lengths=lengths, candidate=candidate)
+    dgi, dh0 = torch.autograd.grad((out, h_T), (leaf, h), (dout, dh))
+    for got, (ref, tol) in zip((out.detach(), h_T.detach(), dgi, dh0), scan_errors(gi, h0, lengths, candidate, dout, dh)):
+        assert float(tol.norm()) <= 1e-4 * float(ref.norm())
+        close(got, ref, tol + rounding(ref, got.dtype))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("T", [3, 140])
@@ -479,6 +545,41 @@ def test_linear_matches_64_bits(dtype, M, K, N):
     x, W, bias, residual, dy = linear_problem(dtype, M, K, N, seed=M + K + N)
     check_linear(x, W, bias, residual, "silu", dy)
     check_linear(x, W, None, None, "none", dy)
+
+
+def linear_plan(M, N, K, dtype, activation="none"):
+    """(CTAs to a tile, columns of a tile, K slices, blocks of 64 terms in a slice, of them in a chunk)."""
+    plan = (ctypes.c_int * 5)()
+    assert _lib.load().b200gru_test_linear_plan(M, N, K, 2 if dtype == torch.float32 else 1, ACTIVATIONS[activation], plan) == 0
+    return tuple(plan)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("activation,residual", [("silu", True), ("gelu", False), ("none", True)])
+@pytest.mark.parametrize("M,K,N", [(4104, 4104, 4104), (16400, 4096, 1024), (9000, 520, 4104)])
+def test_linear_on_pairs_of_ctas(dtype, activation, residual, M, K, N):
+    """256 x 256 tiles of two CTAs in the forward and in the gradients, at remainders, of many chunks, with everything an epilogue does."""
+    forward, dx, dW = linear_plan(M, N, K, dtype, activation), linear_plan(M, K, N, dtype), linear_plan(N, K, M, dtype)
+    assert forward[0] == dW[0] == 2 and (dx[0] == 2 or K == 520)
+    if K > 4000 and dtype != torch.float32 and activation != "none":
+        assert forward[2] == 1 and forward[3] > 3 * forward[4]   # totals that pass through both accumulators, more than once
+    x, W, bias, r, dy = linear_problem(dtype, M, K, N, seed=N)
+    check_linear(x, W, bias, r if residual else None, activation, dy)
+
+
+def test_plans_of_the_large_tests():
+    """Every way a product is cut has a case above: pairs with and without K slices, single CTAs of both widths, one chunk and many."""
+    seen = set()
+    for M, K, N in [(4104, 4104, 4104), (16400, 4096, 1024), (9000, 520, 4104), *LINEAR_SIZES]:
+        for dtype in DTYPES[:2]:
+            for m, n, k in ((M, N, K), (M, K, N), (N, K, M)):
+                ctas, bn, splits, per, chunk = linear_plan(m, n, k, dtype)
+                seen.add((dtype, ctas, bn, splits > 1, per > chunk))
+    for dtype in DTYPES[:2]:
+        for ctas, bn in ((2, 256), (1, 128), (1, 64)):
+            assert (dtype, ctas, bn, False, True) in seen
+            assert any(s[:4] == (dtype, ctas, bn, True) for s in seen) or (ctas == 2 and dtype != torch.float32)
 
 
 @pytest.mark.gpu
