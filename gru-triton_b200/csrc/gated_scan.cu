@@ -1008,19 +1008,23 @@ size_t b200gru_gated_states_bytes(int T, int B, int H) {
   return (size_t)cdiv(T, gated::tile_steps(T, B, H)) * B * H * sizeof(float);
 }
 
-int b200gru_gated_scan_forward(const b200gru_gated_args* p, void* stream) {
+int b200gru_gated_scan_forward(const b200gru_gated_args* p, void* stream) try {
   const int rc = check_scan(p);
   if (rc) return rc;
   if (p->out == nullptr || p->h_T == nullptr || p->out_t <= 0 || p->out_b <= 0) return B200GRU_INVALID_ARGUMENT;
   return gated::launch_forward(to_args(p), p->dtype, static_cast<cudaStream_t>(stream));
+} catch (...) {
+  return B200GRU_LAUNCH_FAILURE;
 }
 
-int b200gru_gated_scan_backward(const b200gru_gated_args* p, void* stream) {
+int b200gru_gated_scan_backward(const b200gru_gated_args* p, void* stream) try {
   const int rc = check_scan(p);
   if (rc) return rc;
   if (p->states == nullptr || p->dgi == nullptr || p->dgi_t <= 0 || p->dgi_b <= 0) return B200GRU_INVALID_ARGUMENT;
   if (p->dout != nullptr && (p->dout_t < 0 || p->dout_b < 0)) return B200GRU_INVALID_ARGUMENT;
   return gated::launch_backward(to_args(p), p->dtype, static_cast<cudaStream_t>(stream));
+} catch (...) {
+  return B200GRU_LAUNCH_FAILURE;
 }
 
 int b200gru_gated_step(int dtype, int candidate_tanh, int B, int H, const void* gi, long long gi_b, const float* h,
