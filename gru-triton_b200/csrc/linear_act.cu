@@ -551,7 +551,8 @@ struct Call {
       }
       T* out = static_cast<T*>(g.C);
       const long long ldc = g.ldc;
-      const bool apart = !on16(g.C, g.ldc, sizeof(T));
+      // a tile store writes whole 16-byte pieces: behind rows that end inside one, too
+      const bool apart = !on16(g.C, g.ldc, sizeof(T)) || g.N * sizeof(T) % 16 != 0;
       if (apart) { g.C = ws.template take<T>(g.M * ld); g.ldc = ld; }
       typedef typename SlopeOf<T>::type S;
       S* slope = static_cast<S*>(g.slope);

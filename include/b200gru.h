@@ -310,7 +310,7 @@ int b200gru_gated_step(int dtype, int candidate_tanh, int B, int H, const void* 
  *   d = dy act'(pre)   dx = d W   dW = d^T x   db = sum over rows of d      (the residual's gradient is dy itself)
  * All of `dtype`; row strides ld* in elements (inputs may have stride 0), rows contiguous; dx, dW and db are packed.
  * bias, residual, dx, dW, db may be NULL.  slope: [M][lds], written by a forward that a backward follows (4 bytes each
- * for fp32, else 2) and read by it; NULL in inference and where there is no activation.  workspace: 256-byte aligned,
+ * for fp32, else 2; columns behind N may be written) and read by it; NULL in inference and where there is no activation.  workspace: 256-byte aligned,
  * b200gru_linear_act_workspace_bytes of the same arguments ((size_t)-1: invalid).  Results repeat their bits; those of a row
  * depend on M to rounding.  No reference counterpart (its
  * projections are F.linear, src/gru_qat/gru_cell.py:410-435). */

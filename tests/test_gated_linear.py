@@ -723,6 +723,42 @@ def test_linear_slopes_of_any_row_pitch(dtype, M, K, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("activation", ["none", "gelu"])
+@pytest.mark.parametrize("M, K, N", [(2, 131, 59), (40, 2045, 131), (300, 133, 267), (300, 130, 266), (1100, 258, 1029), (4100, 1030, 4099)])
+def test_linear_of_column_blocks_of_wider_matrices(dtype, activation, M, K, N):
+    """Odd widths in rows on 16-byte boundaries: what lies beside a block is neither read into a result nor written."""
+    x, W, bias, residual, dy = linear_problem(dtype, M, K, N, seed=9)
+
+    def block(t):
+        big = torch.full((t.shape[0], (t.shape[1] + 7) // 8 * 8 + 16), float("nan"), dtype=dtype, device="cuda")
+        big[:, 8:8 + t.shape[1]] = t
+        return big[:, 8:8 + t.shape[1]]
+
+    want = [t.detach().requires_grad_(True) for t in (x, W, bias, residual)]
+    y = linear_act(*want[:3], activation=activation, residual=want[3])
+    grads = torch.autograd.grad(y, want, dy)
+    got = [t.detach().requires_grad_(True) for t in (block(x), block(W), bias, block(residual))]
+    out = linear_act(*got[:3], activation=activation, residual=got[3])
+    assert torch.equal(out, y)
+    for a, b in zip(torch.autograd.grad(out, got, block(dy)), grads):
+        assert torch.equal(a, b)
+    # a C caller's result is such a block as well
+    lib, stream = _lib.load(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    whole = torch.full((M, (N + 7) // 8 * 8 + 16), 7.0, dtype=dtype, device="cuda")
+    inside = whole[:, 8:8 + N]
+    a = _lib.CLinearArgs()
+    a.M, a.K, a.N, a.dtype, a.activation = M, K, N, DTYPES.index(dtype), ACTIVATIONS[activation]
+    a.x, a.ldx, a.W, a.ldw, a.bias = x.data_ptr(), K, W.data_ptr(), K, bias.data_ptr()
+    a.residual, a.ldr, a.y, a.ldy = residual.data_ptr(), N, inside.data_ptr(), whole.shape[1]
+    n = lib.b200gru_linear_act_workspace_bytes(ctypes.byref(a), 0)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    assert lib.b200gru_linear_act_forward(ctypes.byref(a), stream) == 0
+    assert torch.equal(inside, y) and bool((whole[:, :8] == 7).all()) and bool((whole[:, 8 + N:] == 7).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [5, 200])
 def test_linear_no_rows_some_gradients_and_special_values(M):
     x, W, bias, residual, dy = linear_problem(torch.float32, M, 64, 48)
