@@ -312,8 +312,8 @@ __device__ __forceinline__ void close_group(const Params& p, const CUtensorMap* 
   ++w.sent;
 }
 
-// Out = void: partial sums in fp32.
-template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out>
+// Out = void: partial sums in fp32.  IN_REGISTERS: where the chunks of a tile are added up.
+template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out, bool IN_REGISTERS>
 __global__ void __launch_bounds__(THREADS, 1)
 lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmS,
@@ -535,8 +535,8 @@ lin_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         return open_group<Out, NC>(p, &tmR, w, here ? Corner{at.row, at.col + (g + 1) * G::COLS, 0} : then, here || !last, deadp, status);
       };
       auto close = [&](int g) { close_group<Out, NC>(p, &tmC, &tmS, w, at, g * G::COLS); };
-      if (PL == 1 && ACT != B200GRU_ACT_NONE) {
-        // Long chunks, usually one: a total of more is summed in registers and put back, so that the way out is one: from tensor
+      if (!IN_REGISTERS) {
+        // One chunk, or few long ones: a total of more is summed in registers and put back, so that the way out is one: from tensor
         // memory, the next 32 columns requested before these are finished.
         const int buf0 = c & 1;
         ok = landed(buf0);
@@ -668,9 +668,9 @@ struct Maps {
   alignas(64) CUtensorMap a, b, c, slope, residual;
 };
 
-template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out>
-int launch_variant(Params p, const Maps& m, cudaStream_t st) {
-  auto kernel = lin_gemm_kernel<CTAS, BN, A_MN, B_MN, PL, ACT, Out>;
+template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out, bool IN_REGISTERS>
+int launch_kernel(Params p, const Maps& m, cudaStream_t st) {
+  auto kernel = lin_gemm_kernel<CTAS, BN, A_MN, B_MN, PL, ACT, Out, IN_REGISTERS>;
   constexpr int BH = CTAS == 2 ? 128 : BN, stage = PL * (BM + BH) * 128;
   const int tail = EPI_WARPS * ((1 + p.out_mask + p.with_slope) * WARP_OUT + WARP_COEF);
   p.stages = (227 * 1024 - 1024 - 512 - tail) / stage;       // 512: barriers
@@ -690,6 +690,16 @@ int launch_variant(Params p, const Maps& m, cudaStream_t st) {
   cudaLaunchKernelEx(&cfg, kernel, m.a, m.b, m.c, m.slope, m.residual, p);
   note_launch();
   return check_launch("lin_gemm_kernel");
+}
+
+// Short chunks are added in registers; one chunk alone leaves from tensor memory at once (16384 x 120 -> 608 bf16: 13.4 us against
+// 15.4), and so do the long chunks before an activation.
+template <int CTAS, int BN, bool A_MN, bool B_MN, int PL, int ACT, typename Out>
+int launch_variant(const Params& p, const Maps& m, cudaStream_t st) {
+  if constexpr (PL == 2) return launch_kernel<CTAS, BN, A_MN, B_MN, PL, ACT, Out, true>(p, m, st);
+  else if constexpr (ACT != B200GRU_ACT_NONE) return launch_kernel<CTAS, BN, A_MN, B_MN, PL, ACT, Out, false>(p, m, st);
+  else if (p.kb_per_split > p.chunk_kb) return launch_kernel<CTAS, BN, A_MN, B_MN, PL, ACT, Out, true>(p, m, st);
+  else return launch_kernel<CTAS, BN, A_MN, B_MN, PL, ACT, Out, false>(p, m, st);
 }
 
 template <typename T> struct MapType;
