@@ -9,10 +9,10 @@
 // The tensor core's fp32 accumulator truncates: a sum of K terms loses up to 2^-23 of itself at each of its K / 16 steps, always
 // towards zero.  So sums are built in chunks, in one of two tensor-memory buffers, and the chunks added with round-to-nearest.
 // Planes: 24 steps.  16-bit types without an activation (gates of a recurrence, whose fp32 state carries every rounding of a
-// gate on; gradients): 8 steps where K is at most 512, else 16, added in registers.  With an activation 64 steps, added into the
+// gate on; gradients): 8 steps where K is at most 512, 16 up to 2048, then 32, added in registers.  With an activation 64 steps, added into the
 // next buffer: its epilogue is long, and reading chunks between would hold the products up (32768 x 1024 -> 4096 bf16, gelu: 196 us;
 // 241 with 32 steps, 304 with 16; none: 198 us with 16, 177 with one chunk).  Share of bf16 results that are not the rounding of the exact
-// sum, K 512 / 1024 / 4096: 1.0 / 1.8 / 2.0e-4 (one chunk: 2.8 / 5.6 / 23e-4; fp32 multiply-adds: 1.2 / 1.7 / 3.7e-4).
+// sum, K 512 / 1024 / 4096: 1.0 / 1.8 / 3.4e-4 (one chunk: 2.8 / 5.6 / 23e-4; fp32 multiply-adds: 1.2 / 1.7 / 3.7e-4).
 //
 // Roles of a CTA's ten warps: 0 loads k-blocks by TMA, 1 issues tcgen05.mma, 2-9 drain the accumulator (32 rows and half the
 // columns each; a lane has a row).  Results, slopes and residual move as TMA tiles of 32 rows x 128 bytes through swizzled
@@ -60,7 +60,9 @@ struct Plan {
 Plan plan_gemm(int M, int N, int K, int planes);
 // K-blocks of 64 terms in a chunk (see above).
 inline int chunk_kblocks(int planes, bool activation, int kb_per_split) {
-  return planes == 1 && activation ? 16 : planes == 2 || kb_per_split <= 8 ? 2 : 4;
+  if (planes == 2) return 2;
+  if (activation) return 16;
+  return kb_per_split <= 8 ? 2 : kb_per_split <= 32 ? 4 : 8;
 }
 // T: element type of C (float, __nv_bfloat16, __half).
 template <typename T>

@@ -922,10 +922,12 @@ def rounding_share(x, W, dtype, steps):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES[1:], ids=IDS[1:])
-@pytest.mark.parametrize("activation,K,steps", [("none", 512, 8), ("none", 1024, 16), ("none", 4096, 16), ("relu", 4096, 64)])
+@pytest.mark.parametrize("activation,K,steps", [("none", 512, 8), ("none", 1024, 16), ("none", 4096, 32), ("relu", 4096, 64)])
 def test_linear_16_bit_sums_are_built_in_short_chunks(dtype, activation, K, steps):
     """The share of results that are not the rounding of the exact sum (the tensor core truncates at every step: one chunk of
-    all of K would leave eight times as many at K = 4096)."""
+    all of K would leave seven times as many at K = 4096)."""
+    plan = linear_plan(8192, 1024, K, dtype, activation)
+    assert plan[2] == 1 and min(plan[3:]) * 4 == steps
     x, W, _, _, _ = linear_problem(dtype, 8192, K, 1024, seed=K)
     y = linear_act(x, W, activation=activation)
     ref = act64(x.double() @ W.double().t(), activation)
