@@ -11,7 +11,8 @@ its results (whatever the padding holds), ``out`` and the gradient of ``gi`` are
 the state after its last step.  Lengths outside [0, T] count as the nearer end.
 
 Element types float32, bfloat16 and float16; states (``h0``, ``h_T``) are float32 in all of them, and so
-is everything inside.  The same call repeats its bits.  CUDA tensors only; there is no fallback.  No
+is everything inside: a state is exact to float32 rounding for the gates that came in, a gate to a few units of itself whether it is
+open or closed.  (Gates of 16 bits carry their own rounding into it.)  The same call repeats its bits.  CUDA tensors only; there is no fallback.  No
 counterpart in the reference, whose recurrences all have hidden weights (scan_diagonal.py:79-124).
 """
 
